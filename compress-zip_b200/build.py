@@ -50,7 +50,7 @@ def build_tokenizer() -> str:
 
 def _headers_mtime():
     hs = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".h", ".cuh"))]
-    hs.append(os.path.join(ROOT, "include", "czg.h"))
+    hs += [os.path.join(ROOT, "include", f) for f in ("czg.h", "czg_ops.h")]
     return max(os.path.getmtime(h) for h in hs)
 
 

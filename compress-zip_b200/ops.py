@@ -1,0 +1,353 @@
+"""Operators on device tensors: ctypes binding of include/czg_ops.h (libczg.so).
+
+The int8 product with scales for each token and channel (``quantize_rows``,
+``linear_i8``), and a key/value cache held in 4 bits (``KV4Cache``) with attention
+over it and eviction from it by accumulated attention weight.
+
+Every call queues its work on the current stream of its tensors' device and returns
+without waiting; nothing is allocated but the results and a workspace, both by torch.
+Shapes and types are checked here (ValueError) and again by the library (CzgError).
+What only the device can see -- slots and lengths out of range -- sets bits that
+``KV4Cache.check`` reads.  No fallback: tensors must be on a CUDA device.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import engine as _engine
+from .engine import CZG_OK, CzgError
+
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+# The exported symbols of include/czg_ops.h, checked by the CPU test suite.
+EXPORTS = ["czg_ops_last_error", "czg_quantize_rows", "czg_linear_i8", "czg_linear_i8_workspace",
+           "czg_linear_i8_dynamic", "czg_kv4_append", "czg_kv4_read", "czg_kv4_attend_workspace",
+           "czg_kv4_attend", "czg_kv4_evict"]
+
+STATUS_BITS = {1: "a slot beyond the cache", 2: "a length or entry outside its range",
+               4: "a slot named twice in one call"}
+
+
+class _KV4(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("scales", C.c_void_p), ("weights", C.c_void_p),
+                ("status", C.c_void_p), ("n_slots", C.c_int32), ("n_heads", C.c_int32),
+                ("capacity", C.c_int32), ("head_dim", C.c_int32)]
+
+
+_bound = None
+
+
+def lib() -> C.CDLL:
+    global _bound
+    if _bound is None:
+        L = _engine.lib()
+        P, I, L64, U64 = C.c_void_p, C.c_int32, C.c_int64, C.c_uint64
+        K = C.POINTER(_KV4)
+        sig = {
+            "czg_quantize_rows": [P, I, L64, L64, L64, P, L64, P, P],
+            "czg_linear_i8": [P, L64, P, P, L64, P, P, L64, L64, L64, P, I, L64, P],
+            "czg_linear_i8_dynamic": [P, I, L64, P, L64, P, P, L64, L64, L64, P, I, L64, P, U64, P],
+            "czg_kv4_append": [K, P, L64, L64, L64, P, L64, L64, L64, I, P, P, I, I, P],
+            "czg_kv4_read": [K, P, P, I, I, P, P, I, P],
+            "czg_kv4_attend": [K, P, L64, L64, L64, I, P, P, I, I, I, I, C.c_float, P, L64, L64, L64, P, U64, P],
+            "czg_kv4_evict": [K, P, P, I, I, I, I, P, P, P],
+        }
+        for name, args in sig.items():
+            fn = getattr(L, name)
+            fn.argtypes, fn.restype = args, C.c_int
+        L.czg_linear_i8_workspace.argtypes, L.czg_linear_i8_workspace.restype = [L64, L64], U64
+        L.czg_kv4_attend_workspace.argtypes, L.czg_kv4_attend_workspace.restype = [K, I, I, I, I], U64
+        L.czg_ops_last_error.argtypes, L.czg_ops_last_error.restype = [], C.c_char_p
+        _bound = L
+    return _bound
+
+
+def _raise(status: int) -> None:
+    raise CzgError(status, lib().czg_ops_last_error().decode())
+
+
+def _dtype(t: torch.Tensor, what: str) -> int:
+    code = DTYPES.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{what} must be float32, bfloat16 or float16, not {t.dtype}")
+    return code
+
+
+def _same_device(dev: torch.device, **tensors) -> None:
+    if dev.type != "cuda":
+        raise ValueError(f"tensors must be on a CUDA device, not {dev}")
+    for name, t in tensors.items():
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, the others on {dev}")
+
+
+def _call(dev: torch.device, fn, *args) -> None:
+    """fn(*args, stream) on the current stream of dev, with dev current."""
+    if dev.index == torch.cuda.current_device():
+        st = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            st = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    if st != CZG_OK:
+        _raise(st)
+
+
+# ---- int8 product --------------------------------------------------------------
+
+
+class QRows(NamedTuple):
+    """Rows of int8 codes [n, k] (row stride a multiple of 16 bytes) and their float32 scales [n]."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+
+def _codes(q: QRows, what: str) -> None:
+    c, s = q
+    if c.dtype != torch.int8 or c.dim() != 2 or (c.stride(1) != 1 and c.shape[1] > 1):
+        raise ValueError(f"{what}.codes must be a 2-D int8 tensor with adjacent columns")
+    if s.dtype != torch.float32 or s.dim() != 1 or s.shape[0] != c.shape[0] or (s.stride(0) != 1 and s.shape[0] > 1):
+        raise ValueError(f"{what}.scales must be a contiguous float32 vector, one scale a row")
+    if c.data_ptr() % 16 or (c.stride(0) % 16 and c.shape[0] > 1):
+        raise ValueError(f"{what}.codes' rows must begin on 16-byte boundaries (quantize_rows lays them out so)")
+
+
+def _rows(x: torch.Tensor, what: str) -> None:
+    if x.dim() != 2 or (x.stride(1) != 1 and x.shape[1] > 1):
+        raise ValueError(f"{what} must be 2-D with adjacent columns")
+
+
+def _ld(t: torch.Tensor) -> int:
+    """Row stride; for a single row, whatever satisfies the library's alignment."""
+    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 15) // 16 * 16
+
+
+def quantize_rows(x: torch.Tensor) -> QRows:
+    """Rows of x as int8 codes with one scale each: scale = max |x| / 127, code =
+    round-half-even(127 x / max |x|).  For activations, one scale a token; for a weight
+    [n, k], one scale an output channel."""
+    code = _dtype(x, "x")
+    _rows(x, "x")
+    _same_device(x.device)
+    m, k = x.shape
+    ld = (k + 15) // 16 * 16
+    codes = torch.empty((m, ld), dtype=torch.int8, device=x.device)
+    scales = torch.empty(m, dtype=torch.float32, device=x.device)
+    if m and k:
+        _call(x.device, lib().czg_quantize_rows, x.data_ptr(), code, _ld(x), m, k, codes.data_ptr(), ld,
+              scales.data_ptr())
+    elif m:
+        scales.zero_()
+    return QRows(codes[:, :k], scales)
+
+
+def linear_i8(x, w: QRows, bias: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
+              out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """x @ w.T from int8 codes: exact int32 sums, times the token's and the channel's
+    scale, plus ``bias`` (float32 [n]), rounded once to ``out_dtype``.
+
+    x: a QRows, or a float tensor [..., k] whose rows are quantised in the same call.
+    out_dtype defaults to x's type (bfloat16 for a QRows); ``out``, if given, has
+    adjacent columns and is returned."""
+    _codes(w, "w")
+    n, k = w.codes.shape
+    dev = w.codes.device
+    quantised = isinstance(x, QRows)
+    if quantised:
+        _codes(x, "x")
+        x2, lead = x.codes, x.codes.shape[:1]
+    else:
+        code = _dtype(x, "x")
+        if x.dim() < 1:
+            raise ValueError("x must have a last dimension of k")
+        lead = x.shape[:-1]
+        x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1]) if x.numel() or x.shape[-1] else x.new_empty(lead.numel(), 0)
+        _rows(x2, "x")
+    if x2.shape[1] != k:
+        raise ValueError(f"x has rows of {x2.shape[1]}, w of {k}")
+    m = x2.shape[0]
+    if out is None:
+        kind = out_dtype if out_dtype is not None else torch.bfloat16 if quantised else x.dtype
+        if kind not in DTYPES:
+            raise ValueError(f"out_dtype must be float32, bfloat16 or float16, not {kind}")
+        out2 = None
+    else:
+        if out_dtype is not None and out.dtype != out_dtype:
+            raise ValueError(f"out is of {out.dtype}, out_dtype {out_dtype}")
+        kind = out.dtype
+        _dtype(out, "out")
+        if out.shape != (*lead, n):
+            raise ValueError(f"out must have shape {(*lead, n)}, not {tuple(out.shape)}")
+        out2 = out if out.dim() == 2 else out.view(-1, n)
+        _rows(out2, "out")
+    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (n,) or (n > 1 and bias.stride(0) != 1)):
+        raise ValueError(f"bias must be a contiguous float32 vector of {n}")
+    _same_device(dev, x=x2, x_scales=x.scales if quantised else None, w_scales=w.scales, bias=bias, out=out)
+    if out2 is None:
+        out2 = torch.empty((m, n), dtype=kind, device=dev)
+        out = out2 if len(lead) == 1 else out2.view(*lead, n)
+    if m == 0 or n == 0:
+        return out
+    if k == 0:
+        out2.copy_(torch.zeros((), device=dev) if bias is None else bias)
+        return out
+    L = lib()
+    tail = (w.codes.data_ptr(), _ld(w.codes), w.scales.data_ptr(), 0 if bias is None else bias.data_ptr(), m, n, k,
+            out2.data_ptr(), DTYPES[kind], out2.stride(0) if m > 1 else n)
+    if quantised:
+        _call(dev, L.czg_linear_i8, x2.data_ptr(), _ld(x2), x.scales.data_ptr(), *tail)
+    else:
+        need = L.czg_linear_i8_workspace(m, k)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        _call(dev, L.czg_linear_i8_dynamic, x2.data_ptr(), code, x2.stride(0) if m > 1 else k, *tail, ws.data_ptr(), need)
+    return out
+
+
+# ---- key/value cache in 4 bits ----------------------------------------------------
+
+
+class KV4Cache:
+    """A key/value cache of 4-bit entries over the caller's tensors.
+
+    k, v     uint8 [n_slots, n_heads, capacity, head_dim / 2]
+    scales   bfloat16 [n_slots, n_heads, capacity, 4] (k step, k lo, v step, v lo)
+    weights  None, or float32 [n_slots, n_heads, capacity]: sums of attention weights, grown by
+             ``attend`` and ranked by ``evict``
+
+    ``KV4Cache.empty`` allocates them.  Calls name sequences by ``slots`` (int32 [b]; a
+    negative one is a padded place of the batch) and ``lengths`` (int32 [b], entries of
+    each sequence, the rows of the call among them), both on the device.  Slots of a
+    call that writes (append, evict, attend with weights) are distinct."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, scales: torch.Tensor, weights: Optional[torch.Tensor] = None):
+        if k.dim() != 4 or k.dtype != torch.uint8 or v.shape != k.shape or v.dtype != torch.uint8:
+            raise ValueError("k and v must be uint8 tensors [n_slots, n_heads, capacity, head_dim / 2]")
+        if k.shape[3] not in (32, 64):
+            raise ValueError(f"head_dim must be 64 or 128, not {2 * k.shape[3]}")
+        if scales.shape != (*k.shape[:3], 4) or scales.dtype != torch.bfloat16:
+            raise ValueError("scales must be a bfloat16 tensor [n_slots, n_heads, capacity, 4]")
+        if weights is not None and (weights.shape != k.shape[:3] or weights.dtype != torch.float32):
+            raise ValueError("weights must be a float32 tensor [n_slots, n_heads, capacity]")
+        for name, t in (("k", k), ("v", v), ("scales", scales), ("weights", weights)):
+            if t is not None and (not t.is_contiguous() or t.data_ptr() % 16):
+                raise ValueError(f"{name} must be contiguous and begin on a 16-byte boundary")
+        if k.numel() == 0:
+            raise ValueError("a cache has at least one slot, head and entry")
+        _same_device(k.device, v=v, scales=scales, weights=weights)
+        self.k, self.v, self.scales, self.weights = k, v, scales, weights
+        self.device = k.device
+        self.n_slots, self.n_heads, self.capacity = k.shape[:3]
+        self.head_dim = 2 * k.shape[3]
+        self.status = torch.zeros(1, dtype=torch.int32, device=k.device)
+        self._c = _KV4(k.data_ptr(), v.data_ptr(), scales.data_ptr(), 0 if weights is None else weights.data_ptr(),
+                       self.status.data_ptr(), self.n_slots, self.n_heads, self.capacity, self.head_dim)
+        self._ref = C.byref(self._c)
+
+    @classmethod
+    def empty(cls, n_slots: int, n_heads: int, capacity: int, head_dim: int, track_weights: bool = False,
+              device="cuda") -> "KV4Cache":
+        """A cache of its own tensors: entries are zeros, no sequence holds any."""
+        shape = (n_slots, n_heads, capacity)
+        kv = [torch.zeros(*shape, head_dim // 2, dtype=torch.uint8, device=device) for _ in range(2)]
+        return cls(*kv, torch.zeros(*shape, 4, dtype=torch.bfloat16, device=device),
+                   torch.zeros(shape, dtype=torch.float32, device=device) if track_weights else None)
+
+    def _sequences(self, slots: torch.Tensor, counts: torch.Tensor, name: str) -> int:
+        for what, t in (("slots", slots), (name, counts)):
+            if t.dtype != torch.int32 or t.dim() != 1 or t.shape != slots.shape or (t.stride(0) != 1 and t.shape[0] > 1):
+                raise ValueError(f"{what} must be a contiguous int32 vector, one number a sequence")
+            if t.device != self.device:
+                raise ValueError(f"{what} is on {t.device}, the cache on {self.device}")
+        return slots.shape[0]
+
+    def append(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, lengths: torch.Tensor) -> None:
+        """Quantise rows k, v [b, t, n_heads, head_dim] into entries lengths - t .. lengths - 1
+        of their slots; rows before entry 0 are padding.  Their weights become 0."""
+        b = self._sequences(slots, lengths, "lengths")
+        if k.dim() != 4 or k.shape[0] != b or k.shape[2:] != (self.n_heads, self.head_dim) or v.shape != k.shape:
+            raise ValueError(f"k and v must be [{b}, t, {self.n_heads}, {self.head_dim}]")
+        code = _dtype(k, "k")
+        if v.dtype != k.dtype:
+            raise ValueError("k and v must have the same type")
+        if k.stride(3) != 1 or v.stride(3) != 1:
+            raise ValueError("the last dimension of k and v must be adjacent")
+        _same_device(self.device, k=k, v=v)
+        if k.numel():
+            _call(self.device, lib().czg_kv4_append, self._ref, k.data_ptr(), k.stride(0), k.stride(1), k.stride(2),
+                  v.data_ptr(), v.stride(0), v.stride(1), v.stride(2), code, slots.data_ptr(), lengths.data_ptr(), b,
+                  k.shape[1])
+
+    def read(self, slots: torch.Tensor, starts: torch.Tensor, count: int, dtype: torch.dtype = torch.bfloat16):
+        """Entries starts .. starts + count - 1 of each slot as values: (k, v), each
+        [b, count, n_heads, head_dim]; 0 for places outside the slot."""
+        b = self._sequences(slots, starts, "starts")
+        if dtype not in DTYPES:
+            raise ValueError(f"dtype must be float32, bfloat16 or float16, not {dtype}")
+        if count < 0:
+            raise ValueError("count must not be negative")
+        shape = (b, count, self.n_heads, self.head_dim)
+        k, v = (torch.empty(shape, dtype=dtype, device=self.device) for _ in range(2))
+        if k.numel():
+            _call(self.device, lib().czg_kv4_read, self._ref, slots.data_ptr(), starts.data_ptr(), b, count,
+                  k.data_ptr(), v.data_ptr(), DTYPES[dtype])
+        return k, v
+
+    def attend(self, q: torch.Tensor, slots: torch.Tensor, lengths: torch.Tensor, max_len: Optional[int] = None,
+               scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Attention of q [b, t, hq, head_dim] (bfloat16 or float16) over the sequences'
+        entries, row i seeing the first lengths - (t - 1 - i); rows that see none give 0.
+        hq is a multiple of n_heads.  max_len (default: the capacity) bounds the lengths,
+        scale defaults to head_dim ** -0.5.  With weights, each entry's grows by its
+        probabilities, summed over the rows and query heads of its key head."""
+        b = self._sequences(slots, lengths, "lengths")
+        if q.dim() != 4 or q.shape[0] != b or q.shape[3] != self.head_dim or q.shape[2] % self.n_heads:
+            raise ValueError(f"q must be [{b}, t, a multiple of {self.n_heads}, {self.head_dim}]")
+        if q.dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError(f"q must be bfloat16 or float16, not {q.dtype}")
+        if q.stride(3) != 1:
+            raise ValueError("the last dimension of q must be adjacent")
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        elif out.shape != q.shape or out.dtype != q.dtype or out.stride(3) != 1:
+            raise ValueError("out must have q's shape and type and an adjacent last dimension")
+        _same_device(self.device, q=q, out=out)
+        if q.numel() == 0:
+            return out
+        n = self.capacity if max_len is None else max_len
+        L = lib()
+        t, hq = q.shape[1], q.shape[2]
+        need = L.czg_kv4_attend_workspace(self._ref, b, t, hq, n)
+        ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+        _call(self.device, L.czg_kv4_attend, self._ref, q.data_ptr(), q.stride(0), q.stride(1), q.stride(2),
+              DTYPES[q.dtype], slots.data_ptr(), lengths.data_ptr(), b, t, hq, n,
+              self.head_dim ** -0.5 if scale is None else scale, out.data_ptr(), out.stride(0), out.stride(1),
+              out.stride(2), ws.data_ptr() if need else 0, need)
+        return out
+
+    def evict(self, slots: torch.Tensor, lengths: torch.Tensor, budget: int, recent: int = 0,
+              max_len: Optional[int] = None):
+        """Cut sequences longer than ``budget`` to it: of each head the last ``recent``
+        entries stay and the budget - recent others with the largest weights (ties: the
+        first), in order, moved to the front of the slot.  Returns (kept, new lengths):
+        int32 [b, n_heads, budget] former places (-1 behind a shorter end) and int32 [b]."""
+        b = self._sequences(slots, lengths, "lengths")
+        if self.weights is None:
+            raise ValueError("the cache keeps no weights to rank entries by")
+        if budget < 1 or not 0 <= recent <= budget:
+            raise ValueError("1 <= budget and 0 <= recent <= budget are needed")
+        kept = torch.empty((b, self.n_heads, budget), dtype=torch.int32, device=self.device)
+        new = torch.empty(b, dtype=torch.int32, device=self.device)
+        if b:
+            _call(self.device, lib().czg_kv4_evict, self._ref, slots.data_ptr(), lengths.data_ptr(), b,
+                  self.capacity if max_len is None else max_len, budget, recent, kept.data_ptr(), new.data_ptr())
+        return kept, new
+
+    def check(self) -> None:
+        """Wait for the device and raise CzgError if a call met slots or lengths out of
+        range; the bits are cleared."""
+        bits = int(self.status.item())
+        if bits:
+            self.status.zero_()
+            raise CzgError(1, ", ".join(text for bit, text in STATUS_BITS.items() if bits & bit))

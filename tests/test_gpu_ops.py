@@ -1,0 +1,727 @@
+"""The device-buffer operators (include/czg_ops.h) against their definitions in 64 bits.
+
+Tolerances.  u is half a step of the output type (fp32 2^-24, bf16 2^-8 / 2 ... as
+torch.finfo(t).eps / 2); a result's error is bounded by u |y| for its one rounding plus what the
+arithmetic before it may lose, written out at each comparison.
+"""
+import math
+import os
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
+DEV = "cuda"
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from compress_zip_b200 import ops
+
+    return ops
+
+
+def gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def randn(g, *shape):
+    return torch.randn(*shape, generator=g, device=DEV)
+
+
+def u(t):
+    return torch.finfo(t).eps / 2
+
+
+# ---- quantize_rows ------------------------------------------------------------------
+
+
+def codes_of(x):
+    """(codes, scales) by the definition; the quotients of 16-bit values are exact to 2^-53."""
+    x = x.double()
+    a = x.abs().amax(1, keepdim=True)
+    return torch.where(a > 0, 127 * x / a, 0).round().to(torch.int8), (a / 127).float()[:, 0]
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("m,k", [(1, 1), (1, 16), (3, 17), (5, 384), (2, 4097), (300, 63), (64, 1024), (7, 10007)])
+def test_quantize_rows(ops, dtype, m, k):
+    g = gen(m * k)
+    x = randn(g, m, k + 5).to(dtype)[:, 2:k + 2]   # rows that begin off any boundary
+    if k > 2:
+        x[0, 1] = x[0].abs().max()
+        x[0, 2] = -x[0, 1] / 2                     # 127 x / max = -63.5: the even neighbour
+    got = ops.quantize_rows(x)
+    codes, scales = codes_of(x)
+    assert got.codes.shape == (m, k) and got.codes.stride(0) % 16 == 0
+    if dtype == FP32:   # 127 x and the quotient round (2^-23 in all): codes may differ next to a half alone
+        q = 127 * x.double() / x.double().abs().amax(1, keepdim=True)
+        assert ((got.codes.double() - q).abs() <= 0.5 + 128 * 2.0 ** -23).all()
+    else:
+        assert torch.equal(got.codes, codes)
+    assert torch.equal(got.scales, scales)
+    if k % 16:   # the bytes behind a row are zeros
+        full = got.codes.as_strided((m, got.codes.stride(0)), (got.codes.stride(0), 1))
+        assert not full[:, k:].any()
+
+
+def test_quantize_rows_special(ops):
+    x = torch.zeros(10, 40, device=DEV)
+    x[1] = 3.0
+    x[2, 5] = float("nan")
+    x[3, 39] = float("inf")
+    x[4, 0] = -float("inf")
+    x[5] = torch.linspace(-3e38, 3e38, 40)             # its step overflows: the row is not finite
+    x[9] = torch.linspace(-1, 1, 40) * 3e38
+    x[6] = 1e-45
+    x[7, 3] = -1e-20
+    x[8] = -0.0
+    for dtype in (FP32, BF16):
+        got = ops.quantize_rows(x.to(dtype))
+        s = got.scales
+        assert s[0] == 0 and s[8] == 0 and not got.codes[[0, 8]].any()
+        assert (got.codes[1] == 127).all()
+        assert not torch.isfinite(x[5]).all()
+        assert torch.isnan(s[2:6]).all() and not got.codes[2:6].any()
+        want, scale = codes_of(x.to(dtype)[9:])
+        assert (got.codes[9] - want[0]).abs().max() <= (1 if dtype == FP32 else 0) and s[9] == scale[0]
+        assert got.codes[7, 3] == -127 and got.codes[7].ne(0).sum() == 1
+        if dtype == FP32:
+            assert (got.codes[6] == 127).all()
+    assert ops.quantize_rows(torch.zeros(0, 7, device=DEV)).codes.shape == (0, 7)
+    empty = ops.quantize_rows(torch.zeros(3, 0, device=DEV))
+    assert empty.codes.shape == (3, 0) and not empty.scales.any()
+
+
+# ---- linear_i8 ------------------------------------------------------------------------
+
+
+def rand_codes(ops, g, n, k, pad=0):
+    """Codes whose rows are followed by bytes that must not count."""
+    ld = (k + 15) // 16 * 16 + pad
+    full = torch.randint(-127, 128, (n, ld), generator=g, device=DEV, dtype=torch.int8)
+    return ops.QRows(full[:, :k], 0.001 * (0.5 + torch.rand(n, generator=g, device=DEV)))
+
+
+def check_linear(y, x, w, bias):
+    acc = x.codes.double() @ w.codes.double().t()
+    prod = acc * x.scales.double()[:, None] * w.scales.double()
+    want = prod if bias is None else prod + bias.double()
+    # float(sum), two products and the sum with the bias round once each; then the output type's one
+    tol = u(y.dtype) * want.abs() + 4 * 2.0 ** -24 * (prod.abs() + want.abs())
+    if y.dtype == FP16:
+        tol = tol + 2.0 ** -25   # half a step of its subnormal numbers
+    assert ((y.double() - want).abs() <= tol).all(), ((y.double() - want).abs() - tol).max()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 512, 384), (2, 129, 17), (5, 64, 16), (16, 130, 100), (17, 100, 1100),
+                                   (33, 257, 640), (64, 300, 129), (65, 96, 512), (130, 257, 128), (200, 1000, 48),
+                                   (257, 513, 1000), (600, 640, 2048), (1, 4096, 4096), (24, 4096, 8200)])
+def test_linear_i8(ops, dtype, m, n, k):
+    g = gen(m + n + k)
+    x, w = rand_codes(ops, g, m, k, 32), rand_codes(ops, g, n, k)
+    bias = randn(g, n) if (m + n) % 2 else None
+    check_linear(ops.linear_i8(x, w, bias=bias, out_dtype=dtype), x, w, bias)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("m,n,k", [(1, 512, 384), (3, 70, 33), (50, 1024, 512), (300, 384, 1024)])
+def test_linear_i8_from_floats(ops, dtype, m, n, k):
+    """Quantising in the call is quantize_rows and then the product, bit for bit."""
+    g = gen(m * n)
+    x, w = randn(g, m, k).to(dtype), rand_codes(ops, g, n, k)
+    y = ops.linear_i8(x, w)
+    assert y.dtype == dtype
+    q = ops.quantize_rows(x)
+    assert torch.equal(y, ops.linear_i8(q, w, out_dtype=dtype))
+    check_linear(y, q, w, None)
+    batched = ops.linear_i8(x.view(1, m, k), w)
+    assert batched.shape == (1, m, n) and torch.equal(batched[0], y)
+    assert torch.equal(ops.linear_i8(x.t().contiguous().t().contiguous(), w), y)
+
+
+@pytest.mark.parametrize("m", [1, 7, 40, 150])
+def test_linear_i8_into_a_view(ops, m):
+    """out may be columns of a wider tensor: what lies beside them stays."""
+    g = gen(m)
+    x, w = rand_codes(ops, g, m, 96), rand_codes(ops, g, 45, 96)
+    wide = torch.full((m, 64), 7.0, device=DEV, dtype=BF16)
+    y = ops.linear_i8(x, w, out=wide[:, 3:48])
+    assert y.data_ptr() == wide[:, 3:].data_ptr()
+    check_linear(y, x, w, None)
+    assert (wide[:, :3] == 7).all() and (wide[:, 48:] == 7).all()
+
+
+def test_linear_i8_sums_are_exact(ops):
+    """The longest row at the largest codes: 131,071 * 127 * 127 stays below 2^31."""
+    k = 131071
+    x = ops.QRows(torch.full((3, 131072), 127, dtype=torch.int8, device=DEV)[:, :k], torch.ones(3, device=DEV))
+    w = ops.QRows(torch.full((5, 131072), 127, dtype=torch.int8, device=DEV)[:, :k], torch.ones(5, device=DEV))
+    w.codes[1] = -127
+    w.codes[2, ::2] = -127
+    y = ops.linear_i8(x, w, out_dtype=FP32)
+    want = (x.codes.double() @ w.codes.double().t()).float()
+    assert torch.equal(y, want)
+    with pytest.raises(RuntimeError, match="MAX_K"):
+        big = ops.QRows(torch.zeros(1, 131072, dtype=torch.int8, device=DEV), torch.ones(1, device=DEV))
+        ops.linear_i8(big, big)
+
+
+def test_linear_i8_not_finite(ops):
+    g = gen(4)
+    x, w = rand_codes(ops, g, 40, 64), rand_codes(ops, g, 30, 64)
+    x.scales[3] = float("nan")
+    w.scales[7] = float("inf")
+    y = ops.linear_i8(x, w, out_dtype=FP32)
+    assert torch.isnan(y[3]).all()
+    rest = torch.arange(40, device=DEV) != 3
+    assert not torch.isfinite(y[rest][:, 7]).any()
+    cols = torch.arange(30, device=DEV) != 7
+    assert torch.isfinite(y[rest][:, cols]).all()
+
+
+@pytest.mark.parametrize("n,k", [(512, 384), (130, 100), (4096, 1024)])
+def test_linear_i8_does_not_depend_on_the_batch(ops, n, k):
+    """A row alone gives the bits that it gives among others, wherever it stands."""
+    g = gen(n)
+    x, w, bias = rand_codes(ops, g, 700, k), rand_codes(ops, g, n, k), randn(g, n)
+    full = ops.linear_i8(x, w, bias=bias, out_dtype=FP32)
+    for a, b in ((0, 1), (5, 6), (3, 12), (100, 133), (690, 700), (64, 264)):
+        part = ops.linear_i8(ops.QRows(x.codes[a:b], x.scales[a:b]), w, bias=bias, out_dtype=FP32)
+        assert torch.equal(part, full[a:b])
+
+
+def test_linear_i8_is_the_models_projection(ops, shipped_path, oracle_mod):
+    """With a channel scale of mult / 2^shift (exact powers and small integers) the rounded and
+    clamped product is the engine's requantised projection, on the shipped model's weights."""
+    from compress_zip_b200 import czm
+
+    t = czm.ModelFile.load(shipped_path).tensors
+    wq = torch.from_numpy(np.array(t["layers.0.attn.qkv.weight"])).to(DEV)
+    mult, shift = 819, 20
+    g = gen(1)
+    x = torch.randint(-127, 128, (90, wq.shape[1]), generator=g, device=DEV, dtype=torch.int8)
+    y = ops.linear_i8(ops.QRows(x, torch.full((90,), float(mult), device=DEV)),
+                      ops.QRows(wq, torch.full((wq.shape[0],), 2.0 ** -shift, device=DEV)), out_dtype=FP32)
+    acc = (x.double() @ wq.double().t()).long() * mult
+    down = acc >> shift
+    rest = acc - (down << shift)
+    half = 1 << (shift - 1)
+    rne = down + ((rest > half) | ((rest == half) & (down & 1 == 1))).long()
+    # acc * mult < 2^34 may need more than 24 bits: away from a half by less than 2^-24 of the value
+    # the fp32 product may round onto it, so those places are left out
+    near = (rest - half).abs().double() <= acc.abs().double() * 2.0 ** -23
+    assert near.double().mean() < 0.01
+    got = y.round().clamp(-127, 127).long()
+    assert torch.equal(got[~near], rne.clamp(-127, 127)[~near])
+
+
+# ---- the 4-bit cache --------------------------------------------------------------------
+
+
+def bf16_below(x):
+    m, e = torch.frexp(x)
+    return torch.ldexp(torch.floor(m * 256), e - 8)
+
+
+def held(x):
+    """What an entry holds of rows x, in float64."""
+    x = x.double()
+    lo = bf16_below(x.amin(-1, keepdim=True))
+    step = -bf16_below((lo - x.amax(-1, keepdim=True)) / 15)
+    return lo + step * torch.where(step > 0, (x - lo) / step.clamp(min=1e-300), 0).round(), step[..., 0], lo[..., 0]
+
+
+def int32(*v):
+    return torch.tensor(v, dtype=torch.int32, device=DEV)
+
+
+def entries(c, slot):
+    """All entries of a slot in float64: k, v [heads, capacity, d]."""
+    out = []
+    for x, col in ((c.k, 0), (c.v, 2)):
+        b = x[slot].int()
+        codes = torch.stack([b & 15, b >> 4], -1).flatten(-2).double()
+        s = c.scales[slot].double()
+        out.append(s[..., col + 1:col + 2] + s[..., col:col + 1] * codes)
+    return out
+
+
+def noise_cache(ops, g, n_slots, heads, capacity, d, track):
+    """A cache of arbitrary codes and ranges: what no sequence has written yet is not zero."""
+    def codes():
+        return torch.randint(0, 256, (n_slots, heads, capacity, d // 2), generator=g, device=DEV, dtype=torch.uint8)
+
+    step = 0.05 + 0.3 * torch.rand(n_slots, heads, capacity, 2, generator=g, device=DEV)
+    lo = -step * (6 + 3 * torch.rand(step.shape, generator=g, device=DEV))
+    scales = torch.stack([step[..., 0], lo[..., 0], step[..., 1], lo[..., 1]], -1).to(BF16)
+    w = torch.rand(n_slots, heads, capacity, generator=g, device=DEV) if track else None
+    return ops.KV4Cache(codes(), codes(), scales, w)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+def test_append_and_read(ops, dtype, d):
+    g = gen(d)
+    c = noise_cache(ops, g, 6, 3, 50, d, True)
+    before = [t.clone() for t in (c.k, c.v, c.scales, c.weights)]
+    t = 5
+    # full, one row, a padded place, all padding, up to the end of the slot
+    slots, lengths = int32(4, 0, -1, 2, 5), int32(9, 1, 7, 0, 50)
+    big = randn(g, 5, 3, t + 2, 2 * d + 4).to(dtype)
+    k = big[:, :, 1:t + 1, 2:d + 2].transpose(1, 2)       # strides of its own for every dimension
+    v = randn(g, 5, t, 3, d).to(dtype)
+    k[0, 0, 0] = 0.75                                      # a constant row: exact
+    v[1, 4, 2] = 0                                         # a row of zeros
+    k[4, 1, 1, 7] = float("nan")
+    v[4, 2, 0, 0] = float("inf")
+    c.append(k, v, slots, lengths)
+    c.check()
+    written = torch.zeros(6, 50, dtype=torch.bool, device=DEV)
+    for i, (s, n) in enumerate(zip(slots.tolist(), lengths.tolist())):
+        if s < 0:
+            continue
+        for r in range(t):
+            e = n - t + r
+            if e < 0:
+                continue
+            written[s, e] = True
+            for x, col, name in ((k, 0, "k"), (v, 2, "v")):
+                want, step, lo = held(x[i, r])
+                got = entries(c, s)[0 if name == "k" else 1][:, e]
+                bad = ~torch.isfinite(x[i, r]).all(-1)
+                assert torch.isnan(got[bad]).all()
+                assert torch.equal(got[~bad], want[~bad])
+                assert torch.equal(c.scales[s, :, e, col].double()[~bad], step[~bad])
+                # half a step, and the rounding of the quotient (15 * 2^-24 of a step) next to a half
+                assert ((got - x[i, r].double()).abs() <= step[:, None] * (0.5 + 2.0 ** -20))[~bad].all()
+            assert not c.weights[s, :, e].any()
+    assert torch.equal(entries(c, 4)[0][0, 4], torch.full((d,), 0.75, dtype=torch.float64, device=DEV))
+    assert not entries(c, 0)[1][2, 0].any()
+    for now, old in zip((c.k, c.v, c.scales, c.weights), before):   # nothing else is touched
+        keep = ~written[:, None, :].expand(6, 3, 50)
+        assert torch.equal(now[keep], old[keep])
+    rk, rv = c.read(int32(4, -3, 5), int32(3, 0, 46), 6, dtype=dtype)
+    for got, which in ((rk, 0), (rv, 1)):
+        assert got.shape == (3, 6, 3, d) and not got[1].any() and not got[2, 4:].any()
+        for i, (s, a, n) in enumerate(((4, 3, 6), (-1, 0, 0), (5, 46, 4))):
+            want = entries(c, s)[which][:, a:a + n].transpose(0, 1)
+            ok = torch.isfinite(want)
+            assert torch.equal(torch.isfinite(got[i, :n]), ok)
+            # step * code is exact, the sum rounds to fp32 and then to the output type
+            tol = (u(dtype) + 2.0 ** -24) * want.abs() + (2.0 ** -25 if dtype == FP16 else 0)
+            assert ((got[i, :n].double() - want).abs() <= tol)[ok].all()
+    with pytest.raises(RuntimeError, match="length"):      # the read past the slot's end was reported
+        c.check()
+    c.check()
+
+
+def test_append_extremes(ops):
+    c = ops.KV4Cache.empty(1, 1, 8, 64)
+    x = torch.zeros(1, 4, 1, 64, device=DEV)
+    x[0, 0, 0, 3] = 3e38
+    x[0, 0, 0, 5] = -3e38          # the range overflows fp32
+    x[0, 1] = 1e-30
+    x[0, 1, 0, 9] = -2e-30
+    x[0, 2] = 65504.0
+    x[0, 3, 0, ::2] = 1.0
+    c.append(x, -x, int32(0), int32(4))
+    k, v = entries(c, 0)
+    assert torch.isnan(k[0, 0]).all() and torch.isnan(v[0, 0]).all()
+    for i in (1, 2, 3):
+        assert torch.equal(k[0, i], held(x[0, i])[0][0]) and torch.equal(v[0, i], held(-x[0, i])[0][0])
+    # 1 / 15 rounded up to bf16 is 137 / 2048: the upper end is held as 15 of those
+    assert torch.equal(k[0, 3], x[0, 3, 0].double() * (15 * 137 / 2048))
+
+
+def test_append_out_of_range_is_left_out_and_reported(ops):
+    g = gen(3)
+    for slots, lengths, text in (((0, 3), (2, 2), "slot beyond"), ((0, 1), (2, 11), "length"), ((0, 1), (2, -1), "length"),
+                                 ((1, 1), (2, 2), "twice")):
+        c = noise_cache(ops, g, 3, 2, 10, 64, False)
+        old = c.k.clone()
+        rows = randn(g, 2, 2, 2, 64)
+        c.append(rows, rows, int32(*slots), int32(*lengths))
+        with pytest.raises(RuntimeError, match=text):
+            c.check()
+        assert torch.equal(c.k[2], old[2])
+        if text != "twice":
+            assert torch.equal(entries(c, 0)[0][:, :2], held(rows[0])[0].transpose(0, 1))
+            where = c.k[1] == old[1]
+            assert where[:, :9].all() and (slots != (0, 1) or lengths[1] == 11 or where.all())
+
+
+# ---- attention ---------------------------------------------------------------------------
+
+
+def attention(c, q, slots, lengths, scale, max_len):
+    """(out, its tolerance, added weights, their tolerance) in float64.
+
+    A score's fp32 error is at most (D + 16) 2^-24 E, E the sum of its terms' magnitudes, and the
+    exponential adds 2^-21 (of it and its argument's product with log2 e): a weight is off by the
+    factor 1 + r, r = 2 (D + 16) 2^-24 E + 2^-20, numerator and denominator together twice that.
+    The weights are held in fp16 for the product with the values: 2^-11 of each value's terms."""
+    b, t, hq, d = q.shape
+    g = hq // c.n_heads
+    out, tol = torch.zeros(q.shape, dtype=torch.float64, device=DEV), torch.zeros(q.shape, dtype=torch.float64, device=DEV)
+    add = torch.zeros(c.n_slots, c.n_heads, c.capacity, dtype=torch.float64, device=DEV)
+    add_tol = torch.zeros_like(add)
+    for i, (s, n) in enumerate(zip(slots.tolist(), lengths.tolist())):
+        if not 0 <= s < c.n_slots:
+            continue
+        n = max(0, min(n, max_len, c.capacity))
+        k, v = entries(c, s)
+        sc = c.scales[s].double().abs()
+        k_abs, v_abs = 15 * sc[..., 0] + sc[..., 1], 15 * sc[..., 2] + sc[..., 3]
+        for r in range(t):
+            seen = n - (t - 1 - r)
+            if seen <= 0:
+                continue
+            qr = q[i, r].double().view(c.n_heads, g, d)
+            p = torch.softmax(scale * torch.einsum("hgd,hnd->hgn", qr, k[:, :seen]), -1)
+            e = abs(scale) * qr.abs().sum(-1, keepdim=True) * k_abs[:, None, :seen]
+            rel = 2 * (2 * (d + 16) * 2.0 ** -24 * e.amax(-1, keepdim=True) + 2.0 ** -20)
+            y = torch.einsum("hgn,hnd->hgd", p, v[:, :seen]).reshape(hq, d)
+            out[i, r] = y
+            terms = torch.einsum("hgn,hn->hg", p * (rel + 2.0 ** -11), v_abs[:, :seen]).reshape(hq, 1)
+            tol[i, r] = u(q.dtype) * y.abs() + terms + (2.0 ** -25 if q.dtype == FP16 else 0)
+            add[s, :, :seen] += p.sum(1)
+            add_tol[s, :, :seen] += (p * rel).sum(1)
+    return out, tol, add, add_tol
+
+
+def check_attend(ops, c, q, slots, lengths, max_len=None, scale=None):
+    before = None if c.weights is None else c.weights.clone()
+    y = c.attend(q, slots, lengths, max_len=max_len, scale=scale)
+    out, tol, add, add_tol = attention(c, q, slots, lengths, q.shape[3] ** -0.5 if scale is None else scale,
+                                       c.capacity if max_len is None else max_len)
+    assert y.shape == q.shape and y.dtype == q.dtype
+    assert torch.isfinite(y).all()
+    worst = ((y.double() - out).abs() - tol).max()
+    assert worst <= 0, worst
+    if before is not None:
+        want = before.double() + add
+        rows = q.shape[1] * q.shape[2] // c.n_heads
+        tol = add_tol + (rows + 2) * 2.0 ** -24 * (want.abs() + add)
+        worst = ((c.weights.double() - want).abs() - tol).max()
+        assert worst <= 0, worst
+        same = add == 0
+        assert torch.equal(c.weights[same], before[same])   # entries that no row sees keep their bits
+    return y
+
+
+@pytest.mark.parametrize("track", [False, True])
+@pytest.mark.parametrize("d,heads,g,t,dtype,lens,capacity", [
+    (64, 1, 6, 1, BF16, (1,), 64),
+    (64, 1, 6, 1, BF16, (77, 0, 2, 31, 32, 33), 100),
+    (64, 1, 8, 1, FP16, (512, 511, 513, 64, 63, 65), 520),
+    (64, 2, 1, 1, BF16, (1023, 1, 1024, 1025, 900), 1025),
+    (128, 2, 4, 1, BF16, (300, 17, 0, 129), 300),
+    (128, 1, 8, 1, FP16, (5000, 2047, 1, 2048), 5003),
+    (64, 4, 4, 1, BF16, (20000,), 20000),
+    (128, 1, 16, 1, BF16, (700, 3), 700),
+    (64, 2, 3, 5, BF16, (4, 0, 5, 6, 1, 700, 1030), 1100),
+    (128, 2, 2, 7, FP16, (40, 7, 3, 1500), 1501),
+    (64, 1, 6, 33, BF16, (40, 1, 600), 640),
+    (64, 3, 5, 2, FP16, (95, 96, 97, 128, 160), 161),
+    (128, 8, 7, 3, BF16, (513, 2, 64), 513),
+])
+def test_attend(ops, d, heads, g, t, dtype, lens, capacity, track):
+    r = gen(capacity + t)
+    b = len(lens)
+    c = noise_cache(ops, r, b + 2, heads, capacity, d, track)
+    slots = torch.randperm(b + 2, generator=r, device=DEV)[:b].int()
+    lengths = int32(*lens)
+    for i, n in enumerate(lens):   # what lies behind a sequence's end must not matter
+        c.scales[slots[i].item(), :, n:] = float("nan")
+    q = randn(r, b, t, heads * g, d).to(dtype)
+    y = check_attend(ops, c, q, slots, lengths)
+    c.check()
+    if track:
+        return
+    # the bound of the lengths is no part of the result, nor the batch around a sequence
+    assert torch.equal(c.attend(q, slots, lengths, max_len=max(max(lens), 1)), y)
+    for i in range(b):
+        assert torch.equal(c.attend(q[i:i + 1], slots[i:i + 1], lengths[i:i + 1]), y[i:i + 1])
+
+
+@pytest.mark.parametrize("g,t", [(4, 1), (2, 3)])
+def test_attend_strides_scale_and_padding(ops, g, t):
+    r = gen(g)
+    c = noise_cache(ops, r, 4, 2, 300, 64, True)
+    big = randn(r, 4, 2 * g, t + 1, 70).to(BF16)
+    q = big[:, :, 1:, 3:67].transpose(1, 2)
+    slots, lengths = int32(2, -1, 0, 3), int32(300, 50, 0, 7)
+    y = check_attend(ops, c, q, slots, lengths, scale=0.31)
+    assert not y[1].any() and not y[2].any()
+    out = torch.full((4, 2 * g, t, 80), 9.0, device=DEV, dtype=BF16)
+    view = out[..., 8:72].transpose(1, 2)
+    c.weights.zero_()
+    got = c.attend(q, slots, lengths, scale=0.31, out=view)
+    assert got.data_ptr() == view.data_ptr() and torch.equal(view, y)
+    assert (out[..., :8] == 9).all() and (out[..., 72:] == 9).all()
+    check_attend(ops, c, q, slots, lengths, scale=-0.2)
+    c.attend(q, slots, lengths, scale=0.0)
+    c.check()
+
+
+def test_attend_peaked_and_flat(ops):
+    """Scores far apart, equal scores, and value ranges that lie far apart."""
+    r = gen(8)
+    c = noise_cache(ops, r, 3, 1, 700, 64, True)
+    c.scales[1, :, :, :2] = 0                      # keys all zero: a plain mean of the values
+    c.scales[2, :, ::3, 2:] *= 1024                # a third of the values far above the others
+    c.scales[2, :, 1::3, 2:] *= 2.0 ** -20
+    c.scales[2, :, 5, 2] = 0                       # a constant row of values
+    q = 12 * randn(r, 3, 1, 8, 64).to(BF16)
+    check_attend(ops, c, q, int32(0, 1, 2), int32(700, 699, 640))
+    tiny = (q * 2.0 ** -60).to(BF16)               # exponents that fp16 does not have
+    check_attend(ops, c, tiny, int32(2, 1, 0), int32(513, 1, 30))
+    huge = (q * 2.0 ** 60).to(BF16)
+    check_attend(ops, c, huge, int32(0, 1, 2), int32(512, 20, 1), scale=2.0 ** -66)
+
+
+def test_attend_not_finite(ops):
+    r = gen(9)
+    c = noise_cache(ops, r, 2, 2, 100, 64, False)
+    q = randn(r, 2, 1, 4, 64).to(BF16)
+    y0 = c.attend(q, int32(0, 1), int32(60, 60))
+    c.scales[0, 1, 10, 0] = float("nan")           # one key of head 1 of sequence 0
+    c.scales[1, 0, 59, 3] = float("nan")           # one value of head 0 of sequence 1
+    y = c.attend(q, int32(0, 1), int32(60, 60))
+    assert torch.isnan(y[0, 0, 2:]).all() and torch.equal(y[0, 0, :2], y0[0, 0, :2])
+    assert torch.isnan(y[1, 0, :2]).all() and torch.equal(y[1, 0, 2:], y0[1, 0, 2:])
+    assert torch.isfinite(c.attend(q, int32(0, 1), int32(10, 59))).all()    # neither is seen
+    q[0, 0, 1, 3] = float("nan")
+    q[1, 0, 3, 0] = float("inf")
+    y = c.attend(q, int32(0, 1), int32(10, 59))
+    assert torch.isnan(y[0, 0, 1]).all() and not torch.isfinite(y[1, 0, 3]).any()
+    assert torch.isfinite(y[0, 0, [0, 2, 3]]).all() and torch.isfinite(y[1, 0, :3]).all()
+
+
+def test_attend_out_of_range_is_cut_and_reported(ops):
+    r = gen(10)
+    q = randn(r, 2, 1, 4, 64).to(BF16)
+    for slots, lengths, max_len, text in (((0, 9), (20, 20), None, "slot beyond"), ((0, 1), (20, 51), None, "length"),
+                                          ((0, 1), (20, -5), None, "length"), ((0, 1), (20, 31), 30, "length")):
+        c = noise_cache(ops, r, 2, 2, 50, 64, False)
+        check_attend(ops, c, q, int32(*slots), int32(*lengths), max_len=max_len)
+        with pytest.raises(RuntimeError, match=text):
+            c.check()
+    c = noise_cache(ops, r, 2, 2, 50, 64, False)
+    check_attend(ops, c, q, int32(1, 1), int32(20, 30))   # two sequences may read one slot
+    c.check()
+    c = noise_cache(ops, r, 2, 2, 50, 64, True)
+    c.attend(q, int32(1, 1), int32(20, 30))                # but not add to its weights
+    with pytest.raises(RuntimeError, match="twice"):
+        c.check()
+
+
+def test_offsets_beyond_32_bits(ops):
+    """The last slot of a cache whose codes take more than 2^32 bytes."""
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GB of device memory")
+    slots, heads, capacity, d = 35, 8, 262144, 128
+    shape = (slots, heads, capacity)
+    assert math.prod(shape) * d // 2 > 1 << 32
+    k, v = (torch.empty(*shape, d // 2, dtype=torch.uint8, device=DEV) for _ in range(2))
+    c = ops.KV4Cache(k, v, torch.empty(*shape, 4, dtype=BF16, device=DEV), torch.empty(shape, device=DEV))
+    g = gen(12)
+    n = 300
+    rows_k, rows_v = randn(g, 1, n, heads, d).to(BF16), randn(g, 1, n, heads, d).to(BF16)
+    c.weights[slots - 1].zero_()
+    c.append(rows_k, rows_v, int32(slots - 1), int32(n))
+    rk, rv = c.read(int32(slots - 1), int32(0), n)
+    assert (rk.double()[0] - held(rows_k[0])[0]).abs().max() <= 2.0 ** -8 * 8
+    q = randn(g, 1, 1, 16, d).to(BF16)
+    y = c.attend(q, int32(slots - 1), int32(n))
+    small = ops.KV4Cache(*(x[slots - 1:, :, :512].contiguous() for x in (c.k, c.v, c.scales)))
+    assert torch.equal(y, small.attend(q, int32(0), int32(n)))
+    w = c.weights[slots - 1, :, :n].clone()
+    kept, new = c.evict(int32(slots - 1), int32(n), 200, recent=10)
+    assert new.tolist() == [200]
+    want = torch.cat([w[:, :n - 10].topk(190, dim=1).indices.sort(1).values,
+                      torch.arange(n - 10, n, device=DEV).expand(heads, 10)], 1)
+    assert torch.equal(kept[0].long(), want)
+
+
+# ---- eviction ----------------------------------------------------------------------------
+
+
+def evicted(w, n, budget, recent):
+    """The places that stay, in order, of one head's weights."""
+    if n <= budget:
+        return list(range(n))
+    key = [math.inf if math.isnan(x) else x for x in w[:n - recent].tolist()]
+    nan = [math.isnan(x) for x in w[:n - recent].tolist()]
+    best = sorted(range(n - recent), key=lambda j: (not nan[j], -key[j], j))[:budget - recent]
+    return sorted(best) + list(range(n - recent, n))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lens,budget,recent,kind", [
+    ((1, 2, 3, 0), 1, 0, "random"), ((1, 2, 3, 40), 1, 1, "random"), ((100, 64, 65, 63), 64, 10, "random"),
+    ((513, 512, 1024, 1025), 300, 0, "random"), ((700, 30), 512, 512, "random"), ((900, 850, 13), 511, 100, "equal"),
+    ((600, 601), 257, 3, "few"), ((400,), 100, 20, "special"), ((5000, 3000), 1000, 128, "random"), ((40000,), 20000, 77, "few"),
+])
+def test_evict(ops, d, lens, budget, recent, kind):
+    g = gen(budget)
+    b, heads, capacity = len(lens), 3, max(lens) + 9
+    c = noise_cache(ops, g, b + 1, heads, capacity, d, True)
+    w = c.weights
+    if kind == "random":
+        w.copy_(torch.exp(4 * randn(g, *w.shape)))
+    elif kind == "equal":
+        w.fill_(0.25)
+    elif kind == "few":
+        w.copy_(torch.randint(0, 4, w.shape, generator=g, device=DEV).float())
+    else:
+        w.copy_(randn(g, *w.shape))
+        w[:, :, 3::50] = float("nan")
+        w[:, :, 4::50] = float("inf")
+        w[:, :, 5::50] = -0.0
+        w[:, :, 6::50] = 0.0
+        w[:, :, 7::50] = -float("inf")
+    slots = torch.randperm(b + 1, generator=g, device=DEV)[:b].int()
+    old = [x.clone() for x in (c.k, c.v, c.scales, c.weights)]
+    kept, new = c.evict(slots, int32(*lens), budget, recent)
+    c.check()
+    assert new.tolist() == [min(n, budget) for n in lens]
+    want = [x.clone() for x in old]
+    for i, n in enumerate(lens):
+        s = slots[i].item()
+        for h in range(heads):
+            stay = evicted(old[3][s, h], n, budget, recent)
+            row = kept[i, h].tolist()
+            assert row[:len(stay)] == stay and all(x == -1 for x in row[len(stay):])
+            at = torch.tensor(stay, dtype=torch.long, device=DEV)
+            for x, y in zip(want, old):
+                x[s, h, :len(stay)] = y[s, h, at]
+    for x, y in zip((c.k, c.v, c.scales, c.weights), want):   # the rest is left as it was
+        assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+
+
+def test_evict_padding_and_reports(ops):
+    g = gen(2)
+    c = noise_cache(ops, g, 3, 2, 40, 64, True)
+    kept, new = c.evict(int32(-1, 2), int32(40, 40), 30, 5)
+    c.check()
+    assert new.tolist() == [0, 30] and (kept[0] == -1).all() and (kept[1] >= 0).all()
+    for slots, lengths, text in (((0, 3), (40, 40), "slot beyond"), ((0, 1), (40, 41), "length"), ((0, 0), (40, 40), "twice")):
+        c = noise_cache(ops, g, 3, 2, 40, 64, True)
+        old = c.k.clone()
+        kept, new = c.evict(int32(*slots), int32(*lengths), 30, 5)
+        assert kept[0].max() < 40 and torch.equal(c.k[2], old[2])
+        with pytest.raises(RuntimeError, match=text):
+            c.check()
+    with pytest.raises(ValueError, match="weights"):
+        noise_cache(ops, g, 1, 1, 8, 64, False).evict(int32(0), int32(8), 4)
+
+
+# ---- together ------------------------------------------------------------------------------
+
+
+class Layer:
+    """A serving step of one attention layer: projection, append, attention, projection."""
+
+    def __init__(self, ops, seed, streams=3, heads=8, kv_heads=2, d=64, width=384, capacity=40):
+        g = gen(seed)
+        self.ops, self.h, self.hk, self.d = ops, heads, kv_heads, d
+        rows = (heads + 2 * kv_heads) * d
+        self.w_in = ops.quantize_rows(randn(g, rows, width) / width ** 0.5)
+        self.w_out = ops.quantize_rows(randn(g, width, heads * d) / (heads * d) ** 0.5)
+        self.cache = ops.KV4Cache.empty(streams, kv_heads, capacity, d, track_weights=True)
+
+    def step(self, x, slots, lengths):
+        b, t, width = x.shape
+        qkv = self.ops.linear_i8(x, self.w_in).view(b, t, self.h + 2 * self.hk, self.d)
+        q, k, v = qkv.split([self.h, self.hk, self.hk], 2)
+        self.cache.append(k, v, slots, lengths)
+        return self.ops.linear_i8(self.cache.attend(q, slots, lengths).flatten(2), self.w_out)
+
+
+def test_a_serving_run(ops):
+    """Prompts, single tokens and evictions in turn; every step's attention is compared with the
+    formula on what the cache then holds, and the cache with what was appended and kept."""
+    layer = Layer(ops, 5)
+    c, g = layer.cache, gen(6)
+    slots = int32(2, 0, 1)
+    n = torch.tensor([9, 4, 0], dtype=torch.int32, device=DEV)       # a ragged prompt, padded on the left
+    layer.step(randn(g, 3, 9, 384).to(BF16), slots, n)
+    held_k = {s: entries(c, s)[0].clone() for s in range(3)}
+    for step in range(60):
+        n = n + 1
+        x = randn(g, 3, 1, 384).to(BF16)
+        qkv = ops.linear_i8(x, layer.w_in).view(3, 1, 12, 64)
+        q, k, v = qkv.split([8, 2, 2], 2)
+        c.append(k, v, slots, n)
+        for i, s in enumerate(slots.tolist()):
+            e = n[i].item() - 1
+            assert torch.equal(entries(c, s)[0][:, e], held(k[i, 0])[0])
+            held_k[s][:, e] = entries(c, s)[0][:, e]
+            assert torch.equal(entries(c, s)[0][:, :e], held_k[s][:, :e])
+        check_attend(ops, c, q, slots, n)
+        if step % 15 == 14:
+            kept, n = c.evict(slots, n, budget=16, recent=4)
+            for i, s in enumerate(slots.tolist()):
+                for h in range(2):
+                    at = kept[i, h][kept[i, h] >= 0].long()
+                    held_k[s][h, :len(at)] = held_k[s][h, at]
+    c.check()
+
+
+def test_two_streams_and_graph(ops):
+    """The same steps on another stream and from a captured graph give the same bits; replays go
+    on from what the cache holds."""
+    g = gen(7)
+    slots, xs = int32(1, 0, 2), [randn(g, 3, 2, 384).to(BF16) for _ in range(4)]
+
+    def lengths(i):
+        return torch.full((3,), 2 * (i + 1), dtype=torch.int32, device=DEV)
+
+    eager = Layer(ops, 9)
+    want = [eager.step(x, slots, lengths(i)) for i, x in enumerate(xs)]
+    side = Layer(ops, 9)
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        got = [side.step(x, slots, lengths(i)) for i, x in enumerate(xs)]
+    stream.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert torch.equal(side.cache.weights, eager.cache.weights)
+    layer = Layer(ops, 9)
+    x, n = xs[0].clone(), lengths(0)
+    warm = Layer(ops, 9)
+    with torch.cuda.stream(stream):
+        warm.step(x, slots, n)
+    stream.synchronize()
+    graph, second = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = layer.step(x, slots, n)
+    with torch.cuda.graph(second):       # a second graph of the same cache, with a workspace of its own
+        z = layer.step(x, slots, n)
+    for i in range(4):
+        x.copy_(xs[i])
+        n.copy_(lengths(i))
+        (graph if i % 2 == 0 else second).replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y if i % 2 == 0 else z, want[i])
+    assert torch.equal(layer.cache.weights, eager.cache.weights)
+
+
+def test_every_call_gives_the_same_bits_again(ops):
+    g = gen(13)
+    c = noise_cache(ops, g, 20, 2, 3000, 128, True)
+    q = randn(g, 20, 1, 16, 128).to(BF16)
+    slots = torch.randperm(20, generator=g, device=DEV).int()
+    lengths = torch.randint(0, 3001, (20,), generator=g, device=DEV, dtype=torch.int32)
+    w0 = c.weights.clone()
+    y0 = c.attend(q, slots, lengths)
+    w1 = c.weights.clone()
+    for _ in range(3):
+        c.weights.copy_(w0)
+        assert torch.equal(c.attend(q, slots, lengths), y0) and torch.equal(c.weights, w1)
