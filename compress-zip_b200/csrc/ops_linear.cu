@@ -4,6 +4,7 @@
 #include <string>
 
 #include "ops_common.cuh"
+#include "tc_common.cuh"
 
 namespace czg {
 
@@ -25,62 +26,431 @@ namespace {
 // rounded quotient falls on a half only where the exact one does: with x = X 2^i, a = A 2^j
 // (X, A < 2^11) a quotient q that is no half is 1 / (2 A 2^(j-i)) >= |q| 2^-19 away from
 // one, and the division is off by |q| 2^-24 at most.  (fp32 x: both steps round.)
-// Rows of values beyond 2^100 are scaled by 2^-20 first, which leaves the quotients alone.
-__device__ __forceinline__ int code_of(float x, float a) {
-    return (int)rintf(__fdiv_rn(x * 127.0f, a));
+// x (127 / a) is off by 127 * 2^-23 < 2^-16 at most and decides wherever it is not within
+// 10^-4 of a half; only there is the quotient divided out.
+__device__ __forceinline__ int code_of(float x, float a, float inv) {
+    const float r = x * inv, n = rintf(r);
+    return (int)(fabsf(r - n) < 0.4999f ? n : rintf(__fdiv_rn(x * 127.0f, a)));
 }
 
-// One CTA a row: the row's maximum, then its codes.
+// 8 values of a row from column i on, 0 behind its end.
 template <typename T>
-__global__ void __launch_bounds__(256) k_quantize_rows(const T *__restrict__ x, int64_t ldx, int64_t k,
-                                                       int8_t *__restrict__ codes, int64_t ldc, float *__restrict__ scales) {
+__device__ __forceinline__ void load8(const T *row, int64_t i, int64_t k, bool vec, float (&v)[8]) {
+    if (vec && i + 8 <= k) {
+        __align__(16) T t[8];
+#pragma unroll
+        for (int c = 0; c < (int)sizeof(T) / 2; c++) reinterpret_cast<uint4 *>(t)[c] = reinterpret_cast<const uint4 *>(row + i)[c];
+#pragma unroll
+        for (int c = 0; c < 8; c++) v[c] = to_f32(t[c]);
+    } else {
+#pragma unroll
+        for (int c = 0; c < 8; c++) v[c] = i + c < k ? to_f32(row[i + c]) : 0.0f;
+    }
+}
+
+// One CTA a row: its maximum, then its codes, 8 values a thread and turn; rows of up to
+// kHeld turns stay in registers between the two, longer ones are read again.
+constexpr int kQuantThreads = 256, kHeld = 4;
+template <typename T>
+__global__ void __launch_bounds__(kQuantThreads) k_quantize_rows(const T *__restrict__ x, int64_t ldx, int64_t k, int vec,
+                                                                 int8_t *__restrict__ codes, int64_t ldc,
+                                                                 float *__restrict__ scales) {
+    pdl_trigger();   // the product may set itself up meanwhile
     const T *row = x + (int64_t)blockIdx.x * ldx;
     int8_t *out = codes + (int64_t)blockIdx.x * ldc;
-    __shared__ float part[8];
+    __shared__ float part[kQuantThreads / 32];
+    const int64_t turn = (int64_t)blockDim.x * 8, i0 = threadIdx.x * 8;
+    const bool held = k <= turn * kHeld;
+    float v[kHeld][8];
     float a = 0.0f;
     bool bad = false;
-    for (int64_t i = threadIdx.x; i < k; i += 256) {
-        const float v = fabsf(to_f32(row[i]));
-        bad |= !(v <= 3.402823466e38f);
-        a = fmaxf(a, v);
+    auto most = [&](const float (&w)[8]) {
+#pragma unroll
+        for (int c = 0; c < 8; c++) {
+            const float m = fabsf(w[c]);
+            bad |= !(m <= 3.402823466e38f);
+            a = fmaxf(a, m);
+        }
+    };
+    if (held) {
+#pragma unroll
+        for (int t = 0; t < kHeld; t++)
+            if (i0 + t * turn < k) load8(row, i0 + t * turn, k, vec, v[t]);
+#pragma unroll
+        for (int t = 0; t < kHeld; t++)
+            if (i0 + t * turn < k) most(v[t]);
+    } else {
+        for (int64_t i = i0; i < k; i += turn) {
+            load8(row, i, k, vec, v[0]);
+            most(v[0]);
+        }
     }
     if (bad) a = INFINITY;   // NaN and infinities both end as a row of NaN
     for (int o = 16; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = a;
-    __syncthreads();
-    for (int w = 0; w < 8; w++) a = fmaxf(a, part[w]);
+    if (blockDim.x > 32) {
+        if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = a;
+        __syncthreads();
+        for (int w = 0; w < (int)blockDim.x / 32; w++) a = fmaxf(a, part[w]);
+    }
     const bool fine = a <= 3.402823466e38f;
     if (threadIdx.x == 0) scales[blockIdx.x] = fine ? __fdiv_rn(a, 127.0f) : NAN;
-    const float f = a > 1.2676506e30f ? 9.5367431640625e-7f : 1.0f;
-    const int64_t kp = (k + 15) & ~(int64_t)15;
-    for (int64_t i = threadIdx.x; i < kp; i += 256)
-        out[i] = i < k && fine && a > 0.0f ? (int8_t)code_of(to_f32(row[i]) * f, a * f) : (int8_t)0;
+    // a power of two keeps a, 127 x and 127 / a far from both ends of fp32, and the quotients as they are
+    const float f = a > 1.2676506e30f ? 9.5367431640625e-7f : a < 8.6736174e-19f ? 1.2089258196146292e24f : 1.0f;
+    const float af = a * f, inv = __fdiv_rn(127.0f, af);
+    const bool some = fine && a > 0.0f;
+    auto put = [&](int64_t i, const float (&w)[8]) {
+        uint32_t q[2] = {0, 0};
+        if (some) {
+#pragma unroll
+            for (int c = 0; c < 8; c++) q[c >> 2] |= (uint32_t)(uint8_t)code_of(w[c] * f, af, inv) << (8 * (c & 3));
+        }
+        *reinterpret_cast<uint2 *>(out + i) = make_uint2(q[0], q[1]);
+    };
+    if (held) {
+#pragma unroll
+        for (int t = 0; t < kHeld; t++)
+            if (i0 + t * turn < k) put(i0 + t * turn, v[t]);
+    } else {
+        for (int64_t i = i0; i < k; i += turn) {
+            load8(row, i, k, vec, v[0]);
+            put(i, v[0]);
+        }
+    }
+    // rows of codes end on 16 bytes: the second half of the last 16 may still be to fill
+    const int64_t end = (k + 7) & ~(int64_t)7;
+    if (threadIdx.x == 0 && (end & 15)) *reinterpret_cast<uint2 *>(out + end) = make_uint2(0, 0);
 }
 
-// One thread an output, four products an instruction; rows and columns past the ends
-// read row 0, whose sum is thrown away.
+// ---- the product -------------------------------------------------------------------
+//
+// out^T tile = W tile (128 channels, the M of tcgen05.mma kind::i8) times NT tokens (its N):
+// D[channel][token] in TMEM, so a lane of the epilogue holds one channel, its scale and
+// bias stay in registers, and a warp's store of one token is 32 adjacent channels whatever
+// the row stride of out.
+//   warp 0      one lane loads, by TMA, 128 bytes of k of 128 weight rows and NT token rows
+//               a stage (128-byte swizzle; rows and bytes outside are zeros, which add
+//               nothing to the sums).  Weights do not depend on the kernel before this
+//               one (the quantiser), so the first stages' weight boxes are asked for
+//               before griddepcontrol.wait and only the tokens' after it.
+//   warp 1      one lane issues 4 MMAs (k = 32 each) a stage
+//   the others  epilogue, EW / 4 warps a quadrant of TMEM lanes
+// S = 1: the CTA walks tiles (gridDim.x apart) with two accumulators, so the epilogue of
+// one overlaps the MMAs of the next.  S > 1 (few tokens): a cluster of S CTAs shares one
+// tile, each a stretch of k; each sends its int32 sums of tokens j to CTA j / (NT / S)
+// through distributed shared memory, and that one adds them up: integers, so the split
+// does not show in the result.
+constexpr int LT = 128;   // channels of a tile
+
+__device__ int g_ops_timeout;   // a bounded wait ran out on this device
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void store_remote(uint32_t addr, uint32_t rank, uint32_t v) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
+}
+
+// Barrier of the N threads of the epilogue, and whether any of them says so.
+template <int N>
+__device__ __forceinline__ bool epilogue_any(bool x) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r) : "r"((uint32_t)x), "n"(N) : "memory");
+    return r != 0;
+}
+
+struct LinearArgs {
+    const float *xs, *ws, *bias;
+    void *out;
+    int64_t ldo;
+    int m, n, steps, tiles_n, tiles, stages, split;
+};
+
+template <int NT>
+struct LinearCfg {
+    static constexpr int kStage = LT * TC_BK + NT * TC_BK;
+    static constexpr int kWarps = NT >= 128 ? 10 : 6;
+    static size_t smem(int stages, int split) {
+        return 1024 + (size_t)stages * kStage + (split > 1 ? LT * NT * 4 : 0) + (2 * stages + 5) * 8 + 16 + NT * 4 * 2;
+    }
+};
+
 template <typename T>
-__global__ void __launch_bounds__(256) k_linear_i8(const int8_t *__restrict__ x, int64_t ldx, const float *__restrict__ xs,
-                                                   const int8_t *__restrict__ w, int64_t ldw, const float *__restrict__ ws,
-                                                   const float *__restrict__ bias, int64_t m, int64_t n, int64_t k,
-                                                   T *__restrict__ out, int64_t ldo) {
-    const int64_t i = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4), j = (int64_t)blockIdx.y * 16 + (threadIdx.x & 15);
-    if (i >= m || j >= n) return;
-    const int8_t *a = x + i * ldx, *b = w + j * ldw;
-    int acc = 0;
-    int64_t c = 0;
-    for (; c + 4 <= k; c += 4)
-        acc = __dp4a(*reinterpret_cast<const int *>(a + c), *reinterpret_cast<const int *>(b + c), acc);
-    for (; c < k; c++) acc += (int)a[c] * b[c];
-    float y = __fmul_rn(__fmul_rn((float)acc, xs[i]), ws[j]);
-    if (bias) y = __fadd_rn(y, bias[j]);
-    out[i * ldo + j] = from_f32<T>(y);
+__device__ __forceinline__ T finish(int acc, float xs, float ws, float bias, bool has_bias) {
+    float y = __fmul_rn(__fmul_rn((float)acc, xs), ws);
+    if (has_bias) y = __fadd_rn(y, bias);
+    return from_f32<T>(y);
+}
+
+template <int NT, typename T>
+__global__ void __launch_bounds__(LinearCfg<NT>::kWarps * 32, 1)
+k_linear_tc(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, LinearArgs p) {
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    constexpr int STAGE = LinearCfg<NT>::kStage, W_BYTES = LT * TC_BK, EW = LinearCfg<NT>::kWarps - 2;
+    constexpr int COLS = 2 * NT < 32 ? 32 : 2 * NT;
+    const int STAGES = p.stages, S = p.split;
+    uint8_t *tail = smem + STAGES * STAGE;
+    int *sums = reinterpret_cast<int *>(tail);   // S > 1: [from][token][channel]
+    if (S > 1) tail += LT * NT * 4;
+    uint64_t *full = reinterpret_cast<uint64_t *>(tail);
+    uint64_t *empty = full + STAGES;
+    uint64_t *tfull = empty + STAGES;
+    uint64_t *tempty = tfull + 2;
+    uint64_t *drain = tempty + 2;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
+    float *s_xs = reinterpret_cast<float *>(tmem_slot + 4);   // 2 x NT
+    __shared__ volatile int abort_flag;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = S > 1 ? (int)cluster_rank() : 0;
+    const int k0 = (int)((int64_t)p.steps * rank / S), k1 = (int)((int64_t)p.steps * (rank + 1) / S);
+    const int tile0 = S > 1 ? blockIdx.x / S : blockIdx.x, dt = S > 1 ? gridDim.x / S : gridDim.x;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; s++) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int b = 0; b < 2; b++) {
+            mbar_init(&tfull[b], 1);
+            mbar_init(&tempty[b], EW);
+        }
+        mbar_init(drain, 1);
+        abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(COLS));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = *tmem_slot;
+    if (S > 1) cluster_arrive();   // waited for before the first store to another CTA: it has begun by then
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int it = 0;
+            bool ok = true;
+            const int early = min(STAGES, k1 - k0);   // stages of the first tile that need no wait
+            const int n0 = (tile0 % p.tiles_n) * LT;
+            for (int i = 0; i < early; i++) {
+                mbar_expect_tx(&full[i], STAGE);
+                tma_load_2d(smem + i * STAGE, &map_w, &full[i], (k0 + i) * TC_BK, n0);
+            }
+            pdl_wait();
+            for (int tile = tile0; tile < p.tiles && ok; tile += dt) {
+                const int n0t = (tile % p.tiles_n) * LT, m0 = (tile / p.tiles_n) * NT;
+                for (int kb = k0; kb < k1; kb++, it++) {
+                    const int s = it % STAGES;
+                    uint8_t *sw = smem + s * STAGE;
+                    if (it >= early) {
+                        if (it >= STAGES && !mbar_wait(&empty[s], ((it / STAGES) - 1) & 1, &abort_flag)) {
+                            ok = false;
+                            break;
+                        }
+                        mbar_expect_tx(&full[s], STAGE);
+                        tma_load_2d(sw, &map_w, &full[s], kb * TC_BK, n0t);
+                    }
+                    tma_load_2d(sw + W_BYTES, &map_x, &full[s], kb * TC_BK, m0);
+                }
+            }
+            if (!ok) {
+                atomicOr(&g_ops_timeout, 1);
+                abort_flag = 1;
+                for (int k = max(0, it - STAGES); k < it; k++) mbar_wait(&full[k % STAGES], (k / STAGES) & 1, nullptr);
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            const uint32_t idesc = idesc_i8(LT, NT);
+            int it = 0, tc = 0;
+            bool ok = true;
+            for (int tile = tile0; tile < p.tiles && ok; tile += dt, tc++) {
+                const int b = tc & 1;
+                if (tc >= 2 && !mbar_wait(&tempty[b], ((tc >> 1) - 1) & 1, &abort_flag)) {
+                    ok = false;
+                    break;
+                }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                for (int kb = k0; kb < k1; kb++, it++) {
+                    const int s = it % STAGES;
+                    if (!mbar_wait(&full[s], (it / STAGES) & 1, &abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint64_t wd = smem_desc_sw128(smem_addr(smem + s * STAGE));
+                    const uint64_t xd = smem_desc_sw128(smem_addr(smem + s * STAGE + W_BYTES));
+#pragma unroll
+                    for (int k = 0; k < TC_BK / 32; k++)
+                        mma_i8(tmem + (uint32_t)(b * NT), wd + 2 * k, xd + 2 * k, idesc, kb > k0 || k > 0);
+                    mma_commit(&empty[s]);
+                }
+                if (ok) mma_commit(&tfull[b]);
+            }
+            if (!ok) {
+                atomicOr(&g_ops_timeout, 1);
+                abort_flag = 1;
+            }
+            mma_commit(drain);
+            mbar_wait(drain, 0, nullptr);
+        }
+    } else {
+        const int q = warp & 3;             // TMEM lanes 32q .. 32q + 31
+        const int part = (warp - 2) >> 2;   // of EW / 4 parts of the tokens
+        constexpr int PC = NT / (EW / 4);   // tokens of a part
+        pdl_wait();
+        if (S > 1) cluster_wait();
+        T *out = static_cast<T *>(p.out);
+        int tc = 0;
+        for (int tile = tile0; tile < p.tiles; tile += dt, tc++) {
+            const int b = tc & 1;
+            const int n0 = (tile % p.tiles_n) * LT, m0 = (tile / p.tiles_n) * NT;
+            const int ch = n0 + 32 * q + lane;
+            const bool there = ch < p.n;
+            const float ws = there ? p.ws[ch] : 0.0f, bias = there && p.bias ? p.bias[ch] : 0.0f;
+            float *xs = s_xs + b * NT;      // the accumulator's half: its readers are done when tempty[b] fired
+            if (S == 1)
+                for (int i = threadIdx.x - 64; i < NT; i += EW * 32) xs[i] = m0 + i < p.m ? p.xs[m0 + i] : 0.0f;
+            const bool got = mbar_wait(&tfull[b], (tc >> 1) & 1, &abort_flag);
+            if (epilogue_any<EW * 32>(!got)) {   // one answer for all of them: no warp waits for one that left
+                if (!got) {
+                    atomicOr(&g_ops_timeout, 1);
+                    abort_flag = 1;
+                }
+                break;
+            }
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t tbase = tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(b * NT + part * PC);
+            constexpr int CW = PC < 32 ? 16 : 32;
+#pragma unroll 1
+            for (int c0 = 0; c0 < PC; c0 += CW) {
+                uint32_t v[CW];
+                if constexpr (CW == 32) tmem_ld32(tbase + c0, v); else tmem_ld16(tbase + c0, v);
+                if (c0 + CW == PC) {
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&tempty[b]);
+                }
+                const int j0 = part * PC + c0;
+                if (S > 1) {
+                    const int per = NT / S;
+#pragma unroll
+                    for (int j = 0; j < CW; j++) {
+                        const int to = (j0 + j) / per;
+                        store_remote(smem_addr(sums + (rank * per + (j0 + j) % per) * LT + 32 * q + lane), to, v[j]);
+                    }
+                } else if (there) {
+                    T *o = out + (int64_t)(m0 + j0) * p.ldo + ch;
+                    const int most = p.m - m0 - j0;
+#pragma unroll
+                    for (int j = 0; j < CW; j++)
+                        if (j < most) o[j * p.ldo] = finish<T>((int)v[j], xs[j0 + j], ws, bias, p.bias != nullptr);
+                }
+            }
+        }
+    }
+    if (S > 1) {
+        __syncwarp();
+        if (warp < 2) cluster_wait();
+        cluster_arrive();
+        cluster_wait();   // every CTA of the cluster comes here, whatever it met
+        if (warp >= 2 && !abort_flag) {
+            const int per = NT / S, ch = (tile0 % p.tiles_n) * LT + 32 * (warp & 3) + lane;
+            const int m0 = (tile0 / p.tiles_n) * NT + rank * per;
+            if (ch < p.n) {
+                const float ws = p.ws[ch], bias = p.bias ? p.bias[ch] : 0.0f;
+                for (int j = (warp - 2) >> 2; j < per && m0 + j < p.m; j += EW / 4) {
+                    int acc = 0;
+                    for (int r = 0; r < S; r++) acc += sums[(r * per + j) * LT + 32 * (warp & 3) + lane];
+                    static_cast<T *>(p.out)[(int64_t)(m0 + j) * p.ldo + ch] = finish<T>(acc, p.xs[m0 + j], ws, bias, p.bias != nullptr);
+                }
+            }
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(COLS));
+}
+
+// Rows of codes as a TMA map of boxes of `box` rows by 128 bytes, 128-byte swizzled.
+bool codes_map(CUtensorMap *map, const int8_t *p, int64_t ld, int64_t rows, int64_t k, int box) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return false;
+    cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)(rows > 1 ? ld : (k + 15) / 16 * 16)};
+    cuuint32_t boxes[2] = {TC_BK, (cuuint32_t)box};
+    cuuint32_t one[2] = {1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t *>(p), dims, strides, boxes, one,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int NT, typename T>
+int launch_linear(const int8_t *x, int64_t ldx, const int8_t *w, int64_t ldw, int64_t k, LinearArgs p, bool after_quantise,
+                  cudaStream_t st) {
+    alignas(64) CUtensorMap mw, mx;
+    if (!codes_map(&mw, w, ldw, p.n, k, LT) || !codes_map(&mx, x, ldx, p.m, k, NT))
+        return ops_fail(CZG_E_DEVICE, "no tensor map for the operands");
+    const int64_t tiles = (int64_t)p.tiles_n * ((p.m + NT - 1) / NT);
+    if (tiles > 0x7FFFFFFF) return ops_fail(CZG_E_LIMIT, "too many tiles");
+    p.tiles = (int)tiles;
+    const int per_cta = (p.steps + p.split - 1) / p.split;   // the ring need not be longer than a tile's stretch of k
+    const int fit = (int)((220 * 1024 - (p.split > 1 ? LT * NT * 4 : 0)) / LinearCfg<NT>::kStage);
+    p.stages = per_cta < fit && p.split > 1 ? per_cta : fit;
+    const size_t smem = LinearCfg<NT>::smem(p.stages, p.split);
+    static int ready[64] = {0};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return ops_fail(CZG_E_DEVICE, "no device");
+    if (!ready[dev]) {
+        if (int e = ops_cuda(cudaFuncSetAttribute(k_linear_tc<NT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024)))
+            return e;
+        ready[dev] = 1;
+    }
+    const int grid = p.split > 1 ? p.tiles * p.split : p.tiles < sm_count() ? p.tiles : sm_count();
+    return ops_cuda(ops_launch(k_linear_tc<NT, T>, dim3((unsigned)grid), LinearCfg<NT>::kWarps * 32, smem, st, after_quantise,
+                               p.split, mw, mx, p));
+}
+
+struct LinearShape { int nt, split; };
+
+LinearShape linear_shape(int64_t m, int64_t n, int steps) {
+    const int64_t tiles_n = (n + LT - 1) / LT;
+    const int sms = sm_count();
+    LinearShape best{16, 1};
+    double least = 1e300;
+    for (int nt : {16, 32, 64, 128, 256}) {
+        const int64_t tiles = tiles_n * ((m + nt - 1) / nt);
+        for (int s : {1, 2, 4, 8}) {
+            if (s > 1 && (nt > 64 || s > steps || tiles * s > sms)) break;
+            const double waves = (double)((tiles * s + sms - 1) / sms);
+            const double step = std::fmax(2.0 * nt, (16384.0 + 128.0 * nt) / 48.0);
+            const double cost = waves * ((steps + s - 1) / s) * step + 1500 + 12.0 * nt + (s > 1 ? 1000 : 0);
+            if (cost < least) {
+                least = cost;
+                best = {nt, s};
+            }
+        }
+    }
+    return best;
 }
 
 template <typename T>
 int quantize(const void *x, int64_t ldx, int64_t m, int64_t k, int8_t *codes, int64_t ldc, float *scales, cudaStream_t st) {
-    k_quantize_rows<T><<<(unsigned)m, 256, 0, st>>>(static_cast<const T *>(x), ldx, k, codes, ldc, scales);
-    return ops_cuda(cudaGetLastError());
+    const int64_t turns = (k + 7) / 8;
+    const int threads = turns >= kQuantThreads ? kQuantThreads : (int)((turns + 31) / 32 * 32);
+    const int vec = aligned(x, 16) && (m == 1 || ldx * sizeof(T) % 16 == 0);
+    return ops_cuda(ops_launch(k_quantize_rows<T>, dim3((unsigned)m), threads, 0, st, false, 1, static_cast<const T *>(x), ldx,
+                               k, vec, codes, ldc, scales));
 }
 
 int quantize_any(const void *x, int dtype, int64_t ldx, int64_t m, int64_t k, int8_t *codes, int64_t ldc, float *scales,
@@ -92,17 +462,22 @@ int quantize_any(const void *x, int dtype, int64_t ldx, int64_t m, int64_t k, in
 
 template <typename T>
 int linear(const int8_t *x, int64_t ldx, const float *xs, const int8_t *w, int64_t ldw, const float *ws, const float *bias,
-           int64_t m, int64_t n, int64_t k, void *out, int64_t ldo, cudaStream_t st) {
-    const dim3 grid((unsigned)((m + 15) / 16), (unsigned)((n + 15) / 16));
-    k_linear_i8<T><<<grid, 256, 0, st>>>(x, ldx, xs, w, ldw, ws, bias, m, n, k, static_cast<T *>(out), ldo);
-    return ops_cuda(cudaGetLastError());
+           int64_t m, int64_t n, int64_t k, void *out, int64_t ldo, bool after_quantise, cudaStream_t st) {
+    LinearArgs p{xs, ws, bias, out, ldo, (int)m, (int)n, (int)((k + TC_BK - 1) / TC_BK), (int)((n + LT - 1) / LT), 0, 0, 1};
+    const LinearShape shape = linear_shape(m, n, p.steps);
+    p.split = shape.split;
+    if (shape.nt == 16) return launch_linear<16, T>(x, ldx, w, ldw, k, p, after_quantise, st);
+    if (shape.nt == 32) return launch_linear<32, T>(x, ldx, w, ldw, k, p, after_quantise, st);
+    if (shape.nt == 64) return launch_linear<64, T>(x, ldx, w, ldw, k, p, after_quantise, st);
+    if (shape.nt == 128) return launch_linear<128, T>(x, ldx, w, ldw, k, p, after_quantise, st);
+    return launch_linear<256, T>(x, ldx, w, ldw, k, p, after_quantise, st);
 }
 
-int linear_any(const int8_t *x, int64_t ldx, const float *xs, const int8_t *w, int64_t ldw, const float *ws,
-               const float *bias, int64_t m, int64_t n, int64_t k, void *out, int dtype, int64_t ldo, cudaStream_t st) {
-    if (dtype == CZG_F32) return linear<float>(x, ldx, xs, w, ldw, ws, bias, m, n, k, out, ldo, st);
-    if (dtype == CZG_BF16) return linear<__nv_bfloat16>(x, ldx, xs, w, ldw, ws, bias, m, n, k, out, ldo, st);
-    return linear<__half>(x, ldx, xs, w, ldw, ws, bias, m, n, k, out, ldo, st);
+int linear_any(const int8_t *x, int64_t ldx, const float *xs, const int8_t *w, int64_t ldw, const float *ws, const float *bias,
+               int64_t m, int64_t n, int64_t k, void *out, int dtype, int64_t ldo, bool after_quantise, cudaStream_t st) {
+    if (dtype == CZG_F32) return linear<float>(x, ldx, xs, w, ldw, ws, bias, m, n, k, out, ldo, after_quantise, st);
+    if (dtype == CZG_BF16) return linear<__nv_bfloat16>(x, ldx, xs, w, ldw, ws, bias, m, n, k, out, ldo, after_quantise, st);
+    return linear<__half>(x, ldx, xs, w, ldw, ws, bias, m, n, k, out, ldo, after_quantise, st);
 }
 
 const char *check_codes(const int8_t *p, int64_t ld, int64_t rows, int64_t k) {
@@ -145,6 +520,16 @@ using namespace czg;
 
 extern "C" const char *czg_ops_last_error(void) { return g_ops_error.c_str(); }
 
+extern "C" int czg_ops_check(void) {
+    int bits = 0;
+    if (int st = ops_cuda(cudaDeviceSynchronize())) return st;
+    if (int st = ops_cuda(cudaMemcpyFromSymbol(&bits, g_ops_timeout, sizeof(bits)))) return st;
+    if (bits == 0) return CZG_OK;
+    const int zero = 0;
+    if (int st = ops_cuda(cudaMemcpyToSymbol(g_ops_timeout, &zero, sizeof(zero)))) return st;
+    return ops_fail(CZG_E_TIMEOUT, "a bounded wait of a kernel ran out; its results are incomplete");
+}
+
 extern "C" int czg_quantize_rows(const void *x, int dtype, int64_t ld_x, int64_t m, int64_t k, int8_t *codes,
                                  int64_t ld_codes, float *scales, void *stream) {
     if (m < 0 || k < 1) return ops_fail(CZG_E_ARG, "m must not be negative, k must be at least 1");
@@ -164,7 +549,7 @@ extern "C" int czg_linear_i8(const int8_t *x, int64_t ld_x, const float *x_scale
     if (!x || !x_scale) return ops_fail(CZG_E_ARG, "null pointer");
     if (const char *why = check_codes(x, ld_x, m, k)) return ops_fail(CZG_E_ARG, why);
     if (int st = check_linear(w, ld_w, w_scale, m, n, k, out, out_dtype, ld_out)) return st;
-    return linear_any(x, ld_x, x_scale, w, ld_w, w_scale, bias, m, n, k, out, out_dtype, ld_out,
+    return linear_any(x, ld_x, x_scale, w, ld_w, w_scale, bias, m, n, k, out, out_dtype, ld_out, false,
                       static_cast<cudaStream_t>(stream));
 }
 
@@ -186,5 +571,5 @@ extern "C" int czg_linear_i8_dynamic(const void *x, int dtype, int64_t ld_x, con
     int8_t *codes = static_cast<int8_t *>(ws);
     float *scales = reinterpret_cast<float *>(codes + m * codes_ld(k));
     if (int e = quantize_any(x, dtype, ld_x, m, k, codes, codes_ld(k), scales, st)) return e;
-    return linear_any(codes, codes_ld(k), scales, w, ld_w, w_scale, bias, m, n, k, out, out_dtype, ld_out, st);
+    return linear_any(codes, codes_ld(k), scales, w, ld_w, w_scale, bias, m, n, k, out, out_dtype, ld_out, true, st);
 }

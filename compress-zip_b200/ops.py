@@ -23,7 +23,7 @@ from .engine import CZG_OK, CzgError
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 # The exported symbols of include/czg_ops.h, checked by the CPU test suite.
-EXPORTS = ["czg_ops_last_error", "czg_quantize_rows", "czg_linear_i8", "czg_linear_i8_workspace",
+EXPORTS = ["czg_ops_last_error", "czg_ops_check", "czg_quantize_rows", "czg_linear_i8", "czg_linear_i8_workspace",
            "czg_linear_i8_dynamic", "czg_kv4_append", "czg_kv4_read", "czg_kv4_attend_workspace",
            "czg_kv4_attend", "czg_kv4_evict"]
 
@@ -60,6 +60,7 @@ def lib() -> C.CDLL:
             fn.argtypes, fn.restype = args, C.c_int
         L.czg_linear_i8_workspace.argtypes, L.czg_linear_i8_workspace.restype = [L64, L64], U64
         L.czg_kv4_attend_workspace.argtypes, L.czg_kv4_attend_workspace.restype = [K, I, I, I, I], U64
+        L.czg_ops_check.argtypes, L.czg_ops_check.restype = [], C.c_int
         L.czg_ops_last_error.argtypes, L.czg_ops_last_error.restype = [], C.c_char_p
         _bound = L
     return _bound
@@ -91,6 +92,14 @@ def _call(dev: torch.device, fn, *args) -> None:
     else:
         with torch.cuda.device(dev):
             st = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    if st != CZG_OK:
+        _raise(st)
+
+
+def check(device=None) -> None:
+    """Wait for the device and raise CzgError if a kernel of an operator gave up a bounded wait."""
+    with torch.cuda.device(device):
+        st = lib().czg_ops_check()
     if st != CZG_OK:
         _raise(st)
 
@@ -346,7 +355,8 @@ class KV4Cache:
 
     def check(self) -> None:
         """Wait for the device and raise CzgError if a call met slots or lengths out of
-        range; the bits are cleared."""
+        range, or a kernel gave up a bounded wait; the bits are cleared."""
+        check(self.device)
         bits = int(self.status.item())
         if bits:
             self.status.zero_()

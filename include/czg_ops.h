@@ -37,6 +37,10 @@ enum czg_dtype { CZG_F32 = 0, CZG_BF16 = 1, CZG_F16 = 2 };
 /* Why the last call of this thread that returned another status than CZG_OK did so. */
 const char *czg_ops_last_error(void);
 
+/* Waits for the current device.  CZG_E_TIMEOUT if a kernel of an operator gave up a
+ * bounded wait on it since the last such answer (its results are incomplete). */
+int czg_ops_check(void);
+
 /* ---- int8 product ------------------------------------------------------------- */
 
 /* Rows of x ([m][k] of `dtype`, ld_x elements apart) as int8 codes and one scale each:
