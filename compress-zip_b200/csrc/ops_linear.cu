@@ -27,24 +27,74 @@ namespace {
 // (X, A < 2^11) a quotient q that is no half is 1 / (2 A 2^(j-i)) >= |q| 2^-19 away from
 // one, and the division is off by |q| 2^-24 at most.  (fp32 x: both steps round.)
 // x (127 / a) is off by 127 * 2^-23 < 2^-16 at most and decides wherever it is not within
-// 10^-4 of a half; only there is the quotient divided out.
-__device__ __forceinline__ int code_of(float x, float a, float inv) {
-    const float r = x * inv, n = rintf(r);
-    return (int)(fabsf(r - n) < 0.4999f ? n : rintf(__fdiv_rn(x * 127.0f, a)));
+// 10^-4 of a half; only where one of 8 values is, they are divided out.  Rounding is the
+// addition of M1 = 1.5 * 2^23 (common.cuh), whose sum's low byte is the code.
+__device__ __forceinline__ uint2 codes8(const float (&x)[8], float a, float inv) {
+    uint32_t n[8];
+    float worst = 0.0f;
+#pragma unroll
+    for (int c = 0; c < 8; c++) {
+        const float t = __fmaf_rn(x[c], inv, kM1);
+        n[c] = __float_as_uint(t);
+        worst = fmaxf(worst, fabsf(__fmaf_rn(x[c], inv, -__fsub_rn(t, kM1))));
+    }
+    if (worst > 0.4999f) {
+#pragma unroll
+        for (int c = 0; c < 8; c++) n[c] = __float_as_uint(__fadd_rn(__fdiv_rn(x[c] * 127.0f, a), kM1));
+    }
+    uint2 r;
+    r.x = __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410);
+    r.y = __byte_perm(__byte_perm(n[4], n[5], 0x0040), __byte_perm(n[6], n[7], 0x0040), 0x5410);
+    return r;
 }
 
-// 8 values of a row from column i on, 0 behind its end.
+// 8 values of a row as they lie in memory.  Their magnitudes' bits order like the
+// magnitudes, infinity and NaN above all others.
+template <typename T> struct Raw8;
+template <> struct Raw8<float> {
+    uint32_t w[8];
+    __device__ __forceinline__ uint32_t most(uint32_t m) const {
+#pragma unroll
+        for (int i = 0; i < 8; i++) m = max(m, w[i] & 0x7FFFFFFFu);
+        return m;
+    }
+    __device__ static __forceinline__ float value(uint32_t m) { return __uint_as_float(m); }
+    static constexpr uint32_t kInf = 0x7F800000u;
+    __device__ __forceinline__ void put(int i, float x) { w[i] = __float_as_uint(x); }
+    __device__ __forceinline__ float get(int i) const { return __uint_as_float(w[i]); }
+};
+template <typename T> struct Raw8 {   // 16 bits: two values a word, the maximum of both halves at once
+    uint32_t w[4];
+    __device__ __forceinline__ uint32_t most(uint32_t m) const {
+#pragma unroll
+        for (int i = 0; i < 4; i++) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
+        return m;
+    }
+    static constexpr uint32_t kInf = DType<T>::kCode == CZG_BF16 ? 0x7F80u : 0x7C00u;
+    __device__ static __forceinline__ T half_of(uint32_t h) {
+        const uint16_t u = (uint16_t)h;
+        return *reinterpret_cast<const T *>(&u);
+    }
+    __device__ static __forceinline__ float value(uint32_t m) { return to_f32(half_of(m)); }
+    __device__ __forceinline__ void put(int i, T x) {
+        const uint32_t u = *reinterpret_cast<const uint16_t *>(&x);
+        if (i & 1) w[i / 2] |= u << 16; else w[i / 2] = u;
+    }
+    __device__ __forceinline__ float get(int i) const { return to_f32(half_of(w[i / 2] >> (16 * (i & 1)))); }
+};
+
+// Values i .. i + 7 of a row, 0 behind its end.
 template <typename T>
-__device__ __forceinline__ void load8(const T *row, int64_t i, int64_t k, bool vec, float (&v)[8]) {
+__device__ __forceinline__ void load8(const T *row, int64_t i, int64_t k, bool vec, Raw8<T> &v) {
     if (vec && i + 8 <= k) {
-        __align__(16) T t[8];
 #pragma unroll
-        for (int c = 0; c < (int)sizeof(T) / 2; c++) reinterpret_cast<uint4 *>(t)[c] = reinterpret_cast<const uint4 *>(row + i)[c];
-#pragma unroll
-        for (int c = 0; c < 8; c++) v[c] = to_f32(t[c]);
+        for (int c = 0; c < (int)sizeof(T) / 2; c++) {
+            const uint4 t = __ldg(reinterpret_cast<const uint4 *>(row + i) + c);
+            v.w[4 * c] = t.x; v.w[4 * c + 1] = t.y; v.w[4 * c + 2] = t.z; v.w[4 * c + 3] = t.w;
+        }
     } else {
 #pragma unroll
-        for (int c = 0; c < 8; c++) v[c] = i + c < k ? to_f32(row[i + c]) : 0.0f;
+        for (int c = 0; c < 8; c++) v.put(c, i + c < k ? row[i + c] : from_f32<T>(0.0f));
     }
 }
 
@@ -58,53 +108,44 @@ __global__ void __launch_bounds__(kQuantThreads) k_quantize_rows(const T *__rest
     pdl_trigger();   // the product may set itself up meanwhile
     const T *row = x + (int64_t)blockIdx.x * ldx;
     int8_t *out = codes + (int64_t)blockIdx.x * ldc;
-    __shared__ float part[kQuantThreads / 32];
+    __shared__ uint32_t part[kQuantThreads / 32];
     const int64_t turn = (int64_t)blockDim.x * 8, i0 = threadIdx.x * 8;
     const bool held = k <= turn * kHeld;
-    float v[kHeld][8];
-    float a = 0.0f;
-    bool bad = false;
-    auto most = [&](const float (&w)[8]) {
-#pragma unroll
-        for (int c = 0; c < 8; c++) {
-            const float m = fabsf(w[c]);
-            bad |= !(m <= 3.402823466e38f);
-            a = fmaxf(a, m);
-        }
-    };
+    Raw8<T> v[kHeld];
+    uint32_t m = 0;
     if (held) {
 #pragma unroll
         for (int t = 0; t < kHeld; t++)
             if (i0 + t * turn < k) load8(row, i0 + t * turn, k, vec, v[t]);
 #pragma unroll
         for (int t = 0; t < kHeld; t++)
-            if (i0 + t * turn < k) most(v[t]);
+            if (i0 + t * turn < k) m = v[t].most(m);
     } else {
         for (int64_t i = i0; i < k; i += turn) {
             load8(row, i, k, vec, v[0]);
-            most(v[0]);
+            m = v[0].most(m);
         }
     }
-    if (bad) a = INFINITY;   // NaN and infinities both end as a row of NaN
-    for (int o = 16; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+    if (sizeof(T) == 2) m = max(m & 0xFFFFu, m >> 16);
+    m = __reduce_max_sync(0xffffffffu, m);
     if (blockDim.x > 32) {
-        if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = a;
+        if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = m;
         __syncthreads();
-        for (int w = 0; w < (int)blockDim.x / 32; w++) a = fmaxf(a, part[w]);
+        m = part[(threadIdx.x & 31) < blockDim.x / 32 ? threadIdx.x & 31 : 0];
+        m = __reduce_max_sync(0xffffffffu, m);
     }
-    const bool fine = a <= 3.402823466e38f;
+    const bool fine = m < Raw8<T>::kInf;   // NaN and infinities both end as a row of NaN
+    const float a = Raw8<T>::value(m);
     if (threadIdx.x == 0) scales[blockIdx.x] = fine ? __fdiv_rn(a, 127.0f) : NAN;
     // a power of two keeps a, 127 x and 127 / a far from both ends of fp32, and the quotients as they are
     const float f = a > 1.2676506e30f ? 9.5367431640625e-7f : a < 8.6736174e-19f ? 1.2089258196146292e24f : 1.0f;
     const float af = a * f, inv = __fdiv_rn(127.0f, af);
     const bool some = fine && a > 0.0f;
-    auto put = [&](int64_t i, const float (&w)[8]) {
-        uint32_t q[2] = {0, 0};
-        if (some) {
+    auto put = [&](int64_t i, const Raw8<T> &w) {
+        float x8[8];
 #pragma unroll
-            for (int c = 0; c < 8; c++) q[c >> 2] |= (uint32_t)(uint8_t)code_of(w[c] * f, af, inv) << (8 * (c & 3));
-        }
-        *reinterpret_cast<uint2 *>(out + i) = make_uint2(q[0], q[1]);
+        for (int c = 0; c < 8; c++) x8[c] = w.get(c) * f;
+        *reinterpret_cast<uint2 *>(out + i) = some ? codes8(x8, af, inv) : make_uint2(0, 0);
     };
     if (held) {
 #pragma unroll
@@ -343,12 +384,11 @@ k_linear_tc(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ C
                 }
                 const int j0 = part * PC + c0;
                 if (S > 1) {
-                    const int per = NT / S;
+                    const int lg = 31 - __clz(NT / S), per = NT / S;   // both powers of two
+                    const uint32_t mine = smem_addr(sums + rank * per * LT + 32 * q + lane);
 #pragma unroll
-                    for (int j = 0; j < CW; j++) {
-                        const int to = (j0 + j) / per;
-                        store_remote(smem_addr(sums + (rank * per + (j0 + j) % per) * LT + 32 * q + lane), to, v[j]);
-                    }
+                    for (int j = 0; j < CW; j++)
+                        store_remote(mine + (uint32_t)(((j0 + j) & (per - 1)) * LT * 4), (uint32_t)((j0 + j) >> lg), v[j]);
                 } else if (there) {
                     T *o = out + (int64_t)(m0 + j0) * p.ldo + ch;
                     const int most = p.m - m0 - j0;

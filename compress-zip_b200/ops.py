@@ -13,7 +13,7 @@ What only the device can see -- slots and lengths out of range -- sets bits that
 from __future__ import annotations
 
 import ctypes as C
-from typing import NamedTuple, Optional
+from typing import Optional
 
 import torch
 
@@ -85,13 +85,17 @@ def _same_device(dev: torch.device, **tensors) -> None:
             raise ValueError(f"{name} is on {t.device}, the others on {dev}")
 
 
+_current_device = torch.cuda.current_device
+_raw_stream = torch._C._cuda_getCurrentRawStream   # the handle of the current stream, without a Stream object around it
+
+
 def _call(dev: torch.device, fn, *args) -> None:
     """fn(*args, stream) on the current stream of dev, with dev current."""
-    if dev.index == torch.cuda.current_device():
-        st = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    if dev.index == _current_device():
+        st = fn(*args, _raw_stream(dev.index))
     else:
         with torch.cuda.device(dev):
-            st = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+            st = fn(*args, _raw_stream(dev.index))
     if st != CZG_OK:
         _raise(st)
 
@@ -107,30 +111,28 @@ def check(device=None) -> None:
 # ---- int8 product --------------------------------------------------------------
 
 
-class QRows(NamedTuple):
-    """Rows of int8 codes [n, k] (row stride a multiple of 16 bytes) and their float32 scales [n]."""
-    codes: torch.Tensor
-    scales: torch.Tensor
+class QRows:
+    """Rows of int8 codes [n, k] (beginning on 16-byte boundaries) and their float32 scales [n]."""
+    __slots__ = ("codes", "scales", "n", "k", "ld", "device")
 
-
-def _codes(q: QRows, what: str) -> None:
-    c, s = q
-    if c.dtype != torch.int8 or c.dim() != 2 or (c.stride(1) != 1 and c.shape[1] > 1):
-        raise ValueError(f"{what}.codes must be a 2-D int8 tensor with adjacent columns")
-    if s.dtype != torch.float32 or s.dim() != 1 or s.shape[0] != c.shape[0] or (s.stride(0) != 1 and s.shape[0] > 1):
-        raise ValueError(f"{what}.scales must be a contiguous float32 vector, one scale a row")
-    if c.data_ptr() % 16 or (c.stride(0) % 16 and c.shape[0] > 1):
-        raise ValueError(f"{what}.codes' rows must begin on 16-byte boundaries (quantize_rows lays them out so)")
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
+        if codes.dtype != torch.int8 or codes.dim() != 2 or (codes.stride(1) != 1 and codes.shape[1] > 1):
+            raise ValueError("codes must be a 2-D int8 tensor with adjacent columns")
+        self.n, self.k = codes.shape
+        if scales.dtype != torch.float32 or scales.shape != (self.n,) or (self.n > 1 and scales.stride(0) != 1):
+            raise ValueError("scales must be a contiguous float32 vector, one scale a row")
+        # a single row may have any stride: the library's rule is met with the row's own length
+        self.ld = codes.stride(0) if self.n > 1 else (self.k + 15) // 16 * 16
+        if codes.data_ptr() % 16 or self.ld % 16:
+            raise ValueError("rows of codes must begin on 16-byte boundaries (quantize_rows lays them out so)")
+        if scales.device != codes.device:
+            raise ValueError(f"scales are on {scales.device}, codes on {codes.device}")
+        self.codes, self.scales, self.device = codes, scales, codes.device
 
 
 def _rows(x: torch.Tensor, what: str) -> None:
     if x.dim() != 2 or (x.stride(1) != 1 and x.shape[1] > 1):
         raise ValueError(f"{what} must be 2-D with adjacent columns")
-
-
-def _ld(t: torch.Tensor) -> int:
-    """Row stride; for a single row, whatever satisfies the library's alignment."""
-    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 15) // 16 * 16
 
 
 def quantize_rows(x: torch.Tensor) -> QRows:
@@ -141,11 +143,11 @@ def quantize_rows(x: torch.Tensor) -> QRows:
     _rows(x, "x")
     _same_device(x.device)
     m, k = x.shape
-    ld = (k + 15) // 16 * 16
+    ld = max((k + 15) // 16 * 16, 16)
     codes = torch.empty((m, ld), dtype=torch.int8, device=x.device)
     scales = torch.empty(m, dtype=torch.float32, device=x.device)
     if m and k:
-        _call(x.device, lib().czg_quantize_rows, x.data_ptr(), code, _ld(x), m, k, codes.data_ptr(), ld,
+        _call(x.device, lib().czg_quantize_rows, x.data_ptr(), code, x.stride(0), m, k, codes.data_ptr(), ld,
               scales.data_ptr())
     elif m:
         scales.zero_()
@@ -160,57 +162,67 @@ def linear_i8(x, w: QRows, bias: Optional[torch.Tensor] = None, out_dtype: Optio
     x: a QRows, or a float tensor [..., k] whose rows are quantised in the same call.
     out_dtype defaults to x's type (bfloat16 for a QRows); ``out``, if given, has
     adjacent columns and is returned."""
-    _codes(w, "w")
-    n, k = w.codes.shape
-    dev = w.codes.device
+    n, k, dev = w.n, w.k, w.device
     quantised = isinstance(x, QRows)
     if quantised:
-        _codes(x, "x")
-        x2, lead = x.codes, x.codes.shape[:1]
+        m, width, x2, lead = x.n, x.k, x.codes, None
     else:
         code = _dtype(x, "x")
-        if x.dim() < 1:
+        shape = x.shape
+        if len(shape) == 2:
+            x2, lead = x, None
+        elif len(shape) == 0:
             raise ValueError("x must have a last dimension of k")
-        lead = x.shape[:-1]
-        x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1]) if x.numel() or x.shape[-1] else x.new_empty(lead.numel(), 0)
-        _rows(x2, "x")
-    if x2.shape[1] != k:
-        raise ValueError(f"x has rows of {x2.shape[1]}, w of {k}")
-    m = x2.shape[0]
+        else:
+            lead = shape[:-1]
+            x2 = x.reshape(lead.numel(), shape[-1])
+        m, width = x2.shape
+        if x2.stride(1) != 1 and width > 1:
+            raise ValueError("x must have adjacent columns")
+    if width != k:
+        raise ValueError(f"x has rows of {width}, w of {k}")
+    if x2.device != dev:
+        raise ValueError(f"x is on {x2.device}, w on {dev}")
     if out is None:
         kind = out_dtype if out_dtype is not None else torch.bfloat16 if quantised else x.dtype
-        if kind not in DTYPES:
+        out_code = DTYPES.get(kind)
+        if out_code is None:
             raise ValueError(f"out_dtype must be float32, bfloat16 or float16, not {kind}")
-        out2 = None
     else:
         if out_dtype is not None and out.dtype != out_dtype:
             raise ValueError(f"out is of {out.dtype}, out_dtype {out_dtype}")
-        kind = out.dtype
-        _dtype(out, "out")
-        if out.shape != (*lead, n):
-            raise ValueError(f"out must have shape {(*lead, n)}, not {tuple(out.shape)}")
-        out2 = out if out.dim() == 2 else out.view(-1, n)
-        _rows(out2, "out")
-    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (n,) or (n > 1 and bias.stride(0) != 1)):
-        raise ValueError(f"bias must be a contiguous float32 vector of {n}")
-    _same_device(dev, x=x2, x_scales=x.scales if quantised else None, w_scales=w.scales, bias=bias, out=out)
-    if out2 is None:
+        out_code = _dtype(out, "out")
+        if out.shape != ((m, n) if lead is None else (*lead, n)):
+            raise ValueError(f"out must have shape {(*(lead or (m,)), n)}, not {tuple(out.shape)}")
+        if out.device != dev:
+            raise ValueError(f"out is on {out.device}, w on {dev}")
+    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (n,) or (n > 1 and bias.stride(0) != 1)
+                             or bias.device != dev):
+        raise ValueError(f"bias must be a contiguous float32 vector of {n} on {dev}")
+    if dev.type != "cuda":
+        raise ValueError(f"tensors must be on a CUDA device, not {dev}")
+    if out is None:
         out2 = torch.empty((m, n), dtype=kind, device=dev)
-        out = out2 if len(lead) == 1 else out2.view(*lead, n)
+        out = out2 if lead is None else out2.view(*lead, n)
+    else:
+        out2 = out if lead is None else out.view(m, n)
+        _rows(out2, "out")
     if m == 0 or n == 0:
         return out
     if k == 0:
         out2.copy_(torch.zeros((), device=dev) if bias is None else bias)
         return out
-    L = lib()
-    tail = (w.codes.data_ptr(), _ld(w.codes), w.scales.data_ptr(), 0 if bias is None else bias.data_ptr(), m, n, k,
-            out2.data_ptr(), DTYPES[kind], out2.stride(0) if m > 1 else n)
+    L = _bound or lib()
+    bias_ptr = 0 if bias is None else bias.data_ptr()
+    ldo = out2.stride(0) if m > 1 else n
     if quantised:
-        _call(dev, L.czg_linear_i8, x2.data_ptr(), _ld(x2), x.scales.data_ptr(), *tail)
+        _call(dev, L.czg_linear_i8, x2.data_ptr(), x.ld, x.scales.data_ptr(), w.codes.data_ptr(), w.ld, w.scales.data_ptr(),
+              bias_ptr, m, n, k, out2.data_ptr(), out_code, ldo)
     else:
         need = L.czg_linear_i8_workspace(m, k)
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        _call(dev, L.czg_linear_i8_dynamic, x2.data_ptr(), code, x2.stride(0) if m > 1 else k, *tail, ws.data_ptr(), need)
+        _call(dev, L.czg_linear_i8_dynamic, x2.data_ptr(), code, x2.stride(0) if m > 1 else k, w.codes.data_ptr(), w.ld,
+              w.scales.data_ptr(), bias_ptr, m, n, k, out2.data_ptr(), out_code, ldo, ws.data_ptr(), need)
     return out
 
 
