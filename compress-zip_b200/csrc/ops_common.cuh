@@ -16,7 +16,19 @@ namespace czg {
 int ops_fail(int status, const char *why);
 int ops_cuda(cudaError_t e);   // CZG_OK, or CZG_E_DEVICE with CUDA's text
 
+int kv4_timeouts(int *bits);   // take_timeouts of ops_kv4.cu
+
 namespace {
+
+__device__ int g_ops_timeout;   // a bounded wait of this file's kernels ran out on this device
+
+// Waits of this file's kernels that ran out since the last call (the device is idle).
+inline int take_timeouts(int *bits) {
+    const int zero = 0;
+    *bits = 0;
+    if (int st = ops_cuda(cudaMemcpyFromSymbol(bits, g_ops_timeout, sizeof(*bits)))) return st;
+    return *bits ? ops_cuda(cudaMemcpyToSymbol(g_ops_timeout, &zero, sizeof(zero))) : CZG_OK;
+}
 
 template <typename T> struct DType;
 template <> struct DType<float> { static constexpr int kCode = CZG_F32; };

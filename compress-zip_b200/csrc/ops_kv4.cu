@@ -3,6 +3,7 @@
 #include <cmath>
 
 #include "ops_kv4.cuh"
+#include "tc_common.cuh"
 
 namespace czg {
 namespace {
@@ -133,67 +134,556 @@ __global__ void __launch_bounds__(256) k_kv4_read(czg_kv4 c, const int32_t *__re
     }
 }
 
-// One CTA a sequence and key head, its query rows one after the other: a chunk of 128
-// keys at a time, a thread a key for the scores, a thread a dimension for the sums.
-template <typename T, int D>
-__global__ void __launch_bounds__(128) k_kv4_attend(czg_kv4 c, const T *__restrict__ q, Strides qs,
-                                                    const int32_t *__restrict__ slots, const int32_t *__restrict__ lengths,
-                                                    int t, int g, int max_len, float scale, T *__restrict__ out, Strides os) {
-    __shared__ float sq[D], sp[128], red[4];
-    const int h = blockIdx.x, s = blockIdx.y, tid = threadIdx.x;
-    const int slot = kv4_slot(c, slots, s, tid == 0 && h == 0);
-    const int n = slot < 0 ? 0 : kv4_length(c, lengths, s, min(max_len, c.capacity), tid == 0 && h == 0);
-    const int64_t base = kv4_row(c, slot < 0 ? 0 : slot, h, 0);
-    const KvScale *sc = static_cast<const KvScale *>(c.scales) + base;
-    auto score = [&](int j) {
-        float a = 0.0f, z = 0.0f;
-        for (int i = 0; i < D / 2; i++) {
-            const uint32_t byte = c.k[(base + j) * (D / 2) + i];
-            a += sq[2 * i] * (float)(byte & 15u) + sq[2 * i + 1] * (float)(byte >> 4);
-            z += sq[2 * i] + sq[2 * i + 1];
+// ---- attention ---------------------------------------------------------------------------
+//
+// A CTA takes one unit of a sequence's entries (kUnit, at a fixed place whatever the
+// batch), one key head and up to 8 NB rows (query heads of that key head, times the
+// call's rows).  Its four warps take tiles of 64 entries in turn; each asks for its own
+// tiles at the start, by TMA into swizzled shared memory, so the whole unit is under way
+// at once, and several CTAs share an SM.
+//
+// Products are on mma.sync m16n8k16 (fp16, fp32 sums) with the cache as the A operand and
+// the rows as N: 8 rows fill an MMA, where tcgen05 would need 64 or 128 and the codes
+// unpacked to shared memory first.  A nibble becomes an fp16 number by one AND: bits
+// 0x000n are the subnormal n 2^-24, bits 0x00n0 are 16 n 2^-24, exactly, and the powers of
+// two go into the factors outside.  One word of 8 codes takes a shift and four ANDs:
+//   K: ldmatrix gives a lane 8 dimensions of entries i and i + 8; the pairs (0, 4), (1, 5),
+//      (2, 6), (3, 7) are the k of two MMAs (the query is permuted alike, and its share of
+//      the high nibbles divided by 16);
+//   V: ldmatrix.trans gives a lane 4 dimensions of entries 2c, 2c + 1: nibble i of both is
+//      the pair of dimension 4g + i (odd i: 16-fold, taken out at the end).
+// With x = lo + step c:  s_j = step_j (q.c_j) + lo_j sum(q);  out = sum p_j step_j c_j + sum p_j lo_j.
+// The query is held in fp16 after a power of two that brings its largest value to
+// [2^14, 2^15): exact but for values below 2^-24 of the largest.  p_j step_j is
+// held in fp16 likewise (2^15 for the unit's largest step): off by 2^-12 of itself, against
+// 2^-9 of the result for bf16 and 2^-12 for fp16; its range is 2^39 wide.  Scores, maxima and
+// sums are fp32; exponentials are ex2.approx (2^-22).
+// Between the warps of a CTA, and between units (k_kv4_join), partial results are joined
+// in a fixed order, so a row's bits do not depend on the batch or the grid.
+constexpr int kUnit = 512, kTile = 64, kAttendWarps = 4;
+static_assert(kUnit == 2 * kTile * kAttendWarps, "a warp has two tiles");
+
+struct AttendArgs {
+    czg_kv4 c;
+    const void *q;
+    Strides qs;
+    const int32_t *slots, *lengths;
+    int t, g, rows, row_blocks, max_len, units, vec;
+    float scale_log2;   // scale * log2 e
+    void *out;
+    Strides os;
+    // more than one unit (or row block with weights): partial results
+    float *part;        // [b][head][unit][rows padded][D]
+    float2 *stat;       // [b][head][unit][rows padded] (maximum, sum)
+    float *score;       // weights: [b][head][rows][max_len]
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// What sums taken from the maximum m are worth from the maximum `top` (both may be -infinity).
+__device__ __forceinline__ float share(float m, float top) { return m == top ? 1.0f : ex2(m - top); }
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_trans(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, uint64_t *bar, int x, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+        ::"r"(smem_addr(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar)) : "memory");
+}
+
+// Row r of a sequence and key head: place i = r / g of the call's rows, query head h g + r % g.
+template <typename T>
+__device__ __forceinline__ int64_t row_offset(const Strides &s, int b, int h, int g, int r) {
+    return b * s.b + (r / g) * s.t + (h * g + r % g) * s.h;
+}
+
+template <int D>
+struct AttendSmem {
+    static constexpr int kCodes = kUnit * D / 2;
+    static constexpr int kScales = 2 * kCodes, kBars = kScales + kUnit * 16, kScores = kBars + 128;
+    static size_t bytes(int nb, bool track) { return 1024 + kScores + (track ? (size_t)8 * nb * kUnit * 4 : 0); }
+};
+
+template <typename T, int D, int NB, bool TRACK>
+__global__ void __launch_bounds__(kAttendWarps * 32)
+k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttendArgs p) {
+    using L = AttendSmem<D>;
+    constexpr int CH = D / 32;      // 16-byte chunks of a row of codes
+    constexpr int R = 8 * NB;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    float4 *sc = reinterpret_cast<float4 *>(smem + L::kScales);   // k step, k lo, v step (scaled), v lo
+    uint64_t *bar = reinterpret_cast<uint64_t *>(smem + L::kBars);
+    float *scores = reinterpret_cast<float *>(smem + L::kScores);   // TRACK: [row][entry of the unit]
+    __shared__ float s_m[kAttendWarps][R], s_l[kAttendWarps][R], s_z[kAttendWarps][R];
+    __shared__ uint32_t s_top[kAttendWarps];
+    __shared__ float2 s_row[R];   // maximum and sum over the warps
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, c4 = lane & 3;
+    const int unit = blockIdx.x, h = blockIdx.y / p.row_blocks, rb = blockIdx.y % p.row_blocks, b = blockIdx.z;
+    const bool first = tid == 0 && unit == 0 && blockIdx.y == 0;
+    if (TRACK && unit == 0 && b == 0 && blockIdx.y == 0) kv4_check_distinct(p.c, p.slots, gridDim.z);
+    const int slot = kv4_slot(p.c, p.slots, b, first);
+    const int n = slot < 0 ? 0 : kv4_length(p.c, p.lengths, b, min(p.max_len, p.c.capacity), first);
+    const int j0 = unit * kUnit, here = min(n - j0, kUnit);   // entries of this unit
+    if (here <= 0 && unit > 0) return;
+    const int64_t base = kv4_row(p.c, max(slot, 0), h, 0);
+
+    // each warp asks for its tiles
+    if (lane == 0) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int tile = i * kAttendWarps + warp;
+            mbar_init(&bar[tile], 1);
         }
-        return scale * (to_f32(sc[j].k_step) * a + to_f32(sc[j].k_lo) * z);
-    };
-    auto reduce = [&](float x, bool is_max) {
-        for (int o = 16; o > 0; o >>= 1) {
-            const float y = __shfl_xor_sync(0xffffffffu, x, o);
-            x = is_max ? fmaxf(x, y) : x + y;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int tile = i * kAttendWarps + warp;
+            if (tile * kTile < here) {
+                mbar_expect_tx(&bar[tile], kTile * D);
+                tma_load_3d(smem + tile * kTile * (D / 2), &map_k, &bar[tile], 0, j0 + tile * kTile, slot * p.c.n_heads + h);
+                tma_load_3d(smem + L::kCodes + tile * kTile * (D / 2), &map_v, &bar[tile], 0, j0 + tile * kTile, slot * p.c.n_heads + h);
+            }
         }
-        __syncthreads();
-        if ((tid & 31) == 0) red[tid >> 5] = x;
-        __syncthreads();
-        return is_max ? fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])) : (red[0] + red[1]) + (red[2] + red[3]);
-    };
-    for (int row = 0; row < t * g; row++) {
-        const int i = row / g, hq = h * g + row % g;
-        __syncthreads();
-        if (tid < D) sq[tid] = to_f32(q[s * qs.b + i * qs.t + hq * qs.h + tid]);
-        __syncthreads();
-        const int seen = max(0, n - (t - 1 - i));
-        float m = -INFINITY, l = 0.0f, o = 0.0f;
-        for (int j0 = 0; j0 < seen; j0 += 128) {
-            const int j = j0 + tid;
-            const float x = j < seen ? score(j) : -INFINITY;
-            const float m1 = fmaxf(m, reduce(x, true));
-            const float p = j < seen ? expf(x - m1) : 0.0f;
-            const float f = expf(m - m1);
-            l = l * f + reduce(p, false);
-            o *= f;
-            m = m1;
-            sp[tid] = p;
-            __syncthreads();
-            if (tid < D)
-                for (int e = 0; e < min(128, seen - j0); e++) {
-                    const uint32_t byte = c.v[(base + j0 + e) * (D / 2) + tid / 2];
-                    const float code = (float)(tid & 1 ? byte >> 4 : byte & 15u);
-                    o += sp[e] * (to_f32(sc[j0 + e].v_step) * code + to_f32(sc[j0 + e].v_lo));
-                }
-        }
-        if (tid < D) out[s * os.b + i * os.t + hq * os.h + tid] = from_f32<T>(seen > 0 ? o / l : 0.0f);
-        if (c.weights)
-            for (int j = tid; j < seen; j += 128) c.weights[base + j] += expf(score(j) - m) / l;
     }
-    if (c.weights && h == 0 && s == 0) kv4_check_distinct(c, slots, gridDim.y);
+
+    // ranges of the entries; 0 behind the end, whatever lies there
+    uint2 raw[kUnit / (kAttendWarps * 32)];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < kUnit / (kAttendWarps * 32); i++) {
+        const int j = tid + i * kAttendWarps * 32;
+        raw[i] = j < here ? __ldg(reinterpret_cast<const uint2 *>(static_cast<const KvScale *>(p.c.scales) + base + j0 + j)) : make_uint2(0, 0);
+        const uint32_t step = (raw[i].y & 0xFFFFu) << 16;   // bits of the value's step, never negative
+        if (step < 0x7F800000u) top = max(top, step);
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (lane == 0) s_top[warp] = top;
+
+    // the query's fragments, with its row's power of two, and the row's factors
+    uint32_t qf[NB][CH][4];
+    float qscale[NB][2], qsum[NB][2];   // of rows 2 c4, 2 c4 + 1: what q.c is multiplied by, and sum(q)
+    int seen[NB][2];
+#pragma unroll
+    for (int nb = 0; nb < NB; nb++) {
+        const int r = rb * R + nb * 8 + g8;
+        float x[CH][8], big = 0.0f, sum = 0.0f;
+#pragma unroll
+        for (int ch = 0; ch < CH; ch++) {
+            const T *src = static_cast<const T *>(p.q) + (r < p.rows ? row_offset<T>(p.qs, b, h, p.g, r) : 0) + ch * 32 + c4 * 8;
+            __align__(16) T v[8];
+            if (r >= p.rows) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[i] = from_f32<T>(0.0f);
+            } else if (p.vec) {
+                *reinterpret_cast<uint4 *>(v) = __ldg(reinterpret_cast<const uint4 *>(src));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[i] = src[i];
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                x[ch][i] = to_f32(v[i]);
+                big = fmaxf(big, fabsf(x[ch][i]));
+                sum += x[ch][i];
+            }
+        }
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) {
+            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+            sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        }
+        int e = (int)(__float_as_uint(big) >> 23) - 127;
+        e = e > 127 ? 0 : max(e, -100);
+        const float up = __uint_as_float((uint32_t)(14 - e + 127) << 23);
+#pragma unroll
+        for (int ch = 0; ch < CH; ch++) {
+            const float u16 = up * 0.0625f;
+            qf[nb][ch][0] = pack_half(x[ch][0] * up, x[ch][4] * up);
+            qf[nb][ch][1] = pack_half(x[ch][1] * u16, x[ch][5] * u16);
+            qf[nb][ch][2] = pack_half(x[ch][2] * up, x[ch][6] * up);
+            qf[nb][ch][3] = pack_half(x[ch][3] * u16, x[ch][7] * u16);
+        }
+        const float qs = ldexpf(p.scale_log2, e + 10), zq = p.scale_log2 * sum;   // 2^24 2^(e - 14)
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            qscale[nb][i] = __shfl_sync(0xffffffffu, qs, (2 * c4 + i) * 4);
+            qsum[nb][i] = __shfl_sync(0xffffffffu, zq, (2 * c4 + i) * 4);
+            const int row = rb * R + nb * 8 + 2 * c4 + i;
+            seen[nb][i] = row < p.rows ? n - (p.t - 1 - row / p.g) - j0 : 0x7FFFFFFF;   // entries of this unit that the row sees
+        }
+    }
+    __syncthreads();
+    top = max(max(s_top[0], s_top[1]), max(s_top[2], s_top[3]));
+    // a power of two not below any step, and what brings it to 2^15
+    const int te = top == 0 ? 0 : max((int)(top >> 23) - 126, -100);
+    const float vdown = ldexpf(1.0f, 15 - te);
+#pragma unroll
+    for (int i = 0; i < kUnit / (kAttendWarps * 32); i++)
+        sc[tid + i * kAttendWarps * 32] = make_float4(__uint_as_float(raw[i].x << 16), __uint_as_float(raw[i].x & 0xFFFF0000u),
+                                                      __uint_as_float(raw[i].y << 16) * vdown, __uint_as_float(raw[i].y & 0xFFFF0000u));
+    __syncthreads();
+
+    float m[NB][2], l[NB][2], z[NB][2], o[NB][CH][2][4];
+#pragma unroll
+    for (int nb = 0; nb < NB; nb++) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            m[nb][i] = -INFINITY;
+            l[nb][i] = z[nb][i] = 0.0f;
+        }
+#pragma unroll
+        for (int ch = 0; ch < CH; ch++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) o[nb][ch][i >> 2][i & 3] = 0.0f;
+    }
+    int least = kUnit;   // what every row of the CTA sees at least
+#pragma unroll
+    for (int nb = 0; nb < NB; nb++) least = min(least, min(seen[nb][0], seen[nb][1]));
+    least = __reduce_min_sync(0xffffffffu, least);
+
+    // ldmatrix: lane i gives the address of row i % 8 of matrix i / 8; matrices are
+    // (entries 0-7, 8-15) x (two chunks)
+    const int lm_row = (lane & 7) + (lane & 8), lm_ch = lane >> 4;
+    const uint32_t swz = D == 64 ? (uint32_t)(lm_row >> 2 & 1) : (uint32_t)(lm_row >> 1 & 3);
+#pragma unroll 1
+    for (int it = 0; it < 2; it++) {
+        const int tile = it * kAttendWarps + warp, t0 = tile * kTile;
+        if (t0 >= here) break;
+        if (!mbar_wait(&bar[tile], 0, nullptr)) {
+            atomicOr(&g_ops_timeout, 1);
+            mbar_wait(&bar[tile], 0, nullptr);   // once more for the copies, before anything ends
+        }
+        __syncwarp();
+        const uint32_t ka = smem_addr(smem) + (uint32_t)(t0 + lm_row) * (D / 2), va = ka + L::kCodes;
+        float s[NB][4][4];
+#pragma unroll
+        for (int kb = 0; kb < 4; kb++) {
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) s[nb][kb][i] = 0.0f;
+#pragma unroll
+            for (int cp = 0; cp < CH; cp += 2) {
+                uint32_t w[4];
+                ldsm4(w, ka + kb * 16 * (D / 2) + (((uint32_t)(cp + lm_ch) ^ swz) << 4));
+#pragma unroll
+                for (int ci = 0; ci < 2; ci++) {
+                    const uint32_t a = w[2 * ci], c = w[2 * ci + 1], a8 = a >> 8, c8 = c >> 8;
+#pragma unroll
+                    for (int nb = 0; nb < NB; nb++) {
+                        mma_f16(s[nb][kb], a & 0x000F000Fu, c & 0x000F000Fu, a & 0x00F000F0u, c & 0x00F000F0u, qf[nb][cp + ci][0], qf[nb][cp + ci][1]);
+                        mma_f16(s[nb][kb], a8 & 0x000F000Fu, c8 & 0x000F000Fu, a8 & 0x00F000F0u, c8 & 0x00F000F0u, qf[nb][cp + ci][2], qf[nb][cp + ci][3]);
+                    }
+                }
+            }
+        }
+        float mt[NB][2];
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++) mt[nb][0] = mt[nb][1] = -INFINITY;
+        const bool cut = t0 + kTile > least;
+#pragma unroll
+        for (int kb = 0; kb < 4; kb++)
+#pragma unroll
+            for (int hf = 0; hf < 2; hf++) {
+                const int j = t0 + kb * 16 + hf * 8 + g8;
+                const float2 kr = *reinterpret_cast<const float2 *>(&sc[j]);
+#pragma unroll
+                for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        float x = __fmaf_rn(kr.x, s[nb][kb][2 * hf + i] * qscale[nb][i], kr.y * qsum[nb][i]);
+                        if (cut && j >= seen[nb][i]) x = -INFINITY;
+                        s[nb][kb][2 * hf + i] = x;
+                        mt[nb][i] = fmaxf(mt[nb][i], x);
+                        if (TRACK) scores[(nb * 8 + 2 * c4 + i) * kUnit + j] = x;
+                    }
+            }
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) mt[nb][i] = fmaxf(mt[nb][i], __shfl_xor_sync(0xffffffffu, mt[nb][i], x));
+                const float now = fmaxf(m[nb][i], mt[nb][i]);
+                const float f = now == -INFINITY ? 1.0f : ex2(m[nb][i] - now);
+                m[nb][i] = now;
+                mt[nb][i] = now == -INFINITY ? 0.0f : now;   // what scores are taken from
+                l[nb][i] *= f;
+                z[nb][i] *= f;
+#pragma unroll
+                for (int ch = 0; ch < CH; ch++)
+#pragma unroll
+                    for (int y = 0; y < 2; y++) {
+                        o[nb][ch][y][i] *= f;
+                        o[nb][ch][y][2 + i] *= f;
+                    }
+            }
+#pragma unroll
+        for (int kb = 0; kb < 4; kb++) {
+            uint32_t pf[NB][2];
+#pragma unroll
+            for (int hf = 0; hf < 2; hf++) {
+                const int j = t0 + kb * 16 + hf * 8 + g8;
+                const float2 vr = *(reinterpret_cast<const float2 *>(&sc[j]) + 1);
+#pragma unroll
+                for (int nb = 0; nb < NB; nb++) {
+                    float w[2];
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        const float e = ex2(s[nb][kb][2 * hf + i] - mt[nb][i]);
+                        const bool off = cut && j >= seen[nb][i];   // a value that is not seen may be anything
+                        l[nb][i] += e;
+                        z[nb][i] = off ? z[nb][i] : __fmaf_rn(e, vr.y, z[nb][i]);
+                        w[i] = off ? 0.0f : e * vr.x;
+                    }
+                    pf[nb][hf] = transpose8(pack_half(w[0], w[1]));
+                }
+            }
+#pragma unroll
+            for (int cp = 0; cp < CH; cp += 2) {
+                uint32_t w[4];
+                ldsm4_trans(w, va + kb * 16 * (D / 2) + (((uint32_t)(cp + lm_ch) ^ swz) << 4));
+#pragma unroll
+                for (int ci = 0; ci < 2; ci++) {
+                    const uint32_t a = w[2 * ci], c = w[2 * ci + 1], a8 = a >> 8, c8 = c >> 8;
+#pragma unroll
+                    for (int nb = 0; nb < NB; nb++) {
+                        mma_f16(o[nb][cp + ci][0], a & 0x000F000Fu, a & 0x00F000F0u, c & 0x000F000Fu, c & 0x00F000F0u, pf[nb][0], pf[nb][1]);
+                        mma_f16(o[nb][cp + ci][1], a8 & 0x000F000Fu, a8 & 0x00F000F0u, c8 & 0x000F000Fu, c8 & 0x00F000F0u, pf[nb][0], pf[nb][1]);
+                    }
+                }
+            }
+        }
+    }
+
+    // the four warps' rows together, in their order
+#pragma unroll
+    for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) {
+                l[nb][i] += __shfl_xor_sync(0xffffffffu, l[nb][i], x);
+                z[nb][i] += __shfl_xor_sync(0xffffffffu, z[nb][i], x);
+            }
+            if (g8 == 0) {
+                const int r = nb * 8 + 2 * c4 + i;
+                s_m[warp][r] = m[nb][i];
+                s_l[warp][r] = l[nb][i];
+                s_z[warp][r] = z[nb][i];
+            }
+        }
+    __syncthreads();   // and all codes are read: their place is free for the sums
+    if (tid < R) {
+        const float top_m = fmaxf(fmaxf(s_m[0][tid], s_m[1][tid]), fmaxf(s_m[2][tid], s_m[3][tid]));
+        float sum = 0.0f;
+        for (int w = 0; w < kAttendWarps; w++) sum += s_l[w][tid] * share(s_m[w][tid], top_m);
+        s_row[tid] = make_float2(top_m, sum);
+    }
+    constexpr int LD = D + 4;
+    float *so = reinterpret_cast<float *>(smem);   // [warp][row][LD]
+    static_assert(kAttendWarps * R * LD * 4 <= 2 * L::kCodes, "the warps' sums fit where the codes were");
+    const float vup = ldexpf(1.0f, te);   // and 2^(24 - 15) for the nibbles and vdown
+#pragma unroll
+    for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int r = nb * 8 + 2 * c4 + i;
+            const float f = share(m[nb][i], fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r])));
+            const float zz = s_z[warp][r];
+#pragma unroll
+            for (int ch = 0; ch < CH; ch++)
+#pragma unroll
+                for (int y = 0; y < 2; y++)   // dimensions 32 ch + 4 g8 + 2 y and the next
+                    *reinterpret_cast<float2 *>(&so[(warp * R + r) * LD + ch * 32 + 4 * g8 + 2 * y]) =
+                        make_float2(f * __fmaf_rn(o[nb][ch][y][i] * 512.0f, vup, zz), f * __fmaf_rn(o[nb][ch][y][2 + i] * 32.0f, vup, zz));
+        }
+    __syncthreads();
+    const int rows_here = min(R, p.rows - rb * R);
+    const bool whole = p.part == nullptr;   // nothing to join: this is the result
+    const int64_t at = whole ? 0 : (((int64_t)b * p.c.n_heads + h) * p.units + unit) * ((int64_t)p.row_blocks * R) + rb * R;
+    for (int i = tid; i < rows_here * (D / 2); i += kAttendWarps * 32) {
+        const int r = i / (D / 2), d = 2 * (i % (D / 2));
+        const float2 row = s_row[r];
+        float x = 0.0f, y = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kAttendWarps; w++) {
+            const float2 v = *reinterpret_cast<const float2 *>(&so[(w * R + r) * LD + d]);
+            x += v.x;
+            y += v.y;
+        }
+        if (whole) {
+            T *dst = static_cast<T *>(p.out) + row_offset<T>(p.os, b, h, p.g, rb * R + r) + d;
+            dst[0] = from_f32<T>(row.y == 0.0f ? 0.0f : x / row.y);   // a row that sees nothing: 0
+            dst[1] = from_f32<T>(row.y == 0.0f ? 0.0f : y / row.y);
+        } else {
+            *reinterpret_cast<float2 *>(p.part + (at + r) * D + d) = make_float2(x, y);
+            if (d == 0) p.stat[at + r] = row;
+        }
+    }
+    if (TRACK) {
+        for (int j = tid; j < here; j += kAttendWarps * 32) {
+            if (whole) {
+                float add = 0.0f;
+                for (int r = 0; r < rows_here; r++) {
+                    const float2 row = s_row[r];
+                    if (row.y != 0.0f) add += ex2(scores[r * kUnit + j] - row.x) * (1.0f / row.y);
+                }
+                if (add != 0.0f) p.c.weights[base + j0 + j] += add;
+            } else {
+                for (int r = 0; r < rows_here; r++)
+                    p.score[(((int64_t)b * p.c.n_heads + h) * p.rows + rb * R + r) * p.max_len + j0 + j] = scores[r * kUnit + j];
+            }
+        }
+    }
+}
+
+// Joins the units of a row: the first `rows` CTAs of x write the rows' results, the
+// others the weights of kUnit entries each.  A row's units are taken in 8 interleaved
+// runs and those in order: places that depend on its length alone.
+constexpr int kJoinThreads = 256;
+template <typename T, int D>
+__global__ void __launch_bounds__(kJoinThreads) k_kv4_join(const __grid_constant__ AttendArgs p, int rows_padded) {
+    pdl_wait();
+    constexpr int RUNS = kJoinThreads / (D / 2);   // D / 2 threads a run, two dimensions each
+    __shared__ float red[kJoinThreads / 32];
+    __shared__ float2 runs[RUNS][D / 2];
+    const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
+    const int slot = kv4_slot(p.c, p.slots, b, false);
+    const int n = slot < 0 ? 0 : kv4_length(p.c, p.lengths, b, min(p.max_len, p.c.capacity), false);
+    const int units = (n + kUnit - 1) / kUnit;
+    const int64_t first = ((int64_t)b * p.c.n_heads + h) * p.units * rows_padded;
+    // the maximum of row r over the units
+    auto top_of = [&](int r) {
+        float m = -INFINITY;
+        for (int u = tid; u < units; u += kJoinThreads) m = fmaxf(m, p.stat[first + (int64_t)u * rows_padded + r].x);
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        __syncthreads();
+        if ((tid & 31) == 0) red[tid >> 5] = m;
+        __syncthreads();
+        m = red[0];
+        for (int w = 1; w < kJoinThreads / 32; w++) m = fmaxf(m, red[w]);
+        return m;
+    };
+    if ((int)blockIdx.x < p.rows) {
+        const int r = blockIdx.x, d = tid % (D / 2), run = tid / (D / 2);
+        const float m = top_of(r);
+        float x = 0.0f, y = 0.0f, l = 0.0f;
+        for (int u = run; u < units; u += RUNS) {
+            const int64_t at = first + (int64_t)u * rows_padded + r;
+            const float2 st = p.stat[at];
+            const float2 v = *reinterpret_cast<const float2 *>(p.part + at * D + 2 * d);
+            const float f = share(st.x, m);
+            x = __fmaf_rn(f, v.x, x);
+            y = __fmaf_rn(f, v.y, y);
+            l = __fmaf_rn(f, st.y, l);
+        }
+        __shared__ float run_l[RUNS];
+        runs[run][d] = make_float2(x, y);
+        if (d == 0) run_l[run] = l;
+        __syncthreads();
+        if (run > 0) return;
+        for (int i = 1; i < RUNS; i++) {
+            x += runs[i][d].x;
+            y += runs[i][d].y;
+            l += run_l[i];
+        }
+        T *dst = static_cast<T *>(p.out) + row_offset<T>(p.os, b, h, p.g, r) + 2 * d;
+        dst[0] = from_f32<T>(l == 0.0f ? 0.0f : x / l);
+        dst[1] = from_f32<T>(l == 0.0f ? 0.0f : y / l);
+        return;
+    }
+    const int j0 = ((int)blockIdx.x - p.rows) * kUnit;
+    if (j0 >= n) return;
+    float add[kUnit / kJoinThreads] = {};
+    for (int r = 0; r < p.rows; r++) {
+        const int seen = n - (p.t - 1 - r / p.g);
+        const float m = top_of(r);
+        float l = 0.0f;
+        for (int u = tid; u < units; u += kJoinThreads) {
+            const float2 st = p.stat[first + (int64_t)u * rows_padded + r];
+            l += st.y * share(st.x, m);
+        }
+        for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        __syncthreads();
+        if ((tid & 31) == 0) red[tid >> 5] = l;
+        __syncthreads();
+        l = red[0];
+        for (int w = 1; w < kJoinThreads / 32; w++) l += red[w];
+        const float inv = 1.0f / l;
+        const float *s = p.score + (((int64_t)b * p.c.n_heads + h) * p.rows + r) * p.max_len;
+#pragma unroll
+        for (int i = 0; i < kUnit / kJoinThreads; i++) {
+            const int j = j0 + i * kJoinThreads + tid;
+            if (j < seen) add[i] += ex2(s[j] - m) * inv;
+        }
+    }
+    float *w = p.c.weights + kv4_row(p.c, slot, h, 0);
+#pragma unroll
+    for (int i = 0; i < kUnit / kJoinThreads; i++) {
+        const int j = j0 + i * kJoinThreads + tid;
+        if (j < n && add[i] != 0.0f) w[j] += add[i];
+    }
+}
+
+// Rows of 4-bit codes as a map of boxes of kTile entries of one slot and head.
+bool kv4_map(CUtensorMap *map, uint8_t *p, const czg_kv4 &c) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return false;
+    const cuuint64_t row = (cuuint64_t)c.head_dim / 2;
+    cuuint64_t dims[3] = {row, (cuuint64_t)c.capacity, (cuuint64_t)c.n_slots * c.n_heads};
+    cuuint64_t strides[2] = {row, row * c.capacity};
+    cuuint32_t box[3] = {(cuuint32_t)row, kTile, 1};
+    cuuint32_t one[3] = {1, 1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, p, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              c.head_dim == 64 ? CU_TENSOR_MAP_SWIZZLE_32B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// How a call is cut, and where its workspace's parts lie.
+struct AttendPlan {
+    int rows, nb, row_blocks, units;
+    bool join;
+    uint64_t part, stat, score, bytes;
+};
+
+AttendPlan attend_plan(const czg_kv4 &c, int64_t b, int t, int hq, int max_len) {
+    AttendPlan a{};
+    const int n = max_len < c.capacity ? max_len : c.capacity;
+    a.rows = t * (hq / c.n_heads);
+    a.nb = a.rows <= 8 ? 1 : 2;
+    a.row_blocks = (a.rows + 8 * a.nb - 1) / (8 * a.nb);
+    a.units = n > kUnit ? (n + kUnit - 1) / kUnit : 1;
+    a.join = a.units > 1 || (c.weights && a.row_blocks > 1);
+    if (!a.join) return a;
+    const uint64_t sets = (uint64_t)b * c.n_heads * a.units * a.row_blocks * 8 * a.nb;
+    a.stat = sets * c.head_dim * 4;
+    a.score = a.stat + sets * 8;
+    a.bytes = a.score + (c.weights ? (uint64_t)b * c.n_heads * a.rows * (uint64_t)max_len * 4 : 0);
+    return a;
 }
 
 template <typename T>
@@ -215,20 +705,45 @@ int read(const czg_kv4 &c, const int32_t *slots, const int32_t *starts, int b, i
                                static_cast<T *>(k), static_cast<T *>(v)));
 }
 
+template <typename T, int D, int NB, bool TRACK>
+int attend_with(const AttendPlan &plan, const AttendArgs &p, int b, cudaStream_t st) {
+    alignas(64) CUtensorMap mk, mv;
+    if (!kv4_map(&mk, p.c.k, p.c) || !kv4_map(&mv, p.c.v, p.c)) return ops_fail(CZG_E_DEVICE, "no tensor map for the cache");
+    const size_t smem = AttendSmem<D>::bytes(NB, TRACK);
+    static int ready[64] = {0};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return ops_fail(CZG_E_DEVICE, "no device");
+    if (!ready[dev]) {
+        if (int e = ops_cuda(cudaFuncSetAttribute(k_kv4_attend<T, D, NB, TRACK>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)))
+            return e;
+        ready[dev] = 1;
+    }
+    const dim3 grid((unsigned)plan.units, (unsigned)(p.c.n_heads * plan.row_blocks), (unsigned)b);
+    if (int e = ops_cuda(ops_launch(k_kv4_attend<T, D, NB, TRACK>, grid, kAttendWarps * 32, smem, st, false, 1, mk, mv, p))) return e;
+    if (!plan.join) return CZG_OK;
+    const dim3 join((unsigned)(plan.rows + (TRACK ? plan.units : 0)), (unsigned)p.c.n_heads, (unsigned)b);
+    return ops_cuda(ops_launch(k_kv4_join<T, D>, join, kJoinThreads, 0, st, true, 1, p, plan.row_blocks * 8 * NB));
+}
+
 template <typename T>
-int attend(const czg_kv4 &c, const void *q, Strides qs, const int32_t *slots, const int32_t *lengths, int b, int t, int hq,
-           int max_len, float scale, void *out, Strides os, cudaStream_t st) {
-    auto kern = c.head_dim == 64 ? k_kv4_attend<T, 64> : k_kv4_attend<T, 128>;
-    return ops_cuda(ops_launch(kern, dim3((unsigned)c.n_heads, (unsigned)b), 128, 0, st, false, 1, c,
-                               static_cast<const T *>(q), qs, slots, lengths, t, hq / c.n_heads, max_len, scale,
-                               static_cast<T *>(out), os));
+int attend(const AttendPlan &plan, const AttendArgs &p, int b, cudaStream_t st) {
+    const bool track = p.c.weights != nullptr;
+    if (p.c.head_dim == 64) {
+        if (plan.nb == 1) return track ? attend_with<T, 64, 1, true>(plan, p, b, st) : attend_with<T, 64, 1, false>(plan, p, b, st);
+        return track ? attend_with<T, 64, 2, true>(plan, p, b, st) : attend_with<T, 64, 2, false>(plan, p, b, st);
+    }
+    if (plan.nb == 1) return track ? attend_with<T, 128, 1, true>(plan, p, b, st) : attend_with<T, 128, 1, false>(plan, p, b, st);
+    return track ? attend_with<T, 128, 2, true>(plan, p, b, st) : attend_with<T, 128, 2, false>(plan, p, b, st);
 }
 
 }  // namespace
 
+int kv4_timeouts(int *bits) { return take_timeouts(bits); }
+
 const char *check_kv4(const czg_kv4 *c) {
     if (!c || !c->k || !c->v || !c->scales || !c->status) return "null pointer in the cache";
     if (c->n_slots < 1 || c->n_heads < 1 || c->capacity < 1) return "a cache has at least one slot, head and entry";
+    if ((int64_t)c->n_slots * c->n_heads > 0x7FFFFFFF) return "slots times heads must be below 2^31";
     if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->scales, 8) || !aligned(c->weights, 4) || !aligned(c->status, 4))
         return "the cache's buffers are not aligned";
     return nullptr;
@@ -283,8 +798,10 @@ extern "C" int czg_kv4_read(const czg_kv4 *cache, const int32_t *slots, const in
 }
 
 extern "C" uint64_t czg_kv4_attend_workspace(const czg_kv4 *cache, int32_t b, int32_t t, int32_t hq, int32_t max_len) {
-    (void)cache, (void)b, (void)t, (void)hq, (void)max_len;
-    return 0;
+    if (!cache || cache->n_heads < 1 || cache->capacity < 1 || b < 1 || t < 1 || hq < cache->n_heads || max_len < 0 ||
+        (int64_t)t * hq > 0x7FFFFFFF)
+        return 0;
+    return attend_plan(*cache, b, t, hq, max_len).bytes;
 }
 
 extern "C" int czg_kv4_attend(const czg_kv4 *cache, const void *q, int64_t q_sb, int64_t q_st, int64_t q_sh, int dtype,
@@ -299,10 +816,34 @@ extern "C" int czg_kv4_attend(const czg_kv4 *cache, const void *q, int64_t q_sb,
     if (!q || !out) return ops_fail(CZG_E_ARG, "null pointer");
     if (!aligned(q, 2) || !aligned(out, 2)) return ops_fail(CZG_E_ARG, "q and out must be aligned to their type");
     if ((int64_t)t * hq > 0x7FFFFFFF) return ops_fail(CZG_E_LIMIT, "too many rows");
-    if (ws_bytes < czg_kv4_attend_workspace(cache, b, t, hq, max_len) || !aligned(ws, 16))
+    const AttendPlan plan = attend_plan(*cache, b, t, hq, max_len);
+    if (ws_bytes < plan.bytes || !aligned(ws, 16) || (plan.bytes && !ws))
         return ops_fail(CZG_E_ARG, "the workspace is too small or not 16-byte aligned");
-    const Strides qs{q_sb, q_st, q_sh}, os{o_sb, o_st, o_sh};
+    if ((int64_t)cache->n_heads * plan.row_blocks > kMaxSequences || cache->n_heads > kMaxSequences)
+        return ops_fail(CZG_E_LIMIT, "more than 65,535 blocks of rows");
+    const int es = 2;
+    AttendArgs p{};
+    p.c = *cache;
+    p.q = q;
+    p.qs = {q_sb, q_st, q_sh};
+    p.slots = slots;
+    p.lengths = lengths;
+    p.t = t;
+    p.g = hq / cache->n_heads;
+    p.rows = plan.rows;
+    p.row_blocks = plan.row_blocks;
+    p.max_len = max_len;
+    p.units = plan.units;
+    p.vec = aligned(q, 16) && (q_sb * es) % 16 == 0 && (q_st * es) % 16 == 0 && (q_sh * es) % 16 == 0;
+    p.scale_log2 = (float)((double)scale * 1.4426950408889634);
+    p.out = out;
+    p.os = {o_sb, o_st, o_sh};
+    if (plan.join) {
+        uint8_t *w = static_cast<uint8_t *>(ws);
+        p.part = reinterpret_cast<float *>(w);
+        p.stat = reinterpret_cast<float2 *>(w + plan.stat);
+        p.score = reinterpret_cast<float *>(w + plan.score);
+    }
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (dtype == CZG_BF16) return attend<__nv_bfloat16>(*cache, q, qs, slots, lengths, b, t, hq, max_len, scale, out, os, st);
-    return attend<__half>(*cache, q, qs, slots, lengths, b, t, hq, max_len, scale, out, os, st);
+    return dtype == CZG_BF16 ? attend<__nv_bfloat16>(plan, p, b, st) : attend<__half>(plan, p, b, st);
 }

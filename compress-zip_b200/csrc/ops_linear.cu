@@ -182,8 +182,6 @@ __global__ void __launch_bounds__(kQuantThreads) k_quantize_rows(const T *__rest
 // does not show in the result.
 constexpr int LT = 128;   // channels of a tile
 
-__device__ int g_ops_timeout;   // a bounded wait ran out on this device
-
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -561,13 +559,11 @@ using namespace czg;
 extern "C" const char *czg_ops_last_error(void) { return g_ops_error.c_str(); }
 
 extern "C" int czg_ops_check(void) {
-    int bits = 0;
+    int a = 0, b = 0;
     if (int st = ops_cuda(cudaDeviceSynchronize())) return st;
-    if (int st = ops_cuda(cudaMemcpyFromSymbol(&bits, g_ops_timeout, sizeof(bits)))) return st;
-    if (bits == 0) return CZG_OK;
-    const int zero = 0;
-    if (int st = ops_cuda(cudaMemcpyToSymbol(g_ops_timeout, &zero, sizeof(zero)))) return st;
-    return ops_fail(CZG_E_TIMEOUT, "a bounded wait of a kernel ran out; its results are incomplete");
+    if (int st = take_timeouts(&a)) return st;
+    if (int st = kv4_timeouts(&b)) return st;
+    return a || b ? ops_fail(CZG_E_TIMEOUT, "a bounded wait of a kernel ran out; its results are incomplete") : CZG_OK;
 }
 
 extern "C" int czg_quantize_rows(const void *x, int dtype, int64_t ld_x, int64_t m, int64_t k, int8_t *codes,
