@@ -168,11 +168,12 @@ struct AttendArgs {
     const void *q;
     Strides qs;
     const int32_t *slots, *lengths;
-    int t, g, rows, row_blocks, max_len, units, vec;
+    int t, g, rows, row_blocks, max_len, units, vec, whole;
+    uint64_t g_inv;     // 2^32 / g, rounded up: r g_inv / 2^32 is r / g while r g < 2^32
     float scale_log2;   // scale * log2 e
     void *out;
     Strides os;
-    // more than one unit (or row block with weights): partial results
+    // not whole, that is more than one unit (or row block with weights): partial results to join
     float *part;        // [b][head][unit][rows padded][D]
     float2 *stat;       // [b][head][unit][rows padded] (maximum, sum)
     float *score;       // weights: [b][head][rows][max_len]
@@ -213,16 +214,17 @@ __device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, u
 }
 
 // Row r of a sequence and key head: place i = r / g of the call's rows, query head h g + r % g.
-template <typename T>
-__device__ __forceinline__ int64_t row_offset(const Strides &s, int b, int h, int g, int r) {
-    return b * s.b + (r / g) * s.t + (h * g + r % g) * s.h;
+__device__ __forceinline__ int row_place(const AttendArgs &p, int r) { return (int)((uint64_t)(uint32_t)r * p.g_inv >> 32); }
+__device__ __forceinline__ int64_t row_offset(const AttendArgs &p, const Strides &s, int b, int h, int r) {
+    const int i = row_place(p, r);
+    return b * s.b + i * s.t + (int64_t)((h - i) * p.g + r) * s.h;
 }
 
 template <int D>
 struct AttendSmem {
     static constexpr int kCodes = kUnit * D / 2;
-    static constexpr int kScales = 2 * kCodes, kBars = kScales + kUnit * 16, kScores = kBars + 128;
-    static size_t bytes(int nb, bool track) { return 1024 + kScores + (track ? (size_t)8 * nb * kUnit * 4 : 0); }
+    static constexpr int kScales = 2 * kCodes, kBars = kScales + kUnit * 16;
+    static constexpr size_t kBytes = 1024 + kBars + 64;
 };
 
 template <typename T, int D, int NB, bool TRACK>
@@ -235,8 +237,7 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     float4 *sc = reinterpret_cast<float4 *>(smem + L::kScales);   // k step, k lo, v step (scaled), v lo
     uint64_t *bar = reinterpret_cast<uint64_t *>(smem + L::kBars);
-    float *scores = reinterpret_cast<float *>(smem + L::kScores);   // TRACK: [row][entry of the unit]
-    __shared__ float s_m[kAttendWarps][R], s_l[kAttendWarps][R], s_z[kAttendWarps][R];
+    __shared__ float s_m[kAttendWarps][R], s_l[kAttendWarps][R];
     __shared__ uint32_t s_top[kAttendWarps];
     __shared__ float2 s_row[R];   // maximum and sum over the warps
 
@@ -292,7 +293,7 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
         float x[CH][8], big = 0.0f, sum = 0.0f;
 #pragma unroll
         for (int ch = 0; ch < CH; ch++) {
-            const T *src = static_cast<const T *>(p.q) + (r < p.rows ? row_offset<T>(p.qs, b, h, p.g, r) : 0) + ch * 32 + c4 * 8;
+            const T *src = static_cast<const T *>(p.q) + (r < p.rows ? row_offset(p, p.qs, b, h, r) : 0) + ch * 32 + c4 * 8;
             __align__(16) T v[8];
             if (r >= p.rows) {
 #pragma unroll
@@ -332,7 +333,7 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
             qscale[nb][i] = __shfl_sync(0xffffffffu, qs, (2 * c4 + i) * 4);
             qsum[nb][i] = __shfl_sync(0xffffffffu, zq, (2 * c4 + i) * 4);
             const int row = rb * R + nb * 8 + 2 * c4 + i;
-            seen[nb][i] = row < p.rows ? n - (p.t - 1 - row / p.g) - j0 : 0x7FFFFFFF;   // entries of this unit that the row sees
+            seen[nb][i] = row < p.rows ? n - (p.t - 1 - row_place(p, row)) - j0 : 0x7FFFFFFF;   // entries of this unit that the row sees
         }
     }
     __syncthreads();
@@ -346,13 +347,18 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
                                                       __uint_as_float(raw[i].y << 16) * vdown, __uint_as_float(raw[i].y & 0xFFFF0000u));
     __syncthreads();
 
-    float m[NB][2], l[NB][2], z[NB][2], o[NB][CH][2][4];
+    // scores of this CTA's rows from entry j0 on, kept for the weights
+    float *score = TRACK ? p.score + (((int64_t)b * p.c.n_heads + h) * p.rows + rb * R) * p.max_len + j0 : nullptr;
+    // kExact: what the fp16 weights lost is made good at the middle of the codes, so their
+    // rounding counts from there (a third) and not from code 0; bf16 results do not need it
+    constexpr bool kExact = DType<T>::kCode == CZG_F16;
+    float m[NB][2], l[NB][2], z[NB][2], lost[NB][2], o[NB][CH][2][4];
 #pragma unroll
     for (int nb = 0; nb < NB; nb++) {
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             m[nb][i] = -INFINITY;
-            l[nb][i] = z[nb][i] = 0.0f;
+            l[nb][i] = z[nb][i] = lost[nb][i] = 0.0f;
         }
 #pragma unroll
         for (int ch = 0; ch < CH; ch++)
@@ -418,7 +424,8 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
                         if (cut && j >= seen[nb][i]) x = -INFINITY;
                         s[nb][kb][2 * hf + i] = x;
                         mt[nb][i] = fmaxf(mt[nb][i], x);
-                        if (TRACK) scores[(nb * 8 + 2 * c4 + i) * kUnit + j] = x;
+                        if (TRACK && rb * R + nb * 8 + 2 * c4 + i < p.rows && j < here)
+                            score[(int64_t)(nb * 8 + 2 * c4 + i) * p.max_len + j] = x;
                     }
             }
 #pragma unroll
@@ -428,18 +435,21 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
 #pragma unroll
                 for (int x = 4; x < 32; x <<= 1) mt[nb][i] = fmaxf(mt[nb][i], __shfl_xor_sync(0xffffffffu, mt[nb][i], x));
                 const float now = fmaxf(m[nb][i], mt[nb][i]);
-                const float f = now == -INFINITY ? 1.0f : ex2(m[nb][i] - now);
+                const float f = share(m[nb][i], now);
                 m[nb][i] = now;
                 mt[nb][i] = now == -INFINITY ? 0.0f : now;   // what scores are taken from
-                l[nb][i] *= f;
-                z[nb][i] *= f;
+                if (it > 0) {
+                    l[nb][i] *= f;
+                    z[nb][i] *= f;
+                    lost[nb][i] *= f;
 #pragma unroll
-                for (int ch = 0; ch < CH; ch++)
+                    for (int ch = 0; ch < CH; ch++)
 #pragma unroll
-                    for (int y = 0; y < 2; y++) {
-                        o[nb][ch][y][i] *= f;
-                        o[nb][ch][y][2 + i] *= f;
-                    }
+                        for (int y = 0; y < 2; y++) {
+                            o[nb][ch][y][i] *= f;
+                            o[nb][ch][y][2 + i] *= f;
+                        }
+                }
             }
 #pragma unroll
         for (int kb = 0; kb < 4; kb++) {
@@ -459,7 +469,13 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
                         z[nb][i] = off ? z[nb][i] : __fmaf_rn(e, vr.y, z[nb][i]);
                         w[i] = off ? 0.0f : e * vr.x;
                     }
-                    pf[nb][hf] = transpose8(pack_half(w[0], w[1]));
+                    const uint32_t wp = pack_half(w[0], w[1]);
+                    if (kExact) {
+                        const float2 back = __half22float2(*reinterpret_cast<const __half2 *>(&wp));
+                        lost[nb][0] += w[0] - back.x;
+                        lost[nb][1] += w[1] - back.y;
+                    }
+                    pf[nb][hf] = transpose8(wp);
                 }
             }
 #pragma unroll
@@ -488,12 +504,14 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
             for (int x = 4; x < 32; x <<= 1) {
                 l[nb][i] += __shfl_xor_sync(0xffffffffu, l[nb][i], x);
                 z[nb][i] += __shfl_xor_sync(0xffffffffu, z[nb][i], x);
+                if (kExact) lost[nb][i] += __shfl_xor_sync(0xffffffffu, lost[nb][i], x);
             }
+            // vdown is 2^15 / 2^te
+            if (kExact) z[nb][i] = __fmaf_rn(lost[nb][i] * (7.5f / 32768.0f), ldexpf(1.0f, te), z[nb][i]);
             if (g8 == 0) {
                 const int r = nb * 8 + 2 * c4 + i;
                 s_m[warp][r] = m[nb][i];
                 s_l[warp][r] = l[nb][i];
-                s_z[warp][r] = z[nb][i];
             }
         }
     __syncthreads();   // and all codes are read: their place is free for the sums
@@ -513,7 +531,7 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
         for (int i = 0; i < 2; i++) {
             const int r = nb * 8 + 2 * c4 + i;
             const float f = share(m[nb][i], fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r])));
-            const float zz = s_z[warp][r];
+            const float zz = z[nb][i];
 #pragma unroll
             for (int ch = 0; ch < CH; ch++)
 #pragma unroll
@@ -523,7 +541,7 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
         }
     __syncthreads();
     const int rows_here = min(R, p.rows - rb * R);
-    const bool whole = p.part == nullptr;   // nothing to join: this is the result
+    const bool whole = p.whole;   // nothing to join: this is the result
     const int64_t at = whole ? 0 : (((int64_t)b * p.c.n_heads + h) * p.units + unit) * ((int64_t)p.row_blocks * R) + rb * R;
     for (int i = tid; i < rows_here * (D / 2); i += kAttendWarps * 32) {
         const int r = i / (D / 2), d = 2 * (i % (D / 2));
@@ -536,7 +554,7 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
             y += v.y;
         }
         if (whole) {
-            T *dst = static_cast<T *>(p.out) + row_offset<T>(p.os, b, h, p.g, rb * R + r) + d;
+            T *dst = static_cast<T *>(p.out) + row_offset(p, p.os, b, h, rb * R + r) + d;
             dst[0] = from_f32<T>(row.y == 0.0f ? 0.0f : x / row.y);   // a row that sees nothing: 0
             dst[1] = from_f32<T>(row.y == 0.0f ? 0.0f : y / row.y);
         } else {
@@ -544,21 +562,15 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
             if (d == 0) p.stat[at + r] = row;
         }
     }
-    if (TRACK) {
+    if (TRACK && whole)   // the scores that this CTA wrote
         for (int j = tid; j < here; j += kAttendWarps * 32) {
-            if (whole) {
-                float add = 0.0f;
-                for (int r = 0; r < rows_here; r++) {
-                    const float2 row = s_row[r];
-                    if (row.y != 0.0f) add += ex2(scores[r * kUnit + j] - row.x) * (1.0f / row.y);
-                }
-                if (add != 0.0f) p.c.weights[base + j0 + j] += add;
-            } else {
-                for (int r = 0; r < rows_here; r++)
-                    p.score[(((int64_t)b * p.c.n_heads + h) * p.rows + rb * R + r) * p.max_len + j0 + j] = scores[r * kUnit + j];
+            float add = 0.0f;
+            for (int r = 0; r < rows_here; r++) {
+                const float2 row = s_row[r];
+                if (row.y != 0.0f) add += ex2(score[(int64_t)r * p.max_len + j] - row.x) * (1.0f / row.y);
             }
+            if (add != 0.0f) p.c.weights[base + j0 + j] += add;
         }
-    }
 }
 
 // Joins the units of a row: the first `rows` CTAs of x write the rows' results, the
@@ -611,34 +623,39 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv4_join(const __grid_constant
             y += runs[i][d].y;
             l += run_l[i];
         }
-        T *dst = static_cast<T *>(p.out) + row_offset<T>(p.os, b, h, p.g, r) + 2 * d;
+        T *dst = static_cast<T *>(p.out) + row_offset(p, p.os, b, h, r) + 2 * d;
         dst[0] = from_f32<T>(l == 0.0f ? 0.0f : x / l);
         dst[1] = from_f32<T>(l == 0.0f ? 0.0f : y / l);
         return;
     }
+    // weights of kUnit entries: a warp a row for its maximum and sum, then a thread two entries
     const int j0 = ((int)blockIdx.x - p.rows) * kUnit;
     if (j0 >= n) return;
+    constexpr int RB = 32;   // rows at a time
+    __shared__ float2 s_row[RB];
     float add[kUnit / kJoinThreads] = {};
-    for (int r = 0; r < p.rows; r++) {
-        const int seen = n - (p.t - 1 - r / p.g);
-        const float m = top_of(r);
-        float l = 0.0f;
-        for (int u = tid; u < units; u += kJoinThreads) {
-            const float2 st = p.stat[first + (int64_t)u * rows_padded + r];
-            l += st.y * share(st.x, m);
+    for (int r0 = 0; r0 < p.rows; r0 += RB) {
+        __syncthreads();
+        for (int r = r0 + (tid >> 5); r < min(r0 + RB, p.rows); r += kJoinThreads / 32) {
+            float m = -INFINITY, l = 0.0f;
+            for (int u = tid & 31; u < units; u += 32) m = fmaxf(m, p.stat[first + (int64_t)u * rows_padded + r].x);
+            for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            for (int u = tid & 31; u < units; u += 32) {
+                const float2 st = p.stat[first + (int64_t)u * rows_padded + r];
+                l += st.y * share(st.x, m);
+            }
+            for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+            if ((tid & 31) == 0) s_row[r - r0] = make_float2(m, l == 0.0f ? 0.0f : 1.0f / l);
         }
-        for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
         __syncthreads();
-        if ((tid & 31) == 0) red[tid >> 5] = l;
-        __syncthreads();
-        l = red[0];
-        for (int w = 1; w < kJoinThreads / 32; w++) l += red[w];
-        const float inv = 1.0f / l;
-        const float *s = p.score + (((int64_t)b * p.c.n_heads + h) * p.rows + r) * p.max_len;
+        const float *s = p.score + (((int64_t)b * p.c.n_heads + h) * p.rows + r0) * p.max_len + j0 + tid;
+#pragma unroll 4
+        for (int r = 0; r < min(RB, p.rows - r0); r++) {
+            const int seen = n - (p.t - 1 - row_place(p, r0 + r)) - j0 - tid;
+            const float2 row = s_row[r];
 #pragma unroll
-        for (int i = 0; i < kUnit / kJoinThreads; i++) {
-            const int j = j0 + i * kJoinThreads + tid;
-            if (j < seen) add[i] += ex2(s[j] - m) * inv;
+            for (int i = 0; i < kUnit / kJoinThreads; i++)
+                if (i * kJoinThreads < seen) add[i] += ex2(s[(int64_t)r * p.max_len + i * kJoinThreads] - row.x) * row.y;
         }
     }
     float *w = p.c.weights + kv4_row(p.c, slot, h, 0);
@@ -678,8 +695,7 @@ AttendPlan attend_plan(const czg_kv4 &c, int64_t b, int t, int hq, int max_len) 
     a.row_blocks = (a.rows + 8 * a.nb - 1) / (8 * a.nb);
     a.units = n > kUnit ? (n + kUnit - 1) / kUnit : 1;
     a.join = a.units > 1 || (c.weights && a.row_blocks > 1);
-    if (!a.join) return a;
-    const uint64_t sets = (uint64_t)b * c.n_heads * a.units * a.row_blocks * 8 * a.nb;
+    const uint64_t sets = a.join ? (uint64_t)b * c.n_heads * a.units * a.row_blocks * 8 * a.nb : 0;
     a.stat = sets * c.head_dim * 4;
     a.score = a.stat + sets * 8;
     a.bytes = a.score + (c.weights ? (uint64_t)b * c.n_heads * a.rows * (uint64_t)max_len * 4 : 0);
@@ -709,7 +725,7 @@ template <typename T, int D, int NB, bool TRACK>
 int attend_with(const AttendPlan &plan, const AttendArgs &p, int b, cudaStream_t st) {
     alignas(64) CUtensorMap mk, mv;
     if (!kv4_map(&mk, p.c.k, p.c) || !kv4_map(&mv, p.c.v, p.c)) return ops_fail(CZG_E_DEVICE, "no tensor map for the cache");
-    const size_t smem = AttendSmem<D>::bytes(NB, TRACK);
+    const size_t smem = AttendSmem<D>::kBytes;
     static int ready[64] = {0};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return ops_fail(CZG_E_DEVICE, "no device");
@@ -815,7 +831,8 @@ extern "C" int czg_kv4_attend(const czg_kv4 *cache, const void *q, int64_t q_sb,
     if (b == 0 || t == 0) return CZG_OK;
     if (!q || !out) return ops_fail(CZG_E_ARG, "null pointer");
     if (!aligned(q, 2) || !aligned(out, 2)) return ops_fail(CZG_E_ARG, "q and out must be aligned to their type");
-    if ((int64_t)t * hq > 0x7FFFFFFF) return ops_fail(CZG_E_LIMIT, "too many rows");
+    if ((int64_t)t * hq > 0x7FFFFFFF || (int64_t)t * hq / cache->n_heads * (hq / cache->n_heads) >= 1ll << 32)
+        return ops_fail(CZG_E_LIMIT, "too many rows");
     const AttendPlan plan = attend_plan(*cache, b, t, hq, max_len);
     if (ws_bytes < plan.bytes || !aligned(ws, 16) || (plan.bytes && !ws))
         return ops_fail(CZG_E_ARG, "the workspace is too small or not 16-byte aligned");
@@ -838,12 +855,12 @@ extern "C" int czg_kv4_attend(const czg_kv4 *cache, const void *q, int64_t q_sb,
     p.scale_log2 = (float)((double)scale * 1.4426950408889634);
     p.out = out;
     p.os = {o_sb, o_st, o_sh};
-    if (plan.join) {
-        uint8_t *w = static_cast<uint8_t *>(ws);
-        p.part = reinterpret_cast<float *>(w);
-        p.stat = reinterpret_cast<float2 *>(w + plan.stat);
-        p.score = reinterpret_cast<float *>(w + plan.score);
-    }
+    p.whole = !plan.join;
+    p.g_inv = ((1ull << 32) + p.g - 1) / p.g;
+    uint8_t *w = static_cast<uint8_t *>(ws);
+    p.part = reinterpret_cast<float *>(w);
+    p.stat = reinterpret_cast<float2 *>(w + plan.stat);
+    p.score = reinterpret_cast<float *>(w + plan.score);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     return dtype == CZG_BF16 ? attend<__nv_bfloat16>(plan, p, b, st) : attend<__half>(plan, p, b, st);
 }
