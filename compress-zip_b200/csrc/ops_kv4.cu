@@ -1,6 +1,7 @@
 // ops_kv4.cu -- the key/value cache held in 4 bits (include/czg_ops.h): append, read
 // and attention.
 #include <cmath>
+#include <type_traits>
 
 #include "ops_kv4.cuh"
 #include "tc_common.cuh"
@@ -138,9 +139,9 @@ __global__ void __launch_bounds__(256) k_kv4_read(czg_kv4 c, const int32_t *__re
 //
 // A CTA takes one unit of a sequence's entries (kUnit, at a fixed place whatever the
 // batch), one key head and up to 8 NB rows (query heads of that key head, times the
-// call's rows).  Its four warps take tiles of 64 entries in turn; each asks for its own
-// tiles at the start, by TMA into swizzled shared memory, so the whole unit is under way
-// at once, and several CTAs share an SM.
+// call's rows).  Its two warps take tiles of 64 entries in turn, each through a ring of
+// its own that TMA fills (swizzled for ldmatrix); many such small CTAs share an SM and
+// cover one another's beginnings and ends.
 //
 // Products are on mma.sync m16n8k16 (fp16, fp32 sums) with the cache as the A operand and
 // the rows as N: 8 rows fill an MMA, where tcgen05 would need 64 or 128 and the codes
@@ -154,21 +155,21 @@ __global__ void __launch_bounds__(256) k_kv4_read(czg_kv4 c, const int32_t *__re
 //      the pair of dimension 4g + i (odd i: 16-fold, taken out at the end).
 // With x = lo + step c:  s_j = step_j (q.c_j) + lo_j sum(q);  out = sum p_j step_j c_j + sum p_j lo_j.
 // The query is held in fp16 after a power of two that brings its largest value to
-// [2^14, 2^15): exact but for values below 2^-24 of the largest.  p_j step_j is
+// [2^13, 2^14): exact but for values below 2^-23 of the largest.  p_j step_j is
 // held in fp16 likewise (2^15 for the unit's largest step): off by 2^-12 of itself, against
 // 2^-9 of the result for bf16 and 2^-12 for fp16; its range is 2^39 wide.  Scores, maxima and
 // sums are fp32; exponentials are ex2.approx (2^-22).
 // Between the warps of a CTA, and between units (k_kv4_join), partial results are joined
 // in a fixed order, so a row's bits do not depend on the batch or the grid.
-constexpr int kUnit = 512, kTile = 64, kAttendWarps = 4;
-static_assert(kUnit == 2 * kTile * kAttendWarps, "a warp has two tiles");
+constexpr int kUnit = 512, kTile = 64, kAttendWarps = 2, kRing = 2;
+constexpr int kTurns = kUnit / (kTile * kAttendWarps);   // tiles of a warp
 
 struct AttendArgs {
     czg_kv4 c;
     const void *q;
     Strides qs;
     const int32_t *slots, *lengths;
-    int t, g, rows, row_blocks, max_len, units, vec, whole;
+    int t, g, rows, row_blocks, max_len, units, vec, out_vec, whole;
     uint64_t g_inv;     // 2^32 / g, rounded up: r g_inv / 2^32 is r / g while r g < 2^32
     float scale_log2;   // scale * log2 e
     void *out;
@@ -183,6 +184,23 @@ __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+__device__ __forceinline__ void add_scaled(float4 &x, float f, float4 v) {
+    x.x = __fmaf_rn(f, v.x, x.x);
+    x.y = __fmaf_rn(f, v.y, x.y);
+    x.z = __fmaf_rn(f, v.z, x.z);
+    x.w = __fmaf_rn(f, v.w, x.w);
+}
+// Four dimensions of a result: x f.
+template <typename T>
+__device__ __forceinline__ void store4(T *dst, float4 x, float f, bool vec) {
+    __align__(8) T y[4] = {from_f32<T>(x.x * f), from_f32<T>(x.y * f), from_f32<T>(x.z * f), from_f32<T>(x.w * f)};
+    if (vec) {
+        *reinterpret_cast<uint2 *>(dst) = *reinterpret_cast<const uint2 *>(y);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) dst[i] = y[i];
+    }
 }
 // What sums taken from the maximum m are worth from the maximum `top` (both may be -infinity).
 __device__ __forceinline__ float share(float m, float top) { return m == top ? 1.0f : ex2(m - top); }
@@ -220,11 +238,13 @@ __device__ __forceinline__ int64_t row_offset(const AttendArgs &p, const Strides
     return b * s.b + i * s.t + (int64_t)((h - i) * p.g + r) * s.h;
 }
 
+__device__ __forceinline__ float pow2f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }   // -126 <= e <= 127
+
 template <int D>
 struct AttendSmem {
-    static constexpr int kCodes = kUnit * D / 2;
-    static constexpr int kScales = 2 * kCodes, kBars = kScales + kUnit * 16;
-    static constexpr size_t kBytes = 1024 + kBars + 64;
+    static constexpr int kTileCodes = kTile * D / 2;   // of keys, and as many of values behind them
+    static constexpr int kScales = kAttendWarps * kRing * 2 * kTileCodes, kBars = kScales + kUnit * 8;
+    static constexpr size_t kBytes = 1024 + kBars + kAttendWarps * kRing * 8;
 };
 
 template <typename T, int D, int NB, bool TRACK>
@@ -232,17 +252,21 @@ __global__ void __launch_bounds__(kAttendWarps * 32)
 k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttendArgs p) {
     using L = AttendSmem<D>;
     constexpr int CH = D / 32;      // 16-byte chunks of a row of codes
-    constexpr int R = 8 * NB;
+    constexpr int R = 8 * NB, THREADS = kAttendWarps * 32;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    float4 *sc = reinterpret_cast<float4 *>(smem + L::kScales);   // k step, k lo, v step (scaled), v lo
+    uint2 *sc = reinterpret_cast<uint2 *>(smem + L::kScales);   // the entries' ranges, as they lie in memory
     uint64_t *bar = reinterpret_cast<uint64_t *>(smem + L::kBars);
+    __shared__ uint4 s_q[NB * CH * 32];      // the query as B fragments: [nb][chunk][lane]
+    __shared__ float2 s_qs[R];               // a row's factors
     __shared__ float s_m[kAttendWarps][R], s_l[kAttendWarps][R];
     __shared__ uint32_t s_top[kAttendWarps];
-    __shared__ float2 s_row[R];   // maximum and sum over the warps
+    __shared__ float2 s_row[R];              // maximum and sum over the warps
+    __shared__ int64_t s_out[R];             // where the row's output begins
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, c4 = lane & 3;
-    const int unit = blockIdx.x, h = blockIdx.y / p.row_blocks, rb = blockIdx.y % p.row_blocks, b = blockIdx.z;
+    const int unit = blockIdx.x, h = p.row_blocks == 1 ? blockIdx.y : blockIdx.y / p.row_blocks, b = blockIdx.z;
+    const int rb = blockIdx.y - h * p.row_blocks;
     const bool first = tid == 0 && unit == 0 && blockIdx.y == 0;
     if (TRACK && unit == 0 && b == 0 && blockIdx.y == 0) kv4_check_distinct(p.c, p.slots, gridDim.z);
     const int slot = kv4_slot(p.c, p.slots, b, first);
@@ -251,104 +275,97 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
     if (here <= 0 && unit > 0) return;
     const int64_t base = kv4_row(p.c, max(slot, 0), h, 0);
 
-    // each warp asks for its tiles
+    // each warp asks for its first tiles
+    uint8_t *ring = smem + warp * kRing * 2 * L::kTileCodes;
+    uint64_t *ring_bar = bar + warp * kRing;
+    auto ask = [&](int it) {   // one lane
+        uint8_t *to = ring + (it % kRing) * 2 * L::kTileCodes;
+        const int y = j0 + (it * kAttendWarps + warp) * kTile, z = slot * p.c.n_heads + h;
+        mbar_expect_tx(&ring_bar[it % kRing], 2 * L::kTileCodes);
+        tma_load_3d(to, &map_k, &ring_bar[it % kRing], 0, y, z);
+        tma_load_3d(to + L::kTileCodes, &map_v, &ring_bar[it % kRing], 0, y, z);
+    };
+    const int turns = max(0, (here - warp * kTile + kTile * kAttendWarps - 1) / (kTile * kAttendWarps));   // tiles of this warp
     if (lane == 0) {
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const int tile = i * kAttendWarps + warp;
-            mbar_init(&bar[tile], 1);
-        }
+        for (int i = 0; i < kRing; i++) mbar_init(&ring_bar[i], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        for (int i = 0; i < min(kRing, turns); i++) ask(i);
+    }
+    __syncwarp();
+
+    // ranges of the entries; 0 behind the end, whatever lies there
+    uint2 raw[kUnit / THREADS];
+    uint32_t top = 0;
+    const KvScale *ranges = static_cast<const KvScale *>(p.c.scales) + base + j0;
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const int tile = i * kAttendWarps + warp;
-            if (tile * kTile < here) {
-                mbar_expect_tx(&bar[tile], kTile * D);
-                tma_load_3d(smem + tile * kTile * (D / 2), &map_k, &bar[tile], 0, j0 + tile * kTile, slot * p.c.n_heads + h);
-                tma_load_3d(smem + L::kCodes + tile * kTile * (D / 2), &map_v, &bar[tile], 0, j0 + tile * kTile, slot * p.c.n_heads + h);
+    for (int i = 0; i < kUnit / THREADS; i++)
+        raw[i] = tid + i * THREADS < here ? __ldg(reinterpret_cast<const uint2 *>(ranges + tid + i * THREADS)) : make_uint2(0, 0);
+
+    // the query: D / 8 threads a row, 8 dimensions each, which are one lane's share of a chunk
+    constexpr int TR = D / 8;
+#pragma unroll
+    for (int r0 = 0; r0 < R; r0 += THREADS / TR) {
+        const int r = r0 + tid / TR, part = tid % TR, row = rb * R + r;
+        if (r < R) {   // whole warps
+            const bool there = row < p.rows;
+            const T *src = static_cast<const T *>(p.q) + (there ? row_offset(p, p.qs, b, h, row) : 0) + part * 8;
+            __align__(16) T v[8];
+            if (there && p.vec) {
+                *reinterpret_cast<uint4 *>(v) = __ldg(reinterpret_cast<const uint4 *>(src));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[i] = there ? src[i] : from_f32<T>(0.0f);
+            }
+            float x[8], big = 0.0f, sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                x[i] = to_f32(v[i]);
+                big = fmaxf(big, fabsf(x[i]));
+                sum += x[i];
+            }
+#pragma unroll
+            for (int o = 1; o < TR; o <<= 1) {
+                big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+                sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            }
+            int e = (int)(__float_as_uint(big) >> 23) - 127;
+            e = e > 127 ? 0 : min(max(e, -100), 126);
+            // a negative scale turns the query round, so that larger is larger in what follows
+            const float up = copysignf(pow2f(13 - e), p.scale_log2), u16 = up * 0.0625f;
+            s_q[((r >> 3) * CH + (part >> 2)) * 32 + (r & 7) * 4 + (part & 3)] =
+                make_uint4(pack_half(x[0] * up, x[4] * up), pack_half(x[1] * u16, x[5] * u16),
+                           pack_half(x[2] * up, x[6] * up), pack_half(x[3] * u16, x[7] * u16));
+            if (part == 0) {   // q.c is the MMA's times 2^24 2^(e - 13)
+                s_qs[r] = make_float2(fabsf(p.scale_log2) * 2048.0f * pow2f(e), copysignf(pow2f(-e), p.scale_log2) * (sum * (1.0f / 2048.0f)));
+                s_out[r] = there ? row_offset(p, p.os, b, h, row) : 0;
             }
         }
     }
-
-    // ranges of the entries; 0 behind the end, whatever lies there
-    uint2 raw[kUnit / (kAttendWarps * 32)];
-    uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < kUnit / (kAttendWarps * 32); i++) {
-        const int j = tid + i * kAttendWarps * 32;
-        raw[i] = j < here ? __ldg(reinterpret_cast<const uint2 *>(static_cast<const KvScale *>(p.c.scales) + base + j0 + j)) : make_uint2(0, 0);
+    for (int i = 0; i < kUnit / THREADS; i++) {
         const uint32_t step = (raw[i].y & 0xFFFFu) << 16;   // bits of the value's step, never negative
         if (step < 0x7F800000u) top = max(top, step);
     }
     top = __reduce_max_sync(0xffffffffu, top);
     if (lane == 0) s_top[warp] = top;
-
-    // the query's fragments, with its row's power of two, and the row's factors
-    uint32_t qf[NB][CH][4];
-    float qscale[NB][2], qsum[NB][2];   // of rows 2 c4, 2 c4 + 1: what q.c is multiplied by, and sum(q)
-    int seen[NB][2];
-#pragma unroll
-    for (int nb = 0; nb < NB; nb++) {
-        const int r = rb * R + nb * 8 + g8;
-        float x[CH][8], big = 0.0f, sum = 0.0f;
-#pragma unroll
-        for (int ch = 0; ch < CH; ch++) {
-            const T *src = static_cast<const T *>(p.q) + (r < p.rows ? row_offset(p, p.qs, b, h, r) : 0) + ch * 32 + c4 * 8;
-            __align__(16) T v[8];
-            if (r >= p.rows) {
-#pragma unroll
-                for (int i = 0; i < 8; i++) v[i] = from_f32<T>(0.0f);
-            } else if (p.vec) {
-                *reinterpret_cast<uint4 *>(v) = __ldg(reinterpret_cast<const uint4 *>(src));
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; i++) v[i] = src[i];
-            }
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                x[ch][i] = to_f32(v[i]);
-                big = fmaxf(big, fabsf(x[ch][i]));
-                sum += x[ch][i];
-            }
-        }
-#pragma unroll
-        for (int o = 1; o < 4; o <<= 1) {
-            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-            sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        }
-        int e = (int)(__float_as_uint(big) >> 23) - 127;
-        e = e > 127 ? 0 : max(e, -100);
-        const float up = __uint_as_float((uint32_t)(14 - e + 127) << 23);
-#pragma unroll
-        for (int ch = 0; ch < CH; ch++) {
-            const float u16 = up * 0.0625f;
-            qf[nb][ch][0] = pack_half(x[ch][0] * up, x[ch][4] * up);
-            qf[nb][ch][1] = pack_half(x[ch][1] * u16, x[ch][5] * u16);
-            qf[nb][ch][2] = pack_half(x[ch][2] * up, x[ch][6] * up);
-            qf[nb][ch][3] = pack_half(x[ch][3] * u16, x[ch][7] * u16);
-        }
-        const float qs = ldexpf(p.scale_log2, e + 10), zq = p.scale_log2 * sum;   // 2^24 2^(e - 14)
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            qscale[nb][i] = __shfl_sync(0xffffffffu, qs, (2 * c4 + i) * 4);
-            qsum[nb][i] = __shfl_sync(0xffffffffu, zq, (2 * c4 + i) * 4);
-            const int row = rb * R + nb * 8 + 2 * c4 + i;
-            seen[nb][i] = row < p.rows ? n - (p.t - 1 - row_place(p, row)) - j0 : 0x7FFFFFFF;   // entries of this unit that the row sees
-        }
-    }
     __syncthreads();
-    top = max(max(s_top[0], s_top[1]), max(s_top[2], s_top[3]));
-    // a power of two not below any step, and what brings it to 2^15
-    const int te = top == 0 ? 0 : max((int)(top >> 23) - 126, -100);
-    const float vdown = ldexpf(1.0f, 15 - te);
+    top = s_top[0];
+    for (int w = 1; w < kAttendWarps; w++) top = max(top, s_top[w]);
+    // 2^te is not below any value's step (where 2^-100 is not above all); weights are
+    // taken 2^up-fold, which brings weight times step below 2^15
+    const int te = top == 0 ? 0 : max((int)(top >> 23) - 126, -100), up = 15 - te;
 #pragma unroll
-    for (int i = 0; i < kUnit / (kAttendWarps * 32); i++)
-        sc[tid + i * kAttendWarps * 32] = make_float4(__uint_as_float(raw[i].x << 16), __uint_as_float(raw[i].x & 0xFFFF0000u),
-                                                      __uint_as_float(raw[i].y << 16) * vdown, __uint_as_float(raw[i].y & 0xFFFF0000u));
+    for (int i = 0; i < kUnit / THREADS; i++) sc[tid + i * THREADS] = raw[i];
     __syncthreads();
 
+    const int warps = max(1, min(kAttendWarps, (here + kTile - 1) / kTile));   // that have a tile
+    constexpr int LD = D + 4;
+    float *so = reinterpret_cast<float *>(smem);   // [warp][row][LD], over the codes once all are read
+    static_assert(kAttendWarps * R * LD * 4 <= L::kScales, "the warps' sums fit where the codes were");
     // scores of this CTA's rows from entry j0 on, kept for the weights
     float *score = TRACK ? p.score + (((int64_t)b * p.c.n_heads + h) * p.rows + rb * R) * p.max_len + j0 : nullptr;
+    const int rows_here = min(R, p.rows - rb * R);
     // kExact: what the fp16 weights lost is made good at the middle of the codes, so their
     // rounding counts from there (a third) and not from code 0; bf16 results do not need it
     constexpr bool kExact = DType<T>::kCode == CZG_F16;
@@ -365,205 +382,227 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
 #pragma unroll
             for (int i = 0; i < 8; i++) o[nb][ch][i >> 2][i & 3] = 0.0f;
     }
-    int least = kUnit;   // what every row of the CTA sees at least
+    if (warp < warps) {
+        uint4 qf[NB][CH];
+        float qs[NB][2], zq[NB][2];   // of rows 2 c4, 2 c4 + 1
+        int seen[NB][2], least = kUnit;   // entries of this unit that the row sees; what all rows see at least
 #pragma unroll
-    for (int nb = 0; nb < NB; nb++) least = min(least, min(seen[nb][0], seen[nb][1]));
-    least = __reduce_min_sync(0xffffffffu, least);
-
-    // ldmatrix: lane i gives the address of row i % 8 of matrix i / 8; matrices are
-    // (entries 0-7, 8-15) x (two chunks)
-    const int lm_row = (lane & 7) + (lane & 8), lm_ch = lane >> 4;
-    const uint32_t swz = D == 64 ? (uint32_t)(lm_row >> 2 & 1) : (uint32_t)(lm_row >> 1 & 3);
-#pragma unroll 1
-    for (int it = 0; it < 2; it++) {
-        const int tile = it * kAttendWarps + warp, t0 = tile * kTile;
-        if (t0 >= here) break;
-        if (!mbar_wait(&bar[tile], 0, nullptr)) {
-            atomicOr(&g_ops_timeout, 1);
-            mbar_wait(&bar[tile], 0, nullptr);   // once more for the copies, before anything ends
-        }
-        __syncwarp();
-        const uint32_t ka = smem_addr(smem) + (uint32_t)(t0 + lm_row) * (D / 2), va = ka + L::kCodes;
-        float s[NB][4][4];
+        for (int nb = 0; nb < NB; nb++) {
 #pragma unroll
-        for (int kb = 0; kb < 4; kb++) {
+            for (int ch = 0; ch < CH; ch++) qf[nb][ch] = s_q[(nb * CH + ch) * 32 + lane];
 #pragma unroll
-            for (int nb = 0; nb < NB; nb++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) s[nb][kb][i] = 0.0f;
-#pragma unroll
-            for (int cp = 0; cp < CH; cp += 2) {
-                uint32_t w[4];
-                ldsm4(w, ka + kb * 16 * (D / 2) + (((uint32_t)(cp + lm_ch) ^ swz) << 4));
-#pragma unroll
-                for (int ci = 0; ci < 2; ci++) {
-                    const uint32_t a = w[2 * ci], c = w[2 * ci + 1], a8 = a >> 8, c8 = c >> 8;
-#pragma unroll
-                    for (int nb = 0; nb < NB; nb++) {
-                        mma_f16(s[nb][kb], a & 0x000F000Fu, c & 0x000F000Fu, a & 0x00F000F0u, c & 0x00F000F0u, qf[nb][cp + ci][0], qf[nb][cp + ci][1]);
-                        mma_f16(s[nb][kb], a8 & 0x000F000Fu, c8 & 0x000F000Fu, a8 & 0x00F000F0u, c8 & 0x00F000F0u, qf[nb][cp + ci][2], qf[nb][cp + ci][3]);
-                    }
-                }
+            for (int i = 0; i < 2; i++) {
+                const int r = nb * 8 + 2 * c4 + i;
+                qs[nb][i] = s_qs[r].x;
+                zq[nb][i] = s_qs[r].y;
+                seen[nb][i] = r < rows_here ? here : 0x7FFFFFFF;
+                if (p.t > 1 && r < rows_here) seen[nb][i] = n - (p.t - 1 - row_place(p, rb * R + r)) - j0;
+                least = min(least, seen[nb][i]);
             }
         }
-        float mt[NB][2];
+        least = __reduce_min_sync(0xffffffffu, least);
+        // ldmatrix: lane i gives the address of row i % 8 of matrix i / 8; matrices are
+        // (entries 0-7, 8-15) x (two chunks)
+        const int lm_row = (lane & 7) + (lane & 8), lm_ch = lane >> 4;
+        const uint32_t swz = D == 64 ? (uint32_t)(lm_row >> 2 & 1) : (uint32_t)(lm_row >> 1 & 3);
+
+        auto tile_of = [&](int it, auto cut_of) {
+            constexpr bool CUT = decltype(cut_of)::value;   // some row does not see some of the tile's entries
+            const int t0 = (it * kAttendWarps + warp) * kTile;
+            const uint32_t ka = smem_addr(ring + (it % kRing) * 2 * L::kTileCodes) + (uint32_t)lm_row * (D / 2), va = ka + L::kTileCodes;
+            float s[NB][4][4];
 #pragma unroll
-        for (int nb = 0; nb < NB; nb++) mt[nb][0] = mt[nb][1] = -INFINITY;
-        const bool cut = t0 + kTile > least;
-#pragma unroll
-        for (int kb = 0; kb < 4; kb++)
-#pragma unroll
-            for (int hf = 0; hf < 2; hf++) {
-                const int j = t0 + kb * 16 + hf * 8 + g8;
-                const float2 kr = *reinterpret_cast<const float2 *>(&sc[j]);
+            for (int kb = 0; kb < 4; kb++) {
 #pragma unroll
                 for (int nb = 0; nb < NB; nb++)
 #pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        float x = __fmaf_rn(kr.x, s[nb][kb][2 * hf + i] * qscale[nb][i], kr.y * qsum[nb][i]);
-                        if (cut && j >= seen[nb][i]) x = -INFINITY;
-                        s[nb][kb][2 * hf + i] = x;
-                        mt[nb][i] = fmaxf(mt[nb][i], x);
-                        if (TRACK && rb * R + nb * 8 + 2 * c4 + i < p.rows && j < here)
-                            score[(int64_t)(nb * 8 + 2 * c4 + i) * p.max_len + j] = x;
+                    for (int i = 0; i < 4; i++) s[nb][kb][i] = 0.0f;
+#pragma unroll
+                for (int cp = 0; cp < CH; cp += 2) {
+                    uint32_t w[4];
+                    ldsm4(w, ka + kb * 16 * (D / 2) + (((uint32_t)(cp + lm_ch) ^ swz) << 4));
+#pragma unroll
+                    for (int ci = 0; ci < 2; ci++) {
+                        const uint32_t a = w[2 * ci], c = w[2 * ci + 1], a8 = a >> 8, c8 = c >> 8;
+#pragma unroll
+                        for (int nb = 0; nb < NB; nb++) {
+                            mma_f16(s[nb][kb], a & 0x000F000Fu, c & 0x000F000Fu, a & 0x00F000F0u, c & 0x00F000F0u, qf[nb][cp + ci].x, qf[nb][cp + ci].y);
+                            mma_f16(s[nb][kb], a8 & 0x000F000Fu, c8 & 0x000F000Fu, a8 & 0x00F000F0u, c8 & 0x00F000F0u, qf[nb][cp + ci].z, qf[nb][cp + ci].w);
+                        }
                     }
+                }
             }
+            // scores over the row's factor, their maximum
+            float mt[NB][2];
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++) mt[nb][0] = mt[nb][1] = -INFINITY;
+#pragma unroll
+            for (int kb = 0; kb < 4; kb++)
+#pragma unroll
+                for (int hf = 0; hf < 2; hf++) {
+                    const int j = t0 + kb * 16 + hf * 8 + g8;
+                    const uint32_t kw = sc[j].x;
+                    const float2 kr = make_float2(__uint_as_float(kw << 16), __uint_as_float(kw & 0xFFFF0000u));
+#pragma unroll
+                    for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                        for (int i = 0; i < 2; i++) {
+                            const float x = __fmaf_rn(kr.x, s[nb][kb][2 * hf + i], kr.y * zq[nb][i]);
+                            const bool off = CUT && j >= seen[nb][i];
+                            s[nb][kb][2 * hf + i] = x;
+                            mt[nb][i] = off ? mt[nb][i] : fmaxf(mt[nb][i], x);
+                            if (TRACK && nb * 8 + 2 * c4 + i < rows_here && (!CUT || j < here))
+                                score[(int64_t)(nb * 8 + 2 * c4 + i) * p.max_len + j] = off ? -INFINITY : x * qs[nb][i];
+                        }
+                }
+            float mq[NB][2];   // the maximum times the factor, less `up`
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+#pragma unroll
+                    for (int x = 4; x < 32; x <<= 1) mt[nb][i] = fmaxf(mt[nb][i], __shfl_xor_sync(0xffffffffu, mt[nb][i], x));
+                    const float was = m[nb][i], now = fmaxf(was, mt[nb][i]);
+                    m[nb][i] = now;
+                    mq[nb][i] = now == -INFINITY ? 0.0f : __fmaf_rn(now, qs[nb][i], -(float)up);
+                    if (it > 0) {
+                        const float f = was == now ? 1.0f : was == -INFINITY ? 0.0f : ex2((was - now) * qs[nb][i]);
+                        l[nb][i] *= f;
+                        z[nb][i] *= f;
+                        if (kExact) lost[nb][i] *= f;
+#pragma unroll
+                        for (int ch = 0; ch < CH; ch++)
+#pragma unroll
+                            for (int y = 0; y < 2; y++) {
+                                o[nb][ch][y][i] *= f;
+                                o[nb][ch][y][2 + i] *= f;
+                            }
+                    }
+                }
+#pragma unroll
+            for (int kb = 0; kb < 4; kb++) {
+                uint32_t pf[NB][2];
+#pragma unroll
+                for (int hf = 0; hf < 2; hf++) {
+                    const int j = t0 + kb * 16 + hf * 8 + g8;
+                    const uint32_t vw = sc[j].y;
+                    const float2 vr = make_float2(__uint_as_float(vw << 16), __uint_as_float(vw & 0xFFFF0000u));
+#pragma unroll
+                    for (int nb = 0; nb < NB; nb++) {
+                        float w[2];
+#pragma unroll
+                        for (int i = 0; i < 2; i++) {
+                            const bool off = CUT && j >= seen[nb][i];   // what is not seen may be anything
+                            const float e = off ? 0.0f : ex2(__fmaf_rn(s[nb][kb][2 * hf + i], qs[nb][i], -mq[nb][i]));
+                            l[nb][i] += e;
+                            z[nb][i] = off ? z[nb][i] : __fmaf_rn(e, vr.y, z[nb][i]);
+                            w[i] = off ? 0.0f : e * vr.x;
+                        }
+                        const uint32_t wp = pack_half(w[0], w[1]);
+                        if (kExact) {
+                            const float2 back = __half22float2(*reinterpret_cast<const __half2 *>(&wp));
+                            lost[nb][0] += w[0] - back.x;
+                            lost[nb][1] += w[1] - back.y;
+                        }
+                        pf[nb][hf] = transpose8(wp);
+                    }
+                }
+#pragma unroll
+                for (int cp = 0; cp < CH; cp += 2) {
+                    uint32_t w[4];
+                    ldsm4_trans(w, va + kb * 16 * (D / 2) + (((uint32_t)(cp + lm_ch) ^ swz) << 4));
+#pragma unroll
+                    for (int ci = 0; ci < 2; ci++) {
+                        const uint32_t a = w[2 * ci], c = w[2 * ci + 1], a8 = a >> 8, c8 = c >> 8;
+#pragma unroll
+                        for (int nb = 0; nb < NB; nb++) {
+                            mma_f16(o[nb][cp + ci][0], a & 0x000F000Fu, a & 0x00F000F0u, c & 0x000F000Fu, c & 0x00F000F0u, pf[nb][0], pf[nb][1]);
+                            mma_f16(o[nb][cp + ci][1], a8 & 0x000F000Fu, a8 & 0x00F000F0u, c8 & 0x000F000Fu, c8 & 0x00F000F0u, pf[nb][0], pf[nb][1]);
+                        }
+                    }
+                }
+            }
+        };
+#pragma unroll 1
+        for (int it = 0; it < turns; it++) {
+            if (!mbar_wait(&ring_bar[it % kRing], (it / kRing) & 1, nullptr)) {
+                atomicOr(&g_ops_timeout, 1);
+                mbar_wait(&ring_bar[it % kRing], (it / kRing) & 1, nullptr);   // once more for the copies, before anything ends
+            }
+            __syncwarp();
+            if ((it * kAttendWarps + warp + 1) * kTile > least) tile_of(it, std::true_type{}); else tile_of(it, std::false_type{});
+            __syncwarp();   // all lanes have read the tile
+            if (lane == 0 && it + kRing < turns) ask(it + kRing);
+        }
+        // sums over the lanes that share a row
 #pragma unroll
         for (int nb = 0; nb < NB; nb++)
 #pragma unroll
             for (int i = 0; i < 2; i++) {
 #pragma unroll
-                for (int x = 4; x < 32; x <<= 1) mt[nb][i] = fmaxf(mt[nb][i], __shfl_xor_sync(0xffffffffu, mt[nb][i], x));
-                const float now = fmaxf(m[nb][i], mt[nb][i]);
-                const float f = share(m[nb][i], now);
-                m[nb][i] = now;
-                mt[nb][i] = now == -INFINITY ? 0.0f : now;   // what scores are taken from
-                if (it > 0) {
-                    l[nb][i] *= f;
-                    z[nb][i] *= f;
-                    lost[nb][i] *= f;
-#pragma unroll
-                    for (int ch = 0; ch < CH; ch++)
-#pragma unroll
-                        for (int y = 0; y < 2; y++) {
-                            o[nb][ch][y][i] *= f;
-                            o[nb][ch][y][2 + i] *= f;
-                        }
+                for (int x = 4; x < 32; x <<= 1) {
+                    l[nb][i] += __shfl_xor_sync(0xffffffffu, l[nb][i], x);
+                    z[nb][i] += __shfl_xor_sync(0xffffffffu, z[nb][i], x);
+                    if (kExact) lost[nb][i] += __shfl_xor_sync(0xffffffffu, lost[nb][i], x);
+                }
+                l[nb][i] *= pow2f(-up);
+                z[nb][i] = __fmaf_rn(lost[nb][i], 7.5f, z[nb][i]) * pow2f(-up);
+                m[nb][i] = m[nb][i] == -INFINITY ? -INFINITY : m[nb][i] * qs[nb][i];
+                if (g8 == 0) {
+                    s_m[warp][nb * 8 + 2 * c4 + i] = m[nb][i];
+                    s_l[warp][nb * 8 + 2 * c4 + i] = l[nb][i];
                 }
             }
-#pragma unroll
-        for (int kb = 0; kb < 4; kb++) {
-            uint32_t pf[NB][2];
-#pragma unroll
-            for (int hf = 0; hf < 2; hf++) {
-                const int j = t0 + kb * 16 + hf * 8 + g8;
-                const float2 vr = *(reinterpret_cast<const float2 *>(&sc[j]) + 1);
-#pragma unroll
-                for (int nb = 0; nb < NB; nb++) {
-                    float w[2];
-#pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        const float e = ex2(s[nb][kb][2 * hf + i] - mt[nb][i]);
-                        const bool off = cut && j >= seen[nb][i];   // a value that is not seen may be anything
-                        l[nb][i] += e;
-                        z[nb][i] = off ? z[nb][i] : __fmaf_rn(e, vr.y, z[nb][i]);
-                        w[i] = off ? 0.0f : e * vr.x;
-                    }
-                    const uint32_t wp = pack_half(w[0], w[1]);
-                    if (kExact) {
-                        const float2 back = __half22float2(*reinterpret_cast<const __half2 *>(&wp));
-                        lost[nb][0] += w[0] - back.x;
-                        lost[nb][1] += w[1] - back.y;
-                    }
-                    pf[nb][hf] = transpose8(wp);
-                }
-            }
-#pragma unroll
-            for (int cp = 0; cp < CH; cp += 2) {
-                uint32_t w[4];
-                ldsm4_trans(w, va + kb * 16 * (D / 2) + (((uint32_t)(cp + lm_ch) ^ swz) << 4));
-#pragma unroll
-                for (int ci = 0; ci < 2; ci++) {
-                    const uint32_t a = w[2 * ci], c = w[2 * ci + 1], a8 = a >> 8, c8 = c >> 8;
-#pragma unroll
-                    for (int nb = 0; nb < NB; nb++) {
-                        mma_f16(o[nb][cp + ci][0], a & 0x000F000Fu, a & 0x00F000F0u, c & 0x000F000Fu, c & 0x00F000F0u, pf[nb][0], pf[nb][1]);
-                        mma_f16(o[nb][cp + ci][1], a8 & 0x000F000Fu, a8 & 0x00F000F0u, c8 & 0x000F000Fu, c8 & 0x00F000F0u, pf[nb][0], pf[nb][1]);
-                    }
-                }
-            }
-        }
     }
-
-    // the four warps' rows together, in their order
-#pragma unroll
-    for (int nb = 0; nb < NB; nb++)
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-#pragma unroll
-            for (int x = 4; x < 32; x <<= 1) {
-                l[nb][i] += __shfl_xor_sync(0xffffffffu, l[nb][i], x);
-                z[nb][i] += __shfl_xor_sync(0xffffffffu, z[nb][i], x);
-                if (kExact) lost[nb][i] += __shfl_xor_sync(0xffffffffu, lost[nb][i], x);
-            }
-            // vdown is 2^15 / 2^te
-            if (kExact) z[nb][i] = __fmaf_rn(lost[nb][i] * (7.5f / 32768.0f), ldexpf(1.0f, te), z[nb][i]);
-            if (g8 == 0) {
-                const int r = nb * 8 + 2 * c4 + i;
-                s_m[warp][r] = m[nb][i];
-                s_l[warp][r] = l[nb][i];
-            }
-        }
-    __syncthreads();   // and all codes are read: their place is free for the sums
+    // the warps' rows together, in their order
+    __syncthreads();
     if (tid < R) {
-        const float top_m = fmaxf(fmaxf(s_m[0][tid], s_m[1][tid]), fmaxf(s_m[2][tid], s_m[3][tid]));
-        float sum = 0.0f;
-        for (int w = 0; w < kAttendWarps; w++) sum += s_l[w][tid] * share(s_m[w][tid], top_m);
+        float top_m = s_m[0][tid], sum = 0.0f;
+        for (int w = 1; w < warps; w++) top_m = fmaxf(top_m, s_m[w][tid]);
+        for (int w = 0; w < warps; w++) sum += s_l[w][tid] * share(s_m[w][tid], top_m);
         s_row[tid] = make_float2(top_m, sum);
     }
-    constexpr int LD = D + 4;
-    float *so = reinterpret_cast<float *>(smem);   // [warp][row][LD]
-    static_assert(kAttendWarps * R * LD * 4 <= 2 * L::kCodes, "the warps' sums fit where the codes were");
-    const float vup = ldexpf(1.0f, te);   // and 2^(24 - 15) for the nibbles and vdown
+    if (warp < warps) {
+        const float down = pow2f(-up);
 #pragma unroll
-    for (int nb = 0; nb < NB; nb++)
+        for (int nb = 0; nb < NB; nb++)
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const int r = nb * 8 + 2 * c4 + i;
-            const float f = share(m[nb][i], fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r])));
-            const float zz = z[nb][i];
+            for (int i = 0; i < 2; i++) {
+                const int r = nb * 8 + 2 * c4 + i;
+                float top_m = s_m[0][r];
+                for (int w = 1; w < warps; w++) top_m = fmaxf(top_m, s_m[w][r]);
+                const float f = share(m[nb][i], top_m), zz = z[nb][i] * f, even = down * f, odd = even * 0.0625f;
 #pragma unroll
-            for (int ch = 0; ch < CH; ch++)
+                for (int ch = 0; ch < CH; ch++)
 #pragma unroll
-                for (int y = 0; y < 2; y++)   // dimensions 32 ch + 4 g8 + 2 y and the next
-                    *reinterpret_cast<float2 *>(&so[(warp * R + r) * LD + ch * 32 + 4 * g8 + 2 * y]) =
-                        make_float2(f * __fmaf_rn(o[nb][ch][y][i] * 512.0f, vup, zz), f * __fmaf_rn(o[nb][ch][y][2 + i] * 32.0f, vup, zz));
-        }
+                    for (int y = 0; y < 2; y++)   // dimensions 32 ch + 4 g8 + 2 y and the next
+                        *reinterpret_cast<float2 *>(&so[(warp * R + r) * LD + ch * 32 + 4 * g8 + 2 * y]) =
+                            make_float2(__fmaf_rn(o[nb][ch][y][i] * 16777216.0f, even, zz), __fmaf_rn(o[nb][ch][y][2 + i] * 16777216.0f, odd, zz));
+            }
+    }
     __syncthreads();
-    const int rows_here = min(R, p.rows - rb * R);
     const bool whole = p.whole;   // nothing to join: this is the result
     const int64_t at = whole ? 0 : (((int64_t)b * p.c.n_heads + h) * p.units + unit) * ((int64_t)p.row_blocks * R) + rb * R;
-    for (int i = tid; i < rows_here * (D / 2); i += kAttendWarps * 32) {
-        const int r = i / (D / 2), d = 2 * (i % (D / 2));
+    for (int i = tid; i < rows_here * (D / 4); i += THREADS) {
+        const int r = i / (D / 4), d = 4 * (i % (D / 4));
         const float2 row = s_row[r];
-        float x = 0.0f, y = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kAttendWarps; w++) {
-            const float2 v = *reinterpret_cast<const float2 *>(&so[(w * R + r) * LD + d]);
-            x += v.x;
-            y += v.y;
+        float4 x = *reinterpret_cast<const float4 *>(&so[r * LD + d]);
+        for (int w = 1; w < warps; w++) {
+            const float4 v = *reinterpret_cast<const float4 *>(&so[(w * R + r) * LD + d]);
+            x.x += v.x;
+            x.y += v.y;
+            x.z += v.z;
+            x.w += v.w;
         }
         if (whole) {
-            T *dst = static_cast<T *>(p.out) + row_offset(p, p.os, b, h, rb * R + r) + d;
-            dst[0] = from_f32<T>(row.y == 0.0f ? 0.0f : x / row.y);   // a row that sees nothing: 0
-            dst[1] = from_f32<T>(row.y == 0.0f ? 0.0f : y / row.y);
+            store4(static_cast<T *>(p.out) + s_out[r] + d, x, row.y == 0.0f ? 0.0f : 1.0f / row.y, p.out_vec);   // a row that sees nothing: 0
         } else {
-            *reinterpret_cast<float2 *>(p.part + (at + r) * D + d) = make_float2(x, y);
+            *reinterpret_cast<float4 *>(p.part + (at + r) * D + d) = x;
             if (d == 0) p.stat[at + r] = row;
         }
     }
     if (TRACK && whole)   // the scores that this CTA wrote
-        for (int j = tid; j < here; j += kAttendWarps * 32) {
+        for (int j = tid; j < here; j += THREADS) {
             float add = 0.0f;
             for (int r = 0; r < rows_here; r++) {
                 const float2 row = s_row[r];
@@ -573,59 +612,73 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
         }
 }
 
-// Joins the units of a row: the first `rows` CTAs of x write the rows' results, the
-// others the weights of kUnit entries each.  A row's units are taken in 8 interleaved
-// runs and those in order: places that depend on its length alone.
-constexpr int kJoinThreads = 256;
+// Joins the units of rows: the first `rows` CTAs of x write the rows' results, the others
+// the weights of kUnit entries each.  A row's units are taken in RUNS interleaved runs and
+// those in order: places that depend on its length alone.  Up to kFew units make one run,
+// and the first CTA takes all rows of them.
+constexpr int kJoinThreads = 256, kFew = 16, kMany = 1024;
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads) k_kv4_join(const __grid_constant__ AttendArgs p, int rows_padded) {
     pdl_wait();
-    constexpr int RUNS = kJoinThreads / (D / 2);   // D / 2 threads a run, two dimensions each
-    __shared__ float red[kJoinThreads / 32];
-    __shared__ float2 runs[RUNS][D / 2];
+    constexpr int TR = D / 4, RUNS = kJoinThreads / TR;   // TR threads a run, four dimensions each
     const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
     const int slot = kv4_slot(p.c, p.slots, b, false);
     const int n = slot < 0 ? 0 : kv4_length(p.c, p.lengths, b, min(p.max_len, p.c.capacity), false);
     const int units = (n + kUnit - 1) / kUnit;
     const int64_t first = ((int64_t)b * p.c.n_heads + h) * p.units * rows_padded;
-    // the maximum of row r over the units
-    auto top_of = [&](int r) {
+    if ((int)blockIdx.x < p.rows) {
+        const int d = 4 * (tid % TR), run = tid / TR;
+        if (units <= kFew) {
+            if (blockIdx.x > 0) return;
+            for (int r = run; r < p.rows; r += RUNS) {
+                float m = -INFINITY, l = 0.0f;
+                float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                for (int u = 0; u < units; u++) m = fmaxf(m, p.stat[first + (int64_t)u * rows_padded + r].x);
+#pragma unroll 4
+                for (int u = 0; u < units; u++) {
+                    const int64_t at = first + (int64_t)u * rows_padded + r;
+                    const float2 st = p.stat[at];
+                    add_scaled(x, share(st.x, m), *reinterpret_cast<const float4 *>(p.part + at * D + d));
+                    l = __fmaf_rn(share(st.x, m), st.y, l);
+                }
+                store4(static_cast<T *>(p.out) + row_offset(p, p.os, b, h, r) + d, x, l == 0.0f ? 0.0f : 1.0f / l, p.out_vec);
+            }
+            return;
+        }
+        __shared__ float s_f[kMany], red[kJoinThreads / 32];
+        __shared__ float4 runs[RUNS][TR];
+        const int r = blockIdx.x;
         float m = -INFINITY;
         for (int u = tid; u < units; u += kJoinThreads) m = fmaxf(m, p.stat[first + (int64_t)u * rows_padded + r].x);
         for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        __syncthreads();
         if ((tid & 31) == 0) red[tid >> 5] = m;
         __syncthreads();
-        m = red[0];
-        for (int w = 1; w < kJoinThreads / 32; w++) m = fmaxf(m, red[w]);
-        return m;
-    };
-    if ((int)blockIdx.x < p.rows) {
-        const int r = blockIdx.x, d = tid % (D / 2), run = tid / (D / 2);
-        const float m = top_of(r);
-        float x = 0.0f, y = 0.0f, l = 0.0f;
-        for (int u = run; u < units; u += RUNS) {
-            const int64_t at = first + (int64_t)u * rows_padded + r;
-            const float2 st = p.stat[at];
-            const float2 v = *reinterpret_cast<const float2 *>(p.part + at * D + 2 * d);
-            const float f = share(st.x, m);
-            x = __fmaf_rn(f, v.x, x);
-            y = __fmaf_rn(f, v.y, y);
-            l = __fmaf_rn(f, st.y, l);
+        for (int w = 0; w < kJoinThreads / 32; w++) m = fmaxf(m, red[w]);
+        float l = 0.0f;
+        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int u0 = 0; u0 < units; u0 += kMany) {
+            const int some = min(kMany, units - u0);
+            __syncthreads();
+            for (int u = tid; u < some; u += kJoinThreads) {
+                const float2 st = p.stat[first + (int64_t)(u0 + u) * rows_padded + r];
+                s_f[u] = share(st.x, m);
+                l = __fmaf_rn(s_f[u], st.y, l);
+            }
+            __syncthreads();
+#pragma unroll 8
+            for (int u = run; u < some; u += RUNS)
+                add_scaled(x, s_f[u], *reinterpret_cast<const float4 *>(p.part + (first + (int64_t)(u0 + u) * rows_padded + r) * D + d));
         }
-        __shared__ float run_l[RUNS];
-        runs[run][d] = make_float2(x, y);
-        if (d == 0) run_l[run] = l;
+        runs[run][tid % TR] = x;
+        for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        __syncthreads();
+        if ((tid & 31) == 0) red[tid >> 5] = l;
         __syncthreads();
         if (run > 0) return;
-        for (int i = 1; i < RUNS; i++) {
-            x += runs[i][d].x;
-            y += runs[i][d].y;
-            l += run_l[i];
-        }
-        T *dst = static_cast<T *>(p.out) + row_offset(p, p.os, b, h, r) + 2 * d;
-        dst[0] = from_f32<T>(l == 0.0f ? 0.0f : x / l);
-        dst[1] = from_f32<T>(l == 0.0f ? 0.0f : y / l);
+        l = 0.0f;
+        for (int w = 0; w < kJoinThreads / 32; w++) l += red[w];
+        for (int i = 1; i < RUNS; i++) add_scaled(x, 1.0f, runs[i][tid]);
+        store4(static_cast<T *>(p.out) + row_offset(p, p.os, b, h, r) + d, x, l == 0.0f ? 0.0f : 1.0f / l, p.out_vec);
         return;
     }
     // weights of kUnit entries: a warp a row for its maximum and sum, then a thread two entries
@@ -852,6 +905,7 @@ extern "C" int czg_kv4_attend(const czg_kv4 *cache, const void *q, int64_t q_sb,
     p.max_len = max_len;
     p.units = plan.units;
     p.vec = aligned(q, 16) && (q_sb * es) % 16 == 0 && (q_st * es) % 16 == 0 && (q_sh * es) % 16 == 0;
+    p.out_vec = aligned(out, 8) && o_sb % 4 == 0 && o_st % 4 == 0 && o_sh % 4 == 0;
     p.scale_log2 = (float)((double)scale * 1.4426950408889634);
     p.out = out;
     p.os = {o_sb, o_st, o_sh};
