@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(256) k_kv4_read(czg_kv4 c, const int32_t *__re
 //
 // A CTA takes one unit of a sequence's entries (kUnit, at a fixed place whatever the
 // batch), one key head and up to 8 NB rows (query heads of that key head, times the
-// call's rows).  Its two warps take tiles of 64 entries in turn, each through a ring of
+// call's rows).  Its two warps take tiles of kTile entries in turn, each through a ring of
 // its own that TMA fills (swizzled for ldmatrix); many such small CTAs share an SM and
 // cover one another's beginnings and ends.
 //
@@ -156,13 +156,12 @@ __global__ void __launch_bounds__(256) k_kv4_read(czg_kv4 c, const int32_t *__re
 // With x = lo + step c:  s_j = step_j (q.c_j) + lo_j sum(q);  out = sum p_j step_j c_j + sum p_j lo_j.
 // The query is held in fp16 after a power of two that brings its largest value to
 // [2^13, 2^14): exact but for values below 2^-23 of the largest.  p_j step_j is
-// held in fp16 likewise (2^15 for the unit's largest step): off by 2^-12 of itself, against
-// 2^-9 of the result for bf16 and 2^-12 for fp16; its range is 2^39 wide.  Scores, maxima and
+// held in fp16 likewise (2^7 to 2^15 for the unit's largest): off by 2^-12 of itself, against
+// 2^-9 of the result for bf16 and 2^-12 for fp16; its range is 2^31 wide.  Scores, maxima and
 // sums are fp32; exponentials are ex2.approx (2^-22).
 // Between the warps of a CTA, and between units (k_kv4_join), partial results are joined
 // in a fixed order, so a row's bits do not depend on the batch or the grid.
 constexpr int kUnit = 512, kTile = 64, kAttendWarps = 2, kRing = 2;
-constexpr int kTurns = kUnit / (kTile * kAttendWarps);   // tiles of a warp
 
 struct AttendArgs {
     czg_kv4 c;
@@ -206,19 +205,19 @@ __device__ __forceinline__ void store4(T *dst, float4 x, float f, bool vec) {
 __device__ __forceinline__ float share(float m, float top) { return m == top ? 1.0f : ex2(m - top); }
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
 }
 __device__ __forceinline__ void ldsm4_trans(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
 }
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     uint32_t y;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
@@ -231,6 +230,14 @@ __device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, u
         ::"r"(smem_addr(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar)) : "memory");
 }
 
+__device__ __forceinline__ bool mbar_try(uint64_t *bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done) : "r"(smem_addr(bar)), "r"(parity) : "memory");
+    return done != 0;
+}
+
 // Row r of a sequence and key head: place i = r / g of the call's rows, query head h g + r % g.
 __device__ __forceinline__ int row_place(const AttendArgs &p, int r) { return (int)((uint64_t)(uint32_t)r * p.g_inv >> 32); }
 __device__ __forceinline__ int64_t row_offset(const AttendArgs &p, const Strides &s, int b, int h, int r) {
@@ -240,6 +247,9 @@ __device__ __forceinline__ int64_t row_offset(const AttendArgs &p, const Strides
 
 __device__ __forceinline__ float pow2f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }   // -126 <= e <= 127
 
+// CTAs an SM is to hold: what the sums (D NB / 4 registers), query and scores leave room for
+constexpr int attend_ctas(int d, int nb) { return d == 64 ? (nb == 1 ? 8 : 5) : (nb == 1 ? 6 : 4); }
+
 template <int D>
 struct AttendSmem {
     static constexpr int kTileCodes = kTile * D / 2;   // of keys, and as many of values behind them
@@ -248,7 +258,7 @@ struct AttendSmem {
 };
 
 template <typename T, int D, int NB, bool TRACK>
-__global__ void __launch_bounds__(kAttendWarps * 32)
+__global__ void __launch_bounds__(kAttendWarps * 32, attend_ctas(D, NB))
 k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttendArgs p) {
     using L = AttendSmem<D>;
     constexpr int CH = D / 32;      // 16-byte chunks of a row of codes
@@ -353,16 +363,16 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
     top = s_top[0];
     for (int w = 1; w < kAttendWarps; w++) top = max(top, s_top[w]);
     // 2^te is not below any value's step (where 2^-100 is not above all); weights are
-    // taken 2^up-fold, which brings weight times step below 2^15
-    const int te = top == 0 ? 0 : max((int)(top >> 23) - 126, -100), up = 15 - te;
+    // taken 2^up-fold, which brings weight times step, for weights up to 2^8, below 2^15
+    const int te = top == 0 ? 0 : max((int)(top >> 23) - 126, -100), up = 7 - te;
 #pragma unroll
     for (int i = 0; i < kUnit / THREADS; i++) sc[tid + i * THREADS] = raw[i];
     __syncthreads();
 
     const int warps = max(1, min(kAttendWarps, (here + kTile - 1) / kTile));   // that have a tile
     constexpr int LD = D + 4;
-    float *so = reinterpret_cast<float *>(smem);   // [warp][row][LD], over the codes once all are read
-    static_assert(kAttendWarps * R * LD * 4 <= L::kScales, "the warps' sums fit where the codes were");
+    float *so = reinterpret_cast<float *>(smem);   // [warp][row][LD], over codes and ranges once all are read
+    static_assert(kAttendWarps * R * LD * 4 <= L::kBars, "the warps' sums fit where the codes were");
     // scores of this CTA's rows from entry j0 on, kept for the weights
     float *score = TRACK ? p.score + (((int64_t)b * p.c.n_heads + h) * p.rows + rb * R) * p.max_len + j0 : nullptr;
     const int rows_here = min(R, p.rows - rb * R);
@@ -406,38 +416,38 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
         const int lm_row = (lane & 7) + (lane & 8), lm_ch = lane >> 4;
         const uint32_t swz = D == 64 ? (uint32_t)(lm_row >> 2 & 1) : (uint32_t)(lm_row >> 1 & 3);
 
+        float mq[NB][2];   // reference times factor, less `up`
         auto tile_of = [&](int it, auto cut_of) {
             constexpr bool CUT = decltype(cut_of)::value;   // some row does not see some of the tile's entries
             const int t0 = (it * kAttendWarps + warp) * kTile;
             const uint32_t ka = smem_addr(ring + (it % kRing) * 2 * L::kTileCodes) + (uint32_t)lm_row * (D / 2), va = ka + L::kTileCodes;
-            float s[NB][4][4];
+            constexpr int KB = kTile / 16;
+            float s[NB][KB][4];
 #pragma unroll
-            for (int kb = 0; kb < 4; kb++) {
+            for (int i = 0; i < NB * KB * 4; i++) s[i / (KB * 4)][i / 4 % KB][i % 4] = 0.0f;
+            // entries inside, so that neighbouring MMAs add to different sums
 #pragma unroll
-                for (int nb = 0; nb < NB; nb++)
+            for (int cp = 0; cp < CH; cp += 2) {
+                uint32_t w[KB][4];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) s[nb][kb][i] = 0.0f;
+                for (int kb = 0; kb < KB; kb++) ldsm4(w[kb], ka + kb * 16 * (D / 2) + (((uint32_t)(cp + lm_ch) ^ swz) << 4));
 #pragma unroll
-                for (int cp = 0; cp < CH; cp += 2) {
-                    uint32_t w[4];
-                    ldsm4(w, ka + kb * 16 * (D / 2) + (((uint32_t)(cp + lm_ch) ^ swz) << 4));
+                for (int ci = 0; ci < 2; ci++)
 #pragma unroll
-                    for (int ci = 0; ci < 2; ci++) {
-                        const uint32_t a = w[2 * ci], c = w[2 * ci + 1], a8 = a >> 8, c8 = c >> 8;
+                    for (int half = 0; half < 2; half++)
 #pragma unroll
-                        for (int nb = 0; nb < NB; nb++) {
-                            mma_f16(s[nb][kb], a & 0x000F000Fu, c & 0x000F000Fu, a & 0x00F000F0u, c & 0x00F000F0u, qf[nb][cp + ci].x, qf[nb][cp + ci].y);
-                            mma_f16(s[nb][kb], a8 & 0x000F000Fu, c8 & 0x000F000Fu, a8 & 0x00F000F0u, c8 & 0x00F000F0u, qf[nb][cp + ci].z, qf[nb][cp + ci].w);
+                        for (int kb = 0; kb < KB; kb++) {
+                            const uint32_t a = w[kb][2 * ci] >> (8 * half), c = w[kb][2 * ci + 1] >> (8 * half);
+#pragma unroll
+                            for (int nb = 0; nb < NB; nb++) {
+                                const uint4 &f = qf[nb][cp + ci];
+                                mma_f16(s[nb][kb], a & 0x000F000Fu, c & 0x000F000Fu, a & 0x00F000F0u, c & 0x00F000F0u, half ? f.z : f.x, half ? f.w : f.y);
+                            }
                         }
-                    }
-                }
             }
-            // scores over the row's factor, their maximum
-            float mt[NB][2];
+            // scores over the row's factor
 #pragma unroll
-            for (int nb = 0; nb < NB; nb++) mt[nb][0] = mt[nb][1] = -INFINITY;
-#pragma unroll
-            for (int kb = 0; kb < 4; kb++)
+            for (int kb = 0; kb < KB; kb++)
 #pragma unroll
                 for (int hf = 0; hf < 2; hf++) {
                     const int j = t0 + kb * 16 + hf * 8 + g8;
@@ -447,40 +457,59 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
                     for (int nb = 0; nb < NB; nb++)
 #pragma unroll
                         for (int i = 0; i < 2; i++) {
-                            const float x = __fmaf_rn(kr.x, s[nb][kb][2 * hf + i], kr.y * zq[nb][i]);
-                            const bool off = CUT && j >= seen[nb][i];
-                            s[nb][kb][2 * hf + i] = x;
-                            mt[nb][i] = off ? mt[nb][i] : fmaxf(mt[nb][i], x);
+                            float &x = s[nb][kb][2 * hf + i];
+                            x = __fmaf_rn(kr.x, x, kr.y * zq[nb][i]);
                             if (TRACK && nb * 8 + 2 * c4 + i < rows_here && (!CUT || j < here))
-                                score[(int64_t)(nb * 8 + 2 * c4 + i) * p.max_len + j] = off ? -INFINITY : x * qs[nb][i];
+                                score[(int64_t)(nb * 8 + 2 * c4 + i) * p.max_len + j] = CUT && j >= seen[nb][i] ? -INFINITY : x * qs[nb][i];
                         }
                 }
-            float mq[NB][2];   // the maximum times the factor, less `up`
+            // Weights are taken from a reference that follows the maximum only where a weight
+            // would pass 2^8 (each row by itself, so that its bits are its own): after the
+            // first tile there is hardly anything to look for, or to take down.
+            float mt[NB][2];
+            bool over = it == 0;
 #pragma unroll
             for (int nb = 0; nb < NB; nb++)
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
+                    mt[nb][i] = -INFINITY;
 #pragma unroll
-                    for (int x = 4; x < 32; x <<= 1) mt[nb][i] = fmaxf(mt[nb][i], __shfl_xor_sync(0xffffffffu, mt[nb][i], x));
-                    const float was = m[nb][i], now = fmaxf(was, mt[nb][i]);
-                    m[nb][i] = now;
-                    mq[nb][i] = now == -INFINITY ? 0.0f : __fmaf_rn(now, qs[nb][i], -(float)up);
-                    if (it > 0) {
-                        const float f = was == now ? 1.0f : was == -INFINITY ? 0.0f : ex2((was - now) * qs[nb][i]);
-                        l[nb][i] *= f;
-                        z[nb][i] *= f;
-                        if (kExact) lost[nb][i] *= f;
-#pragma unroll
-                        for (int ch = 0; ch < CH; ch++)
-#pragma unroll
-                            for (int y = 0; y < 2; y++) {
-                                o[nb][ch][y][i] *= f;
-                                o[nb][ch][y][2 + i] *= f;
-                            }
+                    for (int kb = 0; kb < KB; kb++) {
+                        const int j = t0 + kb * 16 + g8;
+                        const float x = CUT && j >= seen[nb][i] ? -INFINITY : s[nb][kb][i];
+                        const float y = CUT && j + 8 >= seen[nb][i] ? -INFINITY : s[nb][kb][2 + i];
+                        mt[nb][i] = fmaxf(mt[nb][i], fmaxf(x, y));
                     }
+                    over |= (mt[nb][i] - m[nb][i]) * qs[nb][i] > 8.0f;
                 }
+            if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
-            for (int kb = 0; kb < 4; kb++) {
+                for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+#pragma unroll
+                        for (int x = 4; x < 32; x <<= 1) mt[nb][i] = fmaxf(mt[nb][i], __shfl_xor_sync(0xffffffffu, mt[nb][i], x));
+                        const float was = m[nb][i];
+                        if (was == -INFINITY || (mt[nb][i] - was) * qs[nb][i] > 8.0f) m[nb][i] = fmaxf(was, mt[nb][i]);
+                        const float now = m[nb][i];
+                        mq[nb][i] = now == -INFINITY ? 0.0f : __fmaf_rn(now, qs[nb][i], -(float)up);
+                        if (it > 0) {
+                            const float f = was == now ? 1.0f : was == -INFINITY ? 0.0f : ex2((was - now) * qs[nb][i]);
+                            l[nb][i] *= f;
+                            z[nb][i] *= f;
+                            if (kExact) lost[nb][i] *= f;
+#pragma unroll
+                            for (int ch = 0; ch < CH; ch++)
+#pragma unroll
+                                for (int y = 0; y < 2; y++) {
+                                    o[nb][ch][y][i] *= f;
+                                    o[nb][ch][y][2 + i] *= f;
+                                }
+                        }
+                    }
+            }
+#pragma unroll
+            for (int kb = 0; kb < KB; kb++) {
                 uint32_t pf[NB][2];
 #pragma unroll
                 for (int hf = 0; hf < 2; hf++) {
@@ -493,10 +522,10 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
 #pragma unroll
                         for (int i = 0; i < 2; i++) {
                             const bool off = CUT && j >= seen[nb][i];   // what is not seen may be anything
-                            const float e = off ? 0.0f : ex2(__fmaf_rn(s[nb][kb][2 * hf + i], qs[nb][i], -mq[nb][i]));
-                            l[nb][i] += e;
-                            z[nb][i] = off ? z[nb][i] : __fmaf_rn(e, vr.y, z[nb][i]);
-                            w[i] = off ? 0.0f : e * vr.x;
+                            const float y = off ? 0.0f : ex2(__fmaf_rn(s[nb][kb][2 * hf + i], qs[nb][i], -mq[nb][i]));
+                            l[nb][i] += y;
+                            z[nb][i] = off ? z[nb][i] : __fmaf_rn(y, vr.y, z[nb][i]);
+                            w[i] = off ? 0.0f : y * vr.x;
                         }
                         const uint32_t wp = pack_half(w[0], w[1]);
                         if (kExact) {
@@ -525,7 +554,7 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
         };
 #pragma unroll 1
         for (int it = 0; it < turns; it++) {
-            if (!mbar_wait(&ring_bar[it % kRing], (it / kRing) & 1, nullptr)) {
+            if (!mbar_try(&ring_bar[it % kRing], (it / kRing) & 1) && !mbar_wait(&ring_bar[it % kRing], (it / kRing) & 1, nullptr)) {
                 atomicOr(&g_ops_timeout, 1);
                 mbar_wait(&ring_bar[it % kRing], (it / kRing) & 1, nullptr);   // once more for the copies, before anything ends
             }
@@ -616,7 +645,7 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
 // the weights of kUnit entries each.  A row's units are taken in RUNS interleaved runs and
 // those in order: places that depend on its length alone.  Up to kFew units make one run,
 // and the first CTA takes all rows of them.
-constexpr int kJoinThreads = 256, kFew = 16, kMany = 1024;
+constexpr int kJoinThreads = 512, kFew = 16, kMany = 1024;
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads) k_kv4_join(const __grid_constant__ AttendArgs p, int rows_padded) {
     pdl_wait();
