@@ -278,6 +278,7 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
     const int unit = blockIdx.x, h = p.row_blocks == 1 ? blockIdx.y : blockIdx.y / p.row_blocks, b = blockIdx.z;
     const int rb = blockIdx.y - h * p.row_blocks;
     const bool first = tid == 0 && unit == 0 && blockIdx.y == 0;
+    pdl_trigger();   // k_kv4_join may begin to launch
     if (TRACK && unit == 0 && b == 0 && blockIdx.y == 0) kv4_check_distinct(p.c, p.slots, gridDim.z);
     const int slot = kv4_slot(p.c, p.slots, b, first);
     const int n = slot < 0 ? 0 : kv4_length(p.c, p.lengths, b, min(p.max_len, p.c.capacity), first);
@@ -641,21 +642,21 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
         }
 }
 
-// Joins the units of rows: the first `rows` CTAs of x write the rows' results, the others
+// Joins the units of rows: the first row_ctas CTAs of x write the rows' results, the others
 // the weights of kUnit entries each.  A row's units are taken in RUNS interleaved runs and
 // those in order: places that depend on its length alone.  Up to kFew units make one run,
-// and the first CTA takes all rows of them.
-constexpr int kJoinThreads = 512, kFew = 16, kMany = 1024;
+// and the first CTA takes all rows of them (row_ctas is 1 where no sequence may have more).
+constexpr int kJoinThreads = 256, kFew = 16, kMany = 1024;
 template <typename T, int D>
-__global__ void __launch_bounds__(kJoinThreads) k_kv4_join(const __grid_constant__ AttendArgs p, int rows_padded) {
-    pdl_wait();
+__global__ void __launch_bounds__(kJoinThreads) k_kv4_join(const __grid_constant__ AttendArgs p, int rows_padded, int row_ctas) {
     constexpr int TR = D / 4, RUNS = kJoinThreads / TR;   // TR threads a run, four dimensions each
     const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
     const int slot = kv4_slot(p.c, p.slots, b, false);
     const int n = slot < 0 ? 0 : kv4_length(p.c, p.lengths, b, min(p.max_len, p.c.capacity), false);
     const int units = (n + kUnit - 1) / kUnit;
     const int64_t first = ((int64_t)b * p.c.n_heads + h) * p.units * rows_padded;
-    if ((int)blockIdx.x < p.rows) {
+    pdl_wait();   // slots and lengths are older than the kernel before this one
+    if ((int)blockIdx.x < row_ctas) {
         const int d = 4 * (tid % TR), run = tid / TR;
         if (units <= kFew) {
             if (blockIdx.x > 0) return;
@@ -663,7 +664,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv4_join(const __grid_constant
                 float m = -INFINITY, l = 0.0f;
                 float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 for (int u = 0; u < units; u++) m = fmaxf(m, p.stat[first + (int64_t)u * rows_padded + r].x);
-#pragma unroll 4
+#pragma unroll 8
                 for (int u = 0; u < units; u++) {
                     const int64_t at = first + (int64_t)u * rows_padded + r;
                     const float2 st = p.stat[at];
@@ -694,7 +695,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv4_join(const __grid_constant
                 l = __fmaf_rn(s_f[u], st.y, l);
             }
             __syncthreads();
-#pragma unroll 8
+#pragma unroll 16
             for (int u = run; u < some; u += RUNS)
                 add_scaled(x, s_f[u], *reinterpret_cast<const float4 *>(p.part + (first + (int64_t)(u0 + u) * rows_padded + r) * D + d));
         }
@@ -711,7 +712,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv4_join(const __grid_constant
         return;
     }
     // weights of kUnit entries: a warp a row for its maximum and sum, then a thread two entries
-    const int j0 = ((int)blockIdx.x - p.rows) * kUnit;
+    const int j0 = ((int)blockIdx.x - row_ctas) * kUnit;
     if (j0 >= n) return;
     constexpr int RB = 32;   // rows at a time
     __shared__ float2 s_row[RB];
@@ -731,7 +732,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv4_join(const __grid_constant
         }
         __syncthreads();
         const float *s = p.score + (((int64_t)b * p.c.n_heads + h) * p.rows + r0) * p.max_len + j0 + tid;
-#pragma unroll 4
+#pragma unroll 8
         for (int r = 0; r < min(RB, p.rows - r0); r++) {
             const int seen = n - (p.t - 1 - row_place(p, r0 + r)) - j0 - tid;
             const float2 row = s_row[r];
@@ -819,8 +820,9 @@ int attend_with(const AttendPlan &plan, const AttendArgs &p, int b, cudaStream_t
     const dim3 grid((unsigned)plan.units, (unsigned)(p.c.n_heads * plan.row_blocks), (unsigned)b);
     if (int e = ops_cuda(ops_launch(k_kv4_attend<T, D, NB, TRACK>, grid, kAttendWarps * 32, smem, st, false, 1, mk, mv, p))) return e;
     if (!plan.join) return CZG_OK;
-    const dim3 join((unsigned)(plan.rows + (TRACK ? plan.units : 0)), (unsigned)p.c.n_heads, (unsigned)b);
-    return ops_cuda(ops_launch(k_kv4_join<T, D>, join, kJoinThreads, 0, st, true, 1, p, plan.row_blocks * 8 * NB));
+    const int row_ctas = plan.units <= kFew ? 1 : plan.rows;
+    const dim3 join((unsigned)(row_ctas + (TRACK ? plan.units : 0)), (unsigned)p.c.n_heads, (unsigned)b);
+    return ops_cuda(ops_launch(k_kv4_join<T, D>, join, kJoinThreads, 0, st, true, 1, p, plan.row_blocks * 8 * NB, row_ctas));
 }
 
 template <typename T>
