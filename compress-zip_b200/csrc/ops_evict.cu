@@ -5,7 +5,10 @@
 namespace czg {
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kDigit = 11, kBins = 1 << kDigit;   // three digits: 11, 11 and 10 bits
+constexpr int kStretch = 8 * kThreads;            // entries sorted out at a time
+constexpr int kTasks = 8;                         // 16-byte pieces a thread holds between reading and writing
 
 // Order of the weights as unsigned numbers: larger weight, larger key; NaN above all.
 __device__ __forceinline__ uint32_t rank_key(float w) {
@@ -14,37 +17,45 @@ __device__ __forceinline__ uint32_t rank_key(float w) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Sum over the CTA of x, and the sum over the threads before this one.
-__device__ __forceinline__ int scan(int x, int *before, int *part) {
+// The sum of x over the CTA (returned) and over the threads before this one.
+__device__ __forceinline__ uint32_t scan(uint32_t x, uint32_t *before, uint32_t *part) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int y = x;
+    uint32_t y = x;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int z = __shfl_up_sync(0xffffffffu, y, o);
+        const uint32_t z = __shfl_up_sync(0xffffffffu, y, o);
         if (lane >= o) y += z;
     }
-    __syncthreads();   // part's readers of the last call are done
+    __syncthreads();   // the readers of part's last contents are done
     if (lane == 31) part[warp] = y;
     __syncthreads();
-    int sum = 0, below = 0;
-    for (int w = 0; w < kThreads / 32; w++) {
-        if (w < warp) below += part[w];
-        sum += part[w];
+    uint32_t sum = 0, below = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; w++) {
+        const uint32_t p = part[w];
+        below += w < warp ? p : 0;
+        sum += p;
     }
     *before = below + y - x;
     return sum;
 }
 
-// One CTA a sequence and head.  The weight that divides the kept from the others is
-// found digit by digit, 8 bits at a time from the top, by counting; then the entries
-// are walked in order, kThreads at a time: what stays is read, the CTA waits, and it is
-// written to its place.  No place is written before it was read: the i-th kept entry
-// lies at i or behind it.
+// One CTA a sequence and head.
+// 1. The weight that divides the kept from the others, digit by digit from the top, by
+//    counting: each pass counts the next digit of the weights that share the digits found
+//    so far, and a scan over the counts finds the digit that the last one kept has.
+// 2. Stretch by stretch, in order: who stays (keys above the threshold, the first ones
+//    equal to it, the recent entries), numbered by a scan.
+// 3. A stretch's entries move, kThreads * kTasks pieces of 16 bytes at a time: all are read,
+//    the CTA waits, all are written.  The i-th kept entry lies at place i or behind it, so
+//    no place is written before it was read.
+// Bound by reading and writing what moves; measured beside the launch below.
 template <int D>
 __global__ void __launch_bounds__(kThreads) k_kv4_evict(czg_kv4 c, const int32_t *__restrict__ slots,
                                                         const int32_t *__restrict__ lengths, int b, int max_len, int budget,
                                                         int recent, int32_t *__restrict__ kept, int32_t *__restrict__ new_len) {
-    __shared__ int hist[256], part[kThreads / 32];
+    __shared__ uint32_t hist[kBins], part[kWarps];
+    __shared__ int stay_list[kStretch];
     __shared__ uint32_t s_prefix;
     __shared__ int s_need;
     const int h = blockIdx.x, s = blockIdx.y, tid = threadIdx.x;
@@ -70,67 +81,98 @@ __global__ void __launch_bounds__(kThreads) k_kv4_evict(czg_kv4 c, const int32_t
         s_need = budget - recent;         // how many of them stay
     }
     __syncthreads();
-    for (int shift = 24; shift >= 0 && budget > recent; shift -= 8) {
-        for (int i = tid; i < 256; i += kThreads) hist[i] = 0;
+    for (int shift = 32 - kDigit; budget > recent; shift = max(shift - kDigit, 0)) {
+        const int bits = shift == 0 ? 32 - 2 * kDigit : kDigit;
+        for (int i = tid; i < kBins; i += kThreads) hist[i] = 0;
         __syncthreads();
-        const uint32_t prefix = s_prefix, mask = shift == 24 ? 0u : 0xFFFFFFFFu << (shift + 8);
+        const uint32_t prefix = s_prefix, mask = bits + shift == 32 ? 0u : 0xFFFFFFFFu << (bits + shift);
+#pragma unroll 8
         for (int i = tid; i < old; i += kThreads) {
             const uint32_t key = rank_key(w[i]);
-            if ((key & mask) == prefix) atomicAdd(&hist[key >> shift & 255u], 1);
+            if ((key & mask) == prefix) atomicAdd(&hist[key >> shift & (kBins - 1u) & ~(~0u << bits)], 1u);
         }
         __syncthreads();
-        if (tid == 0) {
-            int need = s_need, d = 255;
-            while (d > 0 && hist[d] < need) need -= hist[d--];   // d > 0: weights that another call changes meanwhile
-            s_need = need;
-            s_prefix = prefix | (uint32_t)d << shift;
+        // bins from the top: thread i has the four below 4 i, so the scan counts larger keys
+        constexpr int EACH = kBins / kThreads;
+        uint32_t mine[EACH], sum = 0, above;
+#pragma unroll
+        for (int i = 0; i < EACH; i++) sum += mine[i] = hist[kBins - 1 - (tid * EACH + i)];
+        const uint32_t need = (uint32_t)s_need;
+        scan(sum, &above, part);
+        if (above < need && need <= above + sum) {   // one thread, as long as the weights hold still
+            int i = 0;
+            uint32_t left = need - above;
+            while (i < EACH - 1 && mine[i] < left) left -= mine[i++];
+            s_need = (int)left;
+            s_prefix = prefix | (uint32_t)(kBins - 1 - (tid * EACH + i)) << shift;
         }
         __syncthreads();
+        if (shift == 0) break;
     }
     // keys above the threshold stay, and the first s_need of those equal to it
     const uint32_t threshold = s_prefix;
     const int equal = budget > recent ? s_need : 0;
     int done = 0, met = 0;   // kept so far, equal keys met so far
-    for (int i0 = 0; i0 < n; i0 += kThreads) {
-        const int i = i0 + tid;
-        const float wi = i < n ? w[i] : 0.0f;
-        const uint32_t key = rank_key(wi);
-        const bool ranked = i < old && budget > recent;
-        const bool same = ranked && key == threshold;
-        int before_same, before;
-        const int all_same = scan(same, &before_same, part);
-        const bool stay = i < n && (i >= old || (ranked && key > threshold) || (same && met + before_same < equal));
-        const int count = scan(stay, &before, part);
-        uint4 rk[D / 32], rv[D / 32];
-        KvScale sc = {};
-        if (stay) {
-            const uint4 *pk = reinterpret_cast<const uint4 *>(c.k + (base + i) * (D / 2));
-            const uint4 *pv = reinterpret_cast<const uint4 *>(c.v + (base + i) * (D / 2));
+    for (int i0 = 0; i0 < n; i0 += kStretch) {
+        constexpr int EACH = kStretch / kThreads;
+        const int t0 = i0 + tid * EACH;   // this thread's entries, side by side
+        uint32_t flags = 0, same = 0;
 #pragma unroll
-            for (int x = 0; x < D / 32; x++) {
-                rk[x] = pk[x];
-                rv[x] = pv[x];
+        for (int j = 0; j < EACH; j++) {
+            const int i = t0 + j;
+            if (i < old && budget > recent) {
+                const uint32_t key = rank_key(w[i]);
+                if (key > threshold) flags |= 1u << j;
+                if (key == threshold) same |= 1u << j;
+            } else if (i >= old && i < n) {
+                flags |= 1u << j;
             }
-            sc = static_cast<const KvScale *>(c.scales)[base + i];
         }
-        __syncthreads();   // all of this stretch is read
-        const int to = done + before;
-        if (stay && to < budget) {
-            if (to != i) {
-                uint4 *pk = reinterpret_cast<uint4 *>(c.k + (base + to) * (D / 2));
-                uint4 *pv = reinterpret_cast<uint4 *>(c.v + (base + to) * (D / 2));
+        uint32_t before;   // both counts at once: a stretch's fit 16 bits
+        const uint32_t all = scan((uint32_t)__popc(flags) | (uint32_t)__popc(same) << 16, &before, part);
+        const int same_before = met + (int)(before >> 16);
+        int at = (int)(before & 0xFFFFu) + min(same_before, equal) - min(met, equal);   // within the stretch
+        int may = equal - same_before;   // equal keys that may still stay
 #pragma unroll
-                for (int x = 0; x < D / 32; x++) {
-                    pk[x] = rk[x];
-                    pv[x] = rv[x];
-                }
-                static_cast<KvScale *>(c.scales)[base + to] = sc;
-                w[to] = wi;
+        for (int j = 0; j < EACH; j++) {
+            bool stay = flags >> j & 1u;
+            if (same >> j & 1u) stay = may-- > 0;
+            if (stay) stay_list[at++] = t0 + j;
+        }
+        const int same_all = (int)(all >> 16);
+        const int count = min((int)(all & 0xFFFFu) + min(met + same_all, equal) - min(met, equal), max(budget - done, 0));
+        met += same_all;
+        __syncthreads();
+        if (kp)
+            for (int i = tid; i < count; i += kThreads) kp[done + i] = stay_list[i];
+        // a row's pieces: D / 32 of keys, as many of values; its range and weight go with the first
+        constexpr int PIECES = D / 16, ROWS = kThreads * kTasks / PIECES;
+        for (int r0 = 0; r0 < count; r0 += ROWS) {
+            uint4 piece[kTasks];
+            KvScale sc[kTasks];
+            float weight[kTasks];
+#pragma unroll
+            for (int k = 0; k < kTasks; k++) {
+                const int task = k * kThreads + tid, r = r0 + task / PIECES, p = task % PIECES;
+                if (r >= count || stay_list[r] == done + r) continue;
+                const int64_t from = base + stay_list[r];
+                piece[k] = reinterpret_cast<const uint4 *>((p < PIECES / 2 ? c.k : c.v) + from * (D / 2))[p % (PIECES / 2)];
+                if (p == 0) sc[k] = static_cast<const KvScale *>(c.scales)[from];
+                if (p == 1) weight[k] = c.weights[from];
             }
-            if (kp) kp[to] = i;
+            __syncthreads();   // all of these are read
+#pragma unroll
+            for (int k = 0; k < kTasks; k++) {
+                const int task = k * kThreads + tid, r = r0 + task / PIECES, p = task % PIECES;
+                if (r >= count || stay_list[r] == done + r) continue;
+                const int64_t to = base + done + r;
+                reinterpret_cast<uint4 *>((p < PIECES / 2 ? c.k : c.v) + to * (D / 2))[p % (PIECES / 2)] = piece[k];
+                if (p == 0) static_cast<KvScale *>(c.scales)[to] = sc[k];
+                if (p == 1) c.weights[to] = weight[k];
+            }
         }
         done += count;
-        met += all_same;
+        __syncthreads();   // stay_list is read; and this stretch's writes are done before the next weights are read
     }
 }
 

@@ -24,114 +24,126 @@ __device__ __forceinline__ float bf16_up(float x) {
 
 struct Strides { int64_t b, t, h; };
 
-// One warp a row of one head: the row's range by shuffles, then lane i's D / 32 values
-// (dimensions i D/32 ..) as codes.  lo is rounded down and step up (each operation with
-// the same direction), so every quotient lies in [0, 15].
-template <typename T, int D>
-__device__ __forceinline__ void quantise_row(const T *row, uint8_t *codes, __nv_bfloat16 *step_out, __nv_bfloat16 *lo_out) {
-    constexpr int N = D / 32;
-    const int lane = threadIdx.x & 31;
-    float x[N], lo = INFINITY, hi = -INFINITY;
-    bool bad = false;
-#pragma unroll
-    for (int i = 0; i < N; i++) {
-        x[i] = to_f32(row[lane * N + i]);
-        bad |= !(fabsf(x[i]) <= 3.402823466e38f);
-        lo = fminf(lo, x[i]);
-        hi = fmaxf(hi, x[i]);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    }
-    bad = __any_sync(0xffffffffu, bad);
-    lo = bf16_down(lo);
-    float step = bf16_up(__fdiv_ru(__fsub_ru(hi, lo), 15.0f));
-    if (bad || !(fabsf(lo) <= 3.402823466e38f) || !(step <= 3.402823466e38f)) step = lo = NAN;
-    uint32_t byte[N / 2];
-#pragma unroll
-    for (int i = 0; i < N; i += 2) {
-        int c0 = 0, c1 = 0;
-        if (step > 0.0f) {
-            c0 = (int)rintf(__fdiv_rn(__fsub_rn(x[i], lo), step));
-            c1 = (int)rintf(__fdiv_rn(__fsub_rn(x[i + 1], lo), step));
-        }
-        byte[i / 2] = (uint32_t)(c0 | c1 << 4);
-    }
-    if (N == 4)
-        *reinterpret_cast<uint16_t *>(codes + 2 * lane) = (uint16_t)(byte[0] | byte[N / 2 - 1] << 8);
-    else
-        codes[lane] = (uint8_t)byte[0];
-    if (lane == 0) {
-        *step_out = __float2bfloat16_rn(step);
-        *lo_out = __float2bfloat16_rn(lo);
-    }
-}
+constexpr float kFltMax = 3.402823466e38f;
 
-// Two warps a row, one for its key and one for its value; CTA 0 looks for repeated slots.
+// D / 4 lanes a row (a warp takes 128 / D rows side by side), four values each: the row's
+// range by shuffles, then the codes.  lo is rounded down and step up (each operation with
+// the same direction), so every quotient lies in [0, 15].  A key's row and its value's are
+// neighbours.  CTA 0 looks for repeated slots.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) k_kv4_append(czg_kv4 c, const T *__restrict__ k, Strides ks, const T *__restrict__ v,
-                                                    Strides vs, const int32_t *__restrict__ slots,
+                                                    Strides vs, int vec, const int32_t *__restrict__ slots,
                                                     const int32_t *__restrict__ lengths, int b, int t) {
     if (blockIdx.x == 0) {
         kv4_check_distinct(c, slots, b);
         return;
     }
-    const int64_t id = ((int64_t)blockIdx.x - 1) * 8 + (threadIdx.x >> 5);
-    const int64_t row = id >> 1;
-    if (row >= (int64_t)b * t * c.n_heads) return;
-    const int h = (int)(row % c.n_heads), i = (int)(row / c.n_heads % t), s = (int)(row / c.n_heads / t);
-    const bool first = (threadIdx.x & 31) == 0 && h == 0 && (id & 1) == 0;
-    const int slot = kv4_slot(c, slots, s, first);
-    if (slot < 0) return;
-    const int64_t entry = (int64_t)lengths[s] - t + i;
-    if (entry < 0 || entry >= c.capacity) {
-        if (first && (lengths[s] < 0 || entry >= c.capacity)) atomicOr(c.status, CZG_KV4_BAD_LENGTH);
-        return;
+    constexpr int LR = D / 4;
+    const uint32_t id = (blockIdx.x - 1) * (256 / LR) + threadIdx.x / LR, part = threadIdx.x % LR;
+    const uint32_t row = id >> 1;   // fewer than 2^31 of them (checked by the host)
+    uint32_t s = 0, i = 0, h = 0;
+    bool there = row < (uint32_t)b * t * c.n_heads;
+    int slot = -1;
+    int64_t entry = 0;
+    if (there) {
+        const uint32_t of_t = c.n_heads == 1 ? row : row / c.n_heads;
+        h = row - of_t * c.n_heads;
+        s = t == 1 ? of_t : of_t / t;
+        i = of_t - s * t;
+        const bool first = part == 0 && h == 0 && (id & 1) == 0;
+        slot = kv4_slot(c, slots, s, first);
+        const int n = lengths[s];
+        entry = (int64_t)n - t + i;
+        if (slot >= 0 && first && (n < 0 || entry >= c.capacity)) atomicOr(c.status, CZG_KV4_BAD_LENGTH);
+        there = slot >= 0 && entry >= 0 && entry < c.capacity;
+    }
+    const Strides &st = id & 1 ? vs : ks;
+    const T *src = (id & 1 ? v : k) + (there ? s * st.b + i * st.t + h * st.h : 0) + part * 4;
+    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (there && vec) {
+        __align__(16) T y[4];
+        if (sizeof(T) == 4) *reinterpret_cast<uint4 *>(y) = __ldg(reinterpret_cast<const uint4 *>(src));
+        else *reinterpret_cast<uint2 *>(y) = __ldg(reinterpret_cast<const uint2 *>(src));
+#pragma unroll
+        for (int j = 0; j < 4; j++) x[j] = to_f32(y[j]);
+    } else if (there) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) x[j] = to_f32(src[j]);
+    }
+    float lo = INFINITY, hi = -INFINITY;
+    bool fine = true;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        fine &= fabsf(x[j]) <= kFltMax;
+        lo = fminf(lo, x[j]);
+        hi = fmaxf(hi, x[j]);
+    }
+    if (!fine) hi = INFINITY;   // NaN too: the row's range is not finite
+#pragma unroll
+    for (int o = 1; o < LR; o <<= 1) {
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    }
+    if (!there) return;
+    lo = bf16_down(lo);
+    float step = bf16_up(__fdiv_ru(__fsub_ru(hi, lo), 15.0f));
+    if (!(fabsf(lo) <= kFltMax) || !(step <= kFltMax)) step = lo = NAN;
+    uint32_t code = 0;
+    if (step > 0.0f) {
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            code |= (__float_as_uint(__fadd_rn(__fdiv_rn(__fsub_rn(x[j], lo), step), kM1)) & 15u) << (4 * j);   // rounded by the sum
     }
     const int64_t at = kv4_row(c, slot, h, (int)entry);
-    KvScale *sc = static_cast<KvScale *>(c.scales) + at;
-    if (id & 1) {
-        quantise_row<T, D>(v + s * vs.b + i * vs.t + h * vs.h, c.v + at * (D / 2), &sc->v_step, &sc->v_lo);
-    } else {
-        quantise_row<T, D>(k + s * ks.b + i * ks.t + h * ks.h, c.k + at * (D / 2), &sc->k_step, &sc->k_lo);
-        if (c.weights && (threadIdx.x & 31) == 0) c.weights[at] = 0.0f;
+    reinterpret_cast<uint16_t *>((id & 1 ? c.v : c.k) + at * (D / 2))[part] = (uint16_t)code;
+    if (part == 0) {
+        const uint32_t range = __float_as_uint(step) >> 16 | (__float_as_uint(lo) & 0xFFFF0000u);   // both are bf16
+        reinterpret_cast<uint32_t *>(static_cast<KvScale *>(c.scales) + at)[id & 1] = range;
+        if (c.weights && (id & 1) == 0) c.weights[at] = 0.0f;
     }
 }
 
-// A thread reads 8 codes of one row and writes their values.
+// The y of a CTA's grid place is the sequence.  A thread takes 16 codes of a row at a
+// time and writes their values, a row's key and value one after the other.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) k_kv4_read(czg_kv4 c, const int32_t *__restrict__ slots,
-                                                  const int32_t *__restrict__ starts, int b, int count,
+                                                  const int32_t *__restrict__ starts, int count, uint32_t rows,
                                                   T *__restrict__ k_out, T *__restrict__ v_out) {
-    constexpr int P = D / 8;   // threads a row
-    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t row = id / P;
-    if (row >= (int64_t)b * count * c.n_heads) return;
-    const int p = (int)(id % P);
-    const int h = (int)(row % c.n_heads), s = (int)(row / c.n_heads / count);
-    const int64_t entry = (int64_t)starts[s] + row / c.n_heads % count;
-    const int slot = kv4_slot(c, slots, s, p == 0 && h == 0);
+    constexpr int P = D / 16;   // threads a row
+    const int s = blockIdx.y, part = threadIdx.x % P;
+    const int slot = kv4_slot(c, slots, s, threadIdx.x == 0 && blockIdx.x == 0);
+    const int64_t from = starts[s];
+    const uint32_t row = blockIdx.x * (256 / P) + threadIdx.x / P;
+    if (row >= rows) return;
+    const uint32_t place = c.n_heads == 1 ? row : row / c.n_heads, h = row - place * c.n_heads;
+    const int64_t entry = from + place;
     const bool there = slot >= 0 && entry >= 0 && entry < c.capacity;
-    if (slot >= 0 && !there && p == 0 && h == 0) atomicOr(c.status, CZG_KV4_BAD_LENGTH);
+    if (slot >= 0 && !there && part == 0 && h == 0) atomicOr(c.status, CZG_KV4_BAD_LENGTH);
     const int64_t at = there ? kv4_row(c, slot, h, (int)entry) : 0;
-    KvScale sc = {};
-    if (there) sc = static_cast<const KvScale *>(c.scales)[at];
+    uint2 range = make_uint2(0, 0), codes[2] = {make_uint2(0, 0), make_uint2(0, 0)};
+    if (there) {
+        range = *reinterpret_cast<const uint2 *>(static_cast<const KvScale *>(c.scales) + at);
+        if (k_out) codes[0] = reinterpret_cast<const uint2 *>(c.k + at * (D / 2))[part];
+        if (v_out) codes[1] = reinterpret_cast<const uint2 *>(c.v + at * (D / 2))[part];
+    }
 #pragma unroll
     for (int w = 0; w < 2; w++) {
         T *out = w ? v_out : k_out;
         if (!out) continue;
-        const float step = to_f32(w ? sc.v_step : sc.k_step), lo = to_f32(w ? sc.v_lo : sc.k_lo);
-        const uint32_t codes = there ? *reinterpret_cast<const uint32_t *>((w ? c.v : c.k) + at * (D / 2) + 4 * p) : 0u;
-        __align__(16) T y[8];
+        const uint32_t r = w ? range.y : range.x;
+        const float step = __uint_as_float(r << 16), lo = __uint_as_float(r & 0xFFFF0000u);
+        __align__(16) T y[16];
 #pragma unroll
-        for (int i = 0; i < 8; i++)
-            y[i] = from_f32<T>(there ? __fmaf_rn(step, (float)(codes >> (4 * i) & 15u), lo) : 0.0f);
-        uint4 *dst = reinterpret_cast<uint4 *>(out + row * D + 8 * p);
+        for (int i = 0; i < 16; i++) {
+            const uint32_t word = i < 8 ? codes[w].x : codes[w].y;
+            // a code under the bits of 2^23 is 2^23 + code
+            const float code = __fsub_rn(__uint_as_float((word >> (4 * (i & 7)) & 15u) | 0x4B000000u), 8388608.0f);
+            y[i] = from_f32<T>(__fmaf_rn(step, code, lo));
+        }
+        uint4 *dst = reinterpret_cast<uint4 *>(out + ((int64_t)s * rows + row) * D + 16 * part);
         const uint4 *src = reinterpret_cast<const uint4 *>(y);
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; i++) dst[i] = src[i];
+        for (int i = 0; i < (int)sizeof(T); i++) dst[i] = src[i];
     }
 }
 
@@ -788,20 +800,26 @@ AttendPlan attend_plan(const czg_kv4 &c, int64_t b, int t, int hq, int max_len) 
 template <typename T>
 int append(const czg_kv4 &c, const void *k, Strides ks, const void *v, Strides vs, const int32_t *slots,
            const int32_t *lengths, int b, int t, cudaStream_t st) {
-    const int64_t blocks = ((int64_t)b * t * c.n_heads * 2 + 7) / 8 + 1;
-    if (blocks > 0x7FFFFFFF) return ops_fail(CZG_E_LIMIT, "too many rows");
+    const int64_t rows = (int64_t)b * t * c.n_heads;
+    if (rows >= 1ll << 30) return ops_fail(CZG_E_LIMIT, "too many rows");
+    const int64_t per = 1024 / c.head_dim;   // rows of keys and of values a CTA
+    auto vec_of = [](const void *p, const Strides &x) {
+        return aligned(p, 4 * sizeof(T)) && x.b % 4 == 0 && x.t % 4 == 0 && x.h % 4 == 0;
+    };
+    const int vec = vec_of(k, ks) && vec_of(v, vs);
     auto kern = c.head_dim == 64 ? k_kv4_append<T, 64> : k_kv4_append<T, 128>;
-    return ops_cuda(ops_launch(kern, dim3((unsigned)blocks), 256, 0, st, false, 1, c, static_cast<const T *>(k), ks,
-                               static_cast<const T *>(v), vs, slots, lengths, b, t));
+    return ops_cuda(ops_launch(kern, dim3((unsigned)((2 * rows + per - 1) / per + 1)), 256, 0, st, false, 1, c,
+                               static_cast<const T *>(k), ks, static_cast<const T *>(v), vs, vec, slots, lengths, b, t));
 }
 
 template <typename T>
 int read(const czg_kv4 &c, const int32_t *slots, const int32_t *starts, int b, int count, void *k, void *v, cudaStream_t st) {
-    const int64_t blocks = ((int64_t)b * count * c.n_heads * (c.head_dim / 8) + 255) / 256;
-    if (blocks > 0x7FFFFFFF) return ops_fail(CZG_E_LIMIT, "too many entries");
+    const int64_t rows = (int64_t)count * c.n_heads;   // of a sequence
+    if (rows >= 1ll << 30) return ops_fail(CZG_E_LIMIT, "too many entries");
+    const int64_t per = 4096 / c.head_dim;
     auto kern = c.head_dim == 64 ? k_kv4_read<T, 64> : k_kv4_read<T, 128>;
-    return ops_cuda(ops_launch(kern, dim3((unsigned)blocks), 256, 0, st, false, 1, c, slots, starts, b, count,
-                               static_cast<T *>(k), static_cast<T *>(v)));
+    return ops_cuda(ops_launch(kern, dim3((unsigned)((rows + per - 1) / per), (unsigned)b), 256, 0, st, false, 1, c, slots,
+                               starts, count, (uint32_t)rows, static_cast<T *>(k), static_cast<T *>(v)));
 }
 
 template <typename T, int D, int NB, bool TRACK>

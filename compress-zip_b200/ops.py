@@ -21,6 +21,7 @@ from . import engine as _engine
 from .engine import CZG_OK, CzgError
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_INT32 = torch.int32
 
 # The exported symbols of include/czg_ops.h, checked by the CPU test suite.
 EXPORTS = ["czg_ops_last_error", "czg_ops_check", "czg_quantize_rows", "czg_linear_i8", "czg_linear_i8_workspace",
@@ -264,7 +265,7 @@ class KV4Cache:
         self.status = torch.zeros(1, dtype=torch.int32, device=k.device)
         self._c = _KV4(k.data_ptr(), v.data_ptr(), scales.data_ptr(), 0 if weights is None else weights.data_ptr(),
                        self.status.data_ptr(), self.n_slots, self.n_heads, self.capacity, self.head_dim)
-        self._ref = C.byref(self._c)
+        self._ref, self._lib, self._index = C.byref(self._c), lib(), k.get_device()
 
     @classmethod
     def empty(cls, n_slots: int, n_heads: int, capacity: int, head_dim: int, track_weights: bool = False,
@@ -276,43 +277,53 @@ class KV4Cache:
                    torch.zeros(shape, dtype=torch.float32, device=device) if track_weights else None)
 
     def _sequences(self, slots: torch.Tensor, counts: torch.Tensor, name: str) -> int:
-        for what, t in (("slots", slots), (name, counts)):
-            if t.dtype != torch.int32 or t.dim() != 1 or t.shape != slots.shape or (t.stride(0) != 1 and t.shape[0] > 1):
-                raise ValueError(f"{what} must be a contiguous int32 vector, one number a sequence")
-            if t.device != self.device:
-                raise ValueError(f"{what} is on {t.device}, the cache on {self.device}")
-        return slots.shape[0]
+        shape = slots.shape
+        if (slots.dtype is not _INT32 or counts.dtype is not _INT32 or len(shape) != 1 or counts.shape != shape
+                or not slots.is_contiguous() or not counts.is_contiguous()):
+            raise ValueError(f"slots and {name} must be contiguous int32 vectors, one number a sequence")
+        if slots.get_device() != self._index or counts.get_device() != self._index:
+            raise ValueError(f"slots and {name} are on {slots.device} and {counts.device}, the cache on {self.device}")
+        return shape[0]
+
+    def _call(self, fn, *args) -> None:
+        if self._index == _current_device():
+            st = fn(self._ref, *args, _raw_stream(self._index))
+        else:
+            with torch.cuda.device(self._index):
+                st = fn(self._ref, *args, _raw_stream(self._index))
+        if st != CZG_OK:
+            _raise(st)
 
     def append(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, lengths: torch.Tensor) -> None:
         """Quantise rows k, v [b, t, n_heads, head_dim] into entries lengths - t .. lengths - 1
         of their slots; rows before entry 0 are padding.  Their weights become 0."""
         b = self._sequences(slots, lengths, "lengths")
-        if k.dim() != 4 or k.shape[0] != b or k.shape[2:] != (self.n_heads, self.head_dim) or v.shape != k.shape:
+        shape, code = k.shape, DTYPES.get(k.dtype)
+        if len(shape) != 4 or shape[0] != b or shape[2] != self.n_heads or shape[3] != self.head_dim or v.shape != shape:
             raise ValueError(f"k and v must be [{b}, t, {self.n_heads}, {self.head_dim}]")
-        code = _dtype(k, "k")
-        if v.dtype != k.dtype:
-            raise ValueError("k and v must have the same type")
-        if k.stride(3) != 1 or v.stride(3) != 1:
+        if code is None or v.dtype is not k.dtype:
+            raise ValueError(f"k and v must both be float32, bfloat16 or float16, not {k.dtype} and {v.dtype}")
+        ks, vs = k.stride(), v.stride()
+        if ks[3] != 1 or vs[3] != 1:
             raise ValueError("the last dimension of k and v must be adjacent")
-        _same_device(self.device, k=k, v=v)
-        if k.numel():
-            _call(self.device, lib().czg_kv4_append, self._ref, k.data_ptr(), k.stride(0), k.stride(1), k.stride(2),
-                  v.data_ptr(), v.stride(0), v.stride(1), v.stride(2), code, slots.data_ptr(), lengths.data_ptr(), b,
-                  k.shape[1])
+        if k.get_device() != self._index or v.get_device() != self._index:
+            raise ValueError(f"k and v are on {k.device} and {v.device}, the cache on {self.device}")
+        if b and shape[1]:
+            self._call(self._lib.czg_kv4_append, k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2], code,
+                       slots.data_ptr(), lengths.data_ptr(), b, shape[1])
 
     def read(self, slots: torch.Tensor, starts: torch.Tensor, count: int, dtype: torch.dtype = torch.bfloat16):
         """Entries starts .. starts + count - 1 of each slot as values: (k, v), each
         [b, count, n_heads, head_dim]; 0 for places outside the slot."""
         b = self._sequences(slots, starts, "starts")
-        if dtype not in DTYPES:
+        code = DTYPES.get(dtype)
+        if code is None:
             raise ValueError(f"dtype must be float32, bfloat16 or float16, not {dtype}")
         if count < 0:
             raise ValueError("count must not be negative")
-        shape = (b, count, self.n_heads, self.head_dim)
-        k, v = (torch.empty(shape, dtype=dtype, device=self.device) for _ in range(2))
-        if k.numel():
-            _call(self.device, lib().czg_kv4_read, self._ref, slots.data_ptr(), starts.data_ptr(), b, count,
-                  k.data_ptr(), v.data_ptr(), DTYPES[dtype])
+        k, v = torch.empty((2, b, count, self.n_heads, self.head_dim), dtype=dtype, device=self.device).unbind(0)
+        if b and count:
+            self._call(self._lib.czg_kv4_read, slots.data_ptr(), starts.data_ptr(), b, count, k.data_ptr(), v.data_ptr(), code)
         return k, v
 
     def attend(self, q: torch.Tensor, slots: torch.Tensor, lengths: torch.Tensor, max_len: Optional[int] = None,
@@ -323,28 +334,31 @@ class KV4Cache:
         scale defaults to head_dim ** -0.5.  With weights, each entry's grows by its
         probabilities, summed over the rows and query heads of its key head."""
         b = self._sequences(slots, lengths, "lengths")
-        if q.dim() != 4 or q.shape[0] != b or q.shape[3] != self.head_dim or q.shape[2] % self.n_heads:
+        shape, qs = q.shape, q.stride()
+        if len(shape) != 4 or shape[0] != b or shape[3] != self.head_dim or shape[2] % self.n_heads:
             raise ValueError(f"q must be [{b}, t, a multiple of {self.n_heads}, {self.head_dim}]")
-        if q.dtype not in (torch.bfloat16, torch.float16):
+        _, t, hq, _ = shape
+        if q.dtype is not torch.bfloat16 and q.dtype is not torch.float16:
             raise ValueError(f"q must be bfloat16 or float16, not {q.dtype}")
-        if q.stride(3) != 1:
+        if qs[3] != 1:
             raise ValueError("the last dimension of q must be adjacent")
+        if q.get_device() != self._index:
+            raise ValueError(f"q is on {q.device}, the cache on {self.device}")
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        elif out.shape != q.shape or out.dtype != q.dtype or out.stride(3) != 1:
-            raise ValueError("out must have q's shape and type and an adjacent last dimension")
-        _same_device(self.device, q=q, out=out)
-        if q.numel() == 0:
+            out = torch.empty_like(q)
+        elif out.shape != shape or out.dtype is not q.dtype or out.get_device() != self._index:
+            raise ValueError("out must have q's shape, type and device")
+        os = out.stride()
+        if os[3] != 1:
+            raise ValueError("the last dimension of out must be adjacent")
+        if not (b and t and hq):
             return out
         n = self.capacity if max_len is None else max_len
-        L = lib()
-        t, hq = q.shape[1], q.shape[2]
-        need = L.czg_kv4_attend_workspace(self._ref, b, t, hq, n)
+        need = self._lib.czg_kv4_attend_workspace(self._ref, b, t, hq, n)
         ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-        _call(self.device, L.czg_kv4_attend, self._ref, q.data_ptr(), q.stride(0), q.stride(1), q.stride(2),
-              DTYPES[q.dtype], slots.data_ptr(), lengths.data_ptr(), b, t, hq, n,
-              self.head_dim ** -0.5 if scale is None else scale, out.data_ptr(), out.stride(0), out.stride(1),
-              out.stride(2), ws.data_ptr() if need else 0, need)
+        self._call(self._lib.czg_kv4_attend, q.data_ptr(), qs[0], qs[1], qs[2], DTYPES[q.dtype], slots.data_ptr(),
+                   lengths.data_ptr(), b, t, hq, n, self.head_dim ** -0.5 if scale is None else scale, out.data_ptr(),
+                   os[0], os[1], os[2], ws.data_ptr() if need else 0, need)
         return out
 
     def evict(self, slots: torch.Tensor, lengths: torch.Tensor, budget: int, recent: int = 0,
@@ -358,11 +372,11 @@ class KV4Cache:
             raise ValueError("the cache keeps no weights to rank entries by")
         if budget < 1 or not 0 <= recent <= budget:
             raise ValueError("1 <= budget and 0 <= recent <= budget are needed")
-        kept = torch.empty((b, self.n_heads, budget), dtype=torch.int32, device=self.device)
-        new = torch.empty(b, dtype=torch.int32, device=self.device)
+        kept = torch.empty((b, self.n_heads, budget), dtype=_INT32, device=self.device)
+        new = torch.empty_like(slots)
         if b:
-            _call(self.device, lib().czg_kv4_evict, self._ref, slots.data_ptr(), lengths.data_ptr(), b,
-                  self.capacity if max_len is None else max_len, budget, recent, kept.data_ptr(), new.data_ptr())
+            self._call(self._lib.czg_kv4_evict, slots.data_ptr(), lengths.data_ptr(), b,
+                       self.capacity if max_len is None else max_len, budget, recent, kept.data_ptr(), new.data_ptr())
         return kept, new
 
     def check(self) -> None:
