@@ -103,47 +103,58 @@ __global__ void __launch_bounds__(256) k_kv4_append(czg_kv4 c, const T *__restri
     }
 }
 
-// The y of a CTA's grid place is the sequence.  A thread takes 16 codes of a row at a
-// time and writes their values, a row's key and value one after the other.
+// D / 8 threads a row, 8 codes of its key and 8 of its value each; a thread takes two rows.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) k_kv4_read(czg_kv4 c, const int32_t *__restrict__ slots,
-                                                  const int32_t *__restrict__ starts, int count, uint32_t rows,
+                                                  const int32_t *__restrict__ starts, uint32_t rows, uint32_t all,
                                                   T *__restrict__ k_out, T *__restrict__ v_out) {
-    constexpr int P = D / 16;   // threads a row
-    const int s = blockIdx.y, part = threadIdx.x % P;
-    const int slot = kv4_slot(c, slots, s, threadIdx.x == 0 && blockIdx.x == 0);
-    const int64_t from = starts[s];
-    const uint32_t row = blockIdx.x * (256 / P) + threadIdx.x / P;
-    if (row >= rows) return;
-    const uint32_t place = c.n_heads == 1 ? row : row / c.n_heads, h = row - place * c.n_heads;
-    const int64_t entry = from + place;
-    const bool there = slot >= 0 && entry >= 0 && entry < c.capacity;
-    if (slot >= 0 && !there && part == 0 && h == 0) atomicOr(c.status, CZG_KV4_BAD_LENGTH);
-    const int64_t at = there ? kv4_row(c, slot, h, (int)entry) : 0;
-    uint2 range = make_uint2(0, 0), codes[2] = {make_uint2(0, 0), make_uint2(0, 0)};
-    if (there) {
-        range = *reinterpret_cast<const uint2 *>(static_cast<const KvScale *>(c.scales) + at);
-        if (k_out) codes[0] = reinterpret_cast<const uint2 *>(c.k + at * (D / 2))[part];
-        if (v_out) codes[1] = reinterpret_cast<const uint2 *>(c.v + at * (D / 2))[part];
+    constexpr int P = D / 8, N = 2;
+    const int part = threadIdx.x % P;
+    uint2 range[N];
+    uint32_t codes[N][2];
+    bool there[N];
+    const uint32_t row0 = blockIdx.x * (N * 256 / P) + threadIdx.x / P;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const uint32_t row = row0 + i * (256 / P);
+        there[i] = false;
+        range[i] = make_uint2(0, 0);
+        codes[i][0] = codes[i][1] = 0;
+        if (row >= all) continue;
+        const uint32_t s = row / rows, of = row - s * rows, place = c.n_heads == 1 ? of : of / c.n_heads, h = of - place * c.n_heads;
+        const bool first = part == 0 && h == 0;
+        const int slot = kv4_slot(c, slots, s, first);
+        const int64_t entry = (int64_t)starts[s] + place;
+        there[i] = slot >= 0 && entry >= 0 && entry < c.capacity;
+        if (slot >= 0 && !there[i] && first) atomicOr(c.status, CZG_KV4_BAD_LENGTH);
+        if (!there[i]) continue;
+        const int64_t at = kv4_row(c, slot, h, (int)entry);
+        range[i] = *reinterpret_cast<const uint2 *>(static_cast<const KvScale *>(c.scales) + at);
+        if (k_out) codes[i][0] = reinterpret_cast<const uint32_t *>(c.k + at * (D / 2))[part];
+        if (v_out) codes[i][1] = reinterpret_cast<const uint32_t *>(c.v + at * (D / 2))[part];
     }
 #pragma unroll
-    for (int w = 0; w < 2; w++) {
-        T *out = w ? v_out : k_out;
-        if (!out) continue;
-        const uint32_t r = w ? range.y : range.x;
-        const float step = __uint_as_float(r << 16), lo = __uint_as_float(r & 0xFFFF0000u);
-        __align__(16) T y[16];
+    for (int i = 0; i < N; i++) {
+        const uint32_t row = row0 + i * (256 / P);
+        if (row >= all) continue;
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            const uint32_t word = i < 8 ? codes[w].x : codes[w].y;
-            // a code under the bits of 2^23 is 2^23 + code
-            const float code = __fsub_rn(__uint_as_float((word >> (4 * (i & 7)) & 15u) | 0x4B000000u), 8388608.0f);
-            y[i] = from_f32<T>(__fmaf_rn(step, code, lo));
+        for (int w = 0; w < 2; w++) {
+            T *out = w ? v_out : k_out;
+            if (!out) continue;
+            const uint32_t r = w ? range[i].y : range[i].x;
+            const float step = __uint_as_float(r << 16), lo = __uint_as_float(r & 0xFFFF0000u);
+            __align__(16) T y[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                // a code under the bits of 2^23 is 2^23 + code
+                const float code = __fsub_rn(__uint_as_float((codes[i][w] >> (4 * j) & 15u) | 0x4B000000u), 8388608.0f);
+                y[j] = from_f32<T>(__fmaf_rn(step, code, lo));
+            }
+            uint4 *dst = reinterpret_cast<uint4 *>(out + (int64_t)row * D + 8 * part);
+            const uint4 *src = reinterpret_cast<const uint4 *>(y);
+#pragma unroll
+            for (int j = 0; j < (int)sizeof(T) / 2; j++) dst[j] = src[j];
         }
-        uint4 *dst = reinterpret_cast<uint4 *>(out + ((int64_t)s * rows + row) * D + 16 * part);
-        const uint4 *src = reinterpret_cast<const uint4 *>(y);
-#pragma unroll
-        for (int i = 0; i < (int)sizeof(T); i++) dst[i] = src[i];
     }
 }
 
@@ -151,7 +162,7 @@ __global__ void __launch_bounds__(256) k_kv4_read(czg_kv4 c, const int32_t *__re
 //
 // A CTA takes one unit of a sequence's entries (kUnit, at a fixed place whatever the
 // batch), one key head and up to 8 NB rows (query heads of that key head, times the
-// call's rows).  Its two warps take tiles of kTile entries in turn, each through a ring of
+// call's rows).  Its two or four warps take tiles of kTile entries in turn, each through a ring of
 // its own that TMA fills (swizzled for ldmatrix); many such small CTAs share an SM and
 // cover one another's beginnings and ends.
 //
@@ -173,7 +184,8 @@ __global__ void __launch_bounds__(256) k_kv4_read(czg_kv4 c, const int32_t *__re
 // sums are fp32; exponentials are ex2.approx (2^-22).
 // Between the warps of a CTA, and between units (k_kv4_join), partial results are joined
 // in a fixed order, so a row's bits do not depend on the batch or the grid.
-constexpr int kUnit = 512, kTile = 64, kAttendWarps = 2, kRing = 2;
+constexpr int kUnit = 512, kTile = 64, kRing = 2;
+__host__ __device__ constexpr int attend_warps(int nb) { return nb == 1 ? 2 : 4; }   // more rows, longer tiles: more warps to share a unit
 
 struct AttendArgs {
     czg_kv4 c;
@@ -260,29 +272,30 @@ __device__ __forceinline__ int64_t row_offset(const AttendArgs &p, const Strides
 __device__ __forceinline__ float pow2f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }   // -126 <= e <= 127
 
 // CTAs an SM is to hold: what the sums (D NB / 4 registers), query and scores leave room for
-constexpr int attend_ctas(int d, int nb) { return d == 64 ? (nb == 1 ? 8 : 5) : (nb == 1 ? 6 : 4); }
+constexpr int attend_ctas(int d, int nb) { return d == 64 ? (nb == 1 ? 8 : 3) : (nb == 1 ? 6 : 2); }
 
-template <int D>
+template <int D, int W>
 struct AttendSmem {
     static constexpr int kTileCodes = kTile * D / 2;   // of keys, and as many of values behind them
-    static constexpr int kScales = kAttendWarps * kRing * 2 * kTileCodes, kBars = kScales + kUnit * 8;
-    static constexpr size_t kBytes = 1024 + kBars + kAttendWarps * kRing * 8;
+    static constexpr int kScales = W * kRing * 2 * kTileCodes, kBars = kScales + kUnit * 8;
+    static constexpr size_t kBytes = 1024 + kBars + W * kRing * 8;
 };
 
 template <typename T, int D, int NB, bool TRACK>
-__global__ void __launch_bounds__(kAttendWarps * 32, attend_ctas(D, NB))
+__global__ void __launch_bounds__(attend_warps(NB) * 32, attend_ctas(D, NB))
 k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttendArgs p) {
-    using L = AttendSmem<D>;
+    constexpr int kWarps = attend_warps(NB);
+    using L = AttendSmem<D, kWarps>;
     constexpr int CH = D / 32;      // 16-byte chunks of a row of codes
-    constexpr int R = 8 * NB, THREADS = kAttendWarps * 32;
+    constexpr int R = 8 * NB, THREADS = kWarps * 32;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint2 *sc = reinterpret_cast<uint2 *>(smem + L::kScales);   // the entries' ranges, as they lie in memory
     uint64_t *bar = reinterpret_cast<uint64_t *>(smem + L::kBars);
     __shared__ uint4 s_q[NB * CH * 32];      // the query as B fragments: [nb][chunk][lane]
     __shared__ float2 s_qs[R];               // a row's factors
-    __shared__ float s_m[kAttendWarps][R], s_l[kAttendWarps][R];
-    __shared__ uint32_t s_top[kAttendWarps];
+    __shared__ float s_m[kWarps][R], s_l[kWarps][R];
+    __shared__ uint32_t s_top[kWarps];
     __shared__ float2 s_row[R];              // maximum and sum over the warps
     __shared__ int64_t s_out[R];             // where the row's output begins
 
@@ -303,12 +316,12 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
     uint64_t *ring_bar = bar + warp * kRing;
     auto ask = [&](int it) {   // one lane
         uint8_t *to = ring + (it % kRing) * 2 * L::kTileCodes;
-        const int y = j0 + (it * kAttendWarps + warp) * kTile, z = slot * p.c.n_heads + h;
+        const int y = j0 + (it * kWarps + warp) * kTile, z = slot * p.c.n_heads + h;
         mbar_expect_tx(&ring_bar[it % kRing], 2 * L::kTileCodes);
         tma_load_3d(to, &map_k, &ring_bar[it % kRing], 0, y, z);
         tma_load_3d(to + L::kTileCodes, &map_v, &ring_bar[it % kRing], 0, y, z);
     };
-    const int turns = max(0, (here - warp * kTile + kTile * kAttendWarps - 1) / (kTile * kAttendWarps));   // tiles of this warp
+    const int turns = max(0, (here - warp * kTile + kTile * kWarps - 1) / (kTile * kWarps));   // tiles of this warp
     if (lane == 0) {
 #pragma unroll
         for (int i = 0; i < kRing; i++) mbar_init(&ring_bar[i], 1);
@@ -374,7 +387,7 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
     if (lane == 0) s_top[warp] = top;
     __syncthreads();
     top = s_top[0];
-    for (int w = 1; w < kAttendWarps; w++) top = max(top, s_top[w]);
+    for (int w = 1; w < kWarps; w++) top = max(top, s_top[w]);
     // 2^te is not below any value's step (where 2^-100 is not above all); weights are
     // taken 2^up-fold, which brings weight times step, for weights up to 2^8, below 2^15
     const int te = top == 0 ? 0 : max((int)(top >> 23) - 126, -100), up = 7 - te;
@@ -382,10 +395,10 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
     for (int i = 0; i < kUnit / THREADS; i++) sc[tid + i * THREADS] = raw[i];
     __syncthreads();
 
-    const int warps = max(1, min(kAttendWarps, (here + kTile - 1) / kTile));   // that have a tile
+    const int warps = max(1, min(kWarps, (here + kTile - 1) / kTile));   // that have a tile
     constexpr int LD = D + 4;
     float *so = reinterpret_cast<float *>(smem);   // [warp][row][LD], over codes and ranges once all are read
-    static_assert(kAttendWarps * R * LD * 4 <= L::kBars, "the warps' sums fit where the codes were");
+    static_assert(kWarps * R * LD * 4 <= L::kBars, "the warps' sums fit where the codes were");
     // scores of this CTA's rows from entry j0 on, kept for the weights
     float *score = TRACK ? p.score + (((int64_t)b * p.c.n_heads + h) * p.rows + rb * R) * p.max_len + j0 : nullptr;
     const int rows_here = min(R, p.rows - rb * R);
@@ -432,7 +445,7 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
         float mq[NB][2];   // reference times factor, less `up`
         auto tile_of = [&](int it, auto cut_of) {
             constexpr bool CUT = decltype(cut_of)::value;   // some row does not see some of the tile's entries
-            const int t0 = (it * kAttendWarps + warp) * kTile;
+            const int t0 = (it * kWarps + warp) * kTile;
             const uint32_t ka = smem_addr(ring + (it % kRing) * 2 * L::kTileCodes) + (uint32_t)lm_row * (D / 2), va = ka + L::kTileCodes;
             constexpr int KB = kTile / 16;
             float s[NB][KB][4];
@@ -572,7 +585,7 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
                 mbar_wait(&ring_bar[it % kRing], (it / kRing) & 1, nullptr);   // once more for the copies, before anything ends
             }
             __syncwarp();
-            if ((it * kAttendWarps + warp + 1) * kTile > least) tile_of(it, std::true_type{}); else tile_of(it, std::false_type{});
+            if ((it * kWarps + warp + 1) * kTile > least) tile_of(it, std::true_type{}); else tile_of(it, std::false_type{});
             __syncwarp();   // all lanes have read the tile
             if (lane == 0 && it + kRing < turns) ask(it + kRing);
         }
@@ -657,8 +670,8 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
 // Joins the units of rows: the first row_ctas CTAs of x write the rows' results, the others
 // the weights of kUnit entries each.  A row's units are taken in RUNS interleaved runs and
 // those in order: places that depend on its length alone.  Up to kFew units make one run,
-// and the first CTA takes all rows of them (row_ctas is 1 where no sequence may have more).
-constexpr int kJoinThreads = 256, kFew = 16, kMany = 1024;
+// and a CTA takes RUNS rows of them (so fewer row_ctas do where no sequence may have more).
+constexpr int kJoinThreads = 256, kFew = 8, kMany = 1024;
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads) k_kv4_join(const __grid_constant__ AttendArgs p, int rows_padded, int row_ctas) {
     constexpr int TR = D / 4, RUNS = kJoinThreads / TR;   // TR threads a run, four dimensions each
@@ -671,20 +684,32 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv4_join(const __grid_constant
     if ((int)blockIdx.x < row_ctas) {
         const int d = 4 * (tid % TR), run = tid / TR;
         if (units <= kFew) {
-            if (blockIdx.x > 0) return;
-            for (int r = run; r < p.rows; r += RUNS) {
-                float m = -INFINITY, l = 0.0f;
-                float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                for (int u = 0; u < units; u++) m = fmaxf(m, p.stat[first + (int64_t)u * rows_padded + r].x);
-#pragma unroll 8
-                for (int u = 0; u < units; u++) {
-                    const int64_t at = first + (int64_t)u * rows_padded + r;
-                    const float2 st = p.stat[at];
-                    add_scaled(x, share(st.x, m), *reinterpret_cast<const float4 *>(p.part + at * D + d));
-                    l = __fmaf_rn(share(st.x, m), st.y, l);
+            // each CTA the next RUNS rows
+            const int r = blockIdx.x * RUNS + run;
+            if (r >= p.rows) return;
+            float2 st[kFew];
+            float4 v[kFew];
+            float m = -INFINITY, l = 0.0f;
+            float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int u = 0; u < kFew; u++) {
+                const int64_t at = first + (int64_t)min(u, units - 1) * rows_padded + r;
+                if (units > 0) {
+                    st[u] = p.stat[at];
+                    v[u] = *reinterpret_cast<const float4 *>(p.part + at * D + d);
                 }
-                store4(static_cast<T *>(p.out) + row_offset(p, p.os, b, h, r) + d, x, l == 0.0f ? 0.0f : 1.0f / l, p.out_vec);
             }
+#pragma unroll
+            for (int u = 0; u < kFew; u++)
+                if (u < units) m = fmaxf(m, st[u].x);
+#pragma unroll
+            for (int u = 0; u < kFew; u++)
+                if (u < units) {
+                    const float f = share(st[u].x, m);
+                    add_scaled(x, f, v[u]);
+                    l = __fmaf_rn(f, st[u].y, l);
+                }
+            store4(static_cast<T *>(p.out) + row_offset(p, p.os, b, h, r) + d, x, l == 0.0f ? 0.0f : 1.0f / l, p.out_vec);
             return;
         }
         __shared__ float s_f[kMany], red[kJoinThreads / 32];
@@ -731,13 +756,24 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv4_join(const __grid_constant
     float add[kUnit / kJoinThreads] = {};
     for (int r0 = 0; r0 < p.rows; r0 += RB) {
         __syncthreads();
-        for (int r = r0 + (tid >> 5); r < min(r0 + RB, p.rows); r += kJoinThreads / 32) {
-            float m = -INFINITY, l = 0.0f;
-            for (int u = tid & 31; u < units; u += 32) m = fmaxf(m, p.stat[first + (int64_t)u * rows_padded + r].x);
+        constexpr int EACH = RB / (kJoinThreads / 32);
+        float2 st[EACH];   // a warp's rows, the first 32 units of each under way together
+#pragma unroll
+        for (int i = 0; i < EACH; i++) {
+            const int r = r0 + (tid >> 5) + i * (kJoinThreads / 32);
+            st[i] = r < p.rows && (tid & 31) < units ? p.stat[first + (int64_t)(tid & 31) * rows_padded + r] : make_float2(-INFINITY, 0.0f);
+        }
+#pragma unroll
+        for (int i = 0; i < EACH; i++) {
+            const int r = r0 + (tid >> 5) + i * (kJoinThreads / 32);
+            if (r >= p.rows) break;
+            float m = st[i].x;
+            for (int u = (tid & 31) + 32; u < units; u += 32) m = fmaxf(m, p.stat[first + (int64_t)u * rows_padded + r].x);
             for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-            for (int u = tid & 31; u < units; u += 32) {
-                const float2 st = p.stat[first + (int64_t)u * rows_padded + r];
-                l += st.y * share(st.x, m);
+            float l = st[i].y * share(st[i].x, m);
+            for (int u = (tid & 31) + 32; u < units; u += 32) {
+                const float2 more = p.stat[first + (int64_t)u * rows_padded + r];
+                l += more.y * share(more.x, m);
             }
             for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
             if ((tid & 31) == 0) s_row[r - r0] = make_float2(m, l == 0.0f ? 0.0f : 1.0f / l);
@@ -814,19 +850,20 @@ int append(const czg_kv4 &c, const void *k, Strides ks, const void *v, Strides v
 
 template <typename T>
 int read(const czg_kv4 &c, const int32_t *slots, const int32_t *starts, int b, int count, void *k, void *v, cudaStream_t st) {
-    const int64_t rows = (int64_t)count * c.n_heads;   // of a sequence
-    if (rows >= 1ll << 30) return ops_fail(CZG_E_LIMIT, "too many entries");
+    const int64_t rows = (int64_t)count * c.n_heads, all = rows * b;   // of a sequence, of the call
+    if (all >= 1ll << 31) return ops_fail(CZG_E_LIMIT, "too many entries");
     const int64_t per = 4096 / c.head_dim;
     auto kern = c.head_dim == 64 ? k_kv4_read<T, 64> : k_kv4_read<T, 128>;
-    return ops_cuda(ops_launch(kern, dim3((unsigned)((rows + per - 1) / per), (unsigned)b), 256, 0, st, false, 1, c, slots,
-                               starts, count, (uint32_t)rows, static_cast<T *>(k), static_cast<T *>(v)));
+    return ops_cuda(ops_launch(kern, dim3((unsigned)((all + per - 1) / per)), 256, 0, st, false, 1, c, slots, starts,
+                               (uint32_t)rows, (uint32_t)all, static_cast<T *>(k), static_cast<T *>(v)));
 }
 
 template <typename T, int D, int NB, bool TRACK>
 int attend_with(const AttendPlan &plan, const AttendArgs &p, int b, cudaStream_t st) {
     alignas(64) CUtensorMap mk, mv;
     if (!kv4_map(&mk, p.c.k, p.c) || !kv4_map(&mv, p.c.v, p.c)) return ops_fail(CZG_E_DEVICE, "no tensor map for the cache");
-    const size_t smem = AttendSmem<D>::kBytes;
+    constexpr int kWarps = attend_warps(NB);
+    const size_t smem = AttendSmem<D, kWarps>::kBytes;
     static int ready[64] = {0};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return ops_fail(CZG_E_DEVICE, "no device");
@@ -836,9 +873,10 @@ int attend_with(const AttendPlan &plan, const AttendArgs &p, int b, cudaStream_t
         ready[dev] = 1;
     }
     const dim3 grid((unsigned)plan.units, (unsigned)(p.c.n_heads * plan.row_blocks), (unsigned)b);
-    if (int e = ops_cuda(ops_launch(k_kv4_attend<T, D, NB, TRACK>, grid, kAttendWarps * 32, smem, st, false, 1, mk, mv, p))) return e;
+    if (int e = ops_cuda(ops_launch(k_kv4_attend<T, D, NB, TRACK>, grid, kWarps * 32, smem, st, false, 1, mk, mv, p))) return e;
     if (!plan.join) return CZG_OK;
-    const int row_ctas = plan.units <= kFew ? 1 : plan.rows;
+    constexpr int kRuns = kJoinThreads / (D / 4);
+    const int row_ctas = plan.units <= kFew ? (plan.rows + kRuns - 1) / kRuns : plan.rows;
     const dim3 join((unsigned)(row_ctas + (TRACK ? plan.units : 0)), (unsigned)p.c.n_heads, (unsigned)b);
     return ops_cuda(ops_launch(k_kv4_join<T, D>, join, kJoinThreads, 0, st, true, 1, p, plan.row_blocks * 8 * NB, row_ctas));
 }
