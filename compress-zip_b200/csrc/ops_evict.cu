@@ -51,7 +51,7 @@ __device__ __forceinline__ uint32_t scan(uint32_t x, uint32_t *before, uint32_t 
 //    no place is written before it was read.
 // Bound by reading and writing what moves; measured beside the launch below.
 template <int D>
-__global__ void __launch_bounds__(kThreads) k_kv4_evict(czg_kv4 c, const int32_t *__restrict__ slots,
+__global__ void __launch_bounds__(kThreads, 2) k_kv4_evict(czg_kv4 c, const int32_t *__restrict__ slots,
                                                         const int32_t *__restrict__ lengths, int b, int max_len, int budget,
                                                         int recent, int32_t *__restrict__ kept, int32_t *__restrict__ new_len) {
     __shared__ uint32_t hist[kBins], part[kWarps];
@@ -145,30 +145,40 @@ __global__ void __launch_bounds__(kThreads) k_kv4_evict(czg_kv4 c, const int32_t
         __syncthreads();
         if (kp)
             for (int i = tid; i < count; i += kThreads) kp[done + i] = stay_list[i];
-        // a row's pieces: D / 32 of keys, as many of values; its range and weight go with the first
-        constexpr int PIECES = D / 16, ROWS = kThreads * kTasks / PIECES;
+        // a row's pieces: D / 32 of keys and as many of values; ranges and weights go a thread a row
+        constexpr int PIECES = D / 16, ROWS = kThreads * kTasks / PIECES, OWN = ROWS / kThreads;
         for (int r0 = 0; r0 < count; r0 += ROWS) {
             uint4 piece[kTasks];
-            KvScale sc[kTasks];
-            float weight[kTasks];
+            KvScale sc[OWN];
+            float weight[OWN];
 #pragma unroll
             for (int k = 0; k < kTasks; k++) {
                 const int task = k * kThreads + tid, r = r0 + task / PIECES, p = task % PIECES;
-                if (r >= count || stay_list[r] == done + r) continue;
-                const int64_t from = base + stay_list[r];
-                piece[k] = reinterpret_cast<const uint4 *>((p < PIECES / 2 ? c.k : c.v) + from * (D / 2))[p % (PIECES / 2)];
-                if (p == 0) sc[k] = static_cast<const KvScale *>(c.scales)[from];
-                if (p == 1) weight[k] = c.weights[from];
+                if (r < count && stay_list[r] != done + r)
+                    piece[k] = reinterpret_cast<const uint4 *>((p < PIECES / 2 ? c.k : c.v) + (base + stay_list[r]) * (D / 2))[p % (PIECES / 2)];
+            }
+#pragma unroll
+            for (int k = 0; k < OWN; k++) {
+                const int r = r0 + k * kThreads + tid;
+                if (r < count && stay_list[r] != done + r) {
+                    sc[k] = static_cast<const KvScale *>(c.scales)[base + stay_list[r]];
+                    weight[k] = w[stay_list[r]];
+                }
             }
             __syncthreads();   // all of these are read
 #pragma unroll
             for (int k = 0; k < kTasks; k++) {
                 const int task = k * kThreads + tid, r = r0 + task / PIECES, p = task % PIECES;
-                if (r >= count || stay_list[r] == done + r) continue;
-                const int64_t to = base + done + r;
-                reinterpret_cast<uint4 *>((p < PIECES / 2 ? c.k : c.v) + to * (D / 2))[p % (PIECES / 2)] = piece[k];
-                if (p == 0) static_cast<KvScale *>(c.scales)[to] = sc[k];
-                if (p == 1) c.weights[to] = weight[k];
+                if (r < count && stay_list[r] != done + r)
+                    reinterpret_cast<uint4 *>((p < PIECES / 2 ? c.k : c.v) + (base + done + r) * (D / 2))[p % (PIECES / 2)] = piece[k];
+            }
+#pragma unroll
+            for (int k = 0; k < OWN; k++) {
+                const int r = r0 + k * kThreads + tid;
+                if (r < count && stay_list[r] != done + r) {
+                    static_cast<KvScale *>(c.scales)[base + done + r] = sc[k];
+                    w[done + r] = weight[k];
+                }
             }
         }
         done += count;

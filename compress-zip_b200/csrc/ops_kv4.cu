@@ -780,7 +780,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv4_join(const __grid_constant
         }
         __syncthreads();
         const float *s = p.score + (((int64_t)b * p.c.n_heads + h) * p.rows + r0) * p.max_len + j0 + tid;
-#pragma unroll 8
+#pragma unroll 16
         for (int r = 0; r < min(RB, p.rows - r0); r++) {
             const int seen = n - (p.t - 1 - row_place(p, r0 + r)) - j0 - tid;
             const float2 row = s_row[r];
