@@ -688,27 +688,27 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv4_join(const __grid_constant
             const int r = blockIdx.x * RUNS + run;
             if (r >= p.rows) return;
             float2 st[kFew];
-            float4 v[kFew];
             float m = -INFINITY, l = 0.0f;
             float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            const int64_t at = first + r;
 #pragma unroll
-            for (int u = 0; u < kFew; u++) {
-                const int64_t at = first + (int64_t)min(u, units - 1) * rows_padded + r;
-                if (units > 0) {
-                    st[u] = p.stat[at];
-                    v[u] = *reinterpret_cast<const float4 *>(p.part + at * D + d);
-                }
+            for (int u = 0; u < kFew; u++) st[u] = u < units ? p.stat[at + (int64_t)u * rows_padded] : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+            for (int u = 0; u < kFew; u++) m = fmaxf(m, st[u].x);
+#pragma unroll
+            for (int u0 = 0; u0 < kFew; u0 += 4) {
+                float4 v[4];
+#pragma unroll
+                for (int u = 0; u < 4; u++)
+                    if (u0 + u < units) v[u] = *reinterpret_cast<const float4 *>(p.part + (at + (int64_t)(u0 + u) * rows_padded) * D + d);
+#pragma unroll
+                for (int u = 0; u < 4; u++)
+                    if (u0 + u < units) {
+                        const float f = share(st[u0 + u].x, m);
+                        add_scaled(x, f, v[u]);
+                        l = __fmaf_rn(f, st[u0 + u].y, l);
+                    }
             }
-#pragma unroll
-            for (int u = 0; u < kFew; u++)
-                if (u < units) m = fmaxf(m, st[u].x);
-#pragma unroll
-            for (int u = 0; u < kFew; u++)
-                if (u < units) {
-                    const float f = share(st[u].x, m);
-                    add_scaled(x, f, v[u]);
-                    l = __fmaf_rn(f, st[u].y, l);
-                }
             store4(static_cast<T *>(p.out) + row_offset(p, p.os, b, h, r) + d, x, l == 0.0f ? 0.0f : 1.0f / l, p.out_vec);
             return;
         }
@@ -780,7 +780,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv4_join(const __grid_constant
         }
         __syncthreads();
         const float *s = p.score + (((int64_t)b * p.c.n_heads + h) * p.rows + r0) * p.max_len + j0 + tid;
-#pragma unroll 16
+#pragma unroll 8
         for (int r = 0; r < min(RB, p.rows - r0); r++) {
             const int seen = n - (p.t - 1 - row_place(p, r0 + r)) - j0 - tid;
             const float2 row = s_row[r];
