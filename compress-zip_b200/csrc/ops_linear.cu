@@ -177,9 +177,10 @@ __global__ void __launch_bounds__(kQuantThreads) k_quantize_rows(const T *__rest
 //   the others  epilogue, EW / 4 warps a quadrant of TMEM lanes
 // S = 1: the CTA walks tiles (gridDim.x apart) with two accumulators, so the epilogue of
 // one overlaps the MMAs of the next.  S > 1 (few tokens): a cluster of S CTAs shares one
-// tile, each a stretch of k; each sends its int32 sums of tokens j to CTA j / (NT / S)
-// through distributed shared memory, and that one adds them up: integers, so the split
-// does not show in the result.
+// tile, each a stretch of k; each lays its int32 sums down in its shared memory, and CTA r
+// adds up all CTAs' sums of the tokens r NT / S .. (16 bytes a lane through distributed
+// shared memory; 4-byte stores to the other CTAs instead took 4 us more at NT = 64):
+// integers, so the split does not show in the result.
 constexpr int LT = 128;   // channels of a tile
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -189,10 +190,12 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-__device__ __forceinline__ void store_remote(uint32_t addr, uint32_t rank, uint32_t v) {
+__device__ __forceinline__ int4 load_remote(uint32_t addr, uint32_t rank) {
     uint32_t a;
+    int4 v;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
-    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
+    asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+    return v;
 }
 
 // Barrier of the N threads of the epilogue, and whether any of them says so.
@@ -209,7 +212,7 @@ struct LinearArgs {
     const float *xs, *ws, *bias;
     void *out;
     int64_t ldo;
-    int m, n, steps, tiles_n, tiles, stages, split;
+    int m, n, steps, tiles_n, tiles, stages, split, vec_out;
 };
 
 template <int NT>
@@ -237,7 +240,7 @@ k_linear_tc(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ C
     constexpr int COLS = 2 * NT < 32 ? 32 : 2 * NT;
     const int STAGES = p.stages, S = p.split;
     uint8_t *tail = smem + STAGES * STAGE;
-    int *sums = reinterpret_cast<int *>(tail);   // S > 1: [from][token][channel]
+    int *sums = reinterpret_cast<int *>(tail);   // S > 1: [token][channel]
     if (S > 1) tail += LT * NT * 4;
     uint64_t *full = reinterpret_cast<uint64_t *>(tail);
     uint64_t *empty = full + STAGES;
@@ -252,6 +255,7 @@ k_linear_tc(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ C
     const int rank = S > 1 ? (int)cluster_rank() : 0;
     const int k0 = (int)((int64_t)p.steps * rank / S), k1 = (int)((int64_t)p.steps * (rank + 1) / S);
     const int tile0 = S > 1 ? blockIdx.x / S : blockIdx.x, dt = S > 1 ? gridDim.x / S : gridDim.x;
+    const int early = min(STAGES, k1 - k0);   // stages of the first tile that need no wait
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; s++) {
             mbar_init(&full[s], 1);
@@ -264,6 +268,14 @@ k_linear_tc(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ C
         mbar_init(drain, 1);
         abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        // the first loads are on their way before the others are through the setup
+        const int n0 = (tile0 % p.tiles_n) * LT, m0 = (tile0 / p.tiles_n) * NT;
+        for (int i = 0; i < early; i++) {
+            mbar_expect_tx(&full[i], STAGE);
+            tma_load_2d(smem + i * STAGE, &map_w, &full[i], (k0 + i) * TC_BK, n0);
+        }
+        pdl_wait();
+        for (int i = 0; i < early; i++) tma_load_2d(smem + i * STAGE + W_BYTES, &map_x, &full[i], (k0 + i) * TC_BK, m0);
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(COLS));
@@ -273,32 +285,22 @@ k_linear_tc(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ C
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *tmem_slot;
-    if (S > 1) cluster_arrive();   // waited for before the first store to another CTA: it has begun by then
-
     if (warp == 0) {
         if (lane == 0) {
             int it = 0;
             bool ok = true;
-            const int early = min(STAGES, k1 - k0);   // stages of the first tile that need no wait
-            const int n0 = (tile0 % p.tiles_n) * LT;
-            for (int i = 0; i < early; i++) {
-                mbar_expect_tx(&full[i], STAGE);
-                tma_load_2d(smem + i * STAGE, &map_w, &full[i], (k0 + i) * TC_BK, n0);
-            }
-            pdl_wait();
             for (int tile = tile0; tile < p.tiles && ok; tile += dt) {
-                const int n0t = (tile % p.tiles_n) * LT, m0 = (tile / p.tiles_n) * NT;
+                const int n0 = (tile % p.tiles_n) * LT, m0 = (tile / p.tiles_n) * NT;
                 for (int kb = k0; kb < k1; kb++, it++) {
+                    if (it < early) continue;   // under way already
                     const int s = it % STAGES;
                     uint8_t *sw = smem + s * STAGE;
-                    if (it >= early) {
-                        if (it >= STAGES && !mbar_wait(&empty[s], ((it / STAGES) - 1) & 1, &abort_flag)) {
-                            ok = false;
-                            break;
-                        }
-                        mbar_expect_tx(&full[s], STAGE);
-                        tma_load_2d(sw, &map_w, &full[s], kb * TC_BK, n0t);
+                    if (it >= STAGES && !mbar_wait(&empty[s], ((it / STAGES) - 1) & 1, &abort_flag)) {
+                        ok = false;
+                        break;
                     }
+                    mbar_expect_tx(&full[s], STAGE);
+                    tma_load_2d(sw, &map_w, &full[s], kb * TC_BK, n0);
                     tma_load_2d(sw + W_BYTES, &map_x, &full[s], kb * TC_BK, m0);
                 }
             }
@@ -348,7 +350,6 @@ k_linear_tc(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ C
         const int part = (warp - 2) >> 2;   // of EW / 4 parts of the tokens
         constexpr int PC = NT / (EW / 4);   // tokens of a part
         pdl_wait();
-        if (S > 1) cluster_wait();
         T *out = static_cast<T *>(p.out);
         int tc = 0;
         for (int tile = tile0; tile < p.tiles; tile += dt, tc++) {
@@ -382,11 +383,8 @@ k_linear_tc(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ C
                 }
                 const int j0 = part * PC + c0;
                 if (S > 1) {
-                    const int lg = 31 - __clz(NT / S), per = NT / S;   // both powers of two
-                    const uint32_t mine = smem_addr(sums + rank * per * LT + 32 * q + lane);
 #pragma unroll
-                    for (int j = 0; j < CW; j++)
-                        store_remote(mine + (uint32_t)(((j0 + j) & (per - 1)) * LT * 4), (uint32_t)((j0 + j) >> lg), v[j]);
+                    for (int j = 0; j < CW; j++) sums[(j0 + j) * LT + 32 * q + lane] = (int)v[j];
                 } else if (there) {
                     T *o = out + (int64_t)(m0 + j0) * p.ldo + ch;
                     const int most = p.m - m0 - j0;
@@ -399,21 +397,49 @@ k_linear_tc(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ C
     }
     if (S > 1) {
         __syncwarp();
-        if (warp < 2) cluster_wait();
         cluster_arrive();
-        cluster_wait();   // every CTA of the cluster comes here, whatever it met
-        if (warp >= 2 && !abort_flag) {
-            const int per = NT / S, ch = (tile0 % p.tiles_n) * LT + 32 * (warp & 3) + lane;
-            const int m0 = (tile0 / p.tiles_n) * NT + rank * per;
-            if (ch < p.n) {
-                const float ws = p.ws[ch], bias = p.bias ? p.bias[ch] : 0.0f;
-                for (int j = (warp - 2) >> 2; j < per && m0 + j < p.m; j += EW / 4) {
-                    int acc = 0;
-                    for (int r = 0; r < S; r++) acc += sums[(r * per + j) * LT + 32 * (warp & 3) + lane];
-                    static_cast<T *>(p.out)[(int64_t)(m0 + j) * p.ldo + ch] = finish<T>(acc, p.xs[m0 + j], ws, bias, p.bias != nullptr);
+        cluster_wait();   // every CTA of the cluster comes here, whatever it met, and has laid its sums down
+        if (warp >= 2) {
+            const int per = NT / S, n0 = (tile0 % p.tiles_n) * LT + 4 * lane, m0 = (tile0 / p.tiles_n) * NT + rank * per;
+            const bool vec = p.vec_out && n0 + 4 <= p.n;
+            float ws[4], bias[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                ws[i] = n0 + i < p.n ? p.ws[n0 + i] : 0.0f;
+                bias[i] = n0 + i < p.n && p.bias ? p.bias[n0 + i] : 0.0f;
+            }
+#pragma unroll 4
+            for (int j = warp - 2; j < per; j += EW) {
+                if (m0 + j >= p.m) break;
+                int acc[4] = {0, 0, 0, 0};
+                const uint32_t at = smem_addr(sums + (rank * per + j) * LT + 4 * lane);
+#pragma unroll
+                for (int r = 0; r < 8; r++)
+                    if (r < S) {
+                        const int4 v = load_remote(at, r);
+                        acc[0] += v.x;
+                        acc[1] += v.y;
+                        acc[2] += v.z;
+                        acc[3] += v.w;
+                    }
+                const float xs = p.xs[m0 + j];
+                __align__(16) T y[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) y[i] = finish<T>(acc[i], xs, ws[i], bias[i], p.bias != nullptr);
+                T *o = static_cast<T *>(p.out) + (int64_t)(m0 + j) * p.ldo + n0;
+                if (vec) {
+                    if (sizeof(T) == 4) *reinterpret_cast<uint4 *>(o) = *reinterpret_cast<const uint4 *>(y);
+                    else *reinterpret_cast<uint2 *>(o) = *reinterpret_cast<const uint2 *>(y);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (n0 + i < p.n) o[i] = y[i];
                 }
             }
         }
+        __syncwarp();
+        cluster_arrive();
+        cluster_wait();   // no CTA ends while another reads its sums
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
@@ -469,7 +495,7 @@ LinearShape linear_shape(int64_t m, int64_t n, int steps) {
     for (int nt : {16, 32, 64, 128, 256}) {
         const int64_t tiles = tiles_n * ((m + nt - 1) / nt);
         for (int s : {1, 2, 4, 8}) {
-            if (s > 1 && (nt > 64 || s > steps || tiles * s > sms)) break;
+            if (s > 1 && (nt > 128 || nt * s > 256 || s > steps || tiles * s > sms)) break;
             const double waves = (double)((tiles * s + sms - 1) / sms);
             const double step = std::fmax(2.0 * nt, (16384.0 + 128.0 * nt) / 48.0);
             const double cost = waves * ((steps + s - 1) / s) * step + 1500 + 12.0 * nt + (s > 1 ? 1000 : 0);
@@ -501,8 +527,9 @@ int quantize_any(const void *x, int dtype, int64_t ldx, int64_t m, int64_t k, in
 template <typename T>
 int linear(const int8_t *x, int64_t ldx, const float *xs, const int8_t *w, int64_t ldw, const float *ws, const float *bias,
            int64_t m, int64_t n, int64_t k, void *out, int64_t ldo, bool after_quantise, cudaStream_t st) {
-    LinearArgs p{xs, ws, bias, out, ldo, (int)m, (int)n, (int)((k + TC_BK - 1) / TC_BK), (int)((n + LT - 1) / LT), 0, 0, 1};
-    const LinearShape shape = linear_shape(m, n, p.steps);
+    LinearArgs p{xs, ws, bias, out, ldo, (int)m, (int)n, (int)((k + TC_BK - 1) / TC_BK), (int)((n + LT - 1) / LT), 0, 0, 1,
+                 aligned(out, 4 * sizeof(T)) && ldo % 4 == 0};
+    LinearShape shape = linear_shape(m, n, p.steps);
     p.split = shape.split;
     if (shape.nt == 16) return launch_linear<16, T>(x, ldx, w, ldw, k, p, after_quantise, st);
     if (shape.nt == 32) return launch_linear<32, T>(x, ldx, w, ldw, k, p, after_quantise, st);
