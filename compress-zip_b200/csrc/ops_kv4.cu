@@ -1,5 +1,6 @@
 // ops_kv4.cu -- the key/value cache held in 4 bits (include/czg_ops.h): append, read
 // and attention.
+#include <atomic>
 #include <cmath>
 #include <type_traits>
 
@@ -864,7 +865,7 @@ int attend_with(const AttendPlan &plan, const AttendArgs &p, int b, cudaStream_t
     if (!kv4_map(&mk, p.c.k, p.c) || !kv4_map(&mv, p.c.v, p.c)) return ops_fail(CZG_E_DEVICE, "no tensor map for the cache");
     constexpr int kWarps = attend_warps(NB);
     const size_t smem = AttendSmem<D, kWarps>::kBytes;
-    static int ready[64] = {0};
+    static std::atomic<int> ready[64];
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return ops_fail(CZG_E_DEVICE, "no device");
     if (!ready[dev]) {

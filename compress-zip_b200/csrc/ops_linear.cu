@@ -1,7 +1,9 @@
 // ops_linear.cu -- int8 product with a scale for each token and each channel
 // (include/czg_ops.h): the row quantiser and the product.
+#include <atomic>
 #include <cmath>
 #include <string>
+#include <type_traits>
 
 #include "ops_common.cuh"
 #include "tc_common.cuh"
@@ -98,6 +100,28 @@ __device__ __forceinline__ void load8(const T *row, int64_t i, int64_t k, bool v
     }
 }
 
+// What a row's maximum (its magnitude's bits) makes of its values.
+template <typename T>
+struct RowScale {
+    float a, f, af, inv;
+    bool fine;
+    __device__ __forceinline__ explicit RowScale(uint32_t m) {
+        fine = m < Raw8<T>::kInf;   // NaN and infinities both end as a row of NaN
+        a = Raw8<T>::value(m);
+        // a power of two keeps a, 127 x and 127 / a far from both ends of fp32, and the quotients as they are
+        f = a > 1.2676506e30f ? 9.5367431640625e-7f : a < 8.6736174e-19f ? 1.2089258196146292e24f : 1.0f;
+        af = a * f;
+        inv = __fdiv_rn(127.0f, af);
+    }
+    __device__ __forceinline__ float scale() const { return fine ? __fdiv_rn(a, 127.0f) : NAN; }
+    __device__ __forceinline__ uint2 codes(const Raw8<T> &w) const {
+        float x8[8];
+#pragma unroll
+        for (int c = 0; c < 8; c++) x8[c] = w.get(c) * f;
+        return fine && a > 0.0f ? codes8(x8, af, inv) : make_uint2(0, 0);
+    }
+};
+
 // One CTA a row: its maximum, then its codes, 8 values a thread and turn; rows of up to
 // kHeld turns stay in registers between the two, longer ones are read again.
 constexpr int kQuantThreads = 256, kHeld = 4;
@@ -134,19 +158,9 @@ __global__ void __launch_bounds__(kQuantThreads) k_quantize_rows(const T *__rest
         m = part[(threadIdx.x & 31) < blockDim.x / 32 ? threadIdx.x & 31 : 0];
         m = __reduce_max_sync(0xffffffffu, m);
     }
-    const bool fine = m < Raw8<T>::kInf;   // NaN and infinities both end as a row of NaN
-    const float a = Raw8<T>::value(m);
-    if (threadIdx.x == 0) scales[blockIdx.x] = fine ? __fdiv_rn(a, 127.0f) : NAN;
-    // a power of two keeps a, 127 x and 127 / a far from both ends of fp32, and the quotients as they are
-    const float f = a > 1.2676506e30f ? 9.5367431640625e-7f : a < 8.6736174e-19f ? 1.2089258196146292e24f : 1.0f;
-    const float af = a * f, inv = __fdiv_rn(127.0f, af);
-    const bool some = fine && a > 0.0f;
-    auto put = [&](int64_t i, const Raw8<T> &w) {
-        float x8[8];
-#pragma unroll
-        for (int c = 0; c < 8; c++) x8[c] = w.get(c) * f;
-        *reinterpret_cast<uint2 *>(out + i) = some ? codes8(x8, af, inv) : make_uint2(0, 0);
-    };
+    const RowScale<T> rs(m);
+    if (threadIdx.x == 0) scales[blockIdx.x] = rs.scale();
+    auto put = [&](int64_t i, const Raw8<T> &w) { *reinterpret_cast<uint2 *>(out + i) = rs.codes(w); };
     if (held) {
 #pragma unroll
         for (int t = 0; t < kHeld; t++)
@@ -213,7 +227,12 @@ struct LinearArgs {
     void *out;
     int64_t ldo;
     int m, n, steps, tiles_n, tiles, stages, split, vec_out;
+    const void *x;   // of the kernel that quantises: [m][k], ldx elements apart, vec: rows of 16-byte pieces
+    int64_t ldx;
+    int k, vec;
 };
+
+constexpr int kRingBytes = 220 * 1024;   // of shared memory, for the ring and the sums
 
 template <int NT>
 struct LinearCfg {
@@ -231,13 +250,18 @@ __device__ __forceinline__ T finish(int acc, float xs, float ws, float bias, boo
     return from_f32<T>(y);
 }
 
-template <int NT, typename T>
+// TX: void, or the type of x rows that the kernel quantises itself.  Then every CTA reads
+// all of x for the rows' maxima and writes the codes of its stretch of k where TMA would
+// have put them; a cluster has one tile and the ring holds all of it.  For a few short
+// rows, where a launch costs more than reading x once in every CTA.
+template <int NT, typename T, typename TX>
 __global__ void __launch_bounds__(LinearCfg<NT>::kWarps * 32, 1)
 k_linear_tc(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, LinearArgs p) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     constexpr int STAGE = LinearCfg<NT>::kStage, W_BYTES = LT * TC_BK, EW = LinearCfg<NT>::kWarps - 2;
     constexpr int COLS = 2 * NT < 32 ? 32 : 2 * NT;
+    constexpr bool kQuantises = !std::is_void<TX>::value;
     const int STAGES = p.stages, S = p.split;
     uint8_t *tail = smem + STAGES * STAGE;
     int *sums = reinterpret_cast<int *>(tail);   // S > 1: [token][channel]
@@ -271,15 +295,47 @@ k_linear_tc(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ C
         // the first loads are on their way before the others are through the setup
         const int n0 = (tile0 % p.tiles_n) * LT, m0 = (tile0 / p.tiles_n) * NT;
         for (int i = 0; i < early; i++) {
-            mbar_expect_tx(&full[i], STAGE);
+            mbar_expect_tx(&full[i], kQuantises ? W_BYTES : STAGE);
             tma_load_2d(smem + i * STAGE, &map_w, &full[i], (k0 + i) * TC_BK, n0);
         }
         pdl_wait();
-        for (int i = 0; i < early; i++) tma_load_2d(smem + i * STAGE + W_BYTES, &map_x, &full[i], (k0 + i) * TC_BK, m0);
+        for (int i = 0; i < early && !kQuantises; i++) tma_load_2d(smem + i * STAGE + W_BYTES, &map_x, &full[i], (k0 + i) * TC_BK, m0);
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(COLS));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    if constexpr (kQuantises) {
+        constexpr int THREADS = LinearCfg<NT>::kWarps * 32;
+        __shared__ uint32_t s_most[NT];
+        if (threadIdx.x < NT) s_most[threadIdx.x] = 0;
+        __syncthreads();
+        const TX *x = static_cast<const TX *>(p.x);
+#pragma unroll 4
+        for (int r = 0; r < p.m; r++) {
+            uint32_t most = 0;
+#pragma unroll 4
+            for (int i = threadIdx.x * 8; i < p.k; i += THREADS * 8) {
+                Raw8<TX> v;
+                load8(x + r * p.ldx, i, p.k, p.vec, v);
+                most = v.most(most);
+            }
+            if (sizeof(TX) == 2) most = max(most & 0xFFFFu, most >> 16);
+            most = __reduce_max_sync(0xffffffffu, most);
+            if (lane == 0) atomicMax(&s_most[r], most);   // a maximum: in any order
+        }
+        __syncthreads();
+        const int pieces = (k1 - k0) * (TC_BK / 8);   // of 8 values, of a row
+        for (int t = threadIdx.x; t < p.m * pieces; t += THREADS) {
+            const int r = t / pieces, at = t - r * pieces, step = at / (TC_BK / 8), c = at % (TC_BK / 8) / 2;
+            Raw8<TX> v;
+            load8(x + r * p.ldx, (k0 * (TC_BK / 8) + at) * 8, p.k, p.vec, v);
+            // row r of a box, its 16-byte piece c: the 128-byte swizzle
+            *reinterpret_cast<uint2 *>(smem + step * STAGE + W_BYTES + r * TC_BK + ((c ^ (r & 7)) << 4) + 8 * (at & 1)) =
+                RowScale<TX>(s_most[r]).codes(v);
+        }
+        if (threadIdx.x < NT) s_xs[threadIdx.x] = (int)threadIdx.x < p.m ? RowScale<TX>(s_most[threadIdx.x]).scale() : 0.0f;
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the MMAs read what the threads wrote
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
@@ -359,7 +415,7 @@ k_linear_tc(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ C
             const bool there = ch < p.n;
             const float ws = there ? p.ws[ch] : 0.0f, bias = there && p.bias ? p.bias[ch] : 0.0f;
             float *xs = s_xs + b * NT;      // the accumulator's half: its readers are done when tempty[b] fired
-            if (S == 1)
+            if (S == 1 && !kQuantises)
                 for (int i = threadIdx.x - 64; i < NT; i += EW * 32) xs[i] = m0 + i < p.m ? p.xs[m0 + i] : 0.0f;
             const bool got = mbar_wait(&tfull[b], (tc >> 1) & 1, &abort_flag);
             if (epilogue_any<EW * 32>(!got)) {   // one answer for all of them: no warp waits for one that left
@@ -422,7 +478,7 @@ k_linear_tc(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ C
                         acc[2] += v.z;
                         acc[3] += v.w;
                     }
-                const float xs = p.xs[m0 + j];
+                const float xs = kQuantises ? s_xs[rank * per + j] : p.xs[m0 + j];
                 __align__(16) T y[4];
 #pragma unroll
                 for (int i = 0; i < 4; i++) y[i] = finish<T>(acc[i], xs, ws[i], bias[i], p.bias != nullptr);
@@ -459,30 +515,40 @@ bool codes_map(CUtensorMap *map, const int8_t *p, int64_t ld, int64_t rows, int6
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int NT, typename T>
+template <int NT, typename T, typename TX>
 int launch_linear(const int8_t *x, int64_t ldx, const int8_t *w, int64_t ldw, int64_t k, LinearArgs p, bool after_quantise,
                   cudaStream_t st) {
+    constexpr bool kQuantises = !std::is_void<TX>::value;
     alignas(64) CUtensorMap mw, mx;
-    if (!codes_map(&mw, w, ldw, p.n, k, LT) || !codes_map(&mx, x, ldx, p.m, k, NT))
+    if (!codes_map(&mw, w, ldw, p.n, k, LT) || (!kQuantises && !codes_map(&mx, x, ldx, p.m, k, NT)))
         return ops_fail(CZG_E_DEVICE, "no tensor map for the operands");
     const int64_t tiles = (int64_t)p.tiles_n * ((p.m + NT - 1) / NT);
-    if (tiles > 0x7FFFFFFF) return ops_fail(CZG_E_LIMIT, "too many tiles");
+    if (tiles > 0x7FFFFFFF / 8) return ops_fail(CZG_E_LIMIT, "too many tiles");
     p.tiles = (int)tiles;
     const int per_cta = (p.steps + p.split - 1) / p.split;   // the ring need not be longer than a tile's stretch of k
-    const int fit = (int)((220 * 1024 - (p.split > 1 ? LT * NT * 4 : 0)) / LinearCfg<NT>::kStage);
-    p.stages = per_cta < fit && p.split > 1 ? per_cta : fit;
+    const int fit = (int)((kRingBytes - (p.split > 1 ? LT * NT * 4 : 0)) / LinearCfg<NT>::kStage);
+    if (kQuantises && per_cta > fit) return ops_fail(CZG_E_LIMIT, "more steps than the ring holds");
+    p.stages = per_cta < fit && (p.split > 1 || kQuantises) ? per_cta : fit;
     const size_t smem = LinearCfg<NT>::smem(p.stages, p.split);
-    static int ready[64] = {0};
+    static std::atomic<int> ready[64];
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return ops_fail(CZG_E_DEVICE, "no device");
     if (!ready[dev]) {
-        if (int e = ops_cuda(cudaFuncSetAttribute(k_linear_tc<NT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024)))
+        if (int e = ops_cuda(cudaFuncSetAttribute(k_linear_tc<NT, T, TX>, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024)))
             return e;
         ready[dev] = 1;
     }
-    const int grid = p.split > 1 ? p.tiles * p.split : p.tiles < sm_count() ? p.tiles : sm_count();
-    return ops_cuda(ops_launch(k_linear_tc<NT, T>, dim3((unsigned)grid), LinearCfg<NT>::kWarps * 32, smem, st, after_quantise,
+    const int grid = p.split > 1 || kQuantises ? p.tiles * p.split : p.tiles < sm_count() ? p.tiles : sm_count();
+    return ops_cuda(ops_launch(k_linear_tc<NT, T, TX>, dim3((unsigned)grid), LinearCfg<NT>::kWarps * 32, smem, st, after_quantise,
                                p.split, mw, mx, p));
+}
+
+// Calls whose x rows the product quantises itself: at most 16 rows, 64 KB of bf16 in all, so
+// that reading them in every CTA costs less than a launch (1 x 512 x 384: 10.9 us a call from Python, 14.8 with two kernels).
+constexpr int kSmallRows = 16, kSmallValues = 32768, kSmallSteps = 11;   // steps a CTA's ring holds
+static_assert(kSmallSteps * LinearCfg<kSmallRows>::kStage + LT * kSmallRows * 4 <= kRingBytes, "the codes of all steps have their place");
+bool small_call(int64_t m, int64_t k) {
+    return m <= kSmallRows && m * k <= kSmallValues && k <= 8 * kSmallSteps * TC_BK;
 }
 
 struct LinearShape { int nt, split; };
@@ -531,11 +597,11 @@ int linear(const int8_t *x, int64_t ldx, const float *xs, const int8_t *w, int64
                  aligned(out, 4 * sizeof(T)) && ldo % 4 == 0};
     LinearShape shape = linear_shape(m, n, p.steps);
     p.split = shape.split;
-    if (shape.nt == 16) return launch_linear<16, T>(x, ldx, w, ldw, k, p, after_quantise, st);
-    if (shape.nt == 32) return launch_linear<32, T>(x, ldx, w, ldw, k, p, after_quantise, st);
-    if (shape.nt == 64) return launch_linear<64, T>(x, ldx, w, ldw, k, p, after_quantise, st);
-    if (shape.nt == 128) return launch_linear<128, T>(x, ldx, w, ldw, k, p, after_quantise, st);
-    return launch_linear<256, T>(x, ldx, w, ldw, k, p, after_quantise, st);
+    if (shape.nt == 16) return launch_linear<16, T, void>(x, ldx, w, ldw, k, p, after_quantise, st);
+    if (shape.nt == 32) return launch_linear<32, T, void>(x, ldx, w, ldw, k, p, after_quantise, st);
+    if (shape.nt == 64) return launch_linear<64, T, void>(x, ldx, w, ldw, k, p, after_quantise, st);
+    if (shape.nt == 128) return launch_linear<128, T, void>(x, ldx, w, ldw, k, p, after_quantise, st);
+    return launch_linear<256, T, void>(x, ldx, w, ldw, k, p, after_quantise, st);
 }
 
 int linear_any(const int8_t *x, int64_t ldx, const float *xs, const int8_t *w, int64_t ldw, const float *ws, const float *bias,
@@ -543,6 +609,24 @@ int linear_any(const int8_t *x, int64_t ldx, const float *xs, const int8_t *w, i
     if (dtype == CZG_F32) return linear<float>(x, ldx, xs, w, ldw, ws, bias, m, n, k, out, ldo, after_quantise, st);
     if (dtype == CZG_BF16) return linear<__nv_bfloat16>(x, ldx, xs, w, ldw, ws, bias, m, n, k, out, ldo, after_quantise, st);
     return linear<__half>(x, ldx, xs, w, ldw, ws, bias, m, n, k, out, ldo, after_quantise, st);
+}
+
+template <typename T, typename TX>
+int linear_small(const void *x, int64_t ldx, const int8_t *w, int64_t ldw, const float *ws, const float *bias, int64_t m,
+                 int64_t n, int64_t k, void *out, int64_t ldo, cudaStream_t st) {
+    LinearArgs p{nullptr, ws, bias, out, ldo, (int)m, (int)n, (int)((k + TC_BK - 1) / TC_BK), (int)((n + LT - 1) / LT), 0, 0, 1,
+                 aligned(out, 4 * sizeof(T)) && ldo % 4 == 0, x, ldx, (int)k, aligned(x, 16) && (m == 1 || ldx * sizeof(TX) % 16 == 0)};
+    // as many CTAs as there are SMs, of at least two steps each, and no more steps than the ring holds
+    while (p.split < 8 && (p.steps > p.split * kSmallSteps || (p.tiles_n * p.split * 2 <= sm_count() && p.steps >= p.split * 4))) p.split *= 2;
+    return launch_linear<kSmallRows, T, TX>(nullptr, 0, w, ldw, k, p, false, st);
+}
+
+template <typename T>
+int linear_small_of(int dtype, const void *x, int64_t ldx, const int8_t *w, int64_t ldw, const float *ws, const float *bias,
+                    int64_t m, int64_t n, int64_t k, void *out, int64_t ldo, cudaStream_t st) {
+    if (dtype == CZG_F32) return linear_small<T, float>(x, ldx, w, ldw, ws, bias, m, n, k, out, ldo, st);
+    if (dtype == CZG_BF16) return linear_small<T, __nv_bfloat16>(x, ldx, w, ldw, ws, bias, m, n, k, out, ldo, st);
+    return linear_small<T, __half>(x, ldx, w, ldw, ws, bias, m, n, k, out, ldo, st);
 }
 
 const char *check_codes(const int8_t *p, int64_t ld, int64_t rows, int64_t k) {
@@ -617,7 +701,7 @@ extern "C" int czg_linear_i8(const int8_t *x, int64_t ld_x, const float *x_scale
 }
 
 extern "C" uint64_t czg_linear_i8_workspace(int64_t m, int64_t k) {
-    if (m <= 0 || k <= 0) return 0;
+    if (m <= 0 || k <= 0 || small_call(m, k)) return 0;
     return (uint64_t)m * (uint64_t)codes_ld(k) + (((uint64_t)m * 4 + 15) & ~15ull);
 }
 
@@ -628,9 +712,15 @@ extern "C" int czg_linear_i8_dynamic(const void *x, int dtype, int64_t ld_x, con
     if (m == 0 || n == 0) return CZG_OK;
     if (int st = check_x(x, dtype, ld_x, m, k)) return st;
     if (int st = check_linear(w, ld_w, w_scale, m, n, k, out, out_dtype, ld_out)) return st;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (small_call(m, k)) {
+        if (out_dtype == CZG_F32) return linear_small_of<float>(dtype, x, ld_x, w, ld_w, w_scale, bias, m, n, k, out, ld_out, st);
+        if (out_dtype == CZG_BF16)
+            return linear_small_of<__nv_bfloat16>(dtype, x, ld_x, w, ld_w, w_scale, bias, m, n, k, out, ld_out, st);
+        return linear_small_of<__half>(dtype, x, ld_x, w, ld_w, w_scale, bias, m, n, k, out, ld_out, st);
+    }
     if (!ws || !aligned(ws, 16)) return ops_fail(CZG_E_ARG, "the workspace must begin on a 16-byte boundary");
     if (ws_bytes < czg_linear_i8_workspace(m, k)) return ops_fail(CZG_E_ARG, "the workspace is too small");
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
     int8_t *codes = static_cast<int8_t *>(ws);
     float *scales = reinterpret_cast<float *>(codes + m * codes_ld(k));
     if (int e = quantize_any(x, dtype, ld_x, m, k, codes, codes_ld(k), scales, st)) return e;

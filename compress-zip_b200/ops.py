@@ -221,9 +221,9 @@ def linear_i8(x, w: QRows, bias: Optional[torch.Tensor] = None, out_dtype: Optio
               bias_ptr, m, n, k, out2.data_ptr(), out_code, ldo)
     else:
         need = L.czg_linear_i8_workspace(m, k)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         _call(dev, L.czg_linear_i8_dynamic, x2.data_ptr(), code, x2.stride(0) if m > 1 else k, w.codes.data_ptr(), w.ld,
-              w.scales.data_ptr(), bias_ptr, m, n, k, out2.data_ptr(), out_code, ldo, ws.data_ptr(), need)
+              w.scales.data_ptr(), bias_ptr, m, n, k, out2.data_ptr(), out_code, ldo, ws.data_ptr() if need else 0, need)
     return out
 
 

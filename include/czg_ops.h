@@ -45,6 +45,7 @@ int czg_ops_check(void);
 
 /* Rows of x ([m][k] of `dtype`, ld_x elements apart) as int8 codes and one scale each:
  *   scale = max |x| / 127,  code = round-half-even(127 x / max |x|)
+ * (the code exact for 16-bit x; for fp32 x its product and quotient round to fp32)
  * (a row of zeros: scale 0, codes 0; a row with a NaN or an infinity: scale NaN,
  * codes 0).  codes: rows ld_codes bytes apart, 16-byte aligned, ld_codes a multiple
  * of 16; the bytes from k to the next multiple of 16 are set to 0. */
@@ -61,8 +62,9 @@ int czg_linear_i8(const int8_t *x, int64_t ld_x, const float *x_scale, const int
                   const float *w_scale, const float *bias, int64_t m, int64_t n, int64_t k, void *out,
                   int out_dtype, int64_t ld_out, void *stream);
 
-/* czg_quantize_rows into the workspace, then czg_linear_i8.  ws: 16-byte aligned,
- * czg_linear_i8_workspace(m, k) bytes, free again when the queued work is done. */
+/* czg_quantize_rows and then czg_linear_i8, with the same bits.  ws: 16-byte aligned,
+ * czg_linear_i8_workspace(m, k) bytes (0, and NULL will do, for a few short rows, which
+ * one kernel takes), free again when the queued work is done. */
 uint64_t czg_linear_i8_workspace(int64_t m, int64_t k);
 int czg_linear_i8_dynamic(const void *x, int dtype, int64_t ld_x, const int8_t *w, int64_t ld_w,
                           const float *w_scale, const float *bias, int64_t m, int64_t n, int64_t k, void *out,

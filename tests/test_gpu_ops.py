@@ -129,7 +129,8 @@ def test_linear_i8(ops, dtype, m, n, k):
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP16])
-@pytest.mark.parametrize("m,n,k", [(1, 512, 384), (3, 70, 33), (50, 1024, 512), (300, 384, 1024)])
+@pytest.mark.parametrize("m,n,k", [(1, 512, 384), (3, 70, 33), (50, 1024, 512), (300, 384, 1024), (16, 200, 2048), (15, 64, 1),
+                                   (2, 130, 11264), (2, 130, 11265), (2, 130, 12288), (1, 20000, 1100), (17, 300, 640), (5, 1, 4100)])
 def test_linear_i8_from_floats(ops, dtype, m, n, k):
     """Quantising in the call is quantize_rows and then the product, bit for bit."""
     g = gen(m * n)

@@ -76,11 +76,12 @@ def test_linear_refusals(ops, want, text, over):
 
 def test_linear_dynamic_refusals(ops):
     L = ops.lib()
-    need = L.czg_linear_i8_workspace(2, 50)
-    assert need == 2 * 64 + 16 and L.czg_linear_i8_workspace(0, 50) == 0
+    need = L.czg_linear_i8_workspace(21, 50)
+    assert need == 21 * 64 + 96 and L.czg_linear_i8_workspace(0, 50) == 0
+    assert L.czg_linear_i8_workspace(2, 50) == 0      # a few short rows take none
 
     def call(ws=P, n_ws=need, x=P, kind=BF16):
-        return L.czg_linear_i8_dynamic(x, kind, 50, P, 64, P, None, 2, 3, 50, P, BF16, 3, ws, n_ws, None)
+        return L.czg_linear_i8_dynamic(x, kind, 50, P, 64, P, None, 21, 3, 50, P, BF16, 3, ws, n_ws, None)
 
     for args, text in ((dict(ws=None), "workspace"), (dict(ws=P + 8), "workspace"), (dict(n_ws=need - 1), "too small"),
                        (dict(x=None), "null"), (dict(kind=9), "dtype")):
