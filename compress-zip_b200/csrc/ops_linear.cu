@@ -502,6 +502,196 @@ k_linear_tc(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ C
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(COLS));
 }
 
+// ---- the product, two CTAs a tile --------------------------------------------------
+//
+// For large m the loads of 128 x 256 tiles are what one CTA waits for (8192 x 8192 x 4096:
+// 145 of 211 us with the MMAs left out).  A pair of CTAs (tcgen05 cta_group::2) shares
+// 256 channels x 256 tokens: each loads its 128 weight rows and half of the tokens, and
+// the MMAs of the first CTA read both, so a byte loaded serves a third more products.
+// Each CTA's sums of its channels land in its own TMEM; the epilogue is as above.
+//   full[s]   of the first CTA: both CTAs' loads of the stage (64 KB)
+//   empty[s]  of each CTA: the MMAs have read it (committed to both)
+//   tfull[b]  of each CTA; tempty[b] of the first: both CTAs' epilogues have read it
+// A CTA whose wait runs out stops; the other's waits run out after it, and both come to
+// the cluster barrier at the end, so neither leaves while the other may signal it.
+constexpr int kPairTokens = 256, kPairStages = 6, kPairWarps = 10;
+constexpr int kPairStage = LT * TC_BK + kPairTokens / 2 * TC_BK;   // a CTA's bytes
+constexpr size_t kPairSmem = 1024 + (size_t)kPairStages * kPairStage + (2 * kPairStages + 5) * 8 + 16 + 2 * kPairTokens * 4;
+
+// A TMA load into this CTA that counts on the barrier at the same place of the pair's first CTA.
+__device__ __forceinline__ void tma_load_2d_pair(void *dst, const CUtensorMap *map, uint64_t *bar, int x, int y) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+        ::"r"(smem_addr(dst)), "l"(map), "r"(x), "r"(y), "r"(smem_addr(bar) & 0xFEFFFFFFu) : "memory");
+}
+__device__ __forceinline__ void mma_i8_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate));
+}
+__device__ __forceinline__ void mma_commit_pair(uint64_t *bar) {   // on the barrier of both CTAs
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                 ::"r"(smem_addr(bar)), "h"((uint16_t)3) : "memory");
+}
+__device__ __forceinline__ void arrive_first(uint64_t *bar) {   // on the barrier of the pair's first CTA
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_addr(bar)));
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(a) : "memory");
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kPairWarps * 32, 1)
+k_linear_pair(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, LinearArgs p) {
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    constexpr int NT = kPairTokens, STAGES = kPairStages, STAGE = kPairStage, W_BYTES = LT * TC_BK, EW = kPairWarps - 2, COLS = 512;
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + STAGES * STAGE);
+    uint64_t *empty = full + STAGES;
+    uint64_t *tfull = empty + STAGES;
+    uint64_t *tempty = tfull + 2;
+    uint64_t *drain = tempty + 2;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
+    float *s_xs = reinterpret_cast<float *>(tmem_slot + 4);   // 2 x NT
+    __shared__ volatile int abort_flag;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = (int)cluster_rank();
+    const int tile0 = blockIdx.x / 2, dt = gridDim.x / 2;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; s++) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int b = 0; b < 2; b++) {
+            mbar_init(&tfull[b], 1);
+            mbar_init(&tempty[b], 2 * EW);
+        }
+        mbar_init(drain, 1);
+        abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(COLS));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();   // both CTAs' barriers are set up and both have their TMEM
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int it = 0;
+            bool ok = true;
+            pdl_wait();
+            for (int tile = tile0; tile < p.tiles && ok; tile += dt) {
+                const int n0 = (tile % p.tiles_n) * 2 * LT + rank * LT, m0 = (tile / p.tiles_n) * NT + rank * (NT / 2);
+                for (int kb = 0; kb < p.steps; kb++, it++) {
+                    const int s = it % STAGES;
+                    uint8_t *sw = smem + s * STAGE;
+                    if (it >= STAGES && !mbar_wait(&empty[s], ((it / STAGES) - 1) & 1, &abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    if (rank == 0) mbar_expect_tx(&full[s], 2 * STAGE);
+                    tma_load_2d_pair(sw, &map_w, &full[s], kb * TC_BK, n0);
+                    tma_load_2d_pair(sw + W_BYTES, &map_x, &full[s], kb * TC_BK, m0);
+                }
+            }
+            if (!ok) {
+                atomicOr(&g_ops_timeout, 1);
+                abort_flag = 1;
+            }
+            // copies in flight: the first CTA sees all of both
+            if (!ok && rank == 0)
+                for (int k = max(0, it - STAGES); k < it; k++) mbar_wait(&full[k % STAGES], (k / STAGES) & 1, nullptr);
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            const uint32_t idesc = idesc_i8(2 * LT, NT);
+            int it = 0, tc = 0;
+            bool ok = true;
+            for (int tile = tile0; tile < p.tiles && ok; tile += dt, tc++) {
+                const int b = tc & 1;
+                if (tc >= 2 && !mbar_wait(&tempty[b], ((tc >> 1) - 1) & 1, &abort_flag)) {
+                    ok = false;
+                    break;
+                }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                for (int kb = 0; kb < p.steps; kb++, it++) {
+                    const int s = it % STAGES;
+                    if (!mbar_wait(&full[s], (it / STAGES) & 1, &abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint64_t wd = smem_desc_sw128(smem_addr(smem + s * STAGE));
+                    const uint64_t xd = smem_desc_sw128(smem_addr(smem + s * STAGE + W_BYTES));
+#pragma unroll
+                    for (int k = 0; k < TC_BK / 32; k++)
+                        mma_i8_pair(tmem + (uint32_t)(b * NT), wd + 2 * k, xd + 2 * k, idesc, kb > 0 || k > 0);
+                    mma_commit_pair(&empty[s]);
+                }
+                if (ok) mma_commit_pair(&tfull[b]);
+            }
+            if (!ok) {
+                atomicOr(&g_ops_timeout, 1);
+                abort_flag = 1;
+            }
+            asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(drain)) : "memory");
+            mbar_wait(drain, 0, nullptr);
+        }
+    } else {
+        const int q = warp & 3, part = (warp - 2) >> 2;
+        constexpr int PC = NT / (EW / 4);
+        pdl_wait();
+        T *out = static_cast<T *>(p.out);
+        int tc = 0;
+        for (int tile = tile0; tile < p.tiles; tile += dt, tc++) {
+            const int b = tc & 1;
+            const int n0 = (tile % p.tiles_n) * 2 * LT + rank * LT, m0 = (tile / p.tiles_n) * NT;
+            const int ch = n0 + 32 * q + lane;
+            const bool there = ch < p.n;
+            const float ws = there ? p.ws[ch] : 0.0f, bias = there && p.bias ? p.bias[ch] : 0.0f;
+            float *xs = s_xs + b * NT;
+            for (int i = threadIdx.x - 64; i < NT; i += EW * 32) xs[i] = m0 + i < p.m ? p.xs[m0 + i] : 0.0f;
+            const bool got = mbar_wait(&tfull[b], (tc >> 1) & 1, &abort_flag);
+            if (epilogue_any<EW * 32>(!got)) {
+                if (!got) {
+                    atomicOr(&g_ops_timeout, 1);
+                    abort_flag = 1;
+                }
+                break;
+            }
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t tbase = tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(b * NT + part * PC);
+#pragma unroll 1
+            for (int c0 = 0; c0 < PC; c0 += 32) {
+                uint32_t v[32];
+                tmem_ld32(tbase + c0, v);
+                if (c0 + 32 == PC) {
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) arrive_first(&tempty[b]);
+                }
+                if (!there) continue;
+                const int j0 = part * PC + c0, most = p.m - m0 - j0;
+                T *o = out + (int64_t)(m0 + j0) * p.ldo + ch;
+#pragma unroll
+                for (int j = 0; j < 32; j++)
+                    if (j < most) o[j * p.ldo] = finish<T>((int)v[j], xs[j0 + j], ws, bias, p.bias != nullptr);
+            }
+        }
+    }
+    __syncwarp();
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    cluster_arrive();
+    cluster_wait();
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(COLS));
+}
+
 // Rows of codes as a TMA map of boxes of `box` rows by 128 bytes, 128-byte swizzled.
 bool codes_map(CUtensorMap *map, const int8_t *p, int64_t ld, int64_t rows, int64_t k, int box) {
     EncodeTiledFn fn = encode_fn();
@@ -543,6 +733,29 @@ int launch_linear(const int8_t *x, int64_t ldx, const int8_t *w, int64_t ldw, in
                                p.split, mw, mx, p));
 }
 
+template <typename T>
+int launch_pair(const int8_t *x, int64_t ldx, const int8_t *w, int64_t ldw, int64_t k, LinearArgs p, bool after_quantise,
+                cudaStream_t st) {
+    alignas(64) CUtensorMap mw, mx;
+    if (!codes_map(&mw, w, ldw, p.n, k, LT) || !codes_map(&mx, x, ldx, p.m, k, kPairTokens / 2))
+        return ops_fail(CZG_E_DEVICE, "no tensor map for the operands");
+    p.tiles_n = (int)(((int64_t)p.n + 2 * LT - 1) / (2 * LT));
+    const int64_t tiles = (int64_t)p.tiles_n * (((int64_t)p.m + kPairTokens - 1) / kPairTokens);
+    if (tiles > 0x7FFFFFFF / 8) return ops_fail(CZG_E_LIMIT, "too many tiles");
+    p.tiles = (int)tiles;
+    static std::atomic<int> ready[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return ops_fail(CZG_E_DEVICE, "no device");
+    if (!ready[dev]) {
+        if (int e = ops_cuda(cudaFuncSetAttribute(k_linear_pair<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPairSmem)))
+            return e;
+        ready[dev] = 1;
+    }
+    const int pairs = sm_count() / 2;
+    return ops_cuda(ops_launch(k_linear_pair<T>, dim3((unsigned)(2 * (p.tiles < pairs ? p.tiles : pairs))), kPairWarps * 32,
+                               kPairSmem, st, after_quantise, 2, mw, mx, p));
+}
+
 // Calls whose x rows the product quantises itself: at most 16 rows, 64 KB of bf16 in all, so
 // that reading them in every CTA costs less than a launch (1 x 512 x 384: 10.9 us a call from Python, 14.8 with two kernels).
 constexpr int kSmallRows = 16, kSmallValues = 32768, kSmallSteps = 11;   // steps a CTA's ring holds
@@ -551,20 +764,26 @@ bool small_call(int64_t m, int64_t k) {
     return m <= kSmallRows && m * k <= kSmallValues && k <= 8 * kSmallSteps * TC_BK;
 }
 
+// Which tile, and over how many CTAs k is split: the least of a model of the time in
+// cycles.  A step (128 bytes of k) costs about 600 + 1.5 nt in one CTA, whatever its
+// tokens (4096 x 4096 weights, one tile a CTA, 32 steps: 15.2 us at nt = 16, 17.9 at 128,
+// 21 at 256), so more tokens a tile pay as long as the tiles fill the SMs, and below that
+// a split of k does (48 tokens: 17.3 us whole, 9.7 in 4; 128: 17.9 and 10.5).
 struct LinearShape { int nt, split; };
 
 LinearShape linear_shape(int64_t m, int64_t n, int steps) {
-    const int64_t tiles_n = (n + LT - 1) / LT;
     const int sms = sm_count();
     LinearShape best{16, 1};
     double least = 1e300;
-    for (int nt : {16, 32, 64, 128, 256}) {
-        const int64_t tiles = tiles_n * ((m + nt - 1) / nt);
+    for (int nt : {16, 32, 64, 128, 256, 512}) {
+        const bool pair = nt == 512;   // two CTAs, 256 x 256
+        const int64_t tiles = ((n + LT - 1) / LT + pair) / (1 + pair) * ((m + (pair ? 256 : nt) - 1) / (pair ? 256 : nt));
         for (int s : {1, 2, 4, 8}) {
-            if (s > 1 && (nt > 128 || nt * s > 256 || s > steps || tiles * s > sms)) break;
-            const double waves = (double)((tiles * s + sms - 1) / sms);
-            const double step = std::fmax(2.0 * nt, (16384.0 + 128.0 * nt) / 48.0);
-            const double cost = waves * ((steps + s - 1) / s) * step + 1500 + 12.0 * nt + (s > 1 ? 1000 : 0);
+            if (s > 1 && (nt > 128 || nt * s > 512 || s > steps || tiles * s > sms)) break;
+            const int64_t places = pair ? sms / 2 : sms;
+            const double waves = (double)((tiles * s + places - 1) / places);
+            const double step = pair ? 760.0 : 600.0 + 1.5 * nt;
+            const double cost = waves * ((steps + s - 1) / s) * step + 10.0 * nt + (s > 1 ? 1200 + 20.0 * nt : 0);
             if (cost < least) {
                 least = cost;
                 best = {nt, s};
@@ -596,10 +815,12 @@ int linear(const int8_t *x, int64_t ldx, const float *xs, const int8_t *w, int64
     LinearArgs p{xs, ws, bias, out, ldo, (int)m, (int)n, (int)((k + TC_BK - 1) / TC_BK), (int)((n + LT - 1) / LT), 0, 0, 1,
                  aligned(out, 4 * sizeof(T)) && ldo % 4 == 0};
     LinearShape shape = linear_shape(m, n, p.steps);
+
     p.split = shape.split;
     if (shape.nt == 16) return launch_linear<16, T, void>(x, ldx, w, ldw, k, p, after_quantise, st);
     if (shape.nt == 32) return launch_linear<32, T, void>(x, ldx, w, ldw, k, p, after_quantise, st);
     if (shape.nt == 64) return launch_linear<64, T, void>(x, ldx, w, ldw, k, p, after_quantise, st);
+    if (shape.nt == 512) return launch_pair<T>(x, ldx, w, ldw, k, p, after_quantise, st);
     if (shape.nt == 128) return launch_linear<128, T, void>(x, ldx, w, ldw, k, p, after_quantise, st);
     return launch_linear<256, T, void>(x, ldx, w, ldw, k, p, after_quantise, st);
 }

@@ -120,7 +120,8 @@ def check_linear(y, x, w, bias):
 @pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
 @pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 512, 384), (2, 129, 17), (5, 64, 16), (16, 130, 100), (17, 100, 1100),
                                    (33, 257, 640), (64, 300, 129), (65, 96, 512), (130, 257, 128), (200, 1000, 48),
-                                   (257, 513, 1000), (600, 640, 2048), (1, 4096, 4096), (24, 4096, 8200)])
+                                   (257, 513, 1000), (600, 640, 2048), (1, 4096, 4096), (24, 4096, 8200), (128, 1100, 3000),
+                                   (2500, 2100, 200), (2049, 2500, 1000), (5000, 1000, 129), (2560, 8192, 64), (300, 20000, 400)])
 def test_linear_i8(ops, dtype, m, n, k):
     g = gen(m + n + k)
     x, w = rand_codes(ops, g, m, k, 32), rand_codes(ops, g, n, k)
