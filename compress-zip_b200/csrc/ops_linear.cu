@@ -24,13 +24,15 @@ int ops_cuda(cudaError_t e) {
 
 namespace {
 
-// code = rne(127 x / a).  For 16-bit x the product is exact in fp32 (7 + 11 bits), and the
-// rounded quotient falls on a half only where the exact one does: with x = X 2^i, a = A 2^j
-// (X, A < 2^11) a quotient q that is no half is 1 / (2 A 2^(j-i)) >= |q| 2^-19 away from
-// one, and the division is off by |q| 2^-24 at most.  (fp32 x: both steps round.)
-// x (127 / a) is off by 127 * 2^-23 < 2^-16 at most and decides wherever it is not within
-// 10^-4 of a half; only where one of 8 values is, they are divided out.  Rounding is the
-// addition of M1 = 1.5 * 2^23 (common.cuh), whose sum's low byte is the code.
+// code = rne(127 x / a).  r = x (127 / a) in fp32 is off by 127 * 2^-23 < 2^-16 at most and
+// decides wherever it is not within 10^-4 of a half.  Rounding is the addition of
+// M1 = 1.5 * 2^23 (common.cuh), whose sum's low byte is the code.  Where one of 8 values is
+// near a half, all 8 are decided exactly: with k = rne(r - 1/2), which is the integer below
+// the half in question, the code is k + 1, k, or the even one of the two as 127 x is above,
+// below or at (k + 1/2) a.  For 16-bit x both products are exact (7 + 11 and 8 + 11 bits),
+// and a fused multiply-add gives their difference's sign; for fp32 x they are not, and the
+// rounded quotient of the rounded product decides.
+template <bool EXACT>
 __device__ __forceinline__ uint2 codes8(const float (&x)[8], float a, float inv) {
     uint32_t n[8];
     float worst = 0.0f;
@@ -41,8 +43,18 @@ __device__ __forceinline__ uint2 codes8(const float (&x)[8], float a, float inv)
         worst = fmaxf(worst, fabsf(__fmaf_rn(x[c], inv, -__fsub_rn(t, kM1))));
     }
     if (worst > 0.4999f) {
+        const float f = a > 1.2676506e30f ? 9.5367431640625e-7f : 1.0f;   // keeps 127 x inside fp32
 #pragma unroll
-        for (int c = 0; c < 8; c++) n[c] = __float_as_uint(__fadd_rn(__fdiv_rn(x[c] * 127.0f, a), kM1));
+        for (int c = 0; c < 8; c++) {
+            if (EXACT) {
+                const float k = __fsub_rn(__fadd_rn(__fmaf_rn(x[c], inv, -0.5f), kM1), kM1);
+                const float d = __fmaf_rn(x[c] * f, 127.0f, -__fmul_rn(k + 0.5f, a * f));
+                const uint32_t b = __float_as_uint(__fadd_rn(k, kM1));
+                n[c] = b + (d > 0.0f || (d == 0.0f && (b & 1u)));
+            } else {
+                n[c] = __float_as_uint(__fadd_rn(__fdiv_rn(x[c] * f * 127.0f, a * f), kM1));
+            }
+        }
     }
     uint2 r;
     r.x = __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410);
@@ -103,22 +115,25 @@ __device__ __forceinline__ void load8(const T *row, int64_t i, int64_t k, bool v
 // What a row's maximum (its magnitude's bits) makes of its values.
 template <typename T>
 struct RowScale {
-    float a, f, af, inv;
-    bool fine;
+    float a, inv;
+    bool fine, tiny;
     __device__ __forceinline__ explicit RowScale(uint32_t m) {
         fine = m < Raw8<T>::kInf;   // NaN and infinities both end as a row of NaN
         a = Raw8<T>::value(m);
-        // a power of two keeps a, 127 x and 127 / a far from both ends of fp32, and the quotients as they are
-        f = a > 1.2676506e30f ? 9.5367431640625e-7f : a < 8.6736174e-19f ? 1.2089258196146292e24f : 1.0f;
-        af = a * f;
-        inv = __fdiv_rn(127.0f, af);
+        tiny = a < 1.5e-36f;        // 127 / a would overflow: such rows are taken 2^80-fold
+        inv = __fdiv_rn(127.0f, tiny ? a * 1.2089258196146292e24f : a);
     }
     __device__ __forceinline__ float scale() const { return fine ? __fdiv_rn(a, 127.0f) : NAN; }
     __device__ __forceinline__ uint2 codes(const Raw8<T> &w) const {
+        if (!(fine && a > 0.0f)) return make_uint2(0, 0);
         float x8[8];
 #pragma unroll
-        for (int c = 0; c < 8; c++) x8[c] = w.get(c) * f;
-        return fine && a > 0.0f ? codes8(x8, af, inv) : make_uint2(0, 0);
+        for (int c = 0; c < 8; c++) x8[c] = w.get(c);
+        if (tiny) {
+#pragma unroll
+            for (int c = 0; c < 8; c++) x8[c] *= 1.2089258196146292e24f;
+        }
+        return codes8<sizeof(T) == 2>(x8, tiny ? a * 1.2089258196146292e24f : a, inv);
     }
 };
 
@@ -174,6 +189,36 @@ __global__ void __launch_bounds__(kQuantThreads) k_quantize_rows(const T *__rest
     // rows of codes end on 16 bytes: the second half of the last 16 may still be to fill
     const int64_t end = (k + 7) & ~(int64_t)7;
     if (threadIdx.x == 0 && (end & 15)) *reinterpret_cast<uint2 *>(out + end) = make_uint2(0, 0);
+}
+
+// Many rows of up to 256 V values: a warp a row, all of it in registers, no barrier; the
+// CTA's four rows and its neighbours' cover one another's latency.
+template <typename T, int V>
+__global__ void __launch_bounds__(128) k_quantize_rows_warp(const T *__restrict__ x, int64_t ldx, int m, int k, int vec,
+                                                            int8_t *__restrict__ codes, int64_t ldc, float *__restrict__ scales) {
+    pdl_trigger();
+    const int r = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (r >= m) return;
+    const T *row = x + r * ldx;
+    int8_t *out = codes + r * ldc;
+    Raw8<T> v[V];
+    uint32_t most = 0;
+#pragma unroll
+    for (int t = 0; t < V; t++)
+        if ((t * 32 + lane) * 8 < k) load8(row, (t * 32 + lane) * 8, k, vec, v[t]);
+#pragma unroll
+    for (int t = 0; t < V; t++)
+        if ((t * 32 + lane) * 8 < k) most = v[t].most(most);
+    if (sizeof(T) == 2) most = max(most & 0xFFFFu, most >> 16);
+    const RowScale<T> rs(__reduce_max_sync(0xffffffffu, most));
+#pragma unroll
+    for (int t = 0; t < V; t++)
+        if ((t * 32 + lane) * 8 < k) *reinterpret_cast<uint2 *>(out + (t * 32 + lane) * 8) = rs.codes(v[t]);
+    if (lane == 0) {
+        scales[r] = rs.scale();
+        const int end = (k + 7) & ~7;   // as above
+        if (end & 15) *reinterpret_cast<uint2 *>(out + end) = make_uint2(0, 0);
+    }
 }
 
 // ---- the product -------------------------------------------------------------------
@@ -796,8 +841,19 @@ LinearShape linear_shape(int64_t m, int64_t n, int steps) {
 template <typename T>
 int quantize(const void *x, int64_t ldx, int64_t m, int64_t k, int8_t *codes, int64_t ldc, float *scales, cudaStream_t st) {
     const int64_t turns = (k + 7) / 8;
-    const int threads = turns >= kQuantThreads ? kQuantThreads : (int)((turns + 31) / 32 * 32);
     const int vec = aligned(x, 16) && (m == 1 || ldx * sizeof(T) % 16 == 0);
+    // a warp a row once there are rows for all of an SM's warps (8192 x 4096 bf16: MEASUREW)
+    if (m >= 16 * sm_count() && k <= (sizeof(T) == 2 ? 4096 : 2048)) {
+        const dim3 grid((unsigned)((m + 3) / 4));
+        auto go = [&](auto kern) {
+            return ops_cuda(ops_launch(kern, grid, 128, 0, st, false, 1, static_cast<const T *>(x), ldx, (int)m, (int)k, vec, codes, ldc, scales));
+        };
+        if (turns <= 2 * 32) return go(k_quantize_rows_warp<T, 2>);
+        if (turns <= 4 * 32) return go(k_quantize_rows_warp<T, 4>);
+        if (turns <= 8 * 32) return go(k_quantize_rows_warp<T, 8>);
+        return go(k_quantize_rows_warp<T, 16>);
+    }
+    const int threads = turns >= kQuantThreads ? kQuantThreads : (int)((turns + 31) / 32 * 32);
     return ops_cuda(ops_launch(k_quantize_rows<T>, dim3((unsigned)m), threads, 0, st, false, 1, static_cast<const T *>(x), ldx,
                                k, vec, codes, ldc, scales));
 }

@@ -47,7 +47,8 @@ def codes_of(x):
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
-@pytest.mark.parametrize("m,k", [(1, 1), (1, 16), (3, 17), (5, 384), (2, 4097), (300, 63), (64, 1024), (7, 10007)])
+@pytest.mark.parametrize("m,k", [(1, 1), (1, 16), (3, 17), (5, 384), (2, 4097), (300, 63), (64, 1024), (7, 10007),
+                                 (2401, 40), (2370, 1000), (2368, 4096), (5001, 2049), (3000, 300)])
 def test_quantize_rows(ops, dtype, m, k):
     g = gen(m * k)
     x = randn(g, m, k + 5).to(dtype)[:, 2:k + 2]   # rows that begin off any boundary
@@ -66,6 +67,27 @@ def test_quantize_rows(ops, dtype, m, k):
     if k % 16:   # the bytes behind a row are zeros
         full = got.codes.as_strided((m, got.codes.stride(0)), (got.codes.stride(0), 1))
         assert not full[:, k:].any()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_quantize_rows_at_the_halves(ops, dtype):
+    """Rows whose maxima have 127 as a factor, or are twice an entry, are full of exact halves;
+    their neighbours by one step of the type are not."""
+    rows = []
+    for e in (-20, -3, 0, 9) if dtype == FP16 else (-130, -100, -3, 0, 60, 118):
+        for m in (127, 254, 255, 129, 200, 191, 131):
+            top = torch.tensor(m * 2.0 ** (e if dtype == BF16 else max(e, -14) - 7), dtype=torch.float64, device=DEV)
+            k = torch.arange(-127, 128, dtype=torch.float64, device=DEV)
+            v = torch.cat([top[None], top * (k + 0.5) / 127, top * k / 254]).to(dtype)
+            up = torch.nextafter(v.cpu(), torch.full_like(v.cpu(), math.inf)).to(DEV)
+            down = torch.nextafter(v.cpu(), torch.full_like(v.cpu(), -math.inf)).to(DEV)
+            rows.append(torch.cat([v, up, down]).clamp(-top.item(), top.item()))
+    x = torch.stack(rows)
+    assert torch.isfinite(x).all()
+    codes, scales = codes_of(x)
+    for copies in (1, 60):       # a CTA a row, a warp a row
+        got = ops.quantize_rows(x.repeat(copies, 1))
+        assert torch.equal(got.codes, codes.repeat(copies, 1)) and torch.equal(got.scales, scales.repeat(copies))
 
 
 def test_quantize_rows_special(ops):
