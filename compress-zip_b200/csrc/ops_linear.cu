@@ -32,6 +32,30 @@ namespace {
 // below or at (k + 1/2) a.  For 16-bit x both products are exact (7 + 11 and 8 + 11 bits),
 // and a fused multiply-add gives their difference's sign; for fp32 x they are not, and the
 // rounded quotient of the rounded product decides.
+__device__ __forceinline__ uint2 pack8(const uint32_t (&n)[8]) {
+    return make_uint2(__byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410),
+                      __byte_perm(__byte_perm(n[4], n[5], 0x0040), __byte_perm(n[6], n[7], 0x0040), 0x5410));
+}
+// Out of line: one copy of it leaves the unrolled kernels in the instruction cache.
+template <bool EXACT>
+__device__ __noinline__ uint2 codes8_at_halves(float x0, float x1, float x2, float x3, float x4, float x5, float x6, float x7,
+                                               float a, float inv) {
+    const float x[8] = {x0, x1, x2, x3, x4, x5, x6, x7};
+    const float f = a > 1.2676506e30f ? 9.5367431640625e-7f : 1.0f;   // keeps 127 x inside fp32
+    uint32_t n[8];
+#pragma unroll
+    for (int c = 0; c < 8; c++) {
+        if (EXACT) {
+            const float k = __fsub_rn(__fadd_rn(__fmaf_rn(x[c], inv, -0.5f), kM1), kM1);
+            const float d = __fmaf_rn(x[c] * f, 127.0f, -__fmul_rn(k + 0.5f, a * f));
+            const uint32_t b = __float_as_uint(__fadd_rn(k, kM1));
+            n[c] = b + (d > 0.0f || (d == 0.0f && (b & 1u)));
+        } else {
+            n[c] = __float_as_uint(__fadd_rn(__fdiv_rn(x[c] * f * 127.0f, a * f), kM1));
+        }
+    }
+    return pack8(n);
+}
 template <bool EXACT>
 __device__ __forceinline__ uint2 codes8(const float (&x)[8], float a, float inv) {
     uint32_t n[8];
@@ -42,24 +66,8 @@ __device__ __forceinline__ uint2 codes8(const float (&x)[8], float a, float inv)
         n[c] = __float_as_uint(t);
         worst = fmaxf(worst, fabsf(__fmaf_rn(x[c], inv, -__fsub_rn(t, kM1))));
     }
-    if (worst > 0.4999f) {
-        const float f = a > 1.2676506e30f ? 9.5367431640625e-7f : 1.0f;   // keeps 127 x inside fp32
-#pragma unroll
-        for (int c = 0; c < 8; c++) {
-            if (EXACT) {
-                const float k = __fsub_rn(__fadd_rn(__fmaf_rn(x[c], inv, -0.5f), kM1), kM1);
-                const float d = __fmaf_rn(x[c] * f, 127.0f, -__fmul_rn(k + 0.5f, a * f));
-                const uint32_t b = __float_as_uint(__fadd_rn(k, kM1));
-                n[c] = b + (d > 0.0f || (d == 0.0f && (b & 1u)));
-            } else {
-                n[c] = __float_as_uint(__fadd_rn(__fdiv_rn(x[c] * f * 127.0f, a * f), kM1));
-            }
-        }
-    }
-    uint2 r;
-    r.x = __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410);
-    r.y = __byte_perm(__byte_perm(n[4], n[5], 0x0040), __byte_perm(n[6], n[7], 0x0040), 0x5410);
-    return r;
+    if (worst > 0.4999f) return codes8_at_halves<EXACT>(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7], a, inv);
+    return pack8(n);
 }
 
 // 8 values of a row as they lie in memory.  Their magnitudes' bits order like the
