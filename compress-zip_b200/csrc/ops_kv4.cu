@@ -161,8 +161,8 @@ __global__ void __launch_bounds__(256) k_kv4_read(czg_kv4 c, const int32_t *__re
 
 // ---- attention ---------------------------------------------------------------------------
 //
-// A CTA takes one unit of a sequence's entries (kUnit, at a fixed place whatever the
-// batch), one key head and up to 8 NB rows (query heads of that key head, times the
+// A CTA takes one unit of a sequence's entries (unit_of its length, at a fixed place
+// whatever the batch), one key head and up to 8 NB rows (query heads of that key head, times the
 // call's rows).  Its two or four warps take tiles of kTile entries in turn, each through a ring of
 // its own that TMA fills (swizzled for ldmatrix); many such small CTAs share an SM and
 // cover one another's beginnings and ends.
@@ -185,7 +185,14 @@ __global__ void __launch_bounds__(256) k_kv4_read(czg_kv4 c, const int32_t *__re
 // sums are fp32; exponentials are ex2.approx (2^-22).
 // Between the warps of a CTA, and between units (k_kv4_join), partial results are joined
 // in a fixed order, so a row's bits do not depend on the batch or the grid.
-constexpr int kUnit = 512, kTile = 64, kRing = 2;
+constexpr int kChunk = 512, kTile = 32, kRing = 2;
+// Entries of a unit of a sequence of n: enough that none has more than kUnits units.
+constexpr int kUnits = 128;
+__host__ __device__ constexpr int unit_of(int n) {
+    int64_t u = kChunk;
+    while (u * kUnits < n) u *= 2;
+    return u < 0x40000000 ? (int)u : 0x40000000;
+}
 __host__ __device__ constexpr int attend_warps(int nb) { return nb == 1 ? 2 : 4; }   // more rows, longer tiles: more warps to share a unit
 
 struct AttendArgs {
@@ -200,7 +207,7 @@ struct AttendArgs {
     Strides os;
     // not whole, that is more than one unit (or row block with weights): partial results to join
     float *part;        // [b][head][unit][rows padded][D]
-    float2 *stat;       // [b][head][unit][rows padded] (maximum, sum)
+    float4 *stat;       // [b][head][unit][rows padded] (maximum, sum, what a score is multiplied by)
     float *score;       // weights: [b][head][rows][max_len]
 };
 
@@ -273,12 +280,12 @@ __device__ __forceinline__ int64_t row_offset(const AttendArgs &p, const Strides
 __device__ __forceinline__ float pow2f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }   // -126 <= e <= 127
 
 // CTAs an SM is to hold: what the sums (D NB / 4 registers), query and scores leave room for
-constexpr int attend_ctas(int d, int nb) { return d == 64 ? (nb == 1 ? 8 : 3) : (nb == 1 ? 6 : 2); }
+constexpr int attend_ctas(int d, int nb) { return d == 64 ? (nb == 1 ? 10 : 4) : (nb == 1 ? 8 : 3); }
 
 template <int D, int W>
 struct AttendSmem {
     static constexpr int kTileCodes = kTile * D / 2;   // of keys, and as many of values behind them
-    static constexpr int kScales = W * kRing * 2 * kTileCodes, kBars = kScales + kUnit * 8;
+    static constexpr int kScales = W * kRing * 2 * kTileCodes, kBars = kScales + kChunk * 8;
     static constexpr size_t kBytes = 1024 + kBars + W * kRing * 8;
 };
 
@@ -308,8 +315,9 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
     if (TRACK && unit == 0 && b == 0 && blockIdx.y == 0) kv4_check_distinct(p.c, p.slots, gridDim.z);
     const int slot = kv4_slot(p.c, p.slots, b, first);
     const int n = slot < 0 ? 0 : kv4_length(p.c, p.lengths, b, min(p.max_len, p.c.capacity), first);
-    const int j0 = unit * kUnit, here = min(n - j0, kUnit);   // entries of this unit
-    if (here <= 0 && unit > 0) return;
+    const int len = unit_of(n);
+    if (unit > 0 && (int64_t)unit * len >= n) return;
+    const int j0 = unit * len, here = min(n - j0, len);   // entries of this unit
     const int64_t base = kv4_row(p.c, max(slot, 0), h, 0);
 
     // each warp asks for its first tiles
@@ -331,13 +339,34 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
     }
     __syncwarp();
 
-    // ranges of the entries; 0 behind the end, whatever lies there
-    uint2 raw[kUnit / THREADS];
-    uint32_t top = 0;
+    // ranges of the first kChunk entries; 0 behind the end, whatever lies there
+    uint2 raw[kChunk / THREADS];
     const KvScale *ranges = static_cast<const KvScale *>(p.c.scales) + base + j0;
+    auto load_ranges = [&](int from) {
 #pragma unroll
-    for (int i = 0; i < kUnit / THREADS; i++)
-        raw[i] = tid + i * THREADS < here ? __ldg(reinterpret_cast<const uint2 *>(ranges + tid + i * THREADS)) : make_uint2(0, 0);
+        for (int i = 0; i < kChunk / THREADS; i++) {
+            const int j = from + tid + i * THREADS;
+            raw[i] = j < here ? __ldg(reinterpret_cast<const uint2 *>(ranges + j)) : make_uint2(0, 0);
+        }
+    };
+    // lays them down; returns te: 2^te is not below any of their values' steps (where
+    // 2^-100 is not above all)
+    auto put_ranges = [&]() {
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < kChunk / THREADS; i++) {
+            const uint32_t step = (raw[i].y & 0xFFFFu) << 16;   // bits of the value's step, never negative
+            if (step < 0x7F800000u) top = max(top, step);
+            sc[tid + i * THREADS] = raw[i];
+        }
+        top = __reduce_max_sync(0xffffffffu, top);
+        if (lane == 0) s_top[warp] = top;
+        __syncthreads();
+        top = s_top[0];
+        for (int w = 1; w < kWarps; w++) top = max(top, s_top[w]);
+        return top == 0 ? -100 : max((int)(top >> 23) - 126, -100);
+    };
+    load_ranges(0);
 
     // the query: D / 8 threads a row, 8 dimensions each, which are one lane's share of a chunk
     constexpr int TR = D / 8;
@@ -379,22 +408,9 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
             }
         }
     }
-#pragma unroll
-    for (int i = 0; i < kUnit / THREADS; i++) {
-        const uint32_t step = (raw[i].y & 0xFFFFu) << 16;   // bits of the value's step, never negative
-        if (step < 0x7F800000u) top = max(top, step);
-    }
-    top = __reduce_max_sync(0xffffffffu, top);
-    if (lane == 0) s_top[warp] = top;
-    __syncthreads();
-    top = s_top[0];
-    for (int w = 1; w < kWarps; w++) top = max(top, s_top[w]);
-    // 2^te is not below any value's step (where 2^-100 is not above all); weights are
-    // taken 2^up-fold, which brings weight times step, for weights up to 2^8, below 2^15
-    const int te = top == 0 ? 0 : max((int)(top >> 23) - 126, -100), up = 7 - te;
-#pragma unroll
-    for (int i = 0; i < kUnit / THREADS; i++) sc[tid + i * THREADS] = raw[i];
-    __syncthreads();
+    // weights are taken 2^up-fold, up = 7 - te, which brings weight times step, for weights
+    // up to 2^8, below 2^15
+    int te = put_ranges();   // a barrier: the query is there too
 
     const int warps = max(1, min(kWarps, (here + kTile - 1) / kTile));   // that have a tile
     constexpr int LD = D + 4;
@@ -419,10 +435,10 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
 #pragma unroll
             for (int i = 0; i < 8; i++) o[nb][ch][i >> 2][i & 3] = 0.0f;
     }
-    if (warp < warps) {
+    {
         uint4 qf[NB][CH];
         float qs[NB][2], zq[NB][2];   // of rows 2 c4, 2 c4 + 1
-        int seen[NB][2], least = kUnit;   // entries of this unit that the row sees; what all rows see at least
+        int seen[NB][2], least = 0x7FFFFFFF;   // entries of this unit that the row sees; what all rows see at least
 #pragma unroll
         for (int nb = 0; nb < NB; nb++) {
 #pragma unroll
@@ -446,7 +462,8 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
         float mq[NB][2];   // reference times factor, less `up`
         auto tile_of = [&](int it, auto cut_of) {
             constexpr bool CUT = decltype(cut_of)::value;   // some row does not see some of the tile's entries
-            const int t0 = (it * kWarps + warp) * kTile;
+            const int t0 = (it * kWarps + warp) * kTile;   // within the unit
+            const uint2 *range = sc + t0 % kChunk + g8;
             const uint32_t ka = smem_addr(ring + (it % kRing) * 2 * L::kTileCodes) + (uint32_t)lm_row * (D / 2), va = ka + L::kTileCodes;
             constexpr int KB = kTile / 16;
             float s[NB][KB][4];
@@ -478,7 +495,7 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
 #pragma unroll
                 for (int hf = 0; hf < 2; hf++) {
                     const int j = t0 + kb * 16 + hf * 8 + g8;
-                    const uint32_t kw = sc[j].x;
+                    const uint32_t kw = range[kb * 16 + hf * 8].x;
                     const float2 kr = make_float2(__uint_as_float(kw << 16), __uint_as_float(kw & 0xFFFF0000u));
 #pragma unroll
                     for (int nb = 0; nb < NB; nb++)
@@ -487,7 +504,7 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
                             float &x = s[nb][kb][2 * hf + i];
                             x = __fmaf_rn(kr.x, x, kr.y * zq[nb][i]);
                             if (TRACK && nb * 8 + 2 * c4 + i < rows_here && (!CUT || j < here))
-                                score[(int64_t)(nb * 8 + 2 * c4 + i) * p.max_len + j] = CUT && j >= seen[nb][i] ? -INFINITY : x * qs[nb][i];
+                                score[(int64_t)(nb * 8 + 2 * c4 + i) * p.max_len + j] = x;
                         }
                 }
             // Weights are taken from a reference that follows the maximum only where a weight
@@ -519,7 +536,7 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
                         const float was = m[nb][i];
                         if (was == -INFINITY || (mt[nb][i] - was) * qs[nb][i] > 8.0f) m[nb][i] = fmaxf(was, mt[nb][i]);
                         const float now = m[nb][i];
-                        mq[nb][i] = now == -INFINITY ? 0.0f : __fmaf_rn(now, qs[nb][i], -(float)up);
+                        mq[nb][i] = now == -INFINITY ? 0.0f : __fmaf_rn(now, qs[nb][i], (float)(te - 7));
                         if (it > 0) {
                             const float f = was == now ? 1.0f : was == -INFINITY ? 0.0f : ex2((was - now) * qs[nb][i]);
                             l[nb][i] *= f;
@@ -541,7 +558,7 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
 #pragma unroll
                 for (int hf = 0; hf < 2; hf++) {
                     const int j = t0 + kb * 16 + hf * 8 + g8;
-                    const uint32_t vw = sc[j].y;
+                    const uint32_t vw = range[kb * 16 + hf * 8].y;
                     const float2 vr = make_float2(__uint_as_float(vw << 16), __uint_as_float(vw & 0xFFFF0000u));
 #pragma unroll
                     for (int nb = 0; nb < NB; nb++) {
@@ -579,17 +596,47 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
                 }
             }
         };
+        constexpr int kTurns = kChunk / (kTile * kWarps);   // a warp's tiles of a chunk
+        int it = 0;
 #pragma unroll 1
-        for (int it = 0; it < turns; it++) {
-            if (!mbar_try(&ring_bar[it % kRing], (it / kRing) & 1) && !mbar_wait(&ring_bar[it % kRing], (it / kRing) & 1, nullptr)) {
-                atomicOr(&g_ops_timeout, 1);
-                mbar_wait(&ring_bar[it % kRing], (it / kRing) & 1, nullptr);   // once more for the copies, before anything ends
+        for (int j = 0;; j += kChunk) {
+#pragma unroll 1
+            for (const int end = min(turns, j / kChunk * kTurns + kTurns); it < end; it++) {
+                if (!mbar_try(&ring_bar[it % kRing], (it / kRing) & 1) && !mbar_wait(&ring_bar[it % kRing], (it / kRing) & 1, nullptr)) {
+                    atomicOr(&g_ops_timeout, 1);
+                    mbar_wait(&ring_bar[it % kRing], (it / kRing) & 1, nullptr);   // once more for the copies, before anything ends
+                }
+                __syncwarp();
+                if ((it * kWarps + warp + 1) * kTile > least) tile_of(it, std::true_type{}); else tile_of(it, std::false_type{});
+                __syncwarp();   // all lanes have read the tile
+                if (lane == 0 && it + kRing < turns) ask(it + kRing);
             }
-            __syncwarp();
-            if ((it * kWarps + warp + 1) * kTile > least) tile_of(it, std::true_type{}); else tile_of(it, std::false_type{});
-            __syncwarp();   // all lanes have read the tile
-            if (lane == 0 && it + kRing < turns) ask(it + kRing);
+            if (j + kChunk >= here) break;
+            load_ranges(j + kChunk);
+            __syncthreads();   // all warps are through with the last chunk's ranges
+            const int was = te;
+            te = max(te, put_ranges());
+            if (te > was) {    // a larger step: the weights so far, and the next, by a smaller power of two
+                const float f = pow2f(max(was - te, -126)), f2 = pow2f(min(was - te + 126, 0));   // their product is 2^(was - te)
+#pragma unroll
+                for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        l[nb][i] = l[nb][i] * f * f2;
+                        z[nb][i] = z[nb][i] * f * f2;
+                        lost[nb][i] = lost[nb][i] * f * f2;
+                        mq[nb][i] = m[nb][i] == -INFINITY ? 0.0f : __fmaf_rn(m[nb][i], qs[nb][i], (float)(te - 7));
+#pragma unroll
+                        for (int ch = 0; ch < CH; ch++)
+#pragma unroll
+                            for (int y = 0; y < 2; y++) {
+                                o[nb][ch][y][i] = o[nb][ch][y][i] * f * f2;
+                                o[nb][ch][y][2 + i] = o[nb][ch][y][2 + i] * f * f2;
+                            }
+                    }
+            }
         }
+        const float down = pow2f(te - 7);
         // sums over the lanes that share a row
 #pragma unroll
         for (int nb = 0; nb < NB; nb++)
@@ -601,10 +648,10 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
                     z[nb][i] += __shfl_xor_sync(0xffffffffu, z[nb][i], x);
                     if (kExact) lost[nb][i] += __shfl_xor_sync(0xffffffffu, lost[nb][i], x);
                 }
-                l[nb][i] *= pow2f(-up);
-                z[nb][i] = __fmaf_rn(lost[nb][i], 7.5f, z[nb][i]) * pow2f(-up);
+                l[nb][i] *= down;
+                z[nb][i] = __fmaf_rn(lost[nb][i], 7.5f, z[nb][i]) * down;
                 m[nb][i] = m[nb][i] == -INFINITY ? -INFINITY : m[nb][i] * qs[nb][i];
-                if (g8 == 0) {
+                if (g8 == 0 && warp < warps) {
                     s_m[warp][nb * 8 + 2 * c4 + i] = m[nb][i];
                     s_l[warp][nb * 8 + 2 * c4 + i] = l[nb][i];
                 }
@@ -619,7 +666,7 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
         s_row[tid] = make_float2(top_m, sum);
     }
     if (warp < warps) {
-        const float down = pow2f(-up);
+        const float down = pow2f(te - 7);
 #pragma unroll
         for (int nb = 0; nb < NB; nb++)
 #pragma unroll
@@ -654,7 +701,7 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
             store4(static_cast<T *>(p.out) + s_out[r] + d, x, row.y == 0.0f ? 0.0f : 1.0f / row.y, p.out_vec);   // a row that sees nothing: 0
         } else {
             *reinterpret_cast<float4 *>(p.part + (at + r) * D + d) = x;
-            if (d == 0) p.stat[at + r] = row;
+            if (d == 0) p.stat[at + r] = make_float4(row.x, row.y, s_qs[r].x, 0.0f);
         }
     }
     if (TRACK && whole)   // the scores that this CTA wrote
@@ -662,14 +709,15 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
             float add = 0.0f;
             for (int r = 0; r < rows_here; r++) {
                 const float2 row = s_row[r];
-                if (row.y != 0.0f) add += ex2(score[(int64_t)r * p.max_len + j] - row.x) * (1.0f / row.y);
+                if (j < n - (p.t - 1 - row_place(p, rb * R + r)))
+                    add += ex2(__fmaf_rn(score[(int64_t)r * p.max_len + j], s_qs[r].x, -row.x)) * (1.0f / row.y);
             }
             if (add != 0.0f) p.c.weights[base + j0 + j] += add;
         }
 }
 
 // Joins the units of rows: the first row_ctas CTAs of x write the rows' results, the others
-// the weights of kUnit entries each.  A row's units are taken in RUNS interleaved runs and
+// the weights of kChunk entries each.  A row's units are taken in RUNS interleaved runs and
 // those in order: places that depend on its length alone.  Up to kFew units make one run,
 // and a CTA takes RUNS rows of them (so fewer row_ctas do where no sequence may have more).
 constexpr int kJoinThreads = 256, kFew = 8, kMany = 1024;
@@ -679,7 +727,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv4_join(const __grid_constant
     const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
     const int slot = kv4_slot(p.c, p.slots, b, false);
     const int n = slot < 0 ? 0 : kv4_length(p.c, p.lengths, b, min(p.max_len, p.c.capacity), false);
-    const int units = (n + kUnit - 1) / kUnit;
+    const int len = unit_of(n), units = n == 0 ? 0 : (n - 1) / len + 1;
     const int64_t first = ((int64_t)b * p.c.n_heads + h) * p.units * rows_padded;
     pdl_wait();   // slots and lengths are older than the kernel before this one
     if ((int)blockIdx.x < row_ctas) {
@@ -688,12 +736,12 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv4_join(const __grid_constant
             // each CTA the next RUNS rows
             const int r = blockIdx.x * RUNS + run;
             if (r >= p.rows) return;
-            float2 st[kFew];
+            float4 st[kFew];
             float m = -INFINITY, l = 0.0f;
             float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             const int64_t at = first + r;
 #pragma unroll
-            for (int u = 0; u < kFew; u++) st[u] = u < units ? p.stat[at + (int64_t)u * rows_padded] : make_float2(-INFINITY, 0.0f);
+            for (int u = 0; u < kFew; u++) st[u] = u < units ? p.stat[at + (int64_t)u * rows_padded] : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
 #pragma unroll
             for (int u = 0; u < kFew; u++) m = fmaxf(m, st[u].x);
 #pragma unroll
@@ -728,7 +776,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv4_join(const __grid_constant
             const int some = min(kMany, units - u0);
             __syncthreads();
             for (int u = tid; u < some; u += kJoinThreads) {
-                const float2 st = p.stat[first + (int64_t)(u0 + u) * rows_padded + r];
+                const float4 st = p.stat[first + (int64_t)(u0 + u) * rows_padded + r];
                 s_f[u] = share(st.x, m);
                 l = __fmaf_rn(s_f[u], st.y, l);
             }
@@ -749,20 +797,20 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv4_join(const __grid_constant
         store4(static_cast<T *>(p.out) + row_offset(p, p.os, b, h, r) + d, x, l == 0.0f ? 0.0f : 1.0f / l, p.out_vec);
         return;
     }
-    // weights of kUnit entries: a warp a row for its maximum and sum, then a thread two entries
-    const int j0 = ((int)blockIdx.x - row_ctas) * kUnit;
+    // weights of kChunk entries: a warp a row for its maximum and sum, then a thread two entries
+    const int j0 = ((int)blockIdx.x - row_ctas) * kChunk;
     if (j0 >= n) return;
     constexpr int RB = 32;   // rows at a time
-    __shared__ float2 s_row[RB];
-    float add[kUnit / kJoinThreads] = {};
+    __shared__ float4 s_row[RB];
+    float add[kChunk / kJoinThreads] = {};
     for (int r0 = 0; r0 < p.rows; r0 += RB) {
         __syncthreads();
         constexpr int EACH = RB / (kJoinThreads / 32);
-        float2 st[EACH];   // a warp's rows, the first 32 units of each under way together
+        float4 st[EACH];   // a warp's rows, the first 32 units of each under way together
 #pragma unroll
         for (int i = 0; i < EACH; i++) {
             const int r = r0 + (tid >> 5) + i * (kJoinThreads / 32);
-            st[i] = r < p.rows && (tid & 31) < units ? p.stat[first + (int64_t)(tid & 31) * rows_padded + r] : make_float2(-INFINITY, 0.0f);
+            st[i] = r < p.rows && (tid & 31) < units ? p.stat[first + (int64_t)(tid & 31) * rows_padded + r] : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
         }
 #pragma unroll
         for (int i = 0; i < EACH; i++) {
@@ -773,26 +821,26 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv4_join(const __grid_constant
             for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
             float l = st[i].y * share(st[i].x, m);
             for (int u = (tid & 31) + 32; u < units; u += 32) {
-                const float2 more = p.stat[first + (int64_t)u * rows_padded + r];
+                const float4 more = p.stat[first + (int64_t)u * rows_padded + r];
                 l += more.y * share(more.x, m);
             }
             for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-            if ((tid & 31) == 0) s_row[r - r0] = make_float2(m, l == 0.0f ? 0.0f : 1.0f / l);
+            if ((tid & 31) == 0) s_row[r - r0] = make_float4(m, l == 0.0f ? 0.0f : 1.0f / l, st[i].z, 0.0f);
         }
         __syncthreads();
         const float *s = p.score + (((int64_t)b * p.c.n_heads + h) * p.rows + r0) * p.max_len + j0 + tid;
 #pragma unroll 8
         for (int r = 0; r < min(RB, p.rows - r0); r++) {
             const int seen = n - (p.t - 1 - row_place(p, r0 + r)) - j0 - tid;
-            const float2 row = s_row[r];
+            const float4 row = s_row[r];
 #pragma unroll
-            for (int i = 0; i < kUnit / kJoinThreads; i++)
-                if (i * kJoinThreads < seen) add[i] += ex2(s[(int64_t)r * p.max_len + i * kJoinThreads] - row.x) * row.y;
+            for (int i = 0; i < kChunk / kJoinThreads; i++)
+                if (i * kJoinThreads < seen) add[i] += ex2(__fmaf_rn(s[(int64_t)r * p.max_len + i * kJoinThreads], row.z, -row.x)) * row.y;
         }
     }
     float *w = p.c.weights + kv4_row(p.c, slot, h, 0);
 #pragma unroll
-    for (int i = 0; i < kUnit / kJoinThreads; i++) {
+    for (int i = 0; i < kChunk / kJoinThreads; i++) {
         const int j = j0 + i * kJoinThreads + tid;
         if (j < n && add[i] != 0.0f) w[j] += add[i];
     }
@@ -814,7 +862,7 @@ bool kv4_map(CUtensorMap *map, uint8_t *p, const czg_kv4 &c) {
 
 // How a call is cut, and where its workspace's parts lie.
 struct AttendPlan {
-    int rows, nb, row_blocks, units;
+    int rows, nb, row_blocks, units, chunks;
     bool join;
     uint64_t part, stat, score, bytes;
 };
@@ -825,11 +873,12 @@ AttendPlan attend_plan(const czg_kv4 &c, int64_t b, int t, int hq, int max_len) 
     a.rows = t * (hq / c.n_heads);
     a.nb = a.rows <= 8 ? 1 : 2;
     a.row_blocks = (a.rows + 8 * a.nb - 1) / (8 * a.nb);
-    a.units = n > kUnit ? (n + kUnit - 1) / kUnit : 1;
+    a.units = n <= kChunk ? 1 : n > kChunk * kUnits ? kUnits : (n + kChunk - 1) / kChunk;   // of the longest, or of a shorter one
+    a.chunks = (n + kChunk - 1) / kChunk;
     a.join = a.units > 1 || (c.weights && a.row_blocks > 1);
     const uint64_t sets = a.join ? (uint64_t)b * c.n_heads * a.units * a.row_blocks * 8 * a.nb : 0;
     a.stat = sets * c.head_dim * 4;
-    a.score = a.stat + sets * 8;
+    a.score = a.stat + sets * 16;
     a.bytes = a.score + (c.weights ? (uint64_t)b * c.n_heads * a.rows * (uint64_t)max_len * 4 : 0);
     return a;
 }
@@ -878,7 +927,7 @@ int attend_with(const AttendPlan &plan, const AttendArgs &p, int b, cudaStream_t
     if (!plan.join) return CZG_OK;
     constexpr int kRuns = kJoinThreads / (D / 4);
     const int row_ctas = plan.units <= kFew ? (plan.rows + kRuns - 1) / kRuns : plan.rows;
-    const dim3 join((unsigned)(row_ctas + (TRACK ? plan.units : 0)), (unsigned)p.c.n_heads, (unsigned)b);
+    const dim3 join((unsigned)(row_ctas + (TRACK ? plan.chunks : 0)), (unsigned)p.c.n_heads, (unsigned)b);
     return ops_cuda(ops_launch(k_kv4_join<T, D>, join, kJoinThreads, 0, st, true, 1, p, plan.row_blocks * 8 * NB, row_ctas));
 }
 
@@ -1001,7 +1050,7 @@ extern "C" int czg_kv4_attend(const czg_kv4 *cache, const void *q, int64_t q_sb,
     p.g_inv = ((1ull << 32) + p.g - 1) / p.g;
     uint8_t *w = static_cast<uint8_t *>(ws);
     p.part = reinterpret_cast<float *>(w);
-    p.stat = reinterpret_cast<float2 *>(w + plan.stat);
+    p.stat = reinterpret_cast<float4 *>(w + plan.stat);
     p.score = reinterpret_cast<float *>(w + plan.score);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     return dtype == CZG_BF16 ? attend<__nv_bfloat16>(plan, p, b, st) : attend<__half>(plan, p, b, st);

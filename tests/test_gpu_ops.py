@@ -453,6 +453,8 @@ def check_attend(ops, c, q, slots, lengths, max_len=None, scale=None):
     (64, 1, 6, 33, BF16, (40, 1, 600), 640),
     (64, 3, 5, 2, FP16, (95, 96, 97, 128, 160), 161),
     (128, 8, 7, 3, BF16, (513, 2, 64), 513),
+    (64, 1, 8, 1, FP16, (70000, 65537, 500, 65536), 70001),
+    (128, 1, 2, 2, BF16, (131073, 66001), 131073),
 ])
 def test_attend(ops, d, heads, g, t, dtype, lens, capacity, track):
     r = gen(capacity + t)
@@ -507,6 +509,19 @@ def test_attend_peaked_and_flat(ops):
     check_attend(ops, c, tiny, int32(2, 1, 0), int32(513, 1, 30))
     huge = (q * 2.0 ** 60).to(BF16)
     check_attend(ops, c, huge, int32(0, 1, 2), int32(512, 20, 1), scale=2.0 ** -66)
+
+
+def test_attend_ranges_that_grow_along_a_long_sequence(ops):
+    """Later entries' steps far above the earlier ones', which may be 0 at first."""
+    r = gen(18)
+    c = noise_cache(ops, r, 4, 1, 70000, 64, True)
+    for slot, powers in ((0, (0, 9)), (1, (-60, 3)), (2, (0, 60)), (3, (4, -30))):
+        late = (torch.arange(70000, device=DEV) % 1024 >= 512)
+        for part, p in ((~late, powers[0]), (late, powers[1])):
+            c.scales[slot, 0, part, 2:] *= 2.0 ** p
+    c.scales[2, 0, torch.arange(70000, device=DEV) % 1024 < 512, 2] = 0
+    q = 2 * randn(r, 4, 1, 8, 64).to(BF16)
+    check_attend(ops, c, q, int32(0, 1, 2, 3), int32(70000, 69999, 66666, 68000))
 
 
 def test_attend_not_finite(ops):
