@@ -252,6 +252,10 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_f16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t *>(&h);
@@ -285,7 +289,7 @@ constexpr int attend_ctas(int d, int nb) { return d == 64 ? (nb == 1 ? 10 : 4) :
 template <int D, int W>
 struct AttendSmem {
     static constexpr int kTileCodes = kTile * D / 2;   // of keys, and as many of values behind them
-    static constexpr int kScales = W * kRing * 2 * kTileCodes, kBars = kScales + kChunk * 8;
+    static constexpr int kScales = W * kRing * 2 * kTileCodes, kBars = kScales + kChunk * 16;
     static constexpr size_t kBytes = 1024 + kBars + W * kRing * 8;
 };
 
@@ -298,7 +302,7 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
     constexpr int R = 8 * NB, THREADS = kWarps * 32;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint2 *sc = reinterpret_cast<uint2 *>(smem + L::kScales);   // the entries' ranges, as they lie in memory
+    float4 *sc = reinterpret_cast<float4 *>(smem + L::kScales);   // a chunk's ranges: k step, k lo, v step, v lo
     uint64_t *bar = reinterpret_cast<uint64_t *>(smem + L::kBars);
     __shared__ uint4 s_q[NB * CH * 32];      // the query as B fragments: [nb][chunk][lane]
     __shared__ float2 s_qs[R];               // a row's factors
@@ -357,7 +361,8 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
         for (int i = 0; i < kChunk / THREADS; i++) {
             const uint32_t step = (raw[i].y & 0xFFFFu) << 16;   // bits of the value's step, never negative
             if (step < 0x7F800000u) top = max(top, step);
-            sc[tid + i * THREADS] = raw[i];
+            sc[tid + i * THREADS] = make_float4(__uint_as_float(raw[i].x << 16), __uint_as_float(raw[i].x & 0xFFFF0000u),
+                                                __uint_as_float(step), __uint_as_float(raw[i].y & 0xFFFF0000u));
         }
         top = __reduce_max_sync(0xffffffffu, top);
         if (lane == 0) s_top[warp] = top;
@@ -463,12 +468,10 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
         auto tile_of = [&](int it, auto cut_of) {
             constexpr bool CUT = decltype(cut_of)::value;   // some row does not see some of the tile's entries
             const int t0 = (it * kWarps + warp) * kTile;   // within the unit
-            const uint2 *range = sc + t0 % kChunk + g8;
+            const float4 *range = sc + t0 % kChunk + g8;
             const uint32_t ka = smem_addr(ring + (it % kRing) * 2 * L::kTileCodes) + (uint32_t)lm_row * (D / 2), va = ka + L::kTileCodes;
             constexpr int KB = kTile / 16;
             float s[NB][KB][4];
-#pragma unroll
-            for (int i = 0; i < NB * KB * 4; i++) s[i / (KB * 4)][i / 4 % KB][i % 4] = 0.0f;
             // entries inside, so that neighbouring MMAs add to different sums
 #pragma unroll
             for (int cp = 0; cp < CH; cp += 2) {
@@ -485,7 +488,8 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
 #pragma unroll
                             for (int nb = 0; nb < NB; nb++) {
                                 const uint4 &f = qf[nb][cp + ci];
-                                mma_f16(s[nb][kb], a & 0x000F000Fu, c & 0x000F000Fu, a & 0x00F000F0u, c & 0x00F000F0u, half ? f.z : f.x, half ? f.w : f.y);
+                                if (cp + ci + half == 0) mma_f16_first(s[nb][kb], a & 0x000F000Fu, c & 0x000F000Fu, a & 0x00F000F0u, c & 0x00F000F0u, f.x, f.y);
+                                else mma_f16(s[nb][kb], a & 0x000F000Fu, c & 0x000F000Fu, a & 0x00F000F0u, c & 0x00F000F0u, half ? f.z : f.x, half ? f.w : f.y);
                             }
                         }
             }
@@ -495,8 +499,7 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
 #pragma unroll
                 for (int hf = 0; hf < 2; hf++) {
                     const int j = t0 + kb * 16 + hf * 8 + g8;
-                    const uint32_t kw = range[kb * 16 + hf * 8].x;
-                    const float2 kr = make_float2(__uint_as_float(kw << 16), __uint_as_float(kw & 0xFFFF0000u));
+                    const float2 kr = *reinterpret_cast<const float2 *>(&range[kb * 16 + hf * 8]);
 #pragma unroll
                     for (int nb = 0; nb < NB; nb++)
 #pragma unroll
@@ -558,8 +561,7 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
 #pragma unroll
                 for (int hf = 0; hf < 2; hf++) {
                     const int j = t0 + kb * 16 + hf * 8 + g8;
-                    const uint32_t vw = range[kb * 16 + hf * 8].y;
-                    const float2 vr = make_float2(__uint_as_float(vw << 16), __uint_as_float(vw & 0xFFFF0000u));
+                    const float2 vr = *reinterpret_cast<const float2 *>(&range[kb * 16 + hf * 8].z);
 #pragma unroll
                     for (int nb = 0; nb < NB; nb++) {
                         float w[2];
@@ -797,53 +799,55 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv4_join(const __grid_constant
         store4(static_cast<T *>(p.out) + row_offset(p, p.os, b, h, r) + d, x, l == 0.0f ? 0.0f : 1.0f / l, p.out_vec);
         return;
     }
-    // weights of kChunk entries: a warp a row for its maximum and sum, then a thread two entries
+    // weights of kChunk entries, a thread two of them, 8 rows at a time: their scores are
+    // under way while a warp a row makes up the row's maximum and sum
     const int j0 = ((int)blockIdx.x - row_ctas) * kChunk;
     if (j0 >= n) return;
-    constexpr int RB = 32;   // rows at a time
+    constexpr int RB = kJoinThreads / 32, EACH = kChunk / kJoinThreads;
     __shared__ float4 s_row[RB];
-    float add[kChunk / kJoinThreads] = {};
+    float *w = p.c.weights + kv4_row(p.c, slot, h, j0);
+    float add[EACH] = {}, old[EACH];
+#pragma unroll
+    for (int i = 0; i < EACH; i++) old[i] = j0 + i * kJoinThreads + tid < n ? w[i * kJoinThreads + tid] : 0.0f;
     for (int r0 = 0; r0 < p.rows; r0 += RB) {
-        __syncthreads();
-        constexpr int EACH = RB / (kJoinThreads / 32);
-        float4 st[EACH];   // a warp's rows, the first 32 units of each under way together
+        const float *s = p.score + (((int64_t)b * p.c.n_heads + h) * p.rows + r0) * p.max_len + j0 + tid;
+        float v[RB][EACH];
 #pragma unroll
-        for (int i = 0; i < EACH; i++) {
-            const int r = r0 + (tid >> 5) + i * (kJoinThreads / 32);
-            st[i] = r < p.rows && (tid & 31) < units ? p.stat[first + (int64_t)(tid & 31) * rows_padded + r] : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
-        }
+        for (int r = 0; r < RB; r++)
 #pragma unroll
-        for (int i = 0; i < EACH; i++) {
-            const int r = r0 + (tid >> 5) + i * (kJoinThreads / 32);
-            if (r >= p.rows) break;
-            float m = st[i].x;
-            for (int u = (tid & 31) + 32; u < units; u += 32) m = fmaxf(m, p.stat[first + (int64_t)u * rows_padded + r].x);
+            for (int i = 0; i < EACH; i++)
+                if (r0 + r < p.rows && j0 + i * kJoinThreads + tid < n) v[r][i] = s[(int64_t)r * p.max_len + i * kJoinThreads];
+        const int mine = r0 + (tid >> 5), u0 = tid & 31;
+        float4 st = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+        if (mine < p.rows) {
+            if (u0 < units) st = p.stat[first + (int64_t)u0 * rows_padded + mine];
+            float m = st.x;
+            for (int u = u0 + 32; u < units; u += 32) m = fmaxf(m, p.stat[first + (int64_t)u * rows_padded + mine].x);
             for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-            float l = st[i].y * share(st[i].x, m);
-            for (int u = (tid & 31) + 32; u < units; u += 32) {
-                const float4 more = p.stat[first + (int64_t)u * rows_padded + r];
+            float l = st.y * share(st.x, m);
+            for (int u = u0 + 32; u < units; u += 32) {
+                const float4 more = p.stat[first + (int64_t)u * rows_padded + mine];
                 l += more.y * share(more.x, m);
             }
             for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-            if ((tid & 31) == 0) s_row[r - r0] = make_float4(m, l == 0.0f ? 0.0f : 1.0f / l, st[i].z, 0.0f);
+            st = make_float4(m, l == 0.0f ? 0.0f : 1.0f / l, st.z, 0.0f);
         }
+        __syncthreads();   // s_row's readers of the last rows are done
+        if (u0 == 0) s_row[tid >> 5] = st;
         __syncthreads();
-        const float *s = p.score + (((int64_t)b * p.c.n_heads + h) * p.rows + r0) * p.max_len + j0 + tid;
-#pragma unroll 8
-        for (int r = 0; r < min(RB, p.rows - r0); r++) {
+#pragma unroll
+        for (int r = 0; r < RB; r++) {
+            if (r0 + r >= p.rows) break;
             const int seen = n - (p.t - 1 - row_place(p, r0 + r)) - j0 - tid;
             const float4 row = s_row[r];
 #pragma unroll
-            for (int i = 0; i < kChunk / kJoinThreads; i++)
-                if (i * kJoinThreads < seen) add[i] += ex2(__fmaf_rn(s[(int64_t)r * p.max_len + i * kJoinThreads], row.z, -row.x)) * row.y;
+            for (int i = 0; i < EACH; i++)
+                if (i * kJoinThreads < seen) add[i] += ex2(__fmaf_rn(v[r][i], row.z, -row.x)) * row.y;
         }
     }
-    float *w = p.c.weights + kv4_row(p.c, slot, h, 0);
 #pragma unroll
-    for (int i = 0; i < kChunk / kJoinThreads; i++) {
-        const int j = j0 + i * kJoinThreads + tid;
-        if (j < n && add[i] != 0.0f) w[j] += add[i];
-    }
+    for (int i = 0; i < EACH; i++)
+        if (add[i] != 0.0f) w[i * kJoinThreads + tid] = old[i] + add[i];
 }
 
 // Rows of 4-bit codes as a map of boxes of kTile entries of one slot and head.
