@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(256) k_kv4_read(czg_kv4 c, const int32_t *__re
 //      (2, 6), (3, 7) are the k of two MMAs (the query is permuted alike, and its share of
 //      the high nibbles divided by 16);
 //   V: ldmatrix.trans gives a lane 4 dimensions of entries 2c, 2c + 1: nibble i of both is
-//      the pair of dimension 4g + i (odd i: 16-fold, taken out at the end).
+//      the pair of dimension 4g + i (for odd i the byte, taken apart at the end).
 // With x = lo + step c:  s_j = step_j (q.c_j) + lo_j sum(q);  out = sum p_j step_j c_j + sum p_j lo_j.
 // The query is held in fp16 after a power of two that brings its largest value to
 // [2^13, 2^14): exact but for values below 2^-23 of the largest.  p_j step_j is
@@ -588,11 +588,14 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
                     ldsm4_trans(w, va + kb * 16 * (D / 2) + (((uint32_t)(cp + lm_ch) ^ swz) << 4));
 #pragma unroll
                     for (int ci = 0; ci < 2; ci++) {
-                        const uint32_t a = w[2 * ci], c = w[2 * ci + 1], a8 = a >> 8, c8 = c >> 8;
+                        // the odd rows take whole bytes, 16 times their code and the even row's once:
+                        // one operation less than masking the code, and taken off at the end
+                        const uint32_t a = w[2 * ci], c = w[2 * ci + 1];
+                        const uint32_t a8 = __byte_perm(a, 0u, 0x4341), c8 = __byte_perm(c, 0u, 0x4341);
 #pragma unroll
                         for (int nb = 0; nb < NB; nb++) {
-                            mma_f16(o[nb][cp + ci][0], a & 0x000F000Fu, a & 0x00F000F0u, c & 0x000F000Fu, c & 0x00F000F0u, pf[nb][0], pf[nb][1]);
-                            mma_f16(o[nb][cp + ci][1], a8 & 0x000F000Fu, a8 & 0x00F000F0u, c8 & 0x000F000Fu, c8 & 0x00F000F0u, pf[nb][0], pf[nb][1]);
+                            mma_f16(o[nb][cp + ci][0], a & 0x000F000Fu, a & 0x00FF00FFu, c & 0x000F000Fu, c & 0x00FF00FFu, pf[nb][0], pf[nb][1]);
+                            mma_f16(o[nb][cp + ci][1], a8 & 0x000F000Fu, a8, c8 & 0x000F000Fu, c8, pf[nb][0], pf[nb][1]);
                         }
                     }
                 }
@@ -682,7 +685,8 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
 #pragma unroll
                     for (int y = 0; y < 2; y++)   // dimensions 32 ch + 4 g8 + 2 y and the next
                         *reinterpret_cast<float2 *>(&so[(warp * R + r) * LD + ch * 32 + 4 * g8 + 2 * y]) =
-                            make_float2(__fmaf_rn(o[nb][ch][y][i] * 16777216.0f, even, zz), __fmaf_rn(o[nb][ch][y][2 + i] * 16777216.0f, odd, zz));
+                            make_float2(__fmaf_rn(o[nb][ch][y][i] * 16777216.0f, even, zz),
+                                        __fmaf_rn((o[nb][ch][y][2 + i] - o[nb][ch][y][i]) * 16777216.0f, odd, zz));
             }
     }
     __syncthreads();

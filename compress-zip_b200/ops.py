@@ -203,7 +203,7 @@ def linear_i8(x, w: QRows, bias: Optional[torch.Tensor] = None, out_dtype: Optio
     if dev.type != "cuda":
         raise ValueError(f"tensors must be on a CUDA device, not {dev}")
     if out is None:
-        out2 = torch.empty((m, n), dtype=kind, device=dev)
+        out2 = x2.new_empty((m, n)) if x2.dtype is kind else torch.empty((m, n), dtype=kind, device=dev)
         out = out2 if lead is None else out2.view(*lead, n)
     else:
         out2 = out if lead is None else out.view(m, n)
@@ -221,7 +221,7 @@ def linear_i8(x, w: QRows, bias: Optional[torch.Tensor] = None, out_dtype: Optio
               bias_ptr, m, n, k, out2.data_ptr(), out_code, ldo)
     else:
         need = L.czg_linear_i8_workspace(m, k)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        ws = w.codes.new_empty(need) if need else None
         _call(dev, L.czg_linear_i8_dynamic, x2.data_ptr(), code, x2.stride(0) if m > 1 else k, w.codes.data_ptr(), w.ld,
               w.scales.data_ptr(), bias_ptr, m, n, k, out2.data_ptr(), out_code, ldo, ws.data_ptr() if need else 0, need)
     return out
@@ -355,7 +355,7 @@ class KV4Cache:
             return out
         n = self.capacity if max_len is None else max_len
         need = self._lib.czg_kv4_attend_workspace(self._ref, b, t, hq, n)
-        ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+        ws = self.k.new_empty(need) if need else None
         self._call(self._lib.czg_kv4_attend, q.data_ptr(), qs[0], qs[1], qs[2], DTYPES[q.dtype], slots.data_ptr(),
                    lengths.data_ptr(), b, t, hq, n, self.head_dim ** -0.5 if scale is None else scale, out.data_ptr(),
                    os[0], os[1], os[2], ws.data_ptr() if need else 0, need)
