@@ -24,49 +24,39 @@ int ops_cuda(cudaError_t e) {
 
 namespace {
 
-// code = rne(127 x / a).  r = x (127 / a) in fp32 is off by 127 * 2^-23 < 2^-16 at most and
-// decides wherever it is not within 10^-4 of a half.  Rounding is the addition of
-// M1 = 1.5 * 2^23 (common.cuh), whose sum's low byte is the code.  Where one of 8 values is
-// near a half, all 8 are decided exactly: with k = rne(r - 1/2), which is the integer below
-// the half in question, the code is k + 1, k, or the even one of the two as 127 x is above,
-// below or at (k + 1/2) a.  For 16-bit x both products are exact (7 + 11 and 8 + 11 bits),
-// and a fused multiply-add gives their difference's sign; for fp32 x they are not, and the
-// rounded quotient of the rounded product decides.
+// code = rne(127 x / a).  r = x (127 / a) in fp32 is off by 2^-22 of itself at most: where
+// r (1 - 2^-20) and r (1 + 2^-20) round to the same integer, that is the code.  Rounding is
+// the addition of M1 = 1.5 * 2^23 (common.cuh), whose sum's low byte is the code.  Where one
+// of 8 values is nearer to a half than that, all 8 are decided exactly: with
+// k = rne(r - 1/2), which is the integer below the half in question, the code is k + 1, k, or
+// the even one of the two as 127 x is above, below or at (k + 1/2) a.  For 16-bit x both
+// products are exact (7 + 11 and 8 + 11 bits), and a fused multiply-add gives their
+// difference's sign; for fp32 x they are not, and the rounded quotient of the rounded
+// product decides.
 __device__ __forceinline__ uint2 pack8(const uint32_t (&n)[8]) {
     return make_uint2(__byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410),
                       __byte_perm(__byte_perm(n[4], n[5], 0x0040), __byte_perm(n[6], n[7], 0x0040), 0x5410));
 }
 // Out of line: one copy of it leaves the unrolled kernels in the instruction cache.
 template <bool EXACT>
-__device__ __noinline__ uint2 codes8_at_halves(float x0, float x1, float x2, float x3, float x4, float x5, float x6, float x7,
-                                               float a, float inv) {
+__device__ __noinline__ uint2 codes8_at_halves(float x0, float x1, float x2, float x3, float x4, float x5, float x6, float x7, float a) {
     const float x[8] = {x0, x1, x2, x3, x4, x5, x6, x7};
-    const float f = a > 1.2676506e30f ? 9.5367431640625e-7f : 1.0f;   // keeps 127 x inside fp32
+    // a power of two keeps a, 127 x and 127 / a inside fp32
+    const float f = a > 1.2676506e30f ? 9.5367431640625e-7f : a < 8.6736174e-19f ? 1.2089258196146292e24f : 1.0f;
+    const float af = a * f, inv = __fdiv_rn(127.0f, af);
     uint32_t n[8];
 #pragma unroll
     for (int c = 0; c < 8; c++) {
+        const float y = x[c] * f;
         if (EXACT) {
-            const float k = __fsub_rn(__fadd_rn(__fmaf_rn(x[c], inv, -0.5f), kM1), kM1);
-            const float d = __fmaf_rn(x[c] * f, 127.0f, -__fmul_rn(k + 0.5f, a * f));
+            const float k = __fsub_rn(__fadd_rn(__fmaf_rn(y, inv, -0.5f), kM1), kM1);
+            const float d = __fmaf_rn(y, 127.0f, -__fmul_rn(k + 0.5f, af));
             const uint32_t b = __float_as_uint(__fadd_rn(k, kM1));
             n[c] = b + (d > 0.0f || (d == 0.0f && (b & 1u)));
         } else {
-            n[c] = __float_as_uint(__fadd_rn(__fdiv_rn(x[c] * f * 127.0f, a * f), kM1));
+            n[c] = __float_as_uint(__fadd_rn(__fdiv_rn(y * 127.0f, af), kM1));
         }
     }
-    return pack8(n);
-}
-template <bool EXACT>
-__device__ __forceinline__ uint2 codes8(const float (&x)[8], float a, float inv) {
-    uint32_t n[8];
-    float worst = 0.0f;
-#pragma unroll
-    for (int c = 0; c < 8; c++) {
-        const float t = __fmaf_rn(x[c], inv, kM1);
-        n[c] = __float_as_uint(t);
-        worst = fmaxf(worst, fabsf(__fmaf_rn(x[c], inv, -__fsub_rn(t, kM1))));
-    }
-    if (worst > 0.4999f) return codes8_at_halves<EXACT>(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7], a, inv);
     return pack8(n);
 }
 
@@ -123,25 +113,29 @@ __device__ __forceinline__ void load8(const T *row, int64_t i, int64_t k, bool v
 // What a row's maximum (its magnitude's bits) makes of its values.
 template <typename T>
 struct RowScale {
-    float a, inv;
-    bool fine, tiny;
+    float a, low, high;   // 127 / a less and more 2^-20 of itself
+    uint32_t none;          // not 0: 127 / a would overflow, and nothing is decided by it
+    bool fine;
     __device__ __forceinline__ explicit RowScale(uint32_t m) {
         fine = m < Raw8<T>::kInf;   // NaN and infinities both end as a row of NaN
         a = Raw8<T>::value(m);
-        tiny = a < 1.5e-36f;        // 127 / a would overflow: such rows are taken 2^80-fold
-        inv = __fdiv_rn(127.0f, tiny ? a * 1.2089258196146292e24f : a);
+        none = a < 1.5e-36f;
+        const float inv = __fdiv_rn(127.0f, none ? 1.0f : a);
+        low = inv * (1.0f - 9.5367431640625e-7f);
+        high = inv * (1.0f + 9.5367431640625e-7f);
     }
     __device__ __forceinline__ float scale() const { return fine ? __fdiv_rn(a, 127.0f) : NAN; }
     __device__ __forceinline__ uint2 codes(const Raw8<T> &w) const {
         if (!(fine && a > 0.0f)) return make_uint2(0, 0);
-        float x8[8];
+        uint32_t n[8], differ = none;
 #pragma unroll
-        for (int c = 0; c < 8; c++) x8[c] = w.get(c);
-        if (tiny) {
-#pragma unroll
-            for (int c = 0; c < 8; c++) x8[c] *= 1.2089258196146292e24f;
+        for (int c = 0; c < 8; c++) {
+            n[c] = __float_as_uint(__fmaf_rn(w.get(c), low, kM1));
+            differ |= n[c] ^ __float_as_uint(__fmaf_rn(w.get(c), high, kM1));
         }
-        return codes8<sizeof(T) == 2>(x8, tiny ? a * 1.2089258196146292e24f : a, inv);
+        if (differ)
+            return codes8_at_halves<sizeof(T) == 2>(w.get(0), w.get(1), w.get(2), w.get(3), w.get(4), w.get(5), w.get(6), w.get(7), a);
+        return pack8(n);
     }
 };
 
