@@ -1031,6 +1031,22 @@ extern "C" int czg_kv4_attend(const czg_kv4 *cache, const void *q, int64_t q_sb,
     if (!aligned(q, 2) || !aligned(out, 2)) return ops_fail(CZG_E_ARG, "q and out must be aligned to their type");
     if ((int64_t)t * hq > 0x7FFFFFFF || (int64_t)t * hq / cache->n_heads * (hq / cache->n_heads) >= 1ll << 32)
         return ops_fail(CZG_E_LIMIT, "too many rows");
+    const Strides qs{q_sb, q_st, q_sh}, os{o_sb, o_st, o_sh};
+    const int64_t d = cache->head_dim;
+    if ((b > 1 && o_sb == 0) || (t > 1 && o_st == 0) || (hq > 1 && o_sh == 0)) return ops_fail(CZG_E_ARG, "rows of out overlap");
+    // a row's output may take its query's place (both are one CTA's), no other's
+    if (!(q == out && q_sb == o_sb && q_st == o_st && q_sh == o_sh)) {
+        auto last = [&](const void *p, const Strides &s) {
+            return reinterpret_cast<intptr_t>(p) + 2 * ((b - 1) * s.b + (t - 1) * s.t + (hq - 1) * s.h + d);
+        };
+        if (reinterpret_cast<intptr_t>(out) < last(q, qs) && reinterpret_cast<intptr_t>(q) < last(out, os)) {
+            // but for heads side by side in rows of one stride
+            const int64_t width = (hq - 1) * o_sh + d, off = (static_cast<const char *>(q) - static_cast<char *>(out)) / 2;
+            const bool alike = q_sb == o_sb && q_st == o_st && q_sh == o_sh && o_sh > 0 && o_st > 0 && o_sb % o_st == 0;
+            const int64_t from = alike ? (off % o_st + o_st) % o_st : 0;
+            if (!alike || from < width || from + width > o_st) return ops_fail(CZG_E_ARG, "out lies over q");
+        }
+    }
     const AttendPlan plan = attend_plan(*cache, b, t, hq, max_len);
     if (ws_bytes < plan.bytes || !aligned(ws, 16) || (plan.bytes && !ws))
         return ops_fail(CZG_E_ARG, "the workspace is too small or not 16-byte aligned");
@@ -1040,7 +1056,7 @@ extern "C" int czg_kv4_attend(const czg_kv4 *cache, const void *q, int64_t q_sb,
     AttendArgs p{};
     p.c = *cache;
     p.q = q;
-    p.qs = {q_sb, q_st, q_sh};
+    p.qs = qs;
     p.slots = slots;
     p.lengths = lengths;
     p.t = t;
@@ -1053,7 +1069,7 @@ extern "C" int czg_kv4_attend(const czg_kv4 *cache, const void *q, int64_t q_sb,
     p.out_vec = aligned(out, 8) && o_sb % 4 == 0 && o_st % 4 == 0 && o_sh % 4 == 0;
     p.scale_log2 = (float)((double)scale * 1.4426950408889634);
     p.out = out;
-    p.os = {o_sb, o_st, o_sh};
+    p.os = os;
     p.whole = !plan.join;
     p.g_inv = ((1ull << 32) + p.g - 1) / p.g;
     uint8_t *w = static_cast<uint8_t *>(ws);

@@ -2,7 +2,7 @@
 // (include/czg_ops.h): the row quantiser and the product.
 #include <atomic>
 #include <cmath>
-#include <string>
+#include <cstring>
 #include <type_traits>
 
 #include "ops_common.cuh"
@@ -10,10 +10,10 @@
 
 namespace czg {
 
-static thread_local std::string g_ops_error;
+static thread_local char g_ops_error[256];   // no allocation: nothing can throw across the C boundary
 
 int ops_fail(int status, const char *why) {
-    g_ops_error = why;
+    std::strncpy(g_ops_error, why, sizeof(g_ops_error) - 1);
     return status;
 }
 int ops_cuda(cudaError_t e) {
@@ -924,6 +924,19 @@ int check_linear(const int8_t *w, int64_t ldw, const float *ws, int64_t m, int64
     return CZG_OK;
 }
 
+// out must not lie over an operand, whose rows other CTAs may still read: ranges that
+// meet are refused, but for columns side by side in rows of one stride.
+int check_apart(const void *out, int64_t out_ld, int64_t out_row, const void *in, int64_t in_ld, int64_t in_row, int64_t out_rows,
+                int64_t in_rows, const char *why) {   // in bytes
+    const intptr_t a = reinterpret_cast<intptr_t>(out), b = reinterpret_cast<intptr_t>(in);
+    if (a + (out_rows - 1) * out_ld + out_row <= b || b + (in_rows - 1) * in_ld + in_row <= a) return CZG_OK;
+    if (out_ld == in_ld && out_ld > 0) {
+        const int64_t d = ((b - a) % out_ld + out_ld) % out_ld;   // where in's columns begin, counted from out's
+        if (d >= out_row && d + in_row <= out_ld) return CZG_OK;
+    }
+    return ops_fail(CZG_E_ARG, why);
+}
+
 int check_sizes(int64_t m, int64_t n, int64_t k) {
     if (m < 0 || n < 0 || k < 1) return ops_fail(CZG_E_ARG, "m and n must not be negative, k must be at least 1");
     if (k > CZG_LINEAR_MAX_K) return ops_fail(CZG_E_LIMIT, "k is beyond CZG_LINEAR_MAX_K");
@@ -946,7 +959,7 @@ int64_t codes_ld(int64_t k) { return (k + 15) & ~(int64_t)15; }
 
 using namespace czg;
 
-extern "C" const char *czg_ops_last_error(void) { return g_ops_error.c_str(); }
+extern "C" const char *czg_ops_last_error(void) { return g_ops_error; }
 
 extern "C" int czg_ops_check(void) {
     int a = 0, b = 0;
@@ -975,6 +988,9 @@ extern "C" int czg_linear_i8(const int8_t *x, int64_t ld_x, const float *x_scale
     if (!x || !x_scale) return ops_fail(CZG_E_ARG, "null pointer");
     if (const char *why = check_codes(x, ld_x, m, k)) return ops_fail(CZG_E_ARG, why);
     if (int st = check_linear(w, ld_w, w_scale, m, n, k, out, out_dtype, ld_out)) return st;
+    const int eb = elem_bytes(out_dtype);
+    if (int st = check_apart(out, ld_out * eb, n * eb, x, ld_x, k, m, m, "out lies over x")) return st;
+    if (int st = check_apart(out, ld_out * eb, n * eb, w, ld_w, k, m, n, "out lies over w")) return st;
     return linear_any(x, ld_x, x_scale, w, ld_w, w_scale, bias, m, n, k, out, out_dtype, ld_out, false,
                       static_cast<cudaStream_t>(stream));
 }
@@ -991,6 +1007,9 @@ extern "C" int czg_linear_i8_dynamic(const void *x, int dtype, int64_t ld_x, con
     if (m == 0 || n == 0) return CZG_OK;
     if (int st = check_x(x, dtype, ld_x, m, k)) return st;
     if (int st = check_linear(w, ld_w, w_scale, m, n, k, out, out_dtype, ld_out)) return st;
+    const int eb = elem_bytes(out_dtype), xb = elem_bytes(dtype);
+    if (int st = check_apart(out, ld_out * eb, n * eb, x, ld_x * xb, k * xb, m, m, "out lies over x")) return st;
+    if (int st = check_apart(out, ld_out * eb, n * eb, w, ld_w, k, m, n, "out lies over w")) return st;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (small_call(m, k)) {
         if (out_dtype == CZG_F32) return linear_small_of<float>(dtype, x, ld_x, w, ld_w, w_scale, bias, m, n, k, out, ld_out, st);

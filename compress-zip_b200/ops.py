@@ -353,7 +353,7 @@ class KV4Cache:
             raise ValueError("the last dimension of out must be adjacent")
         if not (b and t and hq):
             return out
-        n = self.capacity if max_len is None else max_len
+        n = self.capacity if max_len is None else min(max_len, self.capacity)
         need = self._lib.czg_kv4_attend_workspace(self._ref, b, t, hq, n)
         ws = self.k.new_empty(need) if need else None
         self._call(self._lib.czg_kv4_attend, q.data_ptr(), qs[0], qs[1], qs[2], DTYPES[q.dtype], slots.data_ptr(),
@@ -376,7 +376,7 @@ class KV4Cache:
         new = torch.empty_like(slots)
         if b:
             self._call(self._lib.czg_kv4_evict, slots.data_ptr(), lengths.data_ptr(), b,
-                       self.capacity if max_len is None else max_len, budget, recent, kept.data_ptr(), new.data_ptr())
+                       self.capacity if max_len is None else min(max_len, self.capacity), budget, recent, kept.data_ptr(), new.data_ptr())
         return kept, new
 
     def check(self) -> None:

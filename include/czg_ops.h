@@ -16,9 +16,9 @@
  * see (slots and lengths) is checked there: what is out of range is neither read nor
  * written, and a bit of czg_kv4.status says so.  n = 0 rows or sequences: CZG_OK, nothing queued.
  *
- * A row's result depends on that row's operands alone: not on how many others are in
- * the call, on its place among them, its slot, or the grid.  No result comes out of
- * an atomic whose order could change it.
+ * A row of a product, and a sequence of a cache call, depends on its own operands alone:
+ * not on how many others are in the call, on its place among them, its slot, or the
+ * grid, to the bit.  No result comes out of an atomic whose order could change it.
  */
 #ifndef CZG_OPS_H
 #define CZG_OPS_H
@@ -56,7 +56,7 @@ int czg_quantize_rows(const void *x, int dtype, int64_t ld_x, int64_t m, int64_t
  * the sum exact in int32, the rest in fp32 in this order, one rounding to out_dtype.
  * x: m rows, w: n rows of k codes, ld_x and ld_w bytes apart (16-byte aligned, a
  * multiple of 16; bytes from k on are ignored).  bias may be NULL.  out: rows ld_out
- * elements apart.  k <= CZG_LINEAR_MAX_K (the int32 sum), m, n < 2^31. */
+ * elements apart, not over x or w.  k <= CZG_LINEAR_MAX_K (the int32 sum), m, n < 2^31. */
 #define CZG_LINEAR_MAX_K 131071
 int czg_linear_i8(const int8_t *x, int64_t ld_x, const float *x_scale, const int8_t *w, int64_t ld_w,
                   const float *w_scale, const float *bias, int64_t m, int64_t n, int64_t k, void *out,
@@ -99,7 +99,8 @@ typedef struct {
 
 /* Sequences of a call: slots[b] names the slot of sequence b, a negative one a padded
  * place of the batch (nothing is read or written for it, its outputs are 0).
- * lengths[b] counts its entries, the t rows of this call among them. */
+ * lengths[b] counts its entries, the t rows of this call among them.  At most 65,535
+ * sequences a call (evict: 65,534). */
 
 /* Row i of sequence b (k, v: [b][t][n_heads][head_dim] of `dtype`, strides in elements,
  * the last one 1) becomes entry lengths[b] - t + i; rows before entry 0 are padding and
@@ -117,7 +118,8 @@ int czg_kv4_read(const czg_kv4 *cache, const int32_t *slots, const int32_t *star
 /* Attention of t rows a sequence over its entries: row i sees the first
  * lengths[b] - (t - 1 - i) of them (0 where that leaves none: the row's output is 0).
  * q, out: [b][t][hq][head_dim] of `dtype` (bf16 or fp16), strides in elements, the last one 1;
- * hq a multiple of n_heads, query heads of a key head adjacent.
+ * hq a multiple of n_heads, query heads of a key head adjacent.  out may be q itself, and
+ * lies over no other part of it.
  *   out = sum_j p_j v_j, p = softmax_j(scale q.k_j)
  * cache->weights != NULL: every entry's weight grows by its p, summed over the rows
  * and query heads of its key head.  max_len: no length of the call is above it.

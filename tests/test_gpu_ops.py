@@ -180,6 +180,35 @@ def test_linear_i8_into_a_view(ops, m):
     assert (wide[:, :3] == 7).all() and (wide[:, 48:] == 7).all()
 
 
+@pytest.mark.parametrize("m", [3, 40])
+def test_linear_i8_beside_its_operand(ops, m):
+    """Columns of one buffer: x in some, out in others; over one another they are refused."""
+    g = gen(m)
+    w = rand_codes(ops, g, 45, 64)
+    buf = randn(g, m, 128).to(BF16)
+    x = buf[:, 64:]
+    want = ops.linear_i8(x.clone(), w)
+    before = buf[:, 64:].clone()
+    assert torch.equal(ops.linear_i8(x, w, out=buf[:, 8:53]), want) and torch.equal(buf[:, 64:], before)
+    with pytest.raises(RuntimeError, match="over x"):
+        ops.linear_i8(x, w, out=buf[:, 30:75])
+
+
+def test_attend_in_place(ops):
+    """out may be q itself, or other heads of the buffer that q lies in."""
+    r = gen(21)
+    c = noise_cache(ops, r, 3, 2, 1200, 64, False)
+    for lens in ((100, 7, 40), (1200, 3, 600)):
+        buf = randn(r, 3, 2, 20, 64).to(BF16)
+        want = c.attend(buf[:, :, :8].clone(), int32(0, 1, 2), int32(*lens))
+        c.attend(buf[:, :, :8], int32(0, 1, 2), int32(*lens), out=buf[:, :, 10:18])
+        assert torch.equal(buf[:, :, 10:18], want)
+        c.attend(buf[:, :, :8], int32(0, 1, 2), int32(*lens), out=buf[:, :, :8])
+        assert torch.equal(buf[:, :, :8], want)
+        with pytest.raises(RuntimeError, match="over q"):
+            c.attend(buf[:, :, :8], int32(0, 1, 2), int32(*lens), out=buf[:, :, 4:12])
+
+
 def test_linear_i8_sums_are_exact(ops):
     """The longest row at the largest codes: 131,071 * 127 * 127 stays below 2^31."""
     k = 131071

@@ -56,7 +56,7 @@ def test_quantize_refusals(ops, want, text, args):
 
 
 def linear_args(**over):
-    a = dict(x=P, ldx=64, xs=P, w=P, ldw=64, ws=P, bias=None, m=2, n=3, k=50, out=P, kind=BF16, ldo=3, stream=None)
+    a = dict(x=P, ldx=64, xs=P, w=P, ldw=64, ws=P, bias=None, m=2, n=3, k=50, out=1 << 20, kind=BF16, ldo=3, stream=None)
     a.update(over)
     return tuple(a.values())
 
@@ -69,6 +69,8 @@ def linear_args(**over):
     (E_ARG, "null", dict(ws=None)), (E_ARG, "null", dict(out=None)), (E_ARG, "out_dtype", dict(kind=-1)),
     (E_ARG, "16-byte", dict(ldx=50)), (E_ARG, "16-byte", dict(w=P + 4)), (E_ARG, "overlap", dict(ldw=48)),
     (E_ARG, "aligned", dict(out=P + 2, kind=F32)), (E_ARG, "overlap", dict(ldo=2)),
+    (E_ARG, "over x", dict(out=P)), (E_ARG, "over x", dict(out=P + 64)), (E_ARG, "over w", dict(x=P + 4096, out=P + 128)),
+    (E_ARG, "over x", dict(out=P + 48, ldo=32)), (E_ARG, "over w", dict(x=1 << 21, w=P, ldw=4096, out=P + 4096)),
 ])
 def test_linear_refusals(ops, want, text, over):
     refused(ops, want, text, "czg_linear_i8", *linear_args(**over))
@@ -81,7 +83,7 @@ def test_linear_dynamic_refusals(ops):
     assert L.czg_linear_i8_workspace(2, 50) == 0      # a few short rows take none
 
     def call(ws=P, n_ws=need, x=P, kind=BF16):
-        return L.czg_linear_i8_dynamic(x, kind, 50, P, 64, P, None, 21, 3, 50, P, BF16, 3, ws, n_ws, None)
+        return L.czg_linear_i8_dynamic(x, kind, 50, P, 64, P, None, 21, 3, 50, 1 << 20, BF16, 3, ws, n_ws, None)
 
     for args, text in ((dict(ws=None), "workspace"), (dict(ws=P + 8), "workspace"), (dict(n_ws=need - 1), "too small"),
                        (dict(x=None), "null"), (dict(kind=9), "dtype")):
@@ -103,7 +105,7 @@ def test_cache_refusals(ops, want, text, over):
     c = cache(ops, **over)
     refused(ops, want, text, "czg_kv4_append", c, P, 1, 1, 1, P, 1, 1, 1, BF16, P, P, 2, 1, None)
     refused(ops, want, text, "czg_kv4_read", c, P, P, 2, 1, P, P, BF16, None)
-    refused(ops, want, text, "czg_kv4_attend", c, P, 1, 1, 1, BF16, P, P, 2, 1, 4, 100, 0.1, P, 1, 1, 1, P, 1 << 40, None)
+    refused(ops, want, text, "czg_kv4_attend", c, P, 256, 256, 64, BF16, P, P, 2, 1, 4, 100, 0.1, P, 256, 256, 64, P, 1 << 40, None)
     refused(ops, want, text, "czg_kv4_evict", c, P, P, 2, 100, 10, 2, P, P + 64, None)
 
 
@@ -113,8 +115,8 @@ def test_kv4_call_refusals(ops):
     def append(k=P, v=P, kind=BF16, slots=P, lengths=P, b=2, t=1):
         return ("czg_kv4_append", c, k, 1, 1, 1, v, 1, 1, 1, kind, slots, lengths, b, t, None)
 
-    def attend(q=P, kind=BF16, slots=P, b=2, t=1, hq=4, max_len=100, out=P, ws=P, n_ws=1 << 40):
-        return ("czg_kv4_attend", c, q, 1, 1, 1, kind, slots, P, b, t, hq, max_len, 0.1, out, 1, 1, 1, ws, n_ws, None)
+    def attend(q=P, kind=BF16, slots=P, b=2, t=1, hq=4, max_len=100, out=1 << 20, ws=P, n_ws=1 << 40, os=(256, 256, 64)):
+        return ("czg_kv4_attend", c, q, 256, 256, 64, kind, slots, P, b, t, hq, max_len, 0.1, out, *os, ws, n_ws, None)
 
     def evict(c=c, lengths=P, b=2, max_len=100, budget=10, recent=2, new=P + 64):
         return ("czg_kv4_evict", c, P, lengths, b, max_len, budget, recent, P, new, None)
@@ -126,6 +128,8 @@ def test_kv4_call_refusals(ops):
             (OK, "", attend(b=0)), (OK, "", attend(t=0)), (E_ARG, "multiple", attend(hq=3)), (E_ARG, "multiple", attend(hq=0)),
             (E_UNSUPPORTED, "bf16 or fp16", attend(kind=F32)), (E_ARG, "null", attend(q=None)), (E_ARG, "null", attend(out=None)),
             (E_ARG, "negative", attend(max_len=-1)), (E_ARG, "workspace", attend(ws=P + 8)),
+            (E_ARG, "overlap", attend(os=(0, 256, 64))), (E_ARG, "over q", attend(out=P + 128)), (E_ARG, "over q", attend(out=P - 64)),
+            (E_ARG, "over q", attend(out=P, os=(512, 256, 64))), (E_ARG, "workspace", attend(out=P, ws=P + 8)),
             (OK, "", evict(b=0)), (E_ARG, "budget", evict(budget=0)), (E_ARG, "budget", evict(recent=11)),
             (E_ARG, "budget", evict(recent=-1)), (E_ARG, "weights", evict(c=cache(ops, weights=None))),
             (E_LIMIT, "EVICT_MAX", evict(max_len=(1 << 20) + 1)), (E_ARG, "new_lengths", evict(new=P)),
