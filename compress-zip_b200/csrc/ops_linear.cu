@@ -844,18 +844,22 @@ template <typename T>
 int quantize(const void *x, int64_t ldx, int64_t m, int64_t k, int8_t *codes, int64_t ldc, float *scales, cudaStream_t st) {
     const int64_t turns = (k + 7) / 8;
     const int vec = aligned(x, 16) && (m == 1 || ldx * sizeof(T) % 16 == 0);
-    // a warp a row once there are rows for all of an SM's warps (8192 x 4096 bf16: MEASUREW)
-    if (m >= 16 * sm_count() && k <= (sizeof(T) == 2 ? 4096 : 2048)) {
+    // With rows for all of an SM's warps: a warp a row while it fits its registers (8192 x 2048
+    // bf16: 15.1 us; a CTA a row 16.7), then a CTA of 4 warps (8192 x 4096: 25.0 us, 4.0 TB/s of
+    // rows and codes; a warp a row 28.6, whose few warps load and compute in step; 8 warps
+    // 31.3).  Few rows get 8 warps each.
+    const bool many = m >= 16 * sm_count();
+    if (many && k <= (sizeof(T) == 2 ? 2048 : 1024)) {
         const dim3 grid((unsigned)((m + 3) / 4));
         auto go = [&](auto kern) {
             return ops_cuda(ops_launch(kern, grid, 128, 0, st, false, 1, static_cast<const T *>(x), ldx, (int)m, (int)k, vec, codes, ldc, scales));
         };
         if (turns <= 2 * 32) return go(k_quantize_rows_warp<T, 2>);
         if (turns <= 4 * 32) return go(k_quantize_rows_warp<T, 4>);
-        if (turns <= 8 * 32) return go(k_quantize_rows_warp<T, 8>);
-        return go(k_quantize_rows_warp<T, 16>);
+        return go(k_quantize_rows_warp<T, 8>);
     }
-    const int threads = turns >= kQuantThreads ? kQuantThreads : (int)((turns + 31) / 32 * 32);
+    const int most = many ? kQuantThreads / 2 : kQuantThreads;
+    const int threads = turns >= most ? most : (int)((turns + 31) / 32 * 32);
     return ops_cuda(ops_launch(k_quantize_rows<T>, dim3((unsigned)m), threads, 0, st, false, 1, static_cast<const T *>(x), ldx,
                                k, vec, codes, ldc, scales));
 }
