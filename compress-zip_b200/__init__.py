@@ -3,6 +3,7 @@
 Package layout:
   csrc/          CUDA kernels (sm_100a) and the C-ABI host library libczg.so
   engine.py      ctypes binding of the C-ABI (include/czg.h) -- the GPU path
+  ops.py         ctypes binding of the device-buffer operators (include/czg_ops.h)
   container.py   CZIPv1 outer/inner header and chunk payload
   czm.py         .czm (safetensors) model file reader/writer
   tokenizer.py   BPE tokenizer over the model's embedded JSON
