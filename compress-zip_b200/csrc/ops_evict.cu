@@ -1,5 +1,6 @@
 // ops_evict.cu -- eviction from the 4-bit cache by accumulated attention weight
 // (include/czg_ops.h).
+#include "common.cuh"
 #include "ops_kv4.cuh"
 
 namespace czg {
@@ -59,6 +60,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_evict(czg_kv4 c, const int3
     __shared__ uint32_t s_prefix;
     __shared__ int s_need;
     const int h = blockIdx.x, s = blockIdx.y, tid = threadIdx.x;
+    pdl_wait();
+    pdl_trigger();
     if (s == b) {   // one more sequence's worth of CTAs: the first looks for repeated slots
         if (h == 0) kv4_check_distinct(c, slots, b);
         return;
@@ -205,6 +208,6 @@ extern "C" int czg_kv4_evict(const czg_kv4 *cache, const int32_t *slots, const i
     if (b == 0) return CZG_OK;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     auto kern = cache->head_dim == 64 ? k_kv4_evict<64> : k_kv4_evict<128>;
-    return ops_cuda(ops_launch(kern, dim3((unsigned)cache->n_heads, (unsigned)b + 1), kThreads, 0, st, false, 1, *cache, slots,
+    return ops_cuda(ops_launch(kern, dim3((unsigned)cache->n_heads, (unsigned)b + 1), kThreads, 0, st, true, 1, *cache, slots,
                                lengths, b, max_len, budget, recent, kept, new_lengths));
 }

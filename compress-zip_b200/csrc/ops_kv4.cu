@@ -35,6 +35,8 @@ template <typename T, int D>
 __global__ void __launch_bounds__(256) k_kv4_append(czg_kv4 c, const T *__restrict__ k, Strides ks, const T *__restrict__ v,
                                                     Strides vs, int vec, const int32_t *__restrict__ slots,
                                                     const int32_t *__restrict__ lengths, int b, int t) {
+    pdl_wait();
+    pdl_trigger();
     if (blockIdx.x == 0) {
         kv4_check_distinct(c, slots, b);
         return;
@@ -110,6 +112,8 @@ __global__ void __launch_bounds__(256) k_kv4_read(czg_kv4 c, const int32_t *__re
                                                   const int32_t *__restrict__ starts, uint32_t rows, uint32_t all,
                                                   T *__restrict__ k_out, T *__restrict__ v_out) {
     constexpr int P = D / 8, N = 2;
+    pdl_wait();
+    pdl_trigger();
     const int part = threadIdx.x % P;
     uint2 range[N];
     uint32_t codes[N][2];
@@ -315,6 +319,7 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
     const int unit = blockIdx.x, h = p.row_blocks == 1 ? blockIdx.y : blockIdx.y / p.row_blocks, b = blockIdx.z;
     const int rb = blockIdx.y - h * p.row_blocks;
     const bool first = tid == 0 && unit == 0 && blockIdx.y == 0;
+    pdl_wait();
     pdl_trigger();   // k_kv4_join may begin to launch
     if (TRACK && unit == 0 && b == 0 && blockIdx.y == 0) kv4_check_distinct(p.c, p.slots, gridDim.z);
     const int slot = kv4_slot(p.c, p.slots, b, first);
@@ -735,7 +740,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv4_join(const __grid_constant
     const int n = slot < 0 ? 0 : kv4_length(p.c, p.lengths, b, min(p.max_len, p.c.capacity), false);
     const int len = unit_of(n), units = n == 0 ? 0 : (n - 1) / len + 1;
     const int64_t first = ((int64_t)b * p.c.n_heads + h) * p.units * rows_padded;
-    pdl_wait();   // slots and lengths are older than the kernel before this one
+    pdl_wait();   // slots and lengths are older than the kernel before this one, which waited for them
     if ((int)blockIdx.x < row_ctas) {
         const int d = 4 * (tid % TR), run = tid / TR;
         if (units <= kFew) {
@@ -902,7 +907,7 @@ int append(const czg_kv4 &c, const void *k, Strides ks, const void *v, Strides v
     };
     const int vec = vec_of(k, ks) && vec_of(v, vs);
     auto kern = c.head_dim == 64 ? k_kv4_append<T, 64> : k_kv4_append<T, 128>;
-    return ops_cuda(ops_launch(kern, dim3((unsigned)((2 * rows + per - 1) / per + 1)), 256, 0, st, false, 1, c,
+    return ops_cuda(ops_launch(kern, dim3((unsigned)((2 * rows + per - 1) / per + 1)), 256, 0, st, true, 1, c,
                                static_cast<const T *>(k), ks, static_cast<const T *>(v), vs, vec, slots, lengths, b, t));
 }
 
@@ -912,7 +917,7 @@ int read(const czg_kv4 &c, const int32_t *slots, const int32_t *starts, int b, i
     if (all >= 1ll << 31) return ops_fail(CZG_E_LIMIT, "too many entries");
     const int64_t per = 4096 / c.head_dim;
     auto kern = c.head_dim == 64 ? k_kv4_read<T, 64> : k_kv4_read<T, 128>;
-    return ops_cuda(ops_launch(kern, dim3((unsigned)((all + per - 1) / per)), 256, 0, st, false, 1, c, slots, starts,
+    return ops_cuda(ops_launch(kern, dim3((unsigned)((all + per - 1) / per)), 256, 0, st, true, 1, c, slots, starts,
                                (uint32_t)rows, (uint32_t)all, static_cast<T *>(k), static_cast<T *>(v)));
 }
 
@@ -931,7 +936,7 @@ int attend_with(const AttendPlan &plan, const AttendArgs &p, int b, cudaStream_t
         ready[dev] = 1;
     }
     const dim3 grid((unsigned)plan.units, (unsigned)(p.c.n_heads * plan.row_blocks), (unsigned)b);
-    if (int e = ops_cuda(ops_launch(k_kv4_attend<T, D, NB, TRACK>, grid, kWarps * 32, smem, st, false, 1, mk, mv, p))) return e;
+    if (int e = ops_cuda(ops_launch(k_kv4_attend<T, D, NB, TRACK>, grid, kWarps * 32, smem, st, true, 1, mk, mv, p))) return e;
     if (!plan.join) return CZG_OK;
     constexpr int kRuns = kJoinThreads / (D / 4);
     const int row_ctas = plan.units <= kFew ? (plan.rows + kRuns - 1) / kRuns : plan.rows;

@@ -146,6 +146,7 @@ template <typename T>
 __global__ void __launch_bounds__(kQuantThreads) k_quantize_rows(const T *__restrict__ x, int64_t ldx, int64_t k, int vec,
                                                                  int8_t *__restrict__ codes, int64_t ldc,
                                                                  float *__restrict__ scales) {
+    pdl_wait();
     pdl_trigger();   // the product may set itself up meanwhile
     const T *row = x + (int64_t)blockIdx.x * ldx;
     int8_t *out = codes + (int64_t)blockIdx.x * ldc;
@@ -198,6 +199,7 @@ __global__ void __launch_bounds__(kQuantThreads) k_quantize_rows(const T *__rest
 template <typename T, int V>
 __global__ void __launch_bounds__(128) k_quantize_rows_warp(const T *__restrict__ x, int64_t ldx, int m, int k, int vec,
                                                             int8_t *__restrict__ codes, int64_t ldc, float *__restrict__ scales) {
+    pdl_wait();
     pdl_trigger();
     const int r = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (r >= m) return;
@@ -852,7 +854,7 @@ int quantize(const void *x, int64_t ldx, int64_t m, int64_t k, int8_t *codes, in
     if (many && k <= (sizeof(T) == 2 ? 2048 : 1024)) {
         const dim3 grid((unsigned)((m + 3) / 4));
         auto go = [&](auto kern) {
-            return ops_cuda(ops_launch(kern, grid, 128, 0, st, false, 1, static_cast<const T *>(x), ldx, (int)m, (int)k, vec, codes, ldc, scales));
+            return ops_cuda(ops_launch(kern, grid, 128, 0, st, true, 1, static_cast<const T *>(x), ldx, (int)m, (int)k, vec, codes, ldc, scales));
         };
         if (turns <= 2 * 32) return go(k_quantize_rows_warp<T, 2>);
         if (turns <= 4 * 32) return go(k_quantize_rows_warp<T, 4>);
@@ -860,7 +862,7 @@ int quantize(const void *x, int64_t ldx, int64_t m, int64_t k, int8_t *codes, in
     }
     const int most = many ? kQuantThreads / 2 : kQuantThreads;
     const int threads = turns >= most ? most : (int)((turns + 31) / 32 * 32);
-    return ops_cuda(ops_launch(k_quantize_rows<T>, dim3((unsigned)m), threads, 0, st, false, 1, static_cast<const T *>(x), ldx,
+    return ops_cuda(ops_launch(k_quantize_rows<T>, dim3((unsigned)m), threads, 0, st, true, 1, static_cast<const T *>(x), ldx,
                                k, vec, codes, ldc, scales));
 }
 

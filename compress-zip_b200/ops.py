@@ -265,6 +265,7 @@ class KV4Cache:
         self.status = torch.zeros(1, dtype=torch.int32, device=k.device)
         self._c = _KV4(k.data_ptr(), v.data_ptr(), scales.data_ptr(), 0 if weights is None else weights.data_ptr(),
                        self.status.data_ptr(), self.n_slots, self.n_heads, self.capacity, self.head_dim)
+        self._needs = {}   # workspace bytes by a call's sizes
         self._ref, self._lib, self._index = C.byref(self._c), lib(), k.get_device()
 
     @classmethod
@@ -354,7 +355,11 @@ class KV4Cache:
         if not (b and t and hq):
             return out
         n = self.capacity if max_len is None else min(max_len, self.capacity)
-        need = self._lib.czg_kv4_attend_workspace(self._ref, b, t, hq, n)
+        need = self._needs.get((b, t, hq, n))
+        if need is None:
+            if len(self._needs) > 4096:
+                self._needs.clear()
+            need = self._needs[b, t, hq, n] = self._lib.czg_kv4_attend_workspace(self._ref, b, t, hq, n)
         ws = self.k.new_empty(need) if need else None
         self._call(self._lib.czg_kv4_attend, q.data_ptr(), qs[0], qs[1], qs[2], DTYPES[q.dtype], slots.data_ptr(),
                    lengths.data_ptr(), b, t, hq, n, self.head_dim ** -0.5 if scale is None else scale, out.data_ptr(),

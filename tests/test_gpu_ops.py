@@ -781,6 +781,45 @@ def test_two_streams_and_graph(ops):
     assert torch.equal(layer.cache.weights, eager.cache.weights)
 
 
+def test_graph_of_copies_and_operators(ops):
+    """Copies, fills and torch's kernels before and between the operators of a captured graph."""
+    g = gen(31)
+    layer, slots, n = Layer(ops, 12), int32(0, 1, 2), int32(0, 0, 0)
+    src, x = [randn(g, 3, 1, 384).to(BF16) for _ in range(5)], torch.zeros(3, 1, 384, dtype=BF16, device=DEV)
+    feed, total = torch.zeros_like(x), torch.zeros(3, 1, 384, device=DEV)
+
+    def step():
+        x.copy_(feed)
+        n.add_(1)
+        total.zero_()
+        y = layer.step(x, slots, n)
+        total.add_(y.float())
+        feed.zero_()
+        return y
+
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        step()
+    stream.synchronize()
+    n.zero_()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = step()
+    got = []
+    for s in src:
+        feed.copy_(s)
+        graph.replay()
+        got.append((y.clone(), total.clone()))
+    torch.cuda.synchronize()
+    layer.cache.check()
+    ref, m = Layer(ops, 12), int32(0, 0, 0)
+    for s, (a, b) in zip(src, got):
+        m.add_(1)
+        want = ref.step(s, slots, m)
+        assert torch.equal(a, want) and torch.equal(b, want.float())
+    assert torch.equal(layer.cache.weights[:, :, :5], ref.cache.weights[:, :, :5])
+
+
 def test_every_call_gives_the_same_bits_again(ops):
     g = gen(13)
     c = noise_cache(ops, g, 20, 2, 3000, 128, True)
