@@ -50,7 +50,10 @@ __device__ __forceinline__ uint32_t scan(uint32_t x, uint32_t *before, uint32_t 
 // 3. A stretch's entries move, kThreads * kTasks pieces of 16 bytes at a time: all are read,
 //    the CTA waits, all are written.  The i-th kept entry lies at place i or behind it, so
 //    no place is written before it was read.
-// Bound by reading and writing what moves; measured beside the launch below.
+// Bound by reading and writing what moves: 48 x 8 heads of up to 4096 entries cut to 1024
+// (D = 128, 114 MB moved) take 23.5 us, 4.9 TB/s; one head from 1024 to 700 takes 6.5 us of
+// latency (three passes of counting, two scans, one move).  256 threads a CTA took 4 us
+// more on the batch, one CTA an SM (119 registers) 10 us more.
 template <int D>
 __global__ void __launch_bounds__(kThreads, 2) k_kv4_evict(czg_kv4 c, const int32_t *__restrict__ slots,
                                                         const int32_t *__restrict__ lengths, int b, int max_len, int budget,

@@ -139,7 +139,7 @@ struct RowScale {
     }
 };
 
-// One CTA a row: its maximum, then its codes, 8 values a thread and turn; rows of up to
+// One CTA a row (48 x 4096: 2.8 us): its maximum, then its codes, 8 values a thread and turn; rows of up to
 // kHeld turns stay in registers between the two, longer ones are read again.
 constexpr int kQuantThreads = 256, kHeld = 4;
 template <typename T>
@@ -244,6 +244,8 @@ __global__ void __launch_bounds__(128) k_quantize_rows_warp(const T *__restrict_
 // adds up all CTAs' sums of the tokens r NT / S .. (16 bytes a lane through distributed
 // shared memory; 4-byte stores to the other CTAs instead took 4 us more at NT = 64):
 // integers, so the split does not show in the result.
+// Measured: 48 x 4096 x 4096 (16.8 MB of weights): 9.8 us, and 11 with the quantiser; 4.5 us of
+// any call are the setup, the first loads and the epilogue.  1333 x 1000 x 1100: 10.6 us.
 constexpr int LT = 128;   // channels of a tile
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -556,7 +558,8 @@ k_linear_tc(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ C
 // For large m the loads of 128 x 256 tiles are what one CTA waits for (8192 x 8192 x 4096:
 // 145 of 211 us with the MMAs left out).  A pair of CTAs (tcgen05 cta_group::2) shares
 // 256 channels x 256 tokens: each loads its 128 weight rows and half of the tokens, and
-// the MMAs of the first CTA read both, so a byte loaded serves a third more products.
+// the MMAs of the first CTA read both, so a byte loaded serves a third more products:
+// 191 us, 2.88 POP/s, 87% of twice the measured bf16 rate, the tensor pipe 74% active.
 // Each CTA's sums of its channels land in its own TMEM; the epilogue is as above.
 //   full[s]   of the first CTA: both CTAs' loads of the stage (64 KB)
 //   empty[s]  of each CTA: the MMAs have read it (committed to both)
@@ -943,10 +946,12 @@ int check_apart(const void *out, int64_t out_ld, int64_t out_row, const void *in
     return ops_fail(CZG_E_ARG, why);
 }
 
+constexpr int64_t kMaxRows = 0x7FFFFE00;   // a tile behind the last row is still an int
+
 int check_sizes(int64_t m, int64_t n, int64_t k) {
     if (m < 0 || n < 0 || k < 1) return ops_fail(CZG_E_ARG, "m and n must not be negative, k must be at least 1");
     if (k > CZG_LINEAR_MAX_K) return ops_fail(CZG_E_LIMIT, "k is beyond CZG_LINEAR_MAX_K");
-    if (m > 0x7FFFFFFF || n > 0x7FFFFFFF) return ops_fail(CZG_E_LIMIT, "m and n must be below 2^31");
+    if (m > kMaxRows || n > kMaxRows) return ops_fail(CZG_E_LIMIT, "m and n must be at most 2^31 - 512");
     return CZG_OK;
 }
 
@@ -978,7 +983,7 @@ extern "C" int czg_ops_check(void) {
 extern "C" int czg_quantize_rows(const void *x, int dtype, int64_t ld_x, int64_t m, int64_t k, int8_t *codes,
                                  int64_t ld_codes, float *scales, void *stream) {
     if (m < 0 || k < 1) return ops_fail(CZG_E_ARG, "m must not be negative, k must be at least 1");
-    if (m > 0x7FFFFFFF) return ops_fail(CZG_E_LIMIT, "m must be below 2^31");
+    if (m > kMaxRows) return ops_fail(CZG_E_LIMIT, "m must be at most 2^31 - 512");
     if (m == 0) return CZG_OK;
     if (int st = check_x(x, dtype, ld_x, m, k)) return st;
     if (!codes || !scales) return ops_fail(CZG_E_ARG, "null pointer");

@@ -87,7 +87,8 @@ def _same_device(dev: torch.device, **tensors) -> None:
 
 
 _current_device = torch.cuda.current_device
-_raw_stream = torch._C._cuda_getCurrentRawStream   # the handle of the current stream, without a Stream object around it
+# the handle of a device's current stream, without a Stream object around it where torch has that
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
 
 def _call(dev: torch.device, fn, *args) -> None:

@@ -56,7 +56,7 @@ int czg_quantize_rows(const void *x, int dtype, int64_t ld_x, int64_t m, int64_t
  * the sum exact in int32, the rest in fp32 in this order, one rounding to out_dtype.
  * x: m rows, w: n rows of k codes, ld_x and ld_w bytes apart (16-byte aligned, a
  * multiple of 16; bytes from k on are ignored).  bias may be NULL.  out: rows ld_out
- * elements apart, not over x or w.  k <= CZG_LINEAR_MAX_K (the int32 sum), m, n < 2^31. */
+ * elements apart, not over x or w.  k <= CZG_LINEAR_MAX_K (the int32 sum), m, n <= 2^31 - 512. */
 #define CZG_LINEAR_MAX_K 131071
 int czg_linear_i8(const int8_t *x, int64_t ld_x, const float *x_scale, const int8_t *w, int64_t ld_w,
                   const float *w_scale, const float *bias, int64_t m, int64_t n, int64_t k, void *out,
