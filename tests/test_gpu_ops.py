@@ -484,6 +484,12 @@ def check_attend(ops, c, q, slots, lengths, max_len=None, scale=None):
     (128, 8, 7, 3, BF16, (513, 2, 64), 513),
     (64, 1, 8, 1, FP16, (70000, 65537, 500, 65536), 70001),
     (128, 1, 2, 2, BF16, (131073, 66001), 131073),
+    (64, 1, 2, 1, BF16, (300000,), 300000),
+    (64, 1, 8, 150, BF16, (300, 5, 149, 151), 300),
+    (128, 1, 3, 40, FP16, (1100, 39), 1100),
+    (64, 96, 1, 1, BF16, (70, 1), 70),
+    (64, 1, 40, 1, FP16, (600, 20), 600),
+    (128, 2, 2, 1, BF16, (1, 1, 0), 1),
 ])
 def test_attend(ops, d, heads, g, t, dtype, lens, capacity, track):
     r = gen(capacity + t)
@@ -502,6 +508,49 @@ def test_attend(ops, d, heads, g, t, dtype, lens, capacity, track):
     assert torch.equal(c.attend(q, slots, lengths, max_len=max(max(lens), 1)), y)
     for i in range(b):
         assert torch.equal(c.attend(q[i:i + 1], slots[i:i + 1], lengths[i:i + 1]), y[i:i + 1])
+
+
+def test_many_sequences(ops):
+    """More sequences than any grid dimension's usual size, slots in any order, some of them padding;
+    a cache of slots beyond what one pass of the check for repeated slots covers."""
+    r = gen(40)
+    b, n_slots = 60000, 70000
+    c = noise_cache(ops, r, n_slots, 1, 4, 64, True)
+    before = c.weights.clone()
+    slots = torch.randperm(n_slots, generator=r, device=DEV)[:b].int()
+    slots[::7] = -1
+    lengths = torch.randint(0, 5, (b,), generator=r, device=DEV, dtype=torch.int32)
+    rows, q = randn(r, b, 1, 1, 64).to(BF16), randn(r, b, 1, 2, 64).to(BF16)
+    c.append(rows, -rows, slots, lengths)
+    y = c.attend(q, slots, lengths)
+    c.check()
+    some = (slots >= 0) & (lengths > 0)
+    assert not y[~some].any()
+    at, last = slots[some].long(), lengths[some].long() - 1
+    code = torch.stack([c.k & 15, c.k >> 4], -1).flatten(-2)[:, 0].double()
+    sc = c.scales[:, 0].double()
+    k = sc[..., 1:2] + sc[..., :1] * code
+    code = torch.stack([c.v & 15, c.v >> 4], -1).flatten(-2)[:, 0].double()
+    v = sc[..., 3:] + sc[..., 2:3] * code
+    assert torch.equal(k[at, last], held(rows[some, 0, 0])[0]) and torch.equal(v[at, last], held(-rows[some, 0, 0])[0])
+    s = torch.einsum("bgd,bnd->bgn", q[some, 0].double(), k[at]) / 8
+    s = torch.where(torch.arange(4, device=DEV) <= last[:, None, None], s, -math.inf)
+    p = torch.softmax(s, -1)
+    want = torch.einsum("bgn,bnd->bgd", p, v[at])
+    terms = torch.einsum("bgn,bn->bg", p, (15 * sc[..., 2] + sc[..., 3].abs())[at])[..., None]
+    # attention()'s 2^-11 of the values' terms and 2^-20 of a weight, with room for its scores' rounding
+    assert ((y[some, 0].double() - want).abs() <= u(BF16) * want.abs() + 2.0 ** -10 * terms).all()
+    grown = c.weights.double()[at, 0] - torch.where(torch.arange(4, device=DEV) == last[:, None], 0.0, before[at, 0].double())
+    assert (grown - p.sum(1)).abs().max() < 2.0 ** -18
+    untouched = torch.ones(n_slots, dtype=torch.bool, device=DEV)
+    untouched[at] = False
+    assert torch.equal(c.weights[untouched], before[untouched])
+    kept, new = c.evict(slots, lengths, 2, 1)
+    assert torch.equal(new, torch.where(slots >= 0, lengths, 0).clamp(max=2))
+    slots[b - 1] = slots[1]
+    c.append(rows, rows, slots, lengths)
+    with pytest.raises(RuntimeError, match="twice"):
+        c.check()
 
 
 @pytest.mark.parametrize("g,t", [(4, 1), (2, 3)])
