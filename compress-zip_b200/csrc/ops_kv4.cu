@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(256) k_kv4_read(czg_kv4 c, const int32_t *__re
 // The query is held in fp16 after a power of two that brings its largest value to
 // [2^13, 2^14): exact but for values below 2^-23 of the largest.  p_j step_j is
 // held in fp16 likewise (2^7 to 2^15 for the unit's largest): off by 2^-12 of itself, against
-// 2^-9 of the result for bf16 and 2^-12 for fp16; its range is 2^31 wide.  Scores, maxima and
+// 2^-9 of a bf16 result (for an fp16 one in two parts, to 2^-22); its range is 2^31 wide.  Scores, maxima and
 // sums are fp32; exponentials are ex2.approx (2^-22).
 //
 // Measured: one sequence of 131,071 entries, 32 heads on 8, D = 128, bf16 (143 MB): 37 us with
@@ -440,16 +440,16 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
     // scores of this CTA's rows from entry j0 on, kept for the weights
     float *score = TRACK ? p.score + (((int64_t)b * p.c.n_heads + h) * p.rows + rb * R) * p.max_len + j0 : nullptr;
     const int rows_here = min(R, p.rows - rb * R);
-    // kExact: what the fp16 weights lost is made good at the middle of the codes, so their
-    // rounding counts from there (a third) and not from code 0; bf16 results do not need it
+    // kExact: the weights' rounding to fp16, 2^-12 of each, is as large as that of an fp16
+    // result, so there what it leaves is a second fp16 weight of its own, to 2^-22
     constexpr bool kExact = DType<T>::kCode == CZG_F16;
-    float m[NB][2], l[NB][2], z[NB][2], lost[NB][2], o[NB][CH][2][4];
+    float m[NB][2], l[NB][2], z[NB][2], o[NB][CH][2][4];
 #pragma unroll
     for (int nb = 0; nb < NB; nb++) {
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             m[nb][i] = -INFINITY;
-            l[nb][i] = z[nb][i] = lost[nb][i] = 0.0f;
+            l[nb][i] = z[nb][i] = 0.0f;
         }
 #pragma unroll
         for (int ch = 0; ch < CH; ch++)
@@ -560,7 +560,6 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
                             const float f = was == now ? 1.0f : was == -INFINITY ? 0.0f : ex2((was - now) * qs[nb][i]);
                             l[nb][i] *= f;
                             z[nb][i] *= f;
-                            if (kExact) lost[nb][i] *= f;
 #pragma unroll
                             for (int ch = 0; ch < CH; ch++)
 #pragma unroll
@@ -573,7 +572,7 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
             }
 #pragma unroll
             for (int kb = 0; kb < KB; kb++) {
-                uint32_t pf[NB][2];
+                uint32_t pf[NB][2], pl[NB][2];
 #pragma unroll
                 for (int hf = 0; hf < 2; hf++) {
                     const int j = t0 + kb * 16 + hf * 8 + g8;
@@ -592,8 +591,7 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
                         const uint32_t wp = pack_half(w[0], w[1]);
                         if (kExact) {
                             const float2 back = __half22float2(*reinterpret_cast<const __half2 *>(&wp));
-                            lost[nb][0] += w[0] - back.x;
-                            lost[nb][1] += w[1] - back.y;
+                            pl[nb][hf] = transpose8(pack_half(w[0] - back.x, w[1] - back.y));
                         }
                         pf[nb][hf] = transpose8(wp);
                     }
@@ -612,6 +610,10 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
                         for (int nb = 0; nb < NB; nb++) {
                             mma_f16(o[nb][cp + ci][0], a & 0x000F000Fu, a & 0x00FF00FFu, c & 0x000F000Fu, c & 0x00FF00FFu, pf[nb][0], pf[nb][1]);
                             mma_f16(o[nb][cp + ci][1], a8 & 0x000F000Fu, a8, c8 & 0x000F000Fu, c8, pf[nb][0], pf[nb][1]);
+                            if (kExact) {
+                                mma_f16(o[nb][cp + ci][0], a & 0x000F000Fu, a & 0x00FF00FFu, c & 0x000F000Fu, c & 0x00FF00FFu, pl[nb][0], pl[nb][1]);
+                                mma_f16(o[nb][cp + ci][1], a8 & 0x000F000Fu, a8, c8 & 0x000F000Fu, c8, pl[nb][0], pl[nb][1]);
+                            }
                         }
                     }
                 }
@@ -645,7 +647,6 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
                     for (int i = 0; i < 2; i++) {
                         l[nb][i] = l[nb][i] * f * f2;
                         z[nb][i] = z[nb][i] * f * f2;
-                        lost[nb][i] = lost[nb][i] * f * f2;
                         mq[nb][i] = m[nb][i] == -INFINITY ? 0.0f : __fmaf_rn(m[nb][i], qs[nb][i], (float)(te - 7));
 #pragma unroll
                         for (int ch = 0; ch < CH; ch++)
@@ -667,10 +668,9 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
                 for (int x = 4; x < 32; x <<= 1) {
                     l[nb][i] += __shfl_xor_sync(0xffffffffu, l[nb][i], x);
                     z[nb][i] += __shfl_xor_sync(0xffffffffu, z[nb][i], x);
-                    if (kExact) lost[nb][i] += __shfl_xor_sync(0xffffffffu, lost[nb][i], x);
                 }
                 l[nb][i] *= down;
-                z[nb][i] = __fmaf_rn(lost[nb][i], 7.5f, z[nb][i]) * down;
+                z[nb][i] *= down;
                 m[nb][i] = m[nb][i] == -INFINITY ? -INFINITY : m[nb][i] * qs[nb][i];
                 if (g8 == 0 && warp < warps) {
                     s_m[warp][nb * 8 + 2 * c4 + i] = m[nb][i];
