@@ -298,8 +298,12 @@ __device__ __forceinline__ int64_t row_offset(const AttendArgs &p, const Strides
 
 __device__ __forceinline__ float pow2f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }   // -126 <= e <= 127
 
-// CTAs an SM is to hold: what the sums (D NB / 4 registers), query and scores leave room for
-constexpr int attend_ctas(int d, int nb) { return d == 64 ? (nb == 1 ? 10 : 4) : (nb == 1 ? 8 : 3); }
+// CTAs an SM is to hold: what the sums (D NB / 4 registers), query and scores leave room
+// for.  With the weights in two parts (exact) fewer of them spill less (attend of 64
+// sequences of up to 4096, 32 heads on 4, D = 128, with weights: 43.4 us, 45.0 with 8).
+constexpr int attend_ctas(int d, int nb, bool exact) {
+    return d == 64 ? (nb == 1 ? (exact ? 8 : 10) : exact ? 3 : 4) : nb == 1 ? (exact ? 6 : 8) : exact ? 2 : 3;
+}
 
 template <int D, int W>
 struct AttendSmem {
@@ -309,7 +313,7 @@ struct AttendSmem {
 };
 
 template <typename T, int D, int NB, bool TRACK>
-__global__ void __launch_bounds__(attend_warps(NB) * 32, attend_ctas(D, NB))
+__global__ void __launch_bounds__(attend_warps(NB) * 32, attend_ctas(D, NB, DType<T>::kCode == CZG_F16))
 k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttendArgs p) {
     constexpr int kWarps = attend_warps(NB);
     using L = AttendSmem<D, kWarps>;
