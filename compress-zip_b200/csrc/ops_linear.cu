@@ -852,7 +852,8 @@ int quantize(const void *x, int64_t ldx, int64_t m, int64_t k, int8_t *codes, in
     // With rows for all of an SM's warps: a warp a row while it fits its registers (8192 x 2048
     // bf16: 15.1 us; a CTA a row 16.7), then a CTA of 4 warps (8192 x 4096: 25.0 us, 4.0 TB/s of
     // rows and codes; a warp a row 28.6, whose few warps load and compute in step; 8 warps
-    // 31.3).  Few rows get 8 warps each.
+    // 31.3).  Few rows, and rows that 4 warps would have to read twice (2000 x 8192: 18.7 us,
+    // 13.9 with 8), get 8 warps each.
     const bool many = m >= 16 * sm_count();
     if (many && k <= (sizeof(T) == 2 ? 2048 : 1024)) {
         const dim3 grid((unsigned)((m + 3) / 4));
@@ -863,7 +864,7 @@ int quantize(const void *x, int64_t ldx, int64_t m, int64_t k, int8_t *codes, in
         if (turns <= 4 * 32) return go(k_quantize_rows_warp<T, 4>);
         return go(k_quantize_rows_warp<T, 8>);
     }
-    const int most = many ? kQuantThreads / 2 : kQuantThreads;
+    const int most = many && k <= kQuantThreads / 2 * 8 * kHeld ? kQuantThreads / 2 : kQuantThreads;
     const int threads = turns >= most ? most : (int)((turns + 31) / 32 * 32);
     return ops_cuda(ops_launch(k_quantize_rows<T>, dim3((unsigned)m), threads, 0, st, true, 1, static_cast<const T *>(x), ldx,
                                k, vec, codes, ldc, scales));
