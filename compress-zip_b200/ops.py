@@ -204,7 +204,7 @@ def linear_i8(x, w: QRows, bias: Optional[torch.Tensor] = None, out_dtype: Optio
     if dev.type != "cuda":
         raise ValueError(f"tensors must be on a CUDA device, not {dev}")
     if out is None:
-        out2 = x2.new_empty((m, n)) if x2.dtype is kind else torch.empty((m, n), dtype=kind, device=dev)
+        out2 = x2.new_empty((m, n)) if x2.dtype is kind else x2.new_empty((m, n), dtype=kind)
         out = out2 if lead is None else out2.view(*lead, n)
     else:
         out2 = out if lead is None else out.view(m, n)
@@ -323,7 +323,8 @@ class KV4Cache:
             raise ValueError(f"dtype must be float32, bfloat16 or float16, not {dtype}")
         if count < 0:
             raise ValueError("count must not be negative")
-        k, v = torch.empty((2, b, count, self.n_heads, self.head_dim), dtype=dtype, device=self.device).unbind(0)
+        k = self.k.new_empty((b, count, self.n_heads, self.head_dim), dtype=dtype)
+        v = torch.empty_like(k)
         if b and count:
             self._call(self._lib.czg_kv4_read, slots.data_ptr(), starts.data_ptr(), b, count, k.data_ptr(), v.data_ptr(), code)
         return k, v
@@ -378,7 +379,7 @@ class KV4Cache:
             raise ValueError("the cache keeps no weights to rank entries by")
         if budget < 1 or not 0 <= recent <= budget:
             raise ValueError("1 <= budget and 0 <= recent <= budget are needed")
-        kept = torch.empty((b, self.n_heads, budget), dtype=_INT32, device=self.device)
+        kept = slots.new_empty((b, self.n_heads, budget))
         new = torch.empty_like(slots)
         if b:
             self._call(self._lib.czg_kv4_evict, slots.data_ptr(), lengths.data_ptr(), b,

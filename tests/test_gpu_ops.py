@@ -48,7 +48,7 @@ def codes_of(x):
 
 @pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
 @pytest.mark.parametrize("m,k", [(1, 1), (1, 16), (3, 17), (5, 384), (2, 4097), (300, 63), (64, 1024), (7, 10007),
-                                 (2401, 40), (2370, 1000), (2368, 4096), (5001, 2049), (3000, 300)])
+                                 (2401, 40), (2370, 1000), (2368, 4096), (5001, 2049), (3000, 300), (2370, 5000)])
 def test_quantize_rows(ops, dtype, m, k):
     g = gen(m * k)
     x = randn(g, m, k + 5).to(dtype)[:, 2:k + 2]   # rows that begin off any boundary
