@@ -187,9 +187,11 @@ __global__ void __launch_bounds__(256) k_kv4_read(czg_kv4 c, const int32_t *__re
 // With x = lo + step c:  s_j = step_j (q.c_j) + lo_j sum(q);  out = sum p_j step_j c_j + sum p_j lo_j.
 // The query is held in fp16 after a power of two that brings its largest value to
 // [2^13, 2^14): exact but for values below 2^-23 of the largest.  p_j step_j is
-// held in fp16 likewise (2^7 to 2^15 for the unit's largest): off by 2^-12 of itself, against
-// 2^-9 of a bf16 result (for an fp16 one in two parts, to 2^-22); its range is 2^31 wide.  Scores, maxima and
-// sums are fp32; exponentials are ex2.approx (2^-22).
+// held in fp16 likewise (2^7 to 2^15 for the unit's largest): off by 2^-11 of itself, against
+// 2^-8 of a bf16 result (for an fp16 one in two parts, to 2^-22); its range is 2^31 wide.  That
+// power of two is the step's alone: the sums of p_j and of p_j lo_j are of plain weights, up to
+// 2^8, so that neither their overflow nor what ex2 takes for 0 (weights below 2^-126) depends
+// on the steps.  Scores, maxima and sums are fp32; exponentials are ex2.approx (2^-22).
 //
 // Measured: one sequence of 131,071 entries, 32 heads on 8, D = 128, bf16 (143 MB): 37 us with
 // the join, 3.8 TB/s; 4096 sequences of up to 512, 6 heads on 1, D = 64 (84 MB): 32.5 us.  The
@@ -298,6 +300,9 @@ __device__ __forceinline__ int64_t row_offset(const AttendArgs &p, const Strides
 
 __device__ __forceinline__ float pow2f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }   // -126 <= e <= 127
 
+// The smallest power of two that steps are taken to be of: 2^(7 - te) stays inside fp32.
+constexpr int kLeastTe = -119;
+
 // CTAs an SM is to hold: what the sums (D NB / 4 registers), query and scores leave room
 // for.  With the weights in two parts (exact) fewer of them spill less (attend of 64
 // sequences of up to 4096, 32 heads on 4, D = 128, with weights: 43.4 us, 45.0 with 8).
@@ -363,7 +368,7 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
     }
     __syncwarp();
 
-    // ranges of the first kChunk entries; 0 behind the end, whatever lies there
+    // ranges of kChunk entries; 0 behind the end, whatever lies there
     uint2 raw[kChunk / THREADS];
     const KvScale *ranges = static_cast<const KvScale *>(p.c.scales) + base + j0;
     auto load_ranges = [&](int from) {
@@ -373,23 +378,29 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
             raw[i] = j < here ? __ldg(reinterpret_cast<const uint2 *>(ranges + j)) : make_uint2(0, 0);
         }
     };
-    // lays them down; returns te: 2^te is not below any of their values' steps (where
-    // 2^-100 is not above all)
-    auto put_ranges = [&]() {
-        uint32_t top = 0;
+    // Lays them down and returns te: 2^te is not below any of their values' steps (nor 2^least;
+    // all 0: 2^least).  A value's step carries the 2^(7 - te) of the fp16 weights, so that the
+    // weights themselves, which the sums of fp32 take, need none.
+    auto put_ranges = [&](int least) {
+        uint32_t top = 0;   // a bf16's bits without its sign order like its magnitude
 #pragma unroll
         for (int i = 0; i < kChunk / THREADS; i++) {
-            const uint32_t step = (raw[i].y & 0xFFFFu) << 16;   // bits of the value's step, never negative
-            if (step < 0x7F800000u) top = max(top, step);
-            sc[tid + i * THREADS] = make_float4(__uint_as_float(raw[i].x << 16), __uint_as_float(raw[i].x & 0xFFFF0000u),
-                                                __uint_as_float(step), __uint_as_float(raw[i].y & 0xFFFF0000u));
+            const uint32_t step = raw[i].y & 0x7FFFu;
+            if (step < 0x7F80u) top = max(top, step);
         }
         top = __reduce_max_sync(0xffffffffu, top);
         if (lane == 0) s_top[warp] = top;
         __syncthreads();
         top = s_top[0];
         for (int w = 1; w < kWarps; w++) top = max(top, s_top[w]);
-        return top == 0 ? -100 : max((int)(top >> 23) - 126, -100);
+        const int te = max(top == 0 ? least : (int)(top >> 7) - 126, least);
+        const float up = pow2f(7 - te);
+#pragma unroll
+        for (int i = 0; i < kChunk / THREADS; i++)
+            sc[tid + i * THREADS] = make_float4(__uint_as_float(raw[i].x << 16), __uint_as_float(raw[i].x & 0xFFFF0000u),
+                                                __uint_as_float(raw[i].y << 16) * up, __uint_as_float(raw[i].y & 0xFFFF0000u));
+        __syncthreads();
+        return te;
     };
     load_ranges(0);
 
@@ -433,9 +444,8 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
             }
         }
     }
-    // weights are taken 2^up-fold, up = 7 - te, which brings weight times step, for weights
-    // up to 2^8, below 2^15
-    int te = put_ranges();   // a barrier: the query is there too
+    // weight times 2^(7 - te) times step is below 2^15 for weights up to 2^8
+    int te = put_ranges(kLeastTe);   // a barrier: the query is there too
 
     const int warps = max(1, min(kWarps, (here + kTile - 1) / kTile));   // that have a tile
     constexpr int LD = D + 4;
@@ -484,7 +494,7 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
         const int lm_row = (lane & 7) + (lane & 8), lm_ch = lane >> 4;
         const uint32_t swz = D == 64 ? (uint32_t)(lm_row >> 2 & 1) : (uint32_t)(lm_row >> 1 & 3);
 
-        float mq[NB][2];   // reference times factor, less `up`
+        float mq[NB][2];   // reference times factor
         auto tile_of = [&](int it, auto cut_of) {
             constexpr bool CUT = decltype(cut_of)::value;   // some row does not see some of the tile's entries
             const int t0 = (it * kWarps + warp) * kTile;   // within the unit
@@ -559,7 +569,7 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
                         const float was = m[nb][i];
                         if (was == -INFINITY || (mt[nb][i] - was) * qs[nb][i] > 8.0f) m[nb][i] = fmaxf(was, mt[nb][i]);
                         const float now = m[nb][i];
-                        mq[nb][i] = now == -INFINITY ? 0.0f : __fmaf_rn(now, qs[nb][i], (float)(te - 7));
+                        mq[nb][i] = now == -INFINITY ? 0.0f : now * qs[nb][i];
                         if (it > 0) {
                             const float f = was == now ? 1.0f : was == -INFINITY ? 0.0f : ex2((was - now) * qs[nb][i]);
                             l[nb][i] *= f;
@@ -642,27 +652,17 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
             load_ranges(j + kChunk);
             __syncthreads();   // all warps are through with the last chunk's ranges
             const int was = te;
-            te = max(te, put_ranges());
-            if (te > was) {    // a larger step: the weights so far, and the next, by a smaller power of two
+            te = put_ranges(was);
+            if (te > was) {    // a larger step: the sums of codes so far by the smaller power of two of the next
                 const float f = pow2f(max(was - te, -126)), f2 = pow2f(min(was - te + 126, 0));   // their product is 2^(was - te)
 #pragma unroll
                 for (int nb = 0; nb < NB; nb++)
 #pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        l[nb][i] = l[nb][i] * f * f2;
-                        z[nb][i] = z[nb][i] * f * f2;
-                        mq[nb][i] = m[nb][i] == -INFINITY ? 0.0f : __fmaf_rn(m[nb][i], qs[nb][i], (float)(te - 7));
+                    for (int ch = 0; ch < CH; ch++)
 #pragma unroll
-                        for (int ch = 0; ch < CH; ch++)
-#pragma unroll
-                            for (int y = 0; y < 2; y++) {
-                                o[nb][ch][y][i] = o[nb][ch][y][i] * f * f2;
-                                o[nb][ch][y][2 + i] = o[nb][ch][y][2 + i] * f * f2;
-                            }
-                    }
+                        for (int i = 0; i < 8; i++) o[nb][ch][i >> 2][i & 3] = o[nb][ch][i >> 2][i & 3] * f * f2;
             }
         }
-        const float down = pow2f(te - 7);
         // sums over the lanes that share a row
 #pragma unroll
         for (int nb = 0; nb < NB; nb++)
@@ -673,8 +673,6 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
                     l[nb][i] += __shfl_xor_sync(0xffffffffu, l[nb][i], x);
                     z[nb][i] += __shfl_xor_sync(0xffffffffu, z[nb][i], x);
                 }
-                l[nb][i] *= down;
-                z[nb][i] *= down;
                 m[nb][i] = m[nb][i] == -INFINITY ? -INFINITY : m[nb][i] * qs[nb][i];
                 if (g8 == 0 && warp < warps) {
                     s_m[warp][nb * 8 + 2 * c4 + i] = m[nb][i];

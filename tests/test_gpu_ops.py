@@ -881,3 +881,51 @@ def test_every_call_gives_the_same_bits_again(ops):
     for _ in range(3):
         c.weights.copy_(w0)
         assert torch.equal(c.attend(q, slots, lengths), y0) and torch.equal(c.weights, w1)
+
+
+# ---- attention over values of any size -----------------------------------------------------------
+#
+# The tolerances are attention()'s: rounding to fp16 is off by 2^-11 of a weight or by 2^-25 of what the
+# row's largest weight times step, or (steps alike) the largest step, was brought to, 2^7 at least: for the
+# 512 entries of a unit 2^-23 of the first and, with steps that differ by 2^6, 2^-16 of the second, both far
+# inside what the formula leaves beside 2^-11 of all the terms.
+
+
+def rising_cache(ops, g, n, heads, d, rise, track=False):
+    """A cache of one slot, and a query for it, whose scores (to base 2) rise from 0 to `rise` along n entries."""
+    c = noise_cache(ops, g, 1, heads, n, d, track)
+    s = torch.linspace(0, rise * math.log(2), n, device=DEV)
+    c.scales[0, :, :, 0] = 0
+    c.scales[0, :, :, 1] = (s / d ** 0.5).to(BF16)
+    return c
+
+
+ones = lambda t, hq, d, dtype: torch.ones(1, t, hq, d, device=DEV, dtype=dtype)
+
+
+@pytest.mark.parametrize("track", [False, True])
+@pytest.mark.parametrize("d,dtype", [(64, BF16), (64, FP16), (128, BF16), (128, FP16)])
+@pytest.mark.parametrize("n", [1, 77, 512, 1024, 70000])
+def test_attend_constant_values(ops, n, d, dtype, track):
+    """Value rows whose dimensions are all equal have a step of 0: their mean, whatever they are."""
+    r = gen(n + d)
+    big = torch.finfo(dtype).max if dtype == FP16 else 1e30
+    for rise in (0.0, 7.9, 40.0, -40.0):
+        c = rising_cache(ops, r, n, 1, d, rise, track)
+        sign = torch.where(torch.rand(n, generator=r, device=DEV) < 0.5, -1.0, 1.0)
+        for value in (8192.0, -65504.0, big, 100.0, 64.0 * sign, 8192 * sign, 60000 * sign, big * sign, 2.0 ** -30 * sign):
+            c.scales[0, :, :, 2] = 0
+            c.scales[0, 0, :, 3] = value.to(BF16) if torch.is_tensor(value) else value
+            if dtype == FP16:      # bf16 rounds 65504 up, past what fp16 holds
+                c.scales[0, 0, :, 3] = c.scales[0, 0, :, 3].clamp(-65280, 65280)
+            check_attend(ops, c, ones(1, 2, d, dtype), int32(0), int32(n))
+    c.check()
+
+
+@pytest.mark.parametrize("d,power", [(64, 100), (128, 108), (64, -100), (128, -116)])
+def test_attend_values_of_any_size(ops, d, power):
+    """Weights from 1 to 2^-30 of the largest count alike whatever the values' exponent."""
+    r = gen(power + 200 + d)
+    c = rising_cache(ops, r, 900, 2, d, 30.0)
+    c.scales[0, :, :, 2:] = (c.scales[0, :, :, 2:].double() * 2.0 ** power).to(BF16)
+    check_attend(ops, c, ones(1, 4, d, BF16), int32(0), int32(900))
