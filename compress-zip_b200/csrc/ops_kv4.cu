@@ -224,7 +224,8 @@ struct AttendArgs {
     Strides os;
     // not whole, that is more than one unit (or row block with weights): partial results to join
     float *part;        // [b][head][unit][rows padded][D]
-    float4 *stat;       // [b][head][unit][rows padded] (maximum, sum, what a score is multiplied by)
+    float4 *stat;       // [b][head][unit][rows padded] (maximum, sum, what a score is multiplied by); the
+                        // sum is negative where the partial result is taken kHuge-fold
     float *score;       // weights: [b][head][rows][max_len]
 };
 
@@ -239,10 +240,10 @@ __device__ __forceinline__ void add_scaled(float4 &x, float f, float4 v) {
     x.z = __fmaf_rn(f, v.z, x.z);
     x.w = __fmaf_rn(f, v.w, x.w);
 }
-// Four dimensions of a result: x f.
+// Four dimensions of a result: x f up.
 template <typename T>
-__device__ __forceinline__ void store4(T *dst, float4 x, float f, bool vec) {
-    __align__(8) T y[4] = {from_f32<T>(x.x * f), from_f32<T>(x.y * f), from_f32<T>(x.z * f), from_f32<T>(x.w * f)};
+__device__ __forceinline__ void store4(T *dst, float4 x, float f, float up, bool vec) {
+    __align__(8) T y[4] = {from_f32<T>(x.x * f * up), from_f32<T>(x.y * f * up), from_f32<T>(x.z * f * up), from_f32<T>(x.w * f * up)};
     if (vec) {
         *reinterpret_cast<uint2 *>(dst) = *reinterpret_cast<const uint2 *>(y);
     } else {
@@ -302,6 +303,11 @@ __device__ __forceinline__ float pow2f(int e) { return __uint_as_float((uint32_t
 
 // The smallest power of two that steps are taken to be of: 2^(7 - te) stays inside fp32.
 constexpr int kLeastTe = -119;
+// Sums of weights (below 2^8) times values below 2^87 stay inside fp32 for 2^31 entries.  Where a
+// value of a unit is larger, its values are taken kHuge-fold: below 2^80.
+constexpr float kHuge = 3.5527136788005009e-15f;   // 2^-48
+constexpr int kHugeTe = 83;                        // 15 steps of 2^te and more may pass 2^87
+constexpr uint32_t kHugeLo = (87 + 127) << 7;      // bits of 2^87
 
 // CTAs an SM is to hold: what the sums (D NB / 4 registers), query and scores leave room
 // for.  With the weights in two parts (exact) fewer of them spill less (attend of 64
@@ -378,29 +384,40 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
             raw[i] = j < here ? __ldg(reinterpret_cast<const uint2 *>(ranges + j)) : make_uint2(0, 0);
         }
     };
-    // Lays them down and returns te: 2^te is not below any of their values' steps (nor 2^least;
-    // all 0: 2^least).  A value's step carries the 2^(7 - te) of the fp16 weights, so that the
-    // weights themselves, which the sums of fp32 take, need none.
-    auto put_ranges = [&](int least) {
-        uint32_t top = 0;   // a bf16's bits without its sign order like its magnitude
+    // Lays them down.  2^te is from then on not below any of their values' steps, and huge says
+    // whether some value passes 2^87; neither falls along a unit.  A value's step carries the
+    // 2^(7 - te) of the fp16 weights, so that the weights themselves, which the sums of fp32
+    // take, need none.
+    int te = kLeastTe;
+    bool huge = false;
+    auto put_ranges = [&]() {
+        uint32_t most = 0;   // of the steps and, in the high half, of the lower ends: a bf16's bits without its sign order like its magnitude
 #pragma unroll
-        for (int i = 0; i < kChunk / THREADS; i++) {
-            const uint32_t step = raw[i].y & 0x7FFFu;
-            if (step < 0x7F80u) top = max(top, step);
+        for (int i = 0; i < kChunk / THREADS; i++) most = __vmaxu2(most, raw[i].y & 0x7FFF7FFFu);
+        if (__any_sync(0xffffffffu, (most & 0xFFFFu) >= 0x7F80u || most >= 0x7F800000u)) {   // what is not finite does not count
+            most = 0;
+#pragma unroll
+            for (int i = 0; i < kChunk / THREADS; i++) {
+                const uint32_t step = raw[i].y & 0x7FFFu, lo = raw[i].y & 0x7FFF0000u;
+                most = __vmaxu2(most, (step < 0x7F80u ? step : 0u) | (lo < 0x7F800000u ? lo : 0u));
+            }
         }
-        top = __reduce_max_sync(0xffffffffu, top);
-        if (lane == 0) s_top[warp] = top;
+        uint32_t top = __reduce_max_sync(0xffffffffu, most & 0xFFFFu);
+        const bool far = __any_sync(0xffffffffu, most >> 16 >= kHugeLo);
+        if (lane == 0) s_top[warp] = top | (uint32_t)far << 16;
         __syncthreads();
-        top = s_top[0];
-        for (int w = 1; w < kWarps; w++) top = max(top, s_top[w]);
-        const int te = max(top == 0 ? least : (int)(top >> 7) - 126, least);
-        const float up = pow2f(7 - te);
+        for (int w = 0; w < kWarps; w++) {
+            top = max(top, s_top[w] & 0xFFFFu);
+            huge |= s_top[w] >> 16;
+        }
+        if (top) te = max(te, (int)(top >> 7) - 126);
+        huge |= te > kHugeTe;
+        const float up = pow2f(7 - te), down = huge ? kHuge : 1.0f;
 #pragma unroll
         for (int i = 0; i < kChunk / THREADS; i++)
             sc[tid + i * THREADS] = make_float4(__uint_as_float(raw[i].x << 16), __uint_as_float(raw[i].x & 0xFFFF0000u),
-                                                __uint_as_float(raw[i].y << 16) * up, __uint_as_float(raw[i].y & 0xFFFF0000u));
+                                                __uint_as_float(raw[i].y << 16) * up, __uint_as_float(raw[i].y & 0xFFFF0000u) * down);
         __syncthreads();
-        return te;
     };
     load_ranges(0);
 
@@ -445,7 +462,7 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
         }
     }
     // weight times 2^(7 - te) times step is below 2^15 for weights up to 2^8
-    int te = put_ranges(kLeastTe);   // a barrier: the query is there too
+    put_ranges();   // a barrier: the query is there too
 
     const int warps = max(1, min(kWarps, (here + kTile - 1) / kTile));   // that have a tile
     constexpr int LD = D + 4;
@@ -652,7 +669,14 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
             load_ranges(j + kChunk);
             __syncthreads();   // all warps are through with the last chunk's ranges
             const int was = te;
-            te = put_ranges(was);
+            const bool was_huge = huge;
+            put_ranges();
+            if (huge && !was_huge) {
+#pragma unroll
+                for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                    for (int i = 0; i < 2; i++) z[nb][i] *= kHuge;
+            }
             if (te > was) {    // a larger step: the sums of codes so far by the smaller power of two of the next
                 const float f = pow2f(max(was - te, -126)), f2 = pow2f(min(was - te + 126, 0));   // their product is 2^(was - te)
 #pragma unroll
@@ -689,7 +713,7 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
         s_row[tid] = make_float2(top_m, sum);
     }
     if (warp < warps) {
-        const float down = pow2f(te - 7);
+        const float down = pow2f(te - 7), up24 = huge ? 16777216.0f * kHuge : 16777216.0f;
 #pragma unroll
         for (int nb = 0; nb < NB; nb++)
 #pragma unroll
@@ -703,8 +727,8 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
 #pragma unroll
                     for (int y = 0; y < 2; y++)   // dimensions 32 ch + 4 g8 + 2 y and the next
                         *reinterpret_cast<float2 *>(&so[(warp * R + r) * LD + ch * 32 + 4 * g8 + 2 * y]) =
-                            make_float2(__fmaf_rn(o[nb][ch][y][i] * 16777216.0f, even, zz),
-                                        __fmaf_rn((o[nb][ch][y][2 + i] - o[nb][ch][y][i]) * 16777216.0f, odd, zz));
+                            make_float2(__fmaf_rn(o[nb][ch][y][i] * up24, even, zz),
+                                        __fmaf_rn((o[nb][ch][y][2 + i] - o[nb][ch][y][i]) * up24, odd, zz));
             }
     }
     __syncthreads();
@@ -722,10 +746,10 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
             x.w += v.w;
         }
         if (whole) {
-            store4(static_cast<T *>(p.out) + s_out[r] + d, x, row.y == 0.0f ? 0.0f : 1.0f / row.y, p.out_vec);   // a row that sees nothing: 0
+            store4(static_cast<T *>(p.out) + s_out[r] + d, x, row.y == 0.0f ? 0.0f : 1.0f / row.y, huge ? 1.0f / kHuge : 1.0f, p.out_vec);   // a row that sees nothing: 0
         } else {
             *reinterpret_cast<float4 *>(p.part + (at + r) * D + d) = x;
-            if (d == 0) p.stat[at + r] = make_float4(row.x, row.y, s_qs[r].x, 0.0f);
+            if (d == 0) p.stat[at + r] = make_float4(row.x, huge ? -row.y : row.y, s_qs[r].x, 0.0f);
         }
     }
     if (TRACK && whole)   // the scores that this CTA wrote
@@ -764,12 +788,16 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv4_join(const __grid_constant
             if (r >= p.rows) return;
             float4 st[kFew];
             float m = -INFINITY, l = 0.0f;
+            bool huge = false;   // some partial result is taken kHuge-fold: all are
             float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             const int64_t at = first + r;
 #pragma unroll
             for (int u = 0; u < kFew; u++) st[u] = u < units ? p.stat[at + (int64_t)u * rows_padded] : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-            for (int u = 0; u < kFew; u++) m = fmaxf(m, st[u].x);
+            for (int u = 0; u < kFew; u++) {
+                m = fmaxf(m, st[u].x);
+                huge |= signbit(st[u].y);
+            }
 #pragma unroll
             for (int u0 = 0; u0 < kFew; u0 += 4) {
                 float4 v[4];
@@ -780,21 +808,26 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv4_join(const __grid_constant
                 for (int u = 0; u < 4; u++)
                     if (u0 + u < units) {
                         const float f = share(st[u0 + u].x, m);
-                        add_scaled(x, f, v[u]);
-                        l = __fmaf_rn(f, st[u0 + u].y, l);
+                        add_scaled(x, huge && !signbit(st[u0 + u].y) ? f * kHuge : f, v[u]);
+                        l = __fmaf_rn(f, fabsf(st[u0 + u].y), l);
                     }
             }
-            store4(static_cast<T *>(p.out) + row_offset(p, p.os, b, h, r) + d, x, l == 0.0f ? 0.0f : 1.0f / l, p.out_vec);
+            store4(static_cast<T *>(p.out) + row_offset(p, p.os, b, h, r) + d, x, l == 0.0f ? 0.0f : 1.0f / l, huge ? 1.0f / kHuge : 1.0f, p.out_vec);
             return;
         }
         __shared__ float s_f[kMany], red[kJoinThreads / 32];
         __shared__ float4 runs[RUNS][TR];
         const int r = blockIdx.x;
         float m = -INFINITY;
-        for (int u = tid; u < units; u += kJoinThreads) m = fmaxf(m, p.stat[first + (int64_t)u * rows_padded + r].x);
+        bool huge = false;   // as above
+        for (int u = tid; u < units; u += kJoinThreads) {
+            const float4 st = p.stat[first + (int64_t)u * rows_padded + r];
+            m = fmaxf(m, st.x);
+            huge |= signbit(st.y);
+        }
         for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
         if ((tid & 31) == 0) red[tid >> 5] = m;
-        __syncthreads();
+        huge = __syncthreads_or(huge);
         for (int w = 0; w < kJoinThreads / 32; w++) m = fmaxf(m, red[w]);
         float l = 0.0f;
         float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -803,8 +836,9 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv4_join(const __grid_constant
             __syncthreads();
             for (int u = tid; u < some; u += kJoinThreads) {
                 const float4 st = p.stat[first + (int64_t)(u0 + u) * rows_padded + r];
-                s_f[u] = share(st.x, m);
-                l = __fmaf_rn(s_f[u], st.y, l);
+                const float f = share(st.x, m);
+                l = __fmaf_rn(f, fabsf(st.y), l);
+                s_f[u] = huge && !signbit(st.y) ? f * kHuge : f;
             }
             __syncthreads();
 #pragma unroll 16
@@ -820,7 +854,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv4_join(const __grid_constant
         l = 0.0f;
         for (int w = 0; w < kJoinThreads / 32; w++) l += red[w];
         for (int i = 1; i < RUNS; i++) add_scaled(x, 1.0f, runs[i][tid]);
-        store4(static_cast<T *>(p.out) + row_offset(p, p.os, b, h, r) + d, x, l == 0.0f ? 0.0f : 1.0f / l, p.out_vec);
+        store4(static_cast<T *>(p.out) + row_offset(p, p.os, b, h, r) + d, x, l == 0.0f ? 0.0f : 1.0f / l, huge ? 1.0f / kHuge : 1.0f, p.out_vec);
         return;
     }
     // weights of kChunk entries, a thread two of them, 8 rows at a time: their scores are
@@ -848,10 +882,10 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv4_join(const __grid_constant
             float m = st.x;
             for (int u = u0 + 32; u < units; u += 32) m = fmaxf(m, p.stat[first + (int64_t)u * rows_padded + mine].x);
             for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-            float l = st.y * share(st.x, m);
+            float l = fabsf(st.y) * share(st.x, m);
             for (int u = u0 + 32; u < units; u += 32) {
                 const float4 more = p.stat[first + (int64_t)u * rows_padded + mine];
-                l += more.y * share(more.x, m);
+                l += fabsf(more.y) * share(more.x, m);
             }
             for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
             st = make_float4(m, l == 0.0f ? 0.0f : 1.0f / l, st.z, 0.0f);

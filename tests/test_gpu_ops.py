@@ -929,3 +929,28 @@ def test_attend_values_of_any_size(ops, d, power):
     c = rising_cache(ops, r, 900, 2, d, 30.0)
     c.scales[0, :, :, 2:] = (c.scales[0, :, :, 2:].double() * 2.0 ** power).to(BF16)
     check_attend(ops, c, ones(1, 4, d, BF16), int32(0), int32(900))
+
+
+@pytest.mark.parametrize("d,g,t", [(64, 2, 1), (128, 3, 4)])
+def test_attend_largest_values(ops, d, g, t):
+    """Values up to the end of bf16: sums of many of them stay inside fp32."""
+    r = gen(d)
+    top = torch.finfo(BF16).max
+    for n in (1, 512, 3000, 70000):
+        for rise in (0.0, 7.9, 60.0):
+            c = rising_cache(ops, r, n, 1, d, rise)
+            q = ones(t, g, d, BF16)
+            c.scales[0, :, :, 2] = 0
+            c.scales[0, :, :, 3] = top
+            y = c.attend(q, int32(0), int32(n))
+            seen = torch.arange(t, device=DEV) >= t - n
+            assert not y[0, ~seen].any()
+            assert ((y[0, seen].double() - top).abs() <= 2 * u(BF16) * top).all()
+            c.scales[0, :, ::2, 3] = -top / 4
+            c.scales[0, :, 1::2, 3] = top / 8
+            check_attend(ops, c, q, int32(0), int32(n))
+            c.scales[0, :, 1::2, 2] = 2.0 ** 119          # steps too
+            c.scales[0, :, 1::2, 3] = -(2.0 ** 122)
+            check_attend(ops, c, q, int32(0), int32(n))
+            c.scales[0, :, ::2, 2:] = 1.0
+            check_attend(ops, c, q, int32(0), int32(n))
