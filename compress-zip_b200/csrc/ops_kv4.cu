@@ -187,8 +187,12 @@ __global__ void __launch_bounds__(256) k_kv4_read(czg_kv4 c, const int32_t *__re
 // With x = lo + step c:  s_j = step_j (q.c_j) + lo_j sum(q);  out = sum p_j step_j c_j + sum p_j lo_j.
 // The query is held in fp16 after a power of two that brings its largest value to
 // [2^13, 2^14): exact but for values below 2^-23 of the largest.  p_j step_j is
-// held in fp16 likewise (2^7 to 2^15 for the unit's largest): off by 2^-11 of itself, against
-// 2^-8 of a bf16 result (for an fp16 one in two parts, to 2^-22); its range is 2^31 wide.  That
+// held in fp16 likewise: off by 2^-11 of itself, against 2^-8 of a bf16 result (for an fp16 one
+// in two parts, to 2^-22), and by no less than 2^-25.  Where the steps of a unit are alike, all
+// are brought to one power of two, 2^7 to 2^15 for the largest step at the largest p_j; where
+// some entry's step and lower end are both below 2^-6 of the largest step, an entry far below
+// (or one that a row does not see at all) could push those that count out of fp16's range,
+// and each row has a power of two of its own, which follows its largest p_j step_j.  Either
 // power of two is the step's alone: the sums of p_j and of p_j lo_j are of plain weights, up to
 // 2^8, so that neither their overflow nor what ex2 takes for 0 (weights below 2^-126) depends
 // on the steps.  Scores, maxima and sums are fp32; exponentials are ex2.approx (2^-22).
@@ -303,6 +307,9 @@ __device__ __forceinline__ float pow2f(int e) { return __uint_as_float((uint32_t
 
 // The smallest power of two that steps are taken to be of: 2^(7 - te) stays inside fp32.
 constexpr int kLeastTe = -119;
+// A unit whose least entry (its step, or a sixteenth of its lower end) is below the largest step
+// by more than this power of two keeps a scale for each row.
+constexpr int kAlike = 6;
 // Sums of weights (below 2^8) times values below 2^87 stay inside fp32 for 2^31 entries.  Where a
 // value of a unit is larger, its values are taken kHuge-fold: below 2^80.
 constexpr float kHuge = 3.5527136788005009e-15f;   // 2^-48
@@ -337,7 +344,8 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
     __shared__ uint4 s_q[NB * CH * 32];      // the query as B fragments: [nb][chunk][lane]
     __shared__ float2 s_qs[R];               // a row's factors
     __shared__ float s_m[kWarps][R], s_l[kWarps][R];
-    __shared__ uint32_t s_top[kWarps];
+    __shared__ uint2 s_top[kWarps];          // bits of a block's largest step, and of the unit's least entry
+    __shared__ float2 s_scale[kWarps][R];    // spread: the row's largest weight times step so far, and its power of two
     __shared__ float2 s_row[R];              // maximum and sum over the warps
     __shared__ int64_t s_out[R];             // where the row's output begins
 
@@ -369,6 +377,7 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
     if (lane == 0) {
 #pragma unroll
         for (int i = 0; i < kRing; i++) mbar_init(&ring_bar[i], 1);
+        s_top[warp].y = 0x7FFFu;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         for (int i = 0; i < min(kRing, turns); i++) ask(i);
     }
@@ -384,16 +393,20 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
             raw[i] = j < here ? __ldg(reinterpret_cast<const uint2 *>(ranges + j)) : make_uint2(0, 0);
         }
     };
-    // Lays them down.  2^te is from then on not below any of their values' steps, and huge says
-    // whether some value passes 2^87; neither falls along a unit.  A value's step carries the
-    // 2^(7 - te) of the fp16 weights, so that the weights themselves, which the sums of fp32
-    // take, need none.
+    // Lays them down.  2^te is from then on not below any of their values' steps, huge says
+    // whether some value passes 2^87, and spread whether the entries are not alike; none of
+    // them falls along a unit.  A value's step carries the 2^(7 - te) of the fp16 weights
+    // (spread: none, the rows' scales do), so that the weights themselves, which the sums of
+    // fp32 take, need none.
     int te = kLeastTe;
-    bool huge = false;
-    auto put_ranges = [&]() {
-        uint32_t most = 0;   // of the steps and, in the high half, of the lower ends: a bf16's bits without its sign order like its magnitude
+    bool huge = false, spread = false;
+    auto put_ranges = [&](int from) {
+        uint32_t most = 0, low = 0x7FFF7FFFu;   // of the steps and, in the high half, of the lower ends: a bf16's bits without its sign order like its magnitude
 #pragma unroll
-        for (int i = 0; i < kChunk / THREADS; i++) most = __vmaxu2(most, raw[i].y & 0x7FFF7FFFu);
+        for (int i = 0; i < kChunk / THREADS; i++) {
+            most = __vmaxu2(most, raw[i].y & 0x7FFF7FFFu);
+            if (from + tid + i * THREADS < here) low = __vminu2(low, raw[i].y & 0x7FFF7FFFu);
+        }
         if (__any_sync(0xffffffffu, (most & 0xFFFFu) >= 0x7F80u || most >= 0x7F800000u)) {   // what is not finite does not count
             most = 0;
 #pragma unroll
@@ -404,15 +417,18 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
         }
         uint32_t top = __reduce_max_sync(0xffffffffu, most & 0xFFFFu);
         const bool far = __any_sync(0xffffffffu, most >> 16 >= kHugeLo);
-        if (lane == 0) s_top[warp] = top | (uint32_t)far << 16;
+        uint32_t least = __reduce_min_sync(0xffffffffu, max(low & 0xFFFFu, (low >> 16) - min(low >> 16, 4u << 7)));
+        if (lane == 0) s_top[warp] = make_uint2(top | (uint32_t)far << 16, min(least, s_top[warp].y));
         __syncthreads();
         for (int w = 0; w < kWarps; w++) {
-            top = max(top, s_top[w] & 0xFFFFu);
-            huge |= s_top[w] >> 16;
+            top = max(top, s_top[w].x & 0xFFFFu);
+            least = min(least, s_top[w].y);
+            huge |= s_top[w].x >> 16;
         }
         if (top) te = max(te, (int)(top >> 7) - 126);
         huge |= te > kHugeTe;
-        const float up = pow2f(7 - te), down = huge ? kHuge : 1.0f;
+        spread |= te > kLeastTe && te + 126 - (int)(least >> 7) > kAlike;
+        const float down = huge ? kHuge : 1.0f, up = spread ? down : pow2f(7 - te);
 #pragma unroll
         for (int i = 0; i < kChunk / THREADS; i++)
             sc[tid + i * THREADS] = make_float4(__uint_as_float(raw[i].x << 16), __uint_as_float(raw[i].x & 0xFFFF0000u),
@@ -462,7 +478,9 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
         }
     }
     // weight times 2^(7 - te) times step is below 2^15 for weights up to 2^8
-    put_ranges();   // a barrier: the query is there too
+    put_ranges(0);   // a barrier: the query is there too
+    if (spread && lane < R) s_scale[warp][lane] = make_float2(0.0f, __int_as_float(0));
+    __syncwarp();
 
     const int warps = max(1, min(kWarps, (here + kTile - 1) / kTile));   // that have a tile
     constexpr int LD = D + 4;
@@ -513,7 +531,7 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
 
         float mq[NB][2];   // reference times factor
         auto tile_of = [&](int it, auto cut_of) {
-            constexpr bool CUT = decltype(cut_of)::value;   // some row does not see some of the tile's entries
+            constexpr bool CUT = decltype(cut_of)::value;   // some row does not see some of the tile's entries, or spread
             const int t0 = (it * kWarps + warp) * kTile;   // within the unit
             const float4 *range = sc + t0 % kChunk + g8;
             const uint32_t ka = smem_addr(ring + (it % kRing) * 2 * L::kTileCodes) + (uint32_t)lm_row * (D / 2), va = ka + L::kTileCodes;
@@ -591,6 +609,7 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
                             const float f = was == now ? 1.0f : was == -INFINITY ? 0.0f : ex2((was - now) * qs[nb][i]);
                             l[nb][i] *= f;
                             z[nb][i] *= f;
+                            if (CUT && spread && g8 == 0) s_scale[warp][nb * 8 + 2 * c4 + i].x *= f;
 #pragma unroll
                             for (int ch = 0; ch < CH; ch++)
 #pragma unroll
@@ -604,29 +623,69 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
 #pragma unroll
             for (int kb = 0; kb < KB; kb++) {
                 uint32_t pf[NB][2], pl[NB][2];
+                float w[2][NB][2];
+                auto pack = [&](int hf, int nb) {
+                    const uint32_t wp = pack_half(w[hf][nb][0], w[hf][nb][1]);
+                    if (kExact) {
+                        const float2 back = __half22float2(*reinterpret_cast<const __half2 *>(&wp));
+                        pl[nb][hf] = transpose8(pack_half(w[hf][nb][0] - back.x, w[hf][nb][1] - back.y));
+                    }
+                    pf[nb][hf] = transpose8(wp);
+                };
 #pragma unroll
                 for (int hf = 0; hf < 2; hf++) {
                     const int j = t0 + kb * 16 + hf * 8 + g8;
                     const float2 vr = *reinterpret_cast<const float2 *>(&range[kb * 16 + hf * 8].z);
 #pragma unroll
                     for (int nb = 0; nb < NB; nb++) {
-                        float w[2];
 #pragma unroll
                         for (int i = 0; i < 2; i++) {
                             const bool off = CUT && j >= seen[nb][i];   // what is not seen may be anything
                             const float y = off ? 0.0f : ex2(__fmaf_rn(s[nb][kb][2 * hf + i], qs[nb][i], -mq[nb][i]));
                             l[nb][i] += y;
                             z[nb][i] = off ? z[nb][i] : __fmaf_rn(y, vr.y, z[nb][i]);
-                            w[i] = off ? 0.0f : y * vr.x;
+                            w[hf][nb][i] = off ? 0.0f : y * vr.x;
                         }
-                        const uint32_t wp = pack_half(w[0], w[1]);
-                        if (kExact) {
-                            const float2 back = __half22float2(*reinterpret_cast<const __half2 *>(&wp));
-                            pl[nb][hf] = transpose8(pack_half(w[0] - back.x, w[1] - back.y));
-                        }
-                        pf[nb][hf] = transpose8(wp);
+                        if (!CUT) pack(hf, nb);
                     }
                 }
+                if (CUT && spread) {   // keeps the row's largest weight times step between 2^8 and 2^15
+                    __syncwarp();
+#pragma unroll
+                    for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                        for (int i = 0; i < 2; i++) {
+                            const float2 sc = s_scale[warp][nb * 8 + 2 * c4 + i];
+                            float most = fmaxf(fabsf(w[0][nb][i]), fabsf(w[1][nb][i]));
+#pragma unroll
+                            for (int x = 4; x < 32; x <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, x));
+                            most = fmaxf(most, sc.x);
+                            int k = __float_as_int(sc.y);
+                            const int e = (int)(__float_as_uint(most) >> 23) - 127;
+                            if (e + k < 8 || e + k >= 15 || abs(k) > 126) {
+                                const int was = k;
+                                k = min(max(13 - e, -126), 126);
+                                const int by = min(max(k - was, -252), 252), half = by / 2;
+                                const float f = pow2f(half), f2 = pow2f(by - half);
+#pragma unroll
+                                for (int ch = 0; ch < CH; ch++)
+#pragma unroll
+                                    for (int y = 0; y < 2; y++) {
+                                        o[nb][ch][y][i] = o[nb][ch][y][i] * f * f2;
+                                        o[nb][ch][y][2 + i] = o[nb][ch][y][2 + i] * f * f2;
+                                    }
+                            }
+                            w[0][nb][i] *= pow2f(k);
+                            w[1][nb][i] *= pow2f(k);
+                            __syncwarp();   // all lanes have read it
+                            if (g8 == 0) s_scale[warp][nb * 8 + 2 * c4 + i] = make_float2(most, __int_as_float(k));
+                        }
+                }
+                if (CUT)
+#pragma unroll
+                    for (int hf = 0; hf < 2; hf++)
+#pragma unroll
+                        for (int nb = 0; nb < NB; nb++) pack(hf, nb);
 #pragma unroll
                 for (int cp = 0; cp < CH; cp += 2) {
                     uint32_t w[4];
@@ -661,7 +720,7 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
                     mbar_wait(&ring_bar[it % kRing], (it / kRing) & 1, nullptr);   // once more for the copies, before anything ends
                 }
                 __syncwarp();
-                if ((it * kWarps + warp + 1) * kTile > least) tile_of(it, std::true_type{}); else tile_of(it, std::false_type{});
+                if (spread || (it * kWarps + warp + 1) * kTile > least) tile_of(it, std::true_type{}); else tile_of(it, std::false_type{});
                 __syncwarp();   // all lanes have read the tile
                 if (lane == 0 && it + kRing < turns) ask(it + kRing);
             }
@@ -669,15 +728,24 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
             load_ranges(j + kChunk);
             __syncthreads();   // all warps are through with the last chunk's ranges
             const int was = te;
-            const bool was_huge = huge;
-            put_ranges();
+            const bool was_huge = huge, was_spread = spread;
+            put_ranges(j + kChunk);
             if (huge && !was_huge) {
 #pragma unroll
                 for (int nb = 0; nb < NB; nb++)
 #pragma unroll
                     for (int i = 0; i < 2; i++) z[nb][i] *= kHuge;
             }
-            if (te > was) {    // a larger step: the sums of codes so far by the smaller power of two of the next
+            if (spread) {
+                __syncwarp();
+                if (lane < R) {   // the sums of codes so far have the unit's scale, or lose that of the values
+                    float2 sc = s_scale[warp][lane];
+                    if (!was_spread) sc = make_float2(pow2f(min(was + 7, 126)) * (huge ? kHuge : 1.0f), __int_as_float(7 - was + (huge ? 48 : 0)));
+                    else if (huge && !was_huge) sc = make_float2(sc.x * kHuge, __int_as_float(__float_as_int(sc.y) + 48));
+                    s_scale[warp][lane] = sc;
+                }
+                __syncwarp();
+            } else if (te > was) {    // a larger step: the sums of codes so far by the smaller power of two of the next
                 const float f = pow2f(max(was - te, -126)), f2 = pow2f(min(was - te + 126, 0));   // their product is 2^(was - te)
 #pragma unroll
                 for (int nb = 0; nb < NB; nb++)
@@ -713,7 +781,7 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
         s_row[tid] = make_float2(top_m, sum);
     }
     if (warp < warps) {
-        const float down = pow2f(te - 7), up24 = huge ? 16777216.0f * kHuge : 16777216.0f;
+        float down = pow2f(te - 7), up24 = huge ? 16777216.0f * kHuge : 16777216.0f;
 #pragma unroll
         for (int nb = 0; nb < NB; nb++)
 #pragma unroll
@@ -721,6 +789,11 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
                 const int r = nb * 8 + 2 * c4 + i;
                 float top_m = s_m[0][r];
                 for (int w = 1; w < warps; w++) top_m = fmaxf(top_m, s_m[w][r]);
+                if (spread) {
+                    const int k = __float_as_int(s_scale[warp][r].y);
+                    down = pow2f(max(-k, -126)) * pow2f(min(126 - k, 0));
+                    up24 = 16777216.0f;
+                }
                 const float f = share(m[nb][i], top_m), zz = z[nb][i] * f, even = down * f, odd = even * 0.0625f;
 #pragma unroll
                 for (int ch = 0; ch < CH; ch++)

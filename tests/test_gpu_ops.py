@@ -954,3 +954,78 @@ def test_attend_largest_values(ops, d, g, t):
             check_attend(ops, c, q, int32(0), int32(n))
             c.scales[0, :, ::2, 2:] = 1.0
             check_attend(ops, c, q, int32(0), int32(n))
+
+
+@pytest.mark.parametrize("d,power,far", [(64, 0, -50), (64, 100, -40), (128, 118, -30), (64, -100, -10), (128, -118, -4)])
+def test_attend_small_weights_of_large_values(ops, d, power, far):
+    """Entries of weights 2^far whose values are 2^-2 far times those of the heavy ones, at values' sizes
+    from one end of bf16 to the other: what a weight is held to does not depend on them."""
+    r = gen(power + 200 + d)
+    c = rising_cache(ops, r, 900, 2, d, 0.0)
+    c.scales[0, :, 500:, 1] = -far * math.log(2) / d ** 0.5
+    c.scales[0, :, :, 2:] = (c.scales[0, :, :, 2:].double() * 2.0 ** power).to(BF16)
+    if power >= 0:
+        c.scales[0, :, 500:, 2:] = (c.scales[0, :, 500:, 2:].double() * 2.0 ** (2 * far)).to(BF16)
+    check_attend(ops, c, ones(1, 4, d, BF16), int32(0), int32(900))
+
+
+@pytest.mark.parametrize("dtype,ratio", [(t, p) for t in (BF16, FP16) for p in (6, 7, 12, 26, 60)] + [(BF16, 100)])
+def test_attend_small_step_beside_large_ones(ops, ratio, dtype):
+    """A row's result is as exact beside entries of far larger steps as without them: ones that it does
+    not see, and ones whose scores are far below."""
+    r = gen(ratio)
+    # in one block of ranges, in two of one unit (either order), in two units
+    for d, n, heavy, other in ((64, 40, 3, 1), (128, 700, 650, 600), (64, 70000, 700, 350), (64, 70000, 300, 800),
+                               (128, 66000, 65998, 32000)):
+        # one key far above the others (2^46 and more), whose values have small steps around 0
+        c = noise_cache(ops, r, 1, 1, n, d, False)
+        c.scales[0, 0, :, 0] = 0
+        c.scales[0, 0, :, 1] = 0
+        c.scales[0, 0, heavy, 1] = 1.0
+        c.scales[0, 0, heavy, 2:] = (c.scales[0, 0, heavy, 2:].double() * 2.0 ** (-6 if dtype == FP16 else -30)).to(BF16)
+        q = ones(2, 2, d, dtype) * 4
+        before = c.scales[0, 0, other].clone()
+        c.scales[0, 0, other, 2:] = (c.scales[0, 0, heavy, 2:].double() * 2.0 ** ratio).to(BF16)
+        check_attend(ops, c, q, int32(0), int32(n))
+        c.scales[0, 0, other] = before
+        c.scales[0, 0, n - 1, 2:] = (c.scales[0, 0, heavy, 2:].double() * 2.0 ** ratio).to(BF16)   # the first row does not see it
+        check_attend(ops, c, q, int32(0), int32(n))
+    c.check()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_attend_beside_rows_of_zeros(ops, dtype):
+    """An entry with nearly all the weight whose value is 0: what the others add is all there is."""
+    r = gen(77)
+    for d, n in ((64, 33), (128, 600), (64, 70000)):
+        for above in (10, 20, 28, 45):
+            if dtype == FP16 and above > 10:
+                continue                          # the result itself leaves fp16's range
+            c = noise_cache(ops, r, 1, 2, n, d, True)
+            c.scales[0, :, :, 0] = 0
+            c.scales[0, :, :, 1] = 0
+            c.scales[0, :, 2, 1] = above * math.log(2) / d ** 0.5 + math.log(n) / d ** 0.5
+            c.scales[0, :, 2, 2:] = 0
+            check_attend(ops, c, ones(1, 4, d, dtype), int32(0), int32(n))
+
+
+@pytest.mark.parametrize("g,t", [(8, 1), (2, 9)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_attend_ranges_of_any_exponent(ops, d, g, t):
+    """Every entry's values of a size of their own, from 2^-80 to 2^80, and scores up to 2^60 apart."""
+    r = gen(d + g)
+    for n in (20, 500, 1300, 70000):
+        c = noise_cache(ops, r, 1, 1, n, d, True)
+        power = torch.randint(-80, 81, (n, 1), generator=r, device=DEV).double()
+        c.scales[0, 0, :, 2:] = (c.scales[0, 0, :, 2:].double() * 2.0 ** power).to(BF16)
+        c.scales[0, 0, torch.rand(n, generator=r, device=DEV) < 0.1, 2] = 0
+        for q in (0.3, 4.0):
+            check_attend(ops, c, (q * randn(r, 1, t, g, d)).to(BF16), int32(0), int32(n))
+        # and as large as it goes where the weights are small
+        order = c.scales[0, 0, :, 2].double().argsort(descending=True)
+        ramp = rising_cache(ops, r, n, 1, d, 60.0)
+        ramp.scales[0, 0, :, 2:] = c.scales[0, 0, order, 2:]
+        check_attend(ops, ramp, ones(t, g, d, BF16), int32(0), int32(n))
+        ramp.scales[0, 0, :, 2:] = c.scales[0, 0, order.flip(0), 2:]
+        check_attend(ops, ramp, ones(t, g, d, BF16), int32(0), int32(n))
+    c.check()
