@@ -50,7 +50,9 @@ inline int elem_bytes(int d) { return d == CZG_F32 ? 4 : 2; }
 // One launch.  pdl: the kernel may begin while the one before it on the stream still
 // runs: it calls griddepcontrol.wait before it touches memory that another kernel may
 // write, in every CTA, and lets the next one begin (launch_dependents) only after that, so
-// whatever is older than the kernel before it is complete too.  cluster: CTAs of x.
+// whatever is older than the kernel before it is complete too.  Such a kernel has begun while
+// that memory may still change, so it reads it by plain loads, never by the read-only path
+// (__ldg, const __restrict__ parameters).  cluster: CTAs of x.
 template <typename... KArgs, typename... Args>
 inline cudaError_t ops_launch(void (*kernel)(KArgs...), dim3 grid, int block, size_t smem, cudaStream_t st, bool pdl,
                               int cluster, Args &&...args) {

@@ -55,8 +55,8 @@ __device__ __forceinline__ uint32_t scan(uint32_t x, uint32_t *before, uint32_t 
 // latency (three passes of counting, two scans, one move).  256 threads a CTA took 4 us
 // more on the batch, one CTA an SM (119 registers) 10 us more.
 template <int D>
-__global__ void __launch_bounds__(kThreads, 2) k_kv4_evict(czg_kv4 c, const int32_t *__restrict__ slots,
-                                                        const int32_t *__restrict__ lengths, int b, int max_len, int budget,
+__global__ void __launch_bounds__(kThreads, 2) k_kv4_evict(czg_kv4 c, const int32_t *slots,
+                                                        const int32_t *lengths, int b, int max_len, int budget,
                                                         int recent, int32_t *__restrict__ kept, int32_t *__restrict__ new_len) {
     __shared__ uint32_t hist[kBins], part[kWarps];
     __shared__ int stay_list[kStretch];

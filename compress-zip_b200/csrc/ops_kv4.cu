@@ -32,9 +32,9 @@ constexpr float kFltMax = 3.402823466e38f;
 // the same direction), so every quotient lies in [0, 15].  A key's row and its value's are
 // neighbours.  CTA 0 looks for repeated slots.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) k_kv4_append(czg_kv4 c, const T *__restrict__ k, Strides ks, const T *__restrict__ v,
-                                                    Strides vs, int vec, const int32_t *__restrict__ slots,
-                                                    const int32_t *__restrict__ lengths, int b, int t) {
+__global__ void __launch_bounds__(256) k_kv4_append(czg_kv4 c, const T *k, Strides ks, const T *v,
+                                                    Strides vs, int vec, const int32_t *slots,
+                                                    const int32_t *lengths, int b, int t) {
     pdl_wait();
     pdl_trigger();
     if (blockIdx.x == 0) {
@@ -65,8 +65,8 @@ __global__ void __launch_bounds__(256) k_kv4_append(czg_kv4 c, const T *__restri
     float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     if (there && vec) {
         __align__(16) T y[4];
-        if (sizeof(T) == 4) *reinterpret_cast<uint4 *>(y) = __ldg(reinterpret_cast<const uint4 *>(src));
-        else *reinterpret_cast<uint2 *>(y) = __ldg(reinterpret_cast<const uint2 *>(src));
+        if (sizeof(T) == 4) *reinterpret_cast<uint4 *>(y) = *reinterpret_cast<const uint4 *>(src);
+        else *reinterpret_cast<uint2 *>(y) = *reinterpret_cast<const uint2 *>(src);
 #pragma unroll
         for (int j = 0; j < 4; j++) x[j] = to_f32(y[j]);
     } else if (there) {
@@ -111,8 +111,8 @@ __global__ void __launch_bounds__(256) k_kv4_append(czg_kv4 c, const T *__restri
 // take 47 us, 5.4 TB/s.  (16 codes a thread, whose 32 bytes are written in two halves, were
 // as fast; a grid row a sequence took twice as long for 4096 sequences of one entry.)
 template <typename T, int D>
-__global__ void __launch_bounds__(256) k_kv4_read(czg_kv4 c, const int32_t *__restrict__ slots,
-                                                  const int32_t *__restrict__ starts, uint32_t rows, uint32_t all,
+__global__ void __launch_bounds__(256) k_kv4_read(czg_kv4 c, const int32_t *slots,
+                                                  const int32_t *starts, uint32_t rows, uint32_t all,
                                                   T *__restrict__ k_out, T *__restrict__ v_out) {
     constexpr int P = D / 8, N = 2;
     pdl_wait();
@@ -390,7 +390,7 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
 #pragma unroll
         for (int i = 0; i < kChunk / THREADS; i++) {
             const int j = from + tid + i * THREADS;
-            raw[i] = j < here ? __ldg(reinterpret_cast<const uint2 *>(ranges + j)) : make_uint2(0, 0);
+            raw[i] = j < here ? *reinterpret_cast<const uint2 *>(ranges + j) : make_uint2(0, 0);
         }
     };
     // Lays them down.  2^te is from then on not below any of their values' steps, huge says
@@ -447,7 +447,7 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
             const T *src = static_cast<const T *>(p.q) + (there ? row_offset(p, p.qs, b, h, row) : 0) + part * 8;
             __align__(16) T v[8];
             if (there && p.vec) {
-                *reinterpret_cast<uint4 *>(v) = __ldg(reinterpret_cast<const uint4 *>(src));
+                *reinterpret_cast<uint4 *>(v) = *reinterpret_cast<const uint4 *>(src);
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; i++) v[i] = there ? src[i] : from_f32<T>(0.0f);

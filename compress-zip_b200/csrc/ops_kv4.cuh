@@ -48,7 +48,7 @@ __device__ __forceinline__ void kv4_check_distinct(const czg_kv4 &c, const int32
         __syncthreads();
 #pragma unroll 8
         for (int i = threadIdx.x; i < b; i += blockDim.x) {
-            const int slot = __ldg(slots + i), s = slot - base;
+            const int slot = slots[i], s = slot - base;
             if (slot >= 0 && s >= 0 && s < bits && (atomicOr(&seen[s >> 5], 1u << (s & 31)) >> (s & 31) & 1u))
                 atomicOr(c.status, CZG_KV4_TWICE);
         }

@@ -101,7 +101,7 @@ __device__ __forceinline__ void load8(const T *row, int64_t i, int64_t k, bool v
     if (vec && i + 8 <= k) {
 #pragma unroll
         for (int c = 0; c < (int)sizeof(T) / 2; c++) {
-            const uint4 t = __ldg(reinterpret_cast<const uint4 *>(row + i) + c);
+            const uint4 t = reinterpret_cast<const uint4 *>(row + i)[c];
             v.w[4 * c] = t.x; v.w[4 * c + 1] = t.y; v.w[4 * c + 2] = t.z; v.w[4 * c + 3] = t.w;
         }
     } else {
@@ -143,7 +143,7 @@ struct RowScale {
 // kHeld turns stay in registers between the two, longer ones are read again.
 constexpr int kQuantThreads = 256, kHeld = 4;
 template <typename T>
-__global__ void __launch_bounds__(kQuantThreads) k_quantize_rows(const T *__restrict__ x, int64_t ldx, int64_t k, int vec,
+__global__ void __launch_bounds__(kQuantThreads) k_quantize_rows(const T *x, int64_t ldx, int64_t k, int vec,
                                                                  int8_t *__restrict__ codes, int64_t ldc,
                                                                  float *__restrict__ scales) {
     pdl_wait();
@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(kQuantThreads) k_quantize_rows(const T *__rest
 // Many rows of up to 256 V values: a warp a row, all of it in registers, no barrier; the
 // CTA's four rows and its neighbours' cover one another's latency.
 template <typename T, int V>
-__global__ void __launch_bounds__(128) k_quantize_rows_warp(const T *__restrict__ x, int64_t ldx, int m, int k, int vec,
+__global__ void __launch_bounds__(128) k_quantize_rows_warp(const T *x, int64_t ldx, int m, int k, int vec,
                                                             int8_t *__restrict__ codes, int64_t ldc, float *__restrict__ scales) {
     pdl_wait();
     pdl_trigger();

@@ -172,3 +172,14 @@ def test_python_refusals(ops):
             ("CUDA device", lambda: ops.KV4Cache(k, k, s))):
         with pytest.raises(ValueError, match=text):
             call()
+
+
+def test_no_read_only_loads(root):
+    """The operators' kernels may begin while the kernel before them still writes their operands, and attend's
+    output may be its query: the read-only path promises memory that does not change during a kernel."""
+    folder = os.path.join(root, "compress-zip_b200", "csrc")
+    names = [n for n in os.listdir(folder) if n.startswith("ops_")]
+    assert len(names) >= 5
+    for name in names:
+        text = re.sub(r"//[^\n]*", "", open(os.path.join(folder, name)).read())
+        assert not re.search(r"__ldg\w*\s*\(|\.global\.nc|\bconst\s+\w+\s*\*\s*__restrict__", text), name
