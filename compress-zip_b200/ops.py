@@ -377,8 +377,8 @@ class KV4Cache:
         b = self._sequences(slots, lengths, "lengths")
         if self.weights is None:
             raise ValueError("the cache keeps no weights to rank entries by")
-        if budget < 1 or not 0 <= recent <= budget:
-            raise ValueError("1 <= budget and 0 <= recent <= budget are needed")
+        if not 1 <= budget < 1 << 31 or not 0 <= recent <= budget:
+            raise ValueError("1 <= budget < 2^31 and 0 <= recent <= budget are needed")
         kept = slots.new_empty((b, self.n_heads, budget))
         new = torch.empty_like(slots)
         if b:

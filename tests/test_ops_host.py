@@ -183,3 +183,13 @@ def test_no_read_only_loads(root):
     for name in names:
         text = re.sub(r"//[^\n]*", "", open(os.path.join(folder, name)).read())
         assert not re.search(r"__ldg\w*\s*\(|\.global\.nc|\bconst\s+\w+\s*\*\s*__restrict__", text), name
+
+
+def test_budgets_beyond_an_int(ops):
+    """2^32 + 1 would reach the library as 1."""
+    c = object.__new__(ops.KV4Cache)
+    c._index, c.weights = -1, torch.zeros(1)
+    n = torch.zeros(1, dtype=torch.int32)
+    for budget, recent in ((1 << 31, 0), ((1 << 32) + 1, 0), (0, 0), (5, 6), (5, -1)):
+        with pytest.raises(ValueError, match="budget"):
+            c.evict(n, n, budget, recent)
