@@ -40,10 +40,15 @@ __device__ __forceinline__ int64_t kv4_row(const czg_kv4 &c, int slot, int head,
 // Reports a slot that two sequences of a writing call name.  One CTA; a bit a slot, in
 // ranges of kDistinctBits slots.
 constexpr int kDistinctBits = 32768;
+__host__ __device__ constexpr int distinct_ranges(int n_slots) { return (n_slots - 1) / kDistinctBits + 1; }
+__host__ __device__ constexpr int distinct_base(int range) { return range * kDistinctBits; }
+static_assert(distinct_ranges(1) == 1 && distinct_ranges(kDistinctBits) == 1 && distinct_ranges(kDistinctBits + 1) == 2 &&
+              distinct_base(distinct_ranges(0x7FFFFFFF) - 1) == 0x7FFFFFFF / kDistinctBits * kDistinctBits,
+              "the last range of the most slots still begins at an int");
 __device__ __forceinline__ void kv4_check_distinct(const czg_kv4 &c, const int32_t *slots, int b) {
     __shared__ uint32_t seen[kDistinctBits / 32];
-    for (int base = 0; base < c.n_slots; base += kDistinctBits) {
-        const int bits = min(kDistinctBits, c.n_slots - base);
+    for (int range = 0, ranges = distinct_ranges(c.n_slots); range < ranges; range++) {   // counted: the next base may pass an int
+        const int base = distinct_base(range), bits = min(kDistinctBits, c.n_slots - base);
         for (int i = threadIdx.x; i < (bits + 31) / 32; i += blockDim.x) seen[i] = 0;
         __syncthreads();
 #pragma unroll 8
