@@ -9,6 +9,11 @@ without waiting; nothing is allocated but the results and a workspace, both by t
 Shapes and types are checked here (ValueError) and again by the library (CzgError).
 What only the device can see -- slots and lengths out of range -- sets bits that
 ``KV4Cache.check`` reads.  No fallback: tensors must be on a CUDA device.
+
+There is no backward pass.  ``linear_i8`` and ``KV4Cache.attend`` refuse (ValueError) an
+input that requires a gradient while torch records them: call them under
+``torch.no_grad()``, or detach the input.  ``quantize_rows`` and ``KV4Cache.append`` store codes,
+which have no gradient.
 """
 from __future__ import annotations
 
@@ -87,6 +92,13 @@ def _same_device(dev: torch.device, **tensors) -> None:
 
 
 _current_device = torch.cuda.current_device
+_recording = torch.is_grad_enabled
+
+
+def _no_gradient(what: str) -> None:
+    raise ValueError(f"{what} requires a gradient, which this operator does not have: use torch.no_grad() or detach it")
+
+
 # the handle of a device's current stream, without a Stream object around it where torch has that
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
@@ -201,6 +213,9 @@ def linear_i8(x, w: QRows, bias: Optional[torch.Tensor] = None, out_dtype: Optio
     if bias is not None and (bias.dtype != torch.float32 or bias.shape != (n,) or (n > 1 and bias.stride(0) != 1)
                              or bias.device != dev):
         raise ValueError(f"bias must be a contiguous float32 vector of {n} on {dev}")
+    if _recording() and (x2.requires_grad or w.scales.requires_grad or (bias is not None and bias.requires_grad)
+                         or (quantised and x.scales.requires_grad) or (out is not None and out.requires_grad)):
+        _no_gradient("an input or out")
     if dev.type != "cuda":
         raise ValueError(f"tensors must be on a CUDA device, not {dev}")
     if out is None:
@@ -347,6 +362,8 @@ class KV4Cache:
             raise ValueError("the last dimension of q must be adjacent")
         if q.get_device() != self._index:
             raise ValueError(f"q is on {q.device}, the cache on {self.device}")
+        if _recording() and (q.requires_grad or (out is not None and out.requires_grad)):
+            _no_gradient("q or out")
         if out is None:
             out = torch.empty_like(q)
         elif out.shape != shape or out.dtype is not q.dtype or out.get_device() != self._index:

@@ -193,3 +193,26 @@ def test_budgets_beyond_an_int(ops):
     for budget, recent in ((1 << 31, 0), ((1 << 32) + 1, 0), (0, 0), (5, 6), (5, -1)):
         with pytest.raises(ValueError, match="budget"):
             c.evict(n, n, budget, recent)
+
+
+def test_gradients_are_refused(ops):
+    """There is no backward pass: a result without its gradient would be silent."""
+    x, bias, scales = torch.zeros(4, 32), torch.zeros(8), torch.ones(8)
+    codes = torch.zeros(8, 32, dtype=torch.int8)
+    w = ops.QRows(codes, scales)
+
+    def grad(t):
+        return t.clone().requires_grad_()
+
+    calls = [lambda: ops.linear_i8(grad(x), w), lambda: ops.linear_i8(grad(x).view(2, 2, 32), w), lambda: ops.linear_i8(x, w, bias=grad(bias)),
+             lambda: ops.linear_i8(x, ops.QRows(codes, grad(scales))), lambda: ops.linear_i8(ops.QRows(codes, grad(scales)), w)]
+    c = object.__new__(ops.KV4Cache)
+    c._index, c.n_heads, c.head_dim, c.capacity = -1, 2, 64, 100
+    n, q = torch.zeros(1, dtype=torch.int32), torch.zeros(1, 1, 4, 64, dtype=torch.bfloat16)
+    calls.append(lambda: c.attend(grad(q), n, n))
+    for call in calls:
+        with pytest.raises(ValueError, match="gradient"):
+            call()
+    for call in calls[:5]:        # without gradients the next check answers
+        with torch.no_grad(), pytest.raises(ValueError, match="CUDA device"):
+            call()
