@@ -212,7 +212,7 @@ constexpr int kUnits = 128;
 __host__ __device__ constexpr int unit_of(int n) {
     int64_t u = kChunk;
     while (u * kUnits < n) u *= 2;
-    return u < 0x40000000 ? (int)u : 0x40000000;
+    return (int)u;   // 2^24 at most
 }
 __host__ __device__ constexpr int attend_warps(int nb) { return nb == 1 ? 2 : 4; }   // more rows, longer tiles: more warps to share a unit
 
@@ -843,7 +843,8 @@ k_kv4_attend(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
 // and a CTA takes RUNS rows of them (so fewer row_ctas do where no sequence may have more).
 // Bound by latency, one round of loads each for the statistics and what they scale: 5 us
 // for 128 units of 4 rows and 8 heads, 9 us with the weights of 64 sequences of up to 4096.
-constexpr int kJoinThreads = 256, kFew = 8, kMany = 1024;
+constexpr int kJoinThreads = 256, kFew = 8;
+static_assert(kUnits <= kJoinThreads, "a thread a unit");
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads) k_kv4_join(const __grid_constant__ AttendArgs p, int rows_padded, int row_ctas) {
     constexpr int TR = D / 4, RUNS = kJoinThreads / TR;   // TR threads a run, four dimensions each
@@ -888,36 +889,24 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv4_join(const __grid_constant
             store4(static_cast<T *>(p.out) + row_offset(p, p.os, b, h, r) + d, x, l == 0.0f ? 0.0f : 1.0f / l, huge ? 1.0f / kHuge : 1.0f, p.out_vec);
             return;
         }
-        __shared__ float s_f[kMany], red[kJoinThreads / 32];
+        __shared__ float s_f[kUnits], red[kJoinThreads / 32];
         __shared__ float4 runs[RUNS][TR];
         const int r = blockIdx.x;
-        float m = -INFINITY;
-        bool huge = false;   // as above
-        for (int u = tid; u < units; u += kJoinThreads) {
-            const float4 st = p.stat[first + (int64_t)u * rows_padded + r];
-            m = fmaxf(m, st.x);
-            huge |= signbit(st.y);
-        }
+        float4 st = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+        if (tid < units) st = p.stat[first + (int64_t)tid * rows_padded + r];
+        float m = st.x;
         for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
         if ((tid & 31) == 0) red[tid >> 5] = m;
-        huge = __syncthreads_or(huge);
+        const bool huge = __syncthreads_or(signbit(st.y));   // as above
         for (int w = 0; w < kJoinThreads / 32; w++) m = fmaxf(m, red[w]);
-        float l = 0.0f;
+        const float f = share(st.x, m);
+        float l = f * fabsf(st.y);
+        if (tid < units) s_f[tid] = huge && !signbit(st.y) ? f * kHuge : f;
+        __syncthreads();
         float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int u0 = 0; u0 < units; u0 += kMany) {
-            const int some = min(kMany, units - u0);
-            __syncthreads();
-            for (int u = tid; u < some; u += kJoinThreads) {
-                const float4 st = p.stat[first + (int64_t)(u0 + u) * rows_padded + r];
-                const float f = share(st.x, m);
-                l = __fmaf_rn(f, fabsf(st.y), l);
-                s_f[u] = huge && !signbit(st.y) ? f * kHuge : f;
-            }
-            __syncthreads();
 #pragma unroll 16
-            for (int u = run; u < some; u += RUNS)
-                add_scaled(x, s_f[u], *reinterpret_cast<const float4 *>(p.part + (first + (int64_t)(u0 + u) * rows_padded + r) * D + d));
-        }
+        for (int u = run; u < units; u += RUNS)
+            add_scaled(x, s_f[u], *reinterpret_cast<const float4 *>(p.part + (first + (int64_t)u * rows_padded + r) * D + d));
         runs[run][tid % TR] = x;
         for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
         __syncthreads();

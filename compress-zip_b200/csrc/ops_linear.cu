@@ -861,8 +861,9 @@ int quantize(const void *x, int64_t ldx, int64_t m, int64_t k, int8_t *codes, in
             return ops_cuda(ops_launch(kern, grid, 128, 0, st, true, 1, static_cast<const T *>(x), ldx, (int)m, (int)k, vec, codes, ldc, scales));
         };
         if (turns <= 2 * 32) return go(k_quantize_rows_warp<T, 2>);
-        if (turns <= 4 * 32) return go(k_quantize_rows_warp<T, 4>);
-        return go(k_quantize_rows_warp<T, 8>);
+        if constexpr (sizeof(T) == 2)   // fp32 rows of this branch have 4 turns at most
+            if (turns > 4 * 32) return go(k_quantize_rows_warp<T, 8>);
+        return go(k_quantize_rows_warp<T, 4>);
     }
     const int most = many && k <= kQuantThreads / 2 * 8 * kHeld ? kQuantThreads / 2 : kQuantThreads;
     const int threads = turns >= most ? most : (int)((turns + 31) / 32 * 32);
