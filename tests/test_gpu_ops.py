@@ -1029,3 +1029,75 @@ def test_attend_ranges_of_any_exponent(ops, d, g, t):
         ramp.scales[0, 0, :, 2:] = c.scales[0, 0, order.flip(0), 2:]
         check_attend(ops, ramp, ones(t, g, d, BF16), int32(0), int32(n))
     c.check()
+
+
+# ---- types, strides and scales that the tests above leave out --------------------------------------
+
+
+@pytest.mark.parametrize("with_bias", [False, True])
+@pytest.mark.parametrize("out_dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+def test_linear_i8_from_floats_of_every_type(ops, dtype, out_dtype, with_bias):
+    """Quantising in the call, by one kernel (at most 16 short rows) and by two, for every pair of types, from
+    rows of a wider tensor, with rows of zeros and rows that are not finite."""
+    for m, n, k in ((1, 512, 384), (5, 70, 33), (16, 200, 2048), (9, 130, 1500), (50, 300, 640), (17, 33, 1000)):
+        g = gen(m + n)
+        x = (3 * randn(g, m, k + 11)).to(dtype)[:, 3:k + 3]
+        w, bias = rand_codes(ops, g, n, k), randn(g, n) if with_bias else None
+        fine = torch.ones(m, dtype=torch.bool, device=DEV)
+        if m >= 5:
+            x[1] = 0
+            x[2, k // 2] = float("nan")
+            x[3, k - 1] = float("inf")
+            x[4, 0] = -float("inf")
+            fine[2:5] = False
+        y = ops.linear_i8(x, w, bias=bias, out_dtype=out_dtype)
+        q = ops.quantize_rows(x)
+        two = ops.linear_i8(q, w, bias=bias, out_dtype=out_dtype)
+        assert y.dtype == out_dtype and torch.equal(y[fine], two[fine])
+        assert torch.isnan(y[~fine]).all() and torch.isnan(two[~fine]).all()
+        check_linear(y[fine], ops.quantize_rows(x[fine]), w, bias)
+        if m >= 5:
+            assert torch.equal(y[1], (torch.zeros(n, device=DEV) if bias is None else bias).to(out_dtype))
+
+
+@pytest.mark.parametrize("g,t", [(4, 1), (2, 3)])
+def test_attend_scale_of_zero(ops, g, t):
+    """The plain mean of what a row sees."""
+    r = gen(g + 70)
+    c = noise_cache(ops, r, 4, 2, 900, 64, True)
+    check_attend(ops, c, randn(r, 3, t, 2 * g, 64).to(BF16), int32(2, 0, 3), int32(900, 1, 77), scale=0.0)
+    c.check()
+
+
+def test_attend_one_query_for_all(ops):
+    """Expanded queries (strides of 0) and a bound of the lengths above the capacity."""
+    r = gen(71)
+    c = noise_cache(ops, r, 3, 2, 700, 128, False)
+    q = randn(r, 1, 1, 1, 128).to(FP16).expand(3, 4, 6, 128)
+    y = check_attend(ops, c, q, int32(0, 1, 2), int32(700, 5, 300), max_len=100000)
+    assert torch.equal(y, c.attend(q.contiguous(), int32(0, 1, 2), int32(700, 5, 300)))
+    c.check()
+
+
+def test_two_caches_on_two_streams_at_once(ops):
+    r = gen(72)
+    caches = [noise_cache(ops, r, 40, 2, 2100, 64, True) for _ in range(2)]
+    first = [c.weights.clone() for c in caches]
+    q = randn(r, 40, 1, 8, 64).to(BF16)
+    slots = torch.randperm(40, generator=r, device=DEV).int()
+    lengths = torch.randint(0, 2101, (40,), generator=r, device=DEV, dtype=torch.int32)
+    want = [[c.attend(q, slots, lengths) for _ in range(6)] for c in caches]
+    grown = [c.weights.clone() for c in caches]
+    for c, w in zip(caches, first):
+        c.weights.copy_(w)
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in caches], [[], []]
+    for _ in range(6):
+        for i, c in enumerate(caches):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(c.attend(q, slots, lengths))
+    torch.cuda.synchronize()
+    for i, c in enumerate(caches):
+        assert all(torch.equal(a, b) for a, b in zip(got[i], want[i])) and torch.equal(c.weights, grown[i])
+        c.check()
