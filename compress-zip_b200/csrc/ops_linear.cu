@@ -808,12 +808,31 @@ int launch_pair(const int8_t *x, int64_t ldx, const int8_t *w, int64_t ldw, int6
                                kPairSmem, st, after_quantise, 2, mw, mx, p));
 }
 
-// Calls whose x rows the product quantises itself: at most 16 rows, 64 KB of bf16 in all, so
-// that reading them in every CTA costs less than a launch (1 x 512 x 384: 10.9 us a call from Python, 14.8 with two kernels).
+// Calls whose x rows the product can quantise itself: at most 16 rows, 64 KB of bf16 in all, whose
+// codes a cluster's rings hold.
 constexpr int kSmallRows = 16, kSmallValues = 32768, kSmallSteps = 11;   // steps a CTA's ring holds
 static_assert(kSmallSteps * LinearCfg<kSmallRows>::kStage + LT * kSmallRows * 4 <= kRingBytes, "the codes of all steps have their place");
 bool small_call(int64_t m, int64_t k) {
     return m <= kSmallRows && m * k <= kSmallValues && k <= 8 * kSmallSteps * TC_BK;
+}
+// Over how many CTAs it splits k: as many as there are SMs, of at least two steps each, and
+// no more steps than the ring holds.
+int small_split(int64_t tiles_n, int steps) {
+    int split = 1;
+    while (split < 8 && (steps > split * kSmallSteps || (tiles_n * split * 2 <= sm_count() && steps >= split * 4))) split *= 2;
+    return split;
+}
+// Whether that is the better form.  It saves a launch (4 us of a Python call), but each tile's CTA
+// loads its steps of weights with no other tile's under way behind them, and quantises all of x.  On
+// the device, one kernel and the two of two calls, us, for 1 x 384: 5.0 and 5.6 at 512 channels, 6.2 and 7.5 at
+// 32,768, 15.4 and 14.2 at 128,000; 1 x 2048: 6.1 and 6.9, 31.8 and 18.1, 116 and 50; 8 x 2048: 10.4
+// and 7.1, 54.8 and 18.3, 209 and 51.  So: while an SM has at most kSmallTurns steps to load, one
+// wave of tiles after the other.
+constexpr int64_t kSmallTurns = 8;
+bool small_pays(int64_t n, int64_t k) {
+    const int64_t tiles = (n + LT - 1) / LT, steps = (k + TC_BK - 1) / TC_BK;
+    const int split = small_split(tiles, (int)steps), sms = sm_count();
+    return (tiles * split + sms - 1) / sms * ((steps + split - 1) / split) <= kSmallTurns;
 }
 
 // Which tile, and over how many CTAs k is split: the least of a model of the time in
@@ -906,8 +925,7 @@ int linear_small(const void *x, int64_t ldx, const int8_t *w, int64_t ldw, const
                  int64_t n, int64_t k, void *out, int64_t ldo, cudaStream_t st) {
     LinearArgs p{nullptr, ws, bias, out, ldo, (int)m, (int)n, (int)((k + TC_BK - 1) / TC_BK), (int)((n + LT - 1) / LT), 0, 0, 1,
                  aligned(out, 4 * sizeof(T)) && ldo % 4 == 0, x, ldx, (int)k, aligned(x, 16) && (m == 1 || ldx * sizeof(TX) % 16 == 0)};
-    // as many CTAs as there are SMs, of at least two steps each, and no more steps than the ring holds
-    while (p.split < 8 && (p.steps > p.split * kSmallSteps || (p.tiles_n * p.split * 2 <= sm_count() && p.steps >= p.split * 4))) p.split *= 2;
+    p.split = small_split(p.tiles_n, p.steps);
     return launch_linear<kSmallRows, T, TX>(nullptr, 0, w, ldw, k, p, false, st);
 }
 
@@ -1008,9 +1026,14 @@ extern "C" int czg_linear_i8(const int8_t *x, int64_t ld_x, const float *x_scale
                       static_cast<cudaStream_t>(stream));
 }
 
+static uint64_t rows_workspace(int64_t m, int64_t k) { return (uint64_t)m * (uint64_t)codes_ld(k) + (((uint64_t)m * 4 + 15) & ~15ull); }
+
 extern "C" uint64_t czg_linear_i8_workspace(int64_t m, int64_t k) {
-    if (m <= 0 || k <= 0 || small_call(m, k)) return 0;
-    return (uint64_t)m * (uint64_t)codes_ld(k) + (((uint64_t)m * 4 + 15) & ~15ull);
+    return m <= 0 || k <= 0 || small_call(m, k) ? 0 : rows_workspace(m, k);
+}
+
+extern "C" uint64_t czg_linear_i8_dynamic_workspace(int64_t m, int64_t n, int64_t k) {
+    return m <= 0 || n <= 0 || k <= 0 || (small_call(m, k) && small_pays(n, k)) ? 0 : rows_workspace(m, k);
 }
 
 extern "C" int czg_linear_i8_dynamic(const void *x, int dtype, int64_t ld_x, const int8_t *w, int64_t ld_w,
@@ -1024,7 +1047,7 @@ extern "C" int czg_linear_i8_dynamic(const void *x, int dtype, int64_t ld_x, con
     if (int st = check_apart(out, ld_out * eb, n * eb, x, ld_x * xb, k * xb, m, m, "out lies over x")) return st;
     if (int st = check_apart(out, ld_out * eb, n * eb, w, ld_w, k, m, n, "out lies over w")) return st;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (small_call(m, k)) {
+    if (small_call(m, k) && (!ws || ws_bytes < rows_workspace(m, k) || small_pays(n, k))) {
         if (out_dtype == CZG_F32) return linear_small_of<float>(dtype, x, ld_x, w, ld_w, w_scale, bias, m, n, k, out, ld_out, st);
         if (out_dtype == CZG_BF16)
             return linear_small_of<__nv_bfloat16>(dtype, x, ld_x, w, ld_w, w_scale, bias, m, n, k, out, ld_out, st);

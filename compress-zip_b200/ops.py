@@ -30,7 +30,7 @@ _INT32 = torch.int32
 
 # The exported symbols of include/czg_ops.h, checked by the CPU test suite.
 EXPORTS = ["czg_ops_last_error", "czg_ops_check", "czg_quantize_rows", "czg_linear_i8", "czg_linear_i8_workspace",
-           "czg_linear_i8_dynamic", "czg_kv4_append", "czg_kv4_read", "czg_kv4_attend_workspace",
+           "czg_linear_i8_dynamic_workspace", "czg_linear_i8_dynamic", "czg_kv4_append", "czg_kv4_read", "czg_kv4_attend_workspace",
            "czg_kv4_attend", "czg_kv4_evict"]
 
 STATUS_BITS = {1: "a slot beyond the cache", 2: "a length or entry outside its range",
@@ -65,6 +65,7 @@ def lib() -> C.CDLL:
             fn = getattr(L, name)
             fn.argtypes, fn.restype = args, C.c_int
         L.czg_linear_i8_workspace.argtypes, L.czg_linear_i8_workspace.restype = [L64, L64], U64
+        L.czg_linear_i8_dynamic_workspace.argtypes, L.czg_linear_i8_dynamic_workspace.restype = [L64, L64, L64], U64
         L.czg_kv4_attend_workspace.argtypes, L.czg_kv4_attend_workspace.restype = [K, I, I, I, I], U64
         L.czg_ops_check.argtypes, L.czg_ops_check.restype = [], C.c_int
         L.czg_ops_last_error.argtypes, L.czg_ops_last_error.restype = [], C.c_char_p
@@ -236,7 +237,7 @@ def linear_i8(x, w: QRows, bias: Optional[torch.Tensor] = None, out_dtype: Optio
         _call(dev, L.czg_linear_i8, x2.data_ptr(), x.ld, x.scales.data_ptr(), w.codes.data_ptr(), w.ld, w.scales.data_ptr(),
               bias_ptr, m, n, k, out2.data_ptr(), out_code, ldo)
     else:
-        need = L.czg_linear_i8_workspace(m, k)
+        need = L.czg_linear_i8_dynamic_workspace(m, n, k)
         ws = w.codes.new_empty(need) if need else None
         _call(dev, L.czg_linear_i8_dynamic, x2.data_ptr(), code, x2.stride(0) if m > 1 else k, w.codes.data_ptr(), w.ld,
               w.scales.data_ptr(), bias_ptr, m, n, k, out2.data_ptr(), out_code, ldo, ws.data_ptr() if need else 0, need)

@@ -64,8 +64,11 @@ int czg_linear_i8(const int8_t *x, int64_t ld_x, const float *x_scale, const int
 
 /* czg_quantize_rows and then czg_linear_i8, with the same bits.  ws: 16-byte aligned,
  * czg_linear_i8_workspace(m, k) bytes (0, and NULL will do, for a few short rows, which
- * one kernel takes), free again when the queued work is done. */
+ * one kernel takes), free again when the queued work is done.  With
+ * czg_linear_i8_dynamic_workspace(m, n, k) bytes, which are never fewer, a few short rows on
+ * so many channels that two kernels are faster take two. */
 uint64_t czg_linear_i8_workspace(int64_t m, int64_t k);
+uint64_t czg_linear_i8_dynamic_workspace(int64_t m, int64_t n, int64_t k);
 int czg_linear_i8_dynamic(const void *x, int dtype, int64_t ld_x, const int8_t *w, int64_t ld_w,
                           const float *w_scale, const float *bias, int64_t m, int64_t n, int64_t k, void *out,
                           int out_dtype, int64_t ld_out, void *ws, uint64_t ws_bytes, void *stream);

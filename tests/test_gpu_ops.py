@@ -1101,3 +1101,19 @@ def test_two_caches_on_two_streams_at_once(ops):
     for i, c in enumerate(caches):
         assert all(torch.equal(a, b) for a, b in zip(got[i], want[i])) and torch.equal(c.weights, grown[i])
         c.check()
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 128000, 384), (8, 20000, 2048), (2, 5000, 11264), (16, 40000, 1000)])
+def test_linear_i8_few_rows_on_many_channels(ops, m, n, k):
+    """One kernel or two, with a workspace or without: the same bits."""
+    g = gen(n)
+    x, w, bias = randn(g, m, k).to(BF16), rand_codes(ops, g, n, k), randn(g, n)
+    y = ops.linear_i8(x, w, bias=bias)
+    q = ops.quantize_rows(x)
+    assert torch.equal(y, ops.linear_i8(q, w, bias=bias))
+    check_linear(y, q, w, bias)
+    L, none = ops.lib(), torch.empty_like(y)
+    assert L.czg_linear_i8_dynamic_workspace(m, n, k) > 0 and L.czg_linear_i8_workspace(m, k) == 0
+    st = L.czg_linear_i8_dynamic(x.data_ptr(), 1, k, w.codes.data_ptr(), w.ld, w.scales.data_ptr(), bias.data_ptr(), m, n, k,
+                                 none.data_ptr(), 1, n, None, 0, torch.cuda.current_stream().cuda_stream)
+    assert st == 0 and torch.equal(none, y)

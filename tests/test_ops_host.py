@@ -216,3 +216,14 @@ def test_gradients_are_refused(ops):
     for call in calls[:5]:        # without gradients the next check answers
         with torch.no_grad(), pytest.raises(ValueError, match="CUDA device"):
             call()
+
+
+def test_few_rows_on_many_channels_take_two_kernels(ops):
+    """One kernel quantises a few short rows in every tile of channels: not where tiles come in many waves."""
+    L = ops.lib()
+    for m, n, k, two in ((1, 512, 384, False), (8, 512, 2048, False), (16, 4096, 2048, False), (1, 32768, 384, False),
+                         (1, 128000, 384, True), (1, 16384, 2048, True), (8, 128000, 2048, True), (2, 4096, 11264, True),
+                         (17, 100, 100, True), (0, 512, 384, False), (1, 0, 384, False)):
+        need = L.czg_linear_i8_dynamic_workspace(m, n, k)
+        assert need == (m * ((k + 15) // 16 * 16) + (4 * m + 15) // 16 * 16 if two else 0)
+        assert need >= L.czg_linear_i8_workspace(m, k) or n == 0
