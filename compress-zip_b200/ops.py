@@ -5,7 +5,8 @@ The int8 product with scales for each token and channel (``quantize_rows``,
 over it and eviction from it by accumulated attention weight.
 
 Every call queues its work on the current stream of its tensors' device and returns
-without waiting; nothing is allocated but the results and a workspace, both by torch.
+without waiting; nothing is allocated but the results, a workspace and, in ``linear_i8``, a
+copy of an x whose leading dimensions cannot be viewed as rows, all by torch.
 Shapes and types are checked here (ValueError) and again by the library (CzgError).
 What only the device can see -- slots and lengths out of range -- sets bits that
 ``KV4Cache.check`` reads.  No fallback: tensors must be on a CUDA device.
@@ -351,7 +352,9 @@ class KV4Cache:
         entries, row i seeing the first lengths - (t - 1 - i); rows that see none give 0.
         hq is a multiple of n_heads.  max_len (default: the capacity) bounds the lengths,
         scale defaults to head_dim ** -0.5.  With weights, each entry's grows by its
-        probabilities, summed over the rows and query heads of its key head."""
+        probabilities, summed over the rows and query heads of its key head, and the workspace
+        takes 4 bytes a row, query head and entry of max_len: give it where the capacity is far
+        above the lengths.  A row's last bits may differ between calls of other t."""
         b = self._sequences(slots, lengths, "lengths")
         shape, qs = q.shape, q.stride()
         if len(shape) != 4 or shape[0] != b or shape[3] != self.head_dim or shape[2] % self.n_heads:

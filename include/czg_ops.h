@@ -18,7 +18,10 @@
  *
  * A row of a product, and a sequence of a cache call, depends on its own operands alone:
  * not on how many others are in the call, on its place among them, its slot, or the
- * grid, to the bit.  No result comes out of an atomic whose order could change it.
+ * grid, to the bit.  No result comes out of an atomic whose order could change it.  A
+ * sequence's operands are all its rows and entries of the call: attention of the same row
+ * over the same entries may differ in its last bits between calls of one row (t = 1) and of
+ * several, and between calls that hold more or fewer entries behind those it sees.
  */
 #ifndef CZG_OPS_H
 #define CZG_OPS_H
@@ -80,8 +83,9 @@ int czg_linear_i8_dynamic(const void *x, int dtype, int64_t ld_x, const int8_t *
  * dimension 2i in its low half, and two bf16 numbers:
  *   lo = min x rounded down, step = (max x - lo) / 15 rounded up,
  *   code = round-half-even((x - lo) / step)   (step 0: code 0), held value lo + step * code
- * so that no value is off by more than step / 2.  A row with a NaN or an infinity, or
- * whose range overflows fp32, holds NaN in every place.
+ * so that no value is off by more than step / 2, but for the difference and the quotient,
+ * which round to fp32 before the code does (30 * 2^-24 of a step next to a half).  A row with a
+ * NaN or an infinity, or whose range overflows fp32, holds NaN in every place.
  *   k, v     [n_slots][n_heads][capacity][head_dim / 2] bytes, 16-byte aligned
  *   scales   [n_slots][n_heads][capacity][4] bf16: k step, k lo, v step, v lo; 8-byte aligned
  *   weights  NULL, or [n_slots][n_heads][capacity] sums of attention weights
@@ -124,9 +128,17 @@ int czg_kv4_read(const czg_kv4 *cache, const int32_t *slots, const int32_t *star
  * hq a multiple of n_heads, query heads of a key head adjacent.  out may be q itself, and
  * lies over no other part of it.
  *   out = sum_j p_j v_j, p = softmax_j(scale q.k_j)
+ * Scores, p and the sums are fp32; p below 2^-126 of a row's largest counts as 0.  p_j step_j is
+ * rounded to 11 bits (fp16: 22), and to 2^-25 of the largest p times the largest step of those
+ * that are alike within 2^6, or of the row's largest p_j step_j, so what other entries hold,
+ * seen or not, costs a row nothing.  Values may be as large as bf16 goes.
  * cache->weights != NULL: every entry's weight grows by its p, summed over the rows
  * and query heads of its key head.  max_len: no length of the call is above it.
- * ws: 16-byte aligned, czg_kv4_attend_workspace bytes (may be 0). */
+ * The rows of each key head make blocks of 16 (of 8 where there are no more); all key heads'
+ * blocks of a sequence, about t * hq / 16, are at most 65,535 (CZG_E_LIMIT).
+ * ws: 16-byte aligned, czg_kv4_attend_workspace bytes (may be 0): for calls of more than 512
+ * entries or, with weights, of several blocks of rows, a partial result of each row and unit (at
+ * most 128 units a sequence), and with weights 4 bytes a row, query head and entry of max_len. */
 uint64_t czg_kv4_attend_workspace(const czg_kv4 *cache, int32_t b, int32_t t, int32_t hq, int32_t max_len);
 int czg_kv4_attend(const czg_kv4 *cache, const void *q, int64_t q_sb, int64_t q_st, int64_t q_sh, int dtype,
                    const int32_t *slots, const int32_t *lengths, int32_t b, int32_t t, int32_t hq,

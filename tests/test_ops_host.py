@@ -227,3 +227,17 @@ def test_few_rows_on_many_channels_take_two_kernels(ops):
         need = L.czg_linear_i8_dynamic_workspace(m, n, k)
         assert need == (m * ((k + 15) // 16 * 16) + (4 * m + 15) // 16 * 16 if two else 0)
         assert need >= L.czg_linear_i8_workspace(m, k) or n == 0
+
+
+def test_attend_limit_of_rows(ops):
+    c = cache(ops)
+
+    def attend(t):
+        return ("czg_kv4_attend", c, P, 256, 256, 64, BF16, P, P, 2, t, 4, 100, 0.1, 1 << 40, 256, 256, 64, P, 1 << 50, None)
+
+    refused(ops, E_LIMIT, "65,535 blocks", *attend(32768 * 8))      # 2 key heads of 32,768 blocks of 16 rows
+    refused(ops, E_LIMIT, "too many rows", *attend(1 << 30))
+    need = ops.lib().czg_kv4_attend_workspace        # with weights, scores; with several blocks of rows, partial results
+    assert need(c, 2, 7, 4, 100) == 2 * 7 * 4 * 100 * 4
+    assert need(c, 2, 9, 4, 100) == 2 * 2 * 32 * (64 * 4 + 16) + 2 * 9 * 4 * 100 * 4
+    assert need(cache(ops, weights=None), 2, 9, 4, 100) == 0
