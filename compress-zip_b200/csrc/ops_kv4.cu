@@ -198,10 +198,12 @@ __global__ void __launch_bounds__(256) k_kv4_read(czg_kv4 c, const int32_t *slot
 // on the steps.  Scores, maxima and sums are fp32; exponentials are ex2.approx (2^-22).
 //
 // Measured: one sequence of 131,071 entries, 32 heads on 8, D = 128, bf16 (143 MB): 37 us with
-// the join, 3.8 TB/s; 4096 sequences of up to 512, 6 heads on 1, D = 64 (84 MB): 32.5 us.  The
-// loads alone take 25 and 21 us (the second mostly the CTAs' beginnings and ends), the
-// arithmetic is bound by issue, about half of it unpacking on the half-rate ALU pipe.  Tiles of 32 entries
-// and two stages hold the most CTAs on an SM (8 at D = 128): tiles of 64 took 43 us, three
+// the join, 3.8 TB/s; 4096 sequences of up to 512, 6 heads on 1, D = 64 (84 MB): 33.5 us.  The
+// loads alone take 25 and 21 us (the second mostly the CTAs' beginnings and ends).  No pipe is
+// full (ALU 44%, DRAM 49% and 28%, 18% and 26% of the warps active): loads, arithmetic, half of
+// it unpacking on the half-rate ALU pipe, and a CTA's ends overlap too little.  Units whose rows
+// scale their weights themselves take a quarter to a third more (46.6 and 45.1 us).  Tiles of 32
+// entries and two stages hold the most CTAs on an SM (8 at D = 128): tiles of 64 took 43 us, three
 // and four stages 46 and 47; units of 256 took 7% more, one warp a unit as much.
 //
 // Between the warps of a CTA, and between units (k_kv4_join), partial results are joined
