@@ -131,7 +131,8 @@ int czg_kv4_read(const czg_kv4 *cache, const int32_t *slots, const int32_t *star
  * Scores, p and the sums are fp32; p below 2^-126 of a row's largest counts as 0.  p_j step_j is
  * rounded to 11 bits (fp16: 22), and to 2^-25 of the largest p times the largest step of those
  * that are alike within 2^6, or of the row's largest p_j step_j, so what other entries hold,
- * seen or not, costs a row nothing.  Values may be as large as bf16 goes.
+ * seen or not, costs a row nothing.  Values may be as large as bf16 goes (beside one of 2^87
+ * and more, in the same 512 entries or unit, those below 2^-90 lose bits).
  * cache->weights != NULL: every entry's weight grows by its p, summed over the rows
  * and query heads of its key head.  max_len: no length of the call is above it.
  * The rows of each key head make blocks of 16 (of 8 where there are no more); all key heads'
